@@ -374,6 +374,48 @@ int llmq_awq_dequant(const int32_t* qweight, const void* scales, const int32_t* 
 int llmq_awq_dequant_t(const int32_t* qweight, const void* scales, const int32_t* qzeros, void* out,
                        int64_t K, int64_t N, int64_t group, llmq_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * Block-scaled fp8 (no counterpart in the reference, whose FP8 modules refuse group-wise quantization, linear_fp8.py): activations in e4m3fn with
+ * one fp32 scale per token and 128 channels, weights in e4m3fn with one per block of 128 x 128.
+ * ------------------------------------------------------------------------------------ */
+
+/* q[m, k] = e4m3(x[m, k] / s),  s = a_scale[m, k / 128] = max(max |x[m, 128 (k / 128) ..]|, 1e-12) / 448, in fp32.
+ * x: [M, K] bf16 / f16 (K % 8 == 0, ldx % 8 == 0, 16-byte aligned); q: [M, K] contiguous, 8-byte aligned; scale: fp32 [M, ceil(K / 128)].
+ * The last group of a row may be short.  A group that holds an infinity or a NaN has that as its scale; its codes follow the division. */
+int llmq_quant_fp8_per_group(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* q, float* scale, llmq_stream_t stream);
+
+/* The residual's addition and RMSNorm in one pass, with an output in x_dtype or in 8 bits:
+ *   h = x_dtype(x + residual);  y = (h * inv) * weight, inv = 1 / sqrt(mean(h^2) + eps), in fp32
+ *   LLMQ_NORM_SAME       y (required) = x_dtype(y)
+ *   LLMQ_NORM_I8_TOKEN   q = clamp(rint(y / s), -128, 127), s = max(max |y|, 1e-5) / 127          scale: fp32 [M]
+ *   LLMQ_NORM_FP8_TOKEN  q = e4m3(y / s),                   s = max(max |y|, 1e-12) / 448         scale: fp32 [M]
+ *   LLMQ_NORM_FP8_GROUP  as llmq_quant_fp8_per_group of the fp32 y                                scale: fp32 [M, ceil(K / 128)]
+ * The 8-bit forms write x_dtype(y) too where y is not null.  Unlike llmq_rmsnorm_quant_*, which round h * inv and y to x_dtype as the
+ * reference does, y is not rounded before it is quantized.  residual null: h = x, and h is not written.  h may be the residual itself (the
+ * addition in place) or x; otherwise nothing may overlap.  K % 8 == 0, row strides % 8 == 0, 16-byte aligned (q: 8). */
+enum { LLMQ_NORM_SAME = 0, LLMQ_NORM_I8_TOKEN = 1, LLMQ_NORM_FP8_TOKEN = 2, LLMQ_NORM_FP8_GROUP = 3 };
+int llmq_add_rmsnorm(int out, const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const void* residual, int64_t ldr,
+                     void* h, int64_t ldh, const void* weight, float eps, void* y, void* q, float* scale, llmq_stream_t stream);
+
+/* out[m, n] = out_dtype( sum_b a_scale[m, b] w_scale[n / 128, b] sum_{k in block b} A[m, k] B[n, k]  + bias[n] ), blocks of 128 of K, fp32.
+ * A: e4m3fn [M, K] (lda >= K), B: e4m3fn [N, K] (ldb >= K), 16-byte aligned, K, lda, ldb multiples of 16 and at most 2^23; a_scale: fp32
+ * [M, ceil(K / 128)], w_scale: fp32 [ceil(N / 128), ceil(K / 128)], contiguous; bias: [N] bf16 / f16 / f32 or null; out: bf16 / f16, ldo >= N.
+ * workspace: >= llmq_gemm_fp8_block_workspace_bytes(M, N, K) bytes, 16-byte aligned (may be NULL when that is 0). */
+int llmq_gemm_fp8_block(const uint8_t* A, int64_t lda, const float* a_scale, const uint8_t* B, int64_t ldb, const float* w_scale,
+                        const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                        void* workspace, size_t workspace_bytes, llmq_stream_t stream);
+size_t llmq_gemm_fp8_block_workspace_bytes(int64_t M, int64_t N, int64_t K);
+
+/* The same product by experts: rows offsets[e] .. offsets[e + 1] - 1 of A with the weights of expert e.  B: [experts, N, K], w_scale:
+ * [experts, ceil(N / 128), ceil(K / 128)], bias: [experts, N] or null, all contiguous; offsets: int32 [experts + 1] on the device, ascending;
+ * values outside [0, M] are taken as the nearest inside.  Rows that belong to no expert are not written.  At most 65536 experts.  No workspace;
+ * nothing is read back by the host, so a captured call follows the offsets of its replay. */
+int llmq_gemm_fp8_block_grouped(const uint8_t* A, int64_t lda, const float* a_scale, const uint8_t* B, const float* w_scale,
+                                const int32_t* offsets, int64_t experts, const void* bias, int bias_dtype, void* out, int out_dtype,
+                                int64_t ldo, int64_t M, int64_t N, int64_t K, llmq_stream_t stream);
+/* Tuning / test hook: tile configuration `cfg` (-1: the built-in choice) and K split of later calls of the two products.  Per host thread. */
+int llmq_gemm_fp8_block_force_plan(int cfg, int splits);
+
 #ifdef __cplusplus
 }
 #endif

@@ -80,6 +80,12 @@ SIGNATURES = {
     "llmq_awq_workspace_init": (_int, [_vp, _sz, _vp]),
     "llmq_awq_dequant": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "llmq_awq_dequant_t": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "llmq_quant_fp8_per_group": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "llmq_add_rmsnorm": (_int, [_int, _vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _f32, _vp, _vp, _vp, _vp]),
+    "llmq_gemm_fp8_block": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _vp, _int, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "llmq_gemm_fp8_block_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "llmq_gemm_fp8_block_grouped": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _int, _vp, _int, _i64, _i64, _i64, _i64, _vp]),
+    "llmq_gemm_fp8_block_force_plan": (_int, [_int, _int]),
 }
 
 _lib = None

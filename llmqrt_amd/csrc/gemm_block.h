@@ -1,0 +1,43 @@
+// Block-scaled fp8 products (one scale per token and 128 of K, one per 128 x 128 weights), alone and by experts: what the kernels
+// (gemm_block_tile.hip) and the planner and entry points (gemm_block.hip) share.
+#pragma once
+#include "llmq_common.h"
+
+namespace llmq {
+
+constexpr int kScaleBlock = 128;
+
+struct BlockArgs {
+    const uint8_t* A;      // [M, K] e4m3
+    const float* sa;       // [M, KB]
+    const uint8_t* B;      // [N, K] e4m3, of expert 0
+    const float* sw;       // [NB, KB], of expert 0
+    const void* bias;      // [N] of expert 0, or null
+    void* out;             // [M, N]
+    const int32_t* offsets;  // experts + 1 first rows, or null: one matrix for all rows
+    float* partials;       // K split: [splits, M, N]
+    int64_t lda, ldb, ldo;
+    int M, N, K, KB, NB, experts;
+    int blocks_per_split;  // of 128 of K
+    int bias_dtype, out_dtype;
+};
+
+// Rows [first, last) of expert e, whatever the offsets hold: never outside [0, M].
+__device__ __forceinline__ void expert_rows(const BlockArgs& g, int e, int& first, int& last) {
+    first = min(max(g.offsets[e], 0), g.M);
+    last = min(max(g.offsets[e + 1], first), g.M);
+}
+
+struct BlockTile { int bm, bn, nt; };
+constexpr BlockTile kBlockTiles[] = {
+    {256, 256, 512},  // 0: 8 wavefronts of 128 x 64
+    {128, 256, 512},  // 1: 8 of 64 x 64
+    {128, 128, 256},  // 2: 4 of 64 x 64
+    {64, 128, 256},   // 3: 4 of 32 x 64
+    {32, 128, 256},   // 4: 4 of 32 x 32
+};
+constexpr int kNumBlockTiles = sizeof(kBlockTiles) / sizeof(kBlockTiles[0]);
+
+int launch_block_tile(int cfg, int splits, const BlockArgs& g, hipStream_t st);
+
+}  // namespace llmq

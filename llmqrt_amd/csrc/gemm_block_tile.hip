@@ -1,0 +1,397 @@
+// Block-scaled fp8 product, tile kernel.
+//
+//   out[m, n] = sum_b sa[m, b] sw[n / 128, b] sum_{k in block b} A[m, k] B[n, k]   (+ bias[n])        A, B e4m3, blocks of 128 of K
+//
+// Each block of K is one v_mfma_f32_16x16x128_f8f6f4 per 16 x 16 outputs that starts from zero; its four results per lane are scaled into the
+// fp32 accumulators on the vector unit.  The weights feed the MFMA's row operand, so a lane holds one token (lane % 16) and four
+// channels, and its factor sa sw is one register for all channel tiles of the token.
+#include <type_traits>
+
+#include "gemm_block.h"
+
+namespace llmq {
+namespace {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+constexpr int kNumXcd = 8, kGroupM = 8;
+
+template <int B, int E, class F>
+__device__ __forceinline__ void unrolled(F&& f) {
+    if constexpr (B < E) {
+        f(std::integral_constant<int, B>{});
+        unrolled<B + 1, E>(f);
+    }
+}
+
+// A block of WM x WN wavefronts owns BM tokens x BN channels; a wavefront (16 TM) x (16 TN) of them.
+template <int BM_, int BN_, int WM_, int WN_>
+struct TileCfg {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+    static constexpr int NT = WM * WN * kWave;
+    static constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16, TT = TM * TN;
+    static constexpr int A_LOADS = BM * 8 / NT, B_LOADS = BN * 8 / NT, LPT = A_LOADS + B_LOADS + 1;  // per thread and stage, one of scales
+    static constexpr int DATA = (BM + BN) * 128, STAGE = DATA + NT * 4;  // bytes; the scales' slots are one per thread
+    static constexpr int NS = 4 * STAGE <= 80 * 1024 ? 4 : 3 * STAGE <= 160 * 1024 ? 3 : 2;
+    static constexpr int LDS_BYTES = NS * STAGE;
+    static_assert(TM % 2 == 0 && TN >= 2 && TT % 4 == 0, "fragment parity, pending products");
+    static_assert(BM + (BN + 127) / 128 <= NT && 128 % WTN == 0 && (NT / 8) % 16 == 0, "scale slots, a wavefront's channels in one block, swizzle");
+    static_assert(A_LOADS * NT == BM * 8 && B_LOADS * NT == BN * 8 && (NS - 2) * LPT < 64, "even pieces, vmcnt");
+};
+
+// LDS place of 16-byte chunk c of row r: 16 rows of one chunk fall on 16 places
+__device__ __forceinline__ int chunk_at(int r, int c) { return (r * 8 + (c ^ ((r >> 1) & 7))) * 16; }
+
+// sum over lanes 0 .. lane
+__device__ __forceinline__ int wave_prefix(int v) {
+    const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+    for (int o = 1; o < kWave; o *= 2) {
+        const int up = __shfl_up(v, o);
+        if (lane >= o) v += up;
+    }
+    return v;
+}
+
+// flat id -> (tile of rows, tile of channels): contiguous ranges per XCD, then groups of kGroupM tiles of rows
+__device__ __forceinline__ void tile_of(int bid, int nblk, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int q = nblk / kNumXcd, r = nblk % kNumXcd, xcd = bid % kNumXcd, local = bid / kNumXcd;
+    const int pid = xcd < r ? xcd * (q + 1) + local : r * (q + 1) + (xcd - r) * q + local;
+    const int width = kGroupM * tiles_n, group = pid / width, first = group * kGroupM, size = min(tiles_m - first, kGroupM);
+    tm = first + (pid % width) % size;
+    tn = (pid % width) / size;
+}
+
+template <class C, bool GROUPED, bool SPLIT>
+__global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    constexpr int TM = C::TM, TN = C::TN, NT = C::NT, NS = C::NS, TT = C::TT;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int wm = wave / C::WN, wn = wave % C::WN, l16 = lane & 15, kq = lane >> 4;
+    const int tiles_n = (g.N + C::BN - 1) / C::BN;
+
+    // ---- the block's rows [row0, row_end) and channels from n0
+    int tm, tn, row0, row_end, expert = 0;
+    if (!GROUPED) {
+        const int tiles_m = (g.M + C::BM - 1) / C::BM;
+        tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
+        row0 = tm * C::BM, row_end = g.M;
+    } else {
+        // the experts' tiles of rows, counted by every wavefront for itself: 64 experts at a time
+        int total = 0;
+        for (int e0 = 0; e0 < g.experts; e0 += kWave) {
+            int first = 0, last = 0;
+            if (e0 + lane < g.experts) expert_rows(g, e0 + lane, first, last);
+            total += __shfl(wave_prefix((last - first + C::BM - 1) / C::BM), kWave - 1);
+        }
+        total = __builtin_amdgcn_readfirstlane(total);
+        const int64_t nblk = min((int64_t)gridDim.x, (int64_t)total * tiles_n);
+        if (blockIdx.x >= nblk) return;  // block-uniform
+        tile_of(blockIdx.x, (int)nblk, total, tiles_n, tm, tn);
+        int before = 0;
+        row0 = row_end = 0;
+        for (int e0 = 0; e0 < g.experts; e0 += kWave) {
+            int first = 0, last = 0;
+            if (e0 + lane < g.experts) expert_rows(g, e0 + lane, first, last);
+            const int mine = (last - first + C::BM - 1) / C::BM, upto = before + wave_prefix(mine);
+            const uint64_t has = __ballot(tm >= upto - mine && tm < upto);
+            if (has) {
+                const int at = __ffsll((unsigned long long)has) - 1;
+                expert = e0 + at;
+                row0 = __shfl(first, at) + (tm - __shfl(upto - mine, at)) * C::BM;
+                row_end = __shfl(last, at);
+                break;
+            }
+            before = __shfl(upto, kWave - 1);
+        }
+        expert = __builtin_amdgcn_readfirstlane(expert);
+        row0 = __builtin_amdgcn_readfirstlane(row0);
+        row_end = __builtin_amdgcn_readfirstlane(row_end);
+        if (row0 >= row_end) return;  // block-uniform
+    }
+    const int n0 = tn * C::BN;
+    const int kb0 = SPLIT ? blockIdx.y * g.blocks_per_split : 0, kb1 = SPLIT ? min(g.KB, kb0 + g.blocks_per_split) : g.KB;
+    const int kfull = min(kb1, g.K / kScaleBlock) - kb0;  // whole blocks of this split; a ragged last one comes after them
+    const uint8_t* B = g.B + (int64_t)expert * g.N * g.ldb;
+    const float* sw = g.sw + (int64_t)expert * g.NB * g.KB;
+
+    // ---- global -> LDS.  A thread's pieces are row tid / 8 + i NT / 8 of the tile, LDS slot tid % 8, which holds the row's chunk
+    // slot ^ swizzle.  Rows past the end are the last row again.
+    const int ld_row = tid / 8, ld_chunk = (tid % 8) ^ ((ld_row >> 1) & 7);
+    uint32_t off[C::A_LOADS + C::B_LOADS];
+#pragma unroll
+    for (int i = 0; i < C::A_LOADS; i++) off[i] = (uint32_t)min(ld_row + i * (NT / 8), row_end - 1 - row0) * (uint32_t)g.lda + ld_chunk * 16;
+#pragma unroll
+    for (int i = 0; i < C::B_LOADS; i++) off[C::A_LOADS + i] = (uint32_t)min(ld_row + i * (NT / 8), g.N - 1 - n0) * (uint32_t)g.ldb + ld_chunk * 16;
+    const uint8_t* a_base = g.A + (int64_t)row0 * g.lda;
+    const uint8_t* b_base = B + (int64_t)n0 * g.ldb;
+    // scale slot tid: tokens in the order in which a lane reads them (its TM tokens together), then the blocks of channels
+    const float* s_ptr;
+    if (tid < C::BM) {
+        const int w = tid / C::WTM, r = tid % C::WTM, token = w * C::WTM + (r % TM) * 16 + r / TM;
+        s_ptr = g.sa + (int64_t)min(row0 + token, row_end - 1) * g.KB;
+    } else {
+        s_ptr = sw + (int64_t)min(n0 / kScaleBlock + min(tid - C::BM, (C::BN - 1) / kScaleBlock), g.NB - 1) * g.KB;
+    }
+    const uint32_t lds_base = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) void*)smem);
+    int ld_kb = kb0;
+    auto issue = [&](int stage, auto d_c) __attribute__((always_inline)) {  // piece d of block ld_kb
+        constexpr int d = decltype(d_c)::value;
+        const uint32_t to = lds_base + (uint32_t)stage * C::STAGE;
+        if constexpr (d < C::A_LOADS + C::B_LOADS) {
+            const uint8_t* base = (d < C::A_LOADS ? a_base : b_base) + (int64_t)ld_kb * kScaleBlock;
+            const uint32_t m0v = to + (uint32_t)d * (NT * 16) + (uint32_t)wave * 1024;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(off[d]), "s"(base) : "memory", "m0");
+        } else {
+            const float* p = s_ptr + ld_kb;
+            const uint32_t m0v = to + C::DATA + (uint32_t)wave * 256;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(m0v), "v"(p) : "memory", "m0");
+        }
+    };
+    auto lds_barrier = []() __attribute__((always_inline)) {  // orders LDS traffic only: loads stay in flight across it
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    };
+
+    // ---- LDS -> operands
+    const int a_row = wm * C::WTM + l16, b_row = C::BM + wn * C::WTN + l16;
+    auto fragment = [&](const uint8_t* st, int row) __attribute__((always_inline)) {
+        const uint4 lo = *reinterpret_cast<const uint4*>(st + chunk_at(row, 2 * kq)), hi = *reinterpret_cast<const uint4*>(st + chunk_at(row, 2 * kq + 1));
+        return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+    };
+    v8i a[2], b[TN];
+    v4f acc[TM][TN], p[4];
+    float s[TM], s_next[TM], w_next, s_last = 0.f;
+    auto read_scales = [&](const uint8_t* st) __attribute__((always_inline)) {
+        const float* f = reinterpret_cast<const float*>(st + C::DATA);
+#pragma unroll
+        for (int i = 0; i < TM; i++) s_next[i] = f[wm * C::WTM + l16 * TM + i];
+        w_next = f[C::BM + wn * C::WTN / kScaleBlock];
+    };
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = v4f{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = v4f{0, 0, 0, 0};
+    auto scale_in = [&](auto t_c, float f) __attribute__((always_inline)) {
+        constexpr int t = decltype(t_c)::value, i = t / TN, j = t % TN;
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(p[t & 3][e], f, acc[i][j][e]);
+    };
+    auto wait_loads = [](int younger) __attribute__((always_inline)) {  // until at most `younger` later stages are in flight
+        if (NS > 3 && younger >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NS > 3 ? 2 * C::LPT : 0) : "memory");
+        else if (NS > 2 && younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NS > 2 ? C::LPT : 0) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
+
+    // One block of K.  A product's results are scaled in two MFMAs later, so that the matrix cores never wait for the vector unit; the operands of
+    // the next row of tiles are read under the MFMAs of this one, and those of the next block under the last row, behind the barrier that
+    // publishes its stage and frees this one.
+    auto k_block = [&](const uint8_t* st, const uint8_t* next, int to, int younger, auto load_c, auto next_c) __attribute__((always_inline)) {
+        constexpr bool LOAD = decltype(load_c)::value, NEXT = decltype(next_c)::value;
+        constexpr int PER = (C::LPT + TT - TN - 1) / (TT - TN);  // loads requested behind an MFMA
+        s_last = s[TM - 1];
+#pragma unroll
+        for (int i = 0; i < TM; i++) s[i] = s_next[i] * w_next;
+        unrolled<0, TT>([&](auto t_c) __attribute__((always_inline)) {
+            constexpr int t = decltype(t_c)::value, i = t / TN, j = t % TN;
+            if constexpr (NEXT && i == TM - 1 && j == 0) {
+                wait_loads(younger);
+                lds_barrier();
+            }
+            p[t & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i & 1], v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+            if constexpr (j == 0 && i + 1 < TM) a[(i + 1) & 1] = fragment(st, a_row + (i + 1) * 16);
+            if constexpr (NEXT && i == TM - 1) {
+                b[j] = fragment(next, b_row + j * 16);
+                if constexpr (j == 0) a[0] = fragment(next, a_row), read_scales(next);
+            }
+            if constexpr (t >= 2) scale_in(std::integral_constant<int, t - 2>{}, s[(t - 2) / TN]);
+            else scale_in(std::integral_constant<int, TT - 2 + t>{}, s_last);
+            if constexpr (LOAD)  // all before the last row, whose wait counts them
+                unrolled<(t * PER < C::LPT ? t * PER : C::LPT), ((t + 1) * PER < C::LPT ? (t + 1) * PER : C::LPT)>(
+                    [&](auto d) __attribute__((always_inline)) { issue(to, d); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    auto first_operands = [&](const uint8_t* st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < TN; j++) b[j] = fragment(st, b_row + j * 16);
+        a[0] = fragment(st, a_row);
+        read_scales(st);
+    };
+#pragma unroll
+    for (int i = 0; i < TM; i++) s[i] = 0.f;
+
+    unrolled<0, NS - 1>([&](auto n_c) __attribute__((always_inline)) {
+        constexpr int n = decltype(n_c)::value;
+        if (n < kfull) {
+            unrolled<0, C::LPT>([&](auto d) __attribute__((always_inline)) { issue(n, d); });
+            ld_kb++;
+        }
+    });
+    if (kfull > 0) {
+        wait_loads(min(kfull, NS - 1) - 1);
+        lds_barrier();
+        first_operands(smem);
+    }
+    int stage = 0, kt = 0;
+    auto step = [&](auto load_c, auto next_c, int younger) __attribute__((always_inline)) {
+        const int next = stage == NS - 1 ? 0 : stage + 1, prev = stage == 0 ? NS - 1 : stage - 1;
+        k_block(smem + stage * C::STAGE, smem + next * C::STAGE, prev, younger, load_c, next_c);
+        if (decltype(load_c)::value) ld_kb++;
+        stage = next, kt++;
+    };
+#pragma unroll 1
+    while (kt + NS - 1 < kfull) step(std::true_type{}, std::true_type{}, NS - 2);
+#pragma unroll 1
+    while (kt + 1 < kfull) step(std::false_type{}, std::true_type{}, kfull - 2 - kt);
+    if (kt < kfull) step(std::false_type{}, std::false_type{}, 0);
+    if (kb0 + kfull < kb1) {  // block-uniform: the ragged block, whose missing chunks are zeros, through registers
+        lds_barrier();
+        const int left = g.K - (kb0 + kfull) * kScaleBlock;
+        const int64_t at = (int64_t)(kb0 + kfull) * kScaleBlock;
+#pragma unroll
+        for (int i = 0; i < C::A_LOADS + C::B_LOADS; i++) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (ld_chunk * 16 < left) v = *reinterpret_cast<const uint4*>((i < C::A_LOADS ? a_base : b_base) + at + off[i]);
+            *reinterpret_cast<uint4*>(smem + i * (NT * 16) + tid * 16) = v;
+        }
+        *reinterpret_cast<float*>(smem + C::DATA + tid * 4) = s_ptr[kb0 + kfull];
+        lds_barrier();
+        first_operands(smem);
+        k_block(smem, smem, 0, 0, std::false_type{}, std::false_type{});
+    }
+    scale_in(std::integral_constant<int, TT - 2>{}, s[TM - 1]);
+    scale_in(std::integral_constant<int, TT - 1>{}, s[TM - 1]);
+
+    // ---- a lane holds token l16 of each tile of tokens and channels 4 kq .. + 3 of each tile of channels
+    if constexpr (SPLIT) {
+        float* part = g.partials + (int64_t)blockIdx.y * g.M * g.N;
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            const int m = row0 + wm * C::WTM + i * 16 + l16;
+            if (m >= row_end) continue;
+#pragma unroll
+            for (int j = 0; j < TN; j++) {
+                const int n = n0 + wn * C::WTN + j * 16 + kq * 4;
+                float* to = part + (int64_t)m * g.N + n;
+                if ((g.N & 3) == 0 && n < g.N) *reinterpret_cast<v4f*>(to) = acc[i][j];
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (n + e < g.N) to[e] = acc[i][j][e];
+            }
+        }
+    } else {
+        const bool bf16 = g.out_dtype == LLMQ_BF16;
+        const bool wide = (g.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 7u) == 0;
+#pragma unroll
+        for (int j = 0; j < TN; j++) {
+            const int n = n0 + wn * C::WTN + j * 16 + kq * 4;
+            float bb[4] = {0, 0, 0, 0};
+            if (g.bias) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) bb[e] = load_as_f32(g.bias, g.bias_dtype, (int64_t)expert * g.N + min(n + e, g.N - 1));
+            }
+#pragma unroll
+            for (int i = 0; i < TM; i++) {
+                const int m = row0 + wm * C::WTM + i * 16 + l16;
+                if (m >= row_end || n >= g.N) continue;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = acc[i][j][e] + bb[e];
+                const uint2 h = bf16 ? make_uint2(Lo<LLMQ_BF16>::pack2(v[0], v[1]), Lo<LLMQ_BF16>::pack2(v[2], v[3]))
+                                     : make_uint2(Lo<LLMQ_F16>::pack2(v[0], v[1]), Lo<LLMQ_F16>::pack2(v[2], v[3]));
+                uint16_t* to = reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n;
+                if (wide && n + 3 < g.N) *reinterpret_cast<uint2*>(to) = h;
+                else {
+                    const uint32_t w[2] = {h.x, h.y};
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (n + e < g.N) to[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+                }
+            }
+        }
+    }
+}
+
+// the splits' sums in order, bias, rounding; 4 channels per thread
+__global__ __launch_bounds__(256) void block_reduce_kernel(BlockArgs g, int splits) {
+    const int64_t per_row = (g.N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= per_row * g.M) return;
+    const int m = (int)(i / per_row), n = (int)(i - (int64_t)m * per_row) * 4;
+    const int64_t plane = (int64_t)g.M * g.N;
+    const float* p = g.partials + (int64_t)m * g.N + n;
+    uint16_t* to = reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n;
+    float v[4] = {0, 0, 0, 0};
+    if ((g.N & 3) == 0) {
+        for (int k = 0; k < splits; k++) {
+            const v4f q = *reinterpret_cast<const v4f*>(p + k * plane);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] += q[e];
+        }
+    } else {
+        for (int k = 0; k < splits; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (n + e < g.N) v[e] += p[k * plane + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (n + e >= g.N) continue;
+        const float f = v[e] + (g.bias ? load_as_f32(g.bias, g.bias_dtype, n + e) : 0.f);
+        to[e] = g.out_dtype == LLMQ_BF16 ? Lo<LLMQ_BF16>::from_f32(f) : Lo<LLMQ_F16>::from_f32(f);
+    }
+}
+
+template <class C, bool GROUPED, bool SPLIT>
+int launch_tile(const BlockArgs& g, int splits, hipStream_t st) {
+    auto kernel = block_tile_kernel<C, GROUPED, SPLIT>;
+    if (C::LDS_BYTES > 64 * 1024) {
+        static bool raised[64] = {};  // per device: the attribute belongs to the loaded code object of the current device
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess) return LLMQ_ERR_LAUNCH;
+        if (dev < 0 || dev >= 64 || !raised[dev]) {
+            if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES) != hipSuccess)
+                return LLMQ_ERR_LAUNCH;
+            if (dev >= 0 && dev < 64) raised[dev] = true;
+        }
+    }
+    const int64_t tiles_n = (g.N + C::BN - 1) / C::BN;
+    // by experts: each may end with a tile that is not full
+    const int64_t tiles_m = GROUPED ? g.M / C::BM + (g.experts < g.M ? g.experts : g.M) : (g.M + C::BM - 1) / C::BM;
+    if (tiles_m * tiles_n * C::NT > 0xffffffffLL) return LLMQ_ERR_SHAPE;  // threads of a grid
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * tiles_n), SPLIT ? splits : 1), dim3(C::NT), C::LDS_BYTES, st, g);
+    if (launch_status() != LLMQ_OK) return LLMQ_ERR_LAUNCH;
+    if (SPLIT) {
+        const int64_t n = (int64_t)((g.N + 3) / 4) * g.M;
+        if (n > 0xffffff00LL) return LLMQ_ERR_SHAPE;
+        hipLaunchKernelGGL(block_reduce_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g, splits);
+        return launch_status();
+    }
+    return LLMQ_OK;
+}
+
+template <class C>
+int launch_cfg(const BlockArgs& g, int splits, hipStream_t st) {
+    if (g.offsets) return launch_tile<C, true, false>(g, 1, st);
+    return splits > 1 ? launch_tile<C, false, true>(g, splits, st) : launch_tile<C, false, false>(g, 1, st);
+}
+
+}  // namespace
+
+int launch_block_tile(int cfg, int splits, const BlockArgs& g, hipStream_t st) {
+    switch (cfg) {
+        case 0: return launch_cfg<TileCfg<256, 256, 2, 4>>(g, splits, st);
+        case 1: return launch_cfg<TileCfg<128, 256, 2, 4>>(g, splits, st);
+        case 2: return launch_cfg<TileCfg<128, 128, 2, 2>>(g, splits, st);
+        case 3: return launch_cfg<TileCfg<64, 128, 2, 2>>(g, splits, st);
+        case 4: return launch_cfg<TileCfg<32, 128, 1, 4>>(g, splits, st);
+    }
+    return LLMQ_ERR_SHAPE;
+}
+
+}  // namespace llmq

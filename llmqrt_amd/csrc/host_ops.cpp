@@ -429,6 +429,127 @@ std::optional<std::pair<Tensor, Tensor>> rmsnorm_quant(const Tensor& x, const Te
     return std::make_pair(q, s);
 }
 
+// ---- block-scaled fp8 --------------------------------------------------------------------------------------------
+int64_t blocks128(int64_t n) { return (n + 127) / 128; }
+using Pair = std::pair<Tensor, Tensor>;
+
+std::optional<Pair> quant_groups(const Tensor& x) {
+    const Rows r = rows_of(x);
+    if (!r.ok || !is16(x.scalar_type()) || r.K % 8) return std::nullopt;
+    const Launch l(x.device());
+    Tensor q = make(x.sizes(), at::kFloat8_e4m3fn, x.device()), s = make(out_size(x, blocks128(r.K)), at::kFloat, x.device());
+    check(llmq_quant_fp8_per_group(x.data_ptr(), code(x.scalar_type()), r.M, r.K, r.K, (uint8_t*)q.data_ptr(), (float*)s.data_ptr(), l.stream),
+          "llmq_quant_fp8_per_group");
+    return std::make_pair(q, s);
+}
+
+// out: LLMQ_NORM_*.  Results in order: [codes, scales] (8-bit forms), [y] (same, or normed), [h] (with a residual).
+struct NormOut {
+    Tensor t[4];
+    int n = 0;
+    bool ok = false;
+};
+NormOut add_norm(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& w, double eps, int out, bool normed, bool inplace) {
+    NormOut o;
+    const Rows r = rows_of(x);
+    if (out < LLMQ_NORM_SAME || out > LLMQ_NORM_FP8_GROUP || !norm_ok(x, w, r) || (inplace && !residual)) return o;
+    if (residual && (residual->scalar_type() != x.scalar_type() || residual->sizes() != x.sizes() || !plain_on(*residual, x.device()) || !aligned(*residual)))
+        return o;
+    const Launch l(x.device());
+    Tensor q, s, y, h;
+    if (out != LLMQ_NORM_SAME) {
+        q = make(x.sizes(), out == LLMQ_NORM_I8_TOKEN ? at::kChar : at::kFloat8_e4m3fn, x.device());
+        s = make(out_size(x, out == LLMQ_NORM_FP8_GROUP ? blocks128(r.K) : 1), at::kFloat, x.device());
+        o.t[o.n++] = q, o.t[o.n++] = s;
+    }
+    if (out == LLMQ_NORM_SAME || normed) o.t[o.n++] = y = make(x.sizes(), x.scalar_type(), x.device());
+    if (residual) o.t[o.n++] = h = inplace ? *residual : make(x.sizes(), x.scalar_type(), x.device());
+    check(llmq_add_rmsnorm(out, x.data_ptr(), code(x.scalar_type()), r.M, r.K, r.K, ptr(residual), r.K, residual ? h.data_ptr() : nullptr, r.K,
+                           w.data_ptr(), (float)eps, y.defined() ? y.data_ptr() : nullptr, q.defined() ? q.data_ptr() : nullptr,
+                           s.defined() ? (float*)s.data_ptr() : nullptr, l.stream),
+          "llmq_add_rmsnorm");
+    o.ok = true;
+    return o;
+}
+
+bool block_bias_ok(const std::optional<Tensor>& b, const at::Device& dev, int64_t n) {
+    return !b || (b->numel() == n && plain_on(*b, dev) && (is16(b->scalar_type()) || b->scalar_type() == at::kFloat));
+}
+bool block_weight_ok(const Tensor& w, const Tensor& w_scale, const std::optional<Tensor>& bias, const at::Device& dev, int64_t K) {
+    return weight_ok(w, at::kFloat8_e4m3fn, dev, K) && scale_ok(w_scale, dev, blocks128(w.size(0)) * blocks128(K)) &&
+           block_bias_ok(bias, dev, w.size(0));
+}
+void block_gemm(const void* q, const float* a_scale, const Tensor& w, const Tensor& w_scale, const std::optional<Tensor>& bias, int64_t M, int64_t K,
+                Tensor& out, const Launch& l) {
+    const int64_t N = w.size(0), bytes = (int64_t)llmq_gemm_fp8_block_workspace_bytes(M, N, K);
+    Tensor ws;
+    if (bytes) ws = make({bytes}, at::kByte, out.device());
+    check(llmq_gemm_fp8_block((const uint8_t*)q, K, a_scale, (const uint8_t*)w.data_ptr(), K, (const float*)w_scale.data_ptr(), ptr(bias),
+                              bias ? code(bias->scalar_type()) : LLMQ_BF16, out.data_ptr(), code(out.scalar_type()), N, M, N, K,
+                              bytes ? ws.data_ptr() : nullptr, (size_t)bytes, l.stream),
+          "llmq_gemm_fp8_block");
+}
+std::optional<Tensor> fp8_block(const Tensor& q, const Tensor& a_scale, const Tensor& w, const Tensor& w_scale, const std::optional<Tensor>& bias,
+                                at::ScalarType odt) {
+    const Rows r = rows_of(q);
+    if (!r.ok || !is16(odt) || q.scalar_type() != at::kFloat8_e4m3fn || !block_weight_ok(w, w_scale, bias, q.device(), r.K) ||
+        !scale_ok(a_scale, q.device(), r.M * blocks128(r.K)))
+        return std::nullopt;
+    const Launch l(q.device());
+    Tensor out = make(out_size(q, w.size(0)), odt, q.device());
+    block_gemm(q.data_ptr(), (const float*)a_scale.data_ptr(), w, w_scale, bias, r.M, r.K, out, l);
+    return out;
+}
+// activations not quantized yet; out has their dtype
+std::optional<Tensor> fp8_block_linear(const Tensor& x, const Tensor& w, const Tensor& w_scale, const std::optional<Tensor>& bias) {
+    const Rows r = rows_of(x);
+    if (!r.ok || !is16(x.scalar_type()) || !block_weight_ok(w, w_scale, bias, x.device(), r.K)) return std::nullopt;
+    const Launch l(x.device());
+    const int64_t codes = round16(r.M * r.K);
+    Tensor tmp = make({codes + 4 * r.M * blocks128(r.K)}, at::kByte, x.device());
+    uint8_t* p = (uint8_t*)tmp.data_ptr();
+    float* s = (float*)(p + codes);
+    check(llmq_quant_fp8_per_group(x.data_ptr(), code(x.scalar_type()), r.M, r.K, r.K, p, s, l.stream), "llmq_quant_fp8_per_group");
+    Tensor out = make(out_size(x, w.size(0)), x.scalar_type(), x.device());
+    block_gemm(p, s, w, w_scale, bias, r.M, r.K, out, l);
+    return out;
+}
+
+// rows of x sorted by expert; a_scale absent: x is quantized first.  out: given, or new
+std::optional<Tensor> fp8_block_grouped(const Tensor& x, const std::optional<Tensor>& a_scale, const Tensor& w, const Tensor& w_scale,
+                                        const std::optional<Tensor>& bias, const Tensor& offsets, at::ScalarType odt,
+                                        const std::optional<Tensor>& given) {
+    const Rows r = rows_of(x);
+    const at::Device dev = x.device();
+    if (!r.ok || x.dim() != 2 || !is16(odt) || w.dim() != 3 || w.scalar_type() != at::kFloat8_e4m3fn || w.size(2) != r.K || r.K % 16 || w.numel() == 0 ||
+        !plain_on(w, dev) || !aligned(w))
+        return std::nullopt;
+    const int64_t E = w.size(0), N = w.size(1);
+    if (!scale_ok(w_scale, dev, E * blocks128(N) * blocks128(r.K)) || !block_bias_ok(bias, dev, E * N) || offsets.dim() != 1 ||
+        offsets.numel() != E + 1 || offsets.scalar_type() != at::kInt || !plain_on(offsets, dev) ||
+        (given && (given->scalar_type() != odt || given->dim() != 2 || given->size(0) != r.M || given->size(1) != N || !plain_on(*given, dev))))
+        return std::nullopt;
+    if (a_scale ? (x.scalar_type() != at::kFloat8_e4m3fn || !scale_ok(*a_scale, dev, r.M * blocks128(r.K))) : !is16(x.scalar_type()))
+        return std::nullopt;
+    const Launch l(dev);
+    Tensor tmp;
+    const void* q = x.data_ptr();
+    const float* s = a_scale ? (const float*)a_scale->data_ptr() : nullptr;
+    if (!a_scale) {
+        const int64_t codes = round16(r.M * r.K);
+        tmp = make({codes + 4 * r.M * blocks128(r.K)}, at::kByte, dev);
+        uint8_t* p = (uint8_t*)tmp.data_ptr();
+        check(llmq_quant_fp8_per_group(x.data_ptr(), code(x.scalar_type()), r.M, r.K, r.K, p, (float*)(p + codes), l.stream), "llmq_quant_fp8_per_group");
+        q = p, s = (const float*)(p + codes);
+    }
+    Tensor out = given ? *given : make({r.M, N}, odt, dev);
+    check(llmq_gemm_fp8_block_grouped((const uint8_t*)q, r.K, s, (const uint8_t*)w.data_ptr(), (const float*)w_scale.data_ptr(),
+                                      (const int32_t*)offsets.data_ptr(), E, ptr(bias), bias ? code(bias->scalar_type()) : LLMQ_BF16, out.data_ptr(),
+                                      code(odt), N, r.M, N, r.K, l.stream),
+          "llmq_gemm_fp8_block_grouped");
+    return out;
+}
+
 // ---- Python ----------------------------------------------------------------------------------------------------
 struct NoGil {
     PyThreadState* state = PyEval_SaveThread();
@@ -573,6 +694,69 @@ LLMQ_PY(py_rmsnorm_quant, 4)
     return both;
 LLMQ_PY_END
 
+PyObject* tuple_of(Tensor* t, int n) {
+    PyObject* all = PyTuple_New(n);
+    for (int i = 0; all && i < n; i++) {
+        PyObject* o = THPVariable_Wrap(std::move(t[i]));
+        if (o) PyTuple_SET_ITEM(all, i, o);
+        else Py_CLEAR(all);
+    }
+    return all;
+}
+
+LLMQ_PY(py_quant_groups, 1)
+    const Tensor& x = in.tensor(0);
+    LLMQ_PY_TENSORS;
+    std::optional<Pair> y;
+    { NoGil g; y = quant_groups(x); }
+    if (!y) Py_RETURN_NONE;
+    Tensor t[2] = {std::move(y->first), std::move(y->second)};
+    return tuple_of(t, 2);
+LLMQ_PY_END
+
+LLMQ_PY(py_add_norm, 7)
+    const Tensor &x = in.tensor(0), &w = in.tensor(2);
+    const auto residual = in.optional(1);
+    LLMQ_PY_TENSORS;
+    const double eps = PyFloat_AsDouble(argv[3]);
+    const long out = PyLong_AsLong(argv[4]);
+    const int normed = PyObject_IsTrue(argv[5]), inplace = PyObject_IsTrue(argv[6]);
+    if (PyErr_Occurred()) return nullptr;
+    NormOut y;
+    { NoGil g; y = add_norm(x, residual, w, eps, (int)out, normed != 0, inplace != 0); }
+    if (!y.ok) Py_RETURN_NONE;
+    return tuple_of(y.t, y.n);
+LLMQ_PY_END
+
+LLMQ_PY(py_fp8_block, 6)
+    const Tensor &q = in.tensor(0), &a = in.tensor(1), &w = in.tensor(2), &s = in.tensor(3);
+    const auto bias = in.optional(4);
+    const at::ScalarType odt = in.dtype(5);
+    LLMQ_PY_TENSORS;
+    std::optional<Tensor> y;
+    { NoGil g; y = fp8_block(q, a, w, s, bias, odt); }
+    return wrap(std::move(y));
+LLMQ_PY_END
+
+LLMQ_PY(py_fp8_block_linear, 4)
+    const Tensor &x = in.tensor(0), &w = in.tensor(1), &s = in.tensor(2);
+    const auto bias = in.optional(3);
+    LLMQ_PY_TENSORS;
+    std::optional<Tensor> y;
+    { NoGil g; y = fp8_block_linear(x, w, s, bias); }
+    return wrap(std::move(y));
+LLMQ_PY_END
+
+LLMQ_PY(py_fp8_block_grouped, 8)
+    const Tensor &x = in.tensor(0), &w = in.tensor(2), &s = in.tensor(3), &offsets = in.tensor(5);
+    const auto a = in.optional(1), bias = in.optional(4), out = in.optional(7);
+    const at::ScalarType odt = in.dtype(6);
+    LLMQ_PY_TENSORS;
+    std::optional<Tensor> y;
+    { NoGil g; y = fp8_block_grouped(x, a, w, s, bias, offsets, odt, out); }
+    return wrap(std::move(y));
+LLMQ_PY_END
+
 // the counters of the current stream of a tensor's device
 LLMQ_PY(py_awq_counters, 1)
     const Tensor& x = in.tensor(0);
@@ -607,6 +791,11 @@ PyMethodDef methods[] = {LLMQ_FAST("sq_tensor", py_sq_tensor),
                          LLMQ_FAST("awq", py_awq),
                          LLMQ_FAST("rmsnorm", py_rmsnorm),
                          LLMQ_FAST("rmsnorm_quant", py_rmsnorm_quant),
+                         LLMQ_FAST("quant_groups", py_quant_groups),
+                         LLMQ_FAST("add_norm", py_add_norm),
+                         LLMQ_FAST("fp8_block", py_fp8_block),
+                         LLMQ_FAST("fp8_block_linear", py_fp8_block_linear),
+                         LLMQ_FAST("fp8_block_grouped", py_fp8_block_grouped),
                          LLMQ_FAST("awq_counters", py_awq_counters),
                          {"release_tickets", py_release_counters, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

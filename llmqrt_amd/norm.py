@@ -75,6 +75,95 @@ def rmsnorm_per_token_quantize(x, weight, eps: float = 1e-6, return_normed: bool
     return _fused(x, weight, eps, True, torch.float32, return_normed, _inv_dump)
 
 
+# outputs of llmq_add_rmsnorm
+_SAME, _I8_TOKEN, _FP8_TOKEN, _FP8_GROUP = range(4)
+
+
+def _same_rows(t: torch.Tensor, x: torch.Tensor, what: str) -> torch.Tensor:
+    if t.dtype != x.dtype or t.device != x.device or t.shape != x.shape:
+        raise RuntimeError(f"{what} must have the shape, dtype and device of the activations")
+    return _as_rows(t)
+
+
+@torch.no_grad()
+def _add_norm(x, residual, weight, eps, out, return_normed=False, inplace=False):
+    y = host().add_norm(x, residual, weight, eps, out, return_normed, inplace)
+    if y is not None:
+        return y
+    if inplace and residual is None:
+        raise RuntimeError("inplace needs a residual")
+    rows = _as_rows(x)
+    w = _check_weight(rows, weight)
+    M, K = rows.shape
+    dev = rows.device
+    res = h = None
+    if residual is not None:
+        res = _same_rows(residual, x, "the residual")
+        if not inplace:
+            h = torch.empty((M, K), dtype=rows.dtype, device=dev)
+        elif res.data_ptr() != residual.data_ptr():
+            raise RuntimeError("a residual that is updated in place needs rows of one stride that is a multiple of 16 bytes, 16-byte aligned")
+        else:
+            h = res
+    groups = (K + 127) // 128
+    q = scale = y = None
+    if out != _SAME:
+        q = torch.empty((M, K), dtype=torch.int8 if out == _I8_TOKEN else torch.float8_e4m3fn, device=dev)
+        scale = torch.empty((M, groups if out == _FP8_GROUP else 1), dtype=torch.float32, device=dev)
+    if out == _SAME or return_normed:
+        y = torch.empty((M, K), dtype=rows.dtype, device=dev)
+    if M:
+        with torch.cuda.device(dev):
+            _abi.check(_abi.lib().llmq_add_rmsnorm(
+                out, rows.data_ptr(), _abi.dtype_code(rows.dtype), M, K, rows.stride(0) if M > 1 else K, _abi.ptr(res),
+                res.stride(0) if res is not None and M > 1 else K, _abi.ptr(h), h.stride(0) if h is not None and M > 1 else K, w.data_ptr(), float(eps),
+                _abi.ptr(y), _abi.ptr(q), _abi.ptr(scale), _abi.stream_of(rows)), "llmq_add_rmsnorm")
+    result = [] if q is None else [q.view(x.shape), scale.view(*x.shape[:-1], scale.shape[-1])]
+    if y is not None:
+        result.append(y.view(x.shape))
+    if h is not None:
+        result.append(residual if inplace else h.view(x.shape))
+    return tuple(result)
+
+
+def add_rmsnorm(x, residual, weight, eps: float = 1e-6, inplace: bool = False):
+    """The residual's addition and RMSNorm in one pass: h = (x + residual).to(x.dtype), y = (h * rsqrt(mean(h^2) + eps) * weight) in fp32,
+    rounded once to x.dtype.  -> (y, h).  ``inplace`` writes h over the residual (and returns it)."""
+    if residual is None:
+        raise RuntimeError("add_rmsnorm needs a residual (rmsnorm is the form without)")
+    return _add_norm(x, residual, weight, eps, _SAME, inplace=inplace)
+
+
+def add_rmsnorm_quantize_activation_per_token_absmax(x, residual, weight, eps: float = 1e-6, return_normed: bool = False, inplace: bool = False):
+    """add_rmsnorm with y quantized to int8 per token: -> (int8 like x, fp32 scales [.., 1][, y], h).  scale = max(absmax, 1e-5) / 127.
+
+    y is quantized as it is in fp32.  (The pair without a residual, rmsnorm_quantize_activation_per_token_absmax, rounds the normalised
+    row, y, scale and quotients to x.dtype, as its reference does.)"""
+    if residual is None:
+        raise RuntimeError("add_rmsnorm_quantize_activation_per_token_absmax needs a residual")
+    return _add_norm(x, residual, weight, eps, _I8_TOKEN, return_normed, inplace)
+
+
+def add_rmsnorm_per_token_quantize(x, residual, weight, eps: float = 1e-6, return_normed: bool = False, inplace: bool = False):
+    """add_rmsnorm with y quantized to e4m3fn per token: -> (codes, fp32 scales [.., 1][, y], h).  scale = max(absmax, 1e-12) / 448."""
+    if residual is None:
+        raise RuntimeError("add_rmsnorm_per_token_quantize needs a residual")
+    return _add_norm(x, residual, weight, eps, _FP8_TOKEN, return_normed, inplace)
+
+
+def add_rmsnorm_per_group_quantize(x, residual, weight, eps: float = 1e-6, return_normed: bool = False, inplace: bool = False):
+    """add_rmsnorm with y quantized to e4m3fn per token and 128 channels, for a block-scaled Linear: -> (codes, fp32 scales
+    [.., ceil(K / 128)][, y], h)."""
+    if residual is None:
+        raise RuntimeError("add_rmsnorm_per_group_quantize needs a residual (rmsnorm_per_group_quantize is the form without)")
+    return _add_norm(x, residual, weight, eps, _FP8_GROUP, return_normed, inplace)
+
+
+def rmsnorm_per_group_quantize(x, weight, eps: float = 1e-6, return_normed: bool = False):
+    """RMSNorm with an output in e4m3fn per token and 128 channels, without a residual: -> (codes, fp32 scales [.., ceil(K / 128)][, y])."""
+    return _add_norm(x, None, weight, eps, _FP8_GROUP, return_normed)
+
+
 class RMSNorm(nn.Module):
     """Drop-in for the reference RMSNorm: same constructor (a ready weight tensor, eps) and forward."""
 

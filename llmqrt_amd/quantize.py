@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _abi
+from ._native import host
 
 
 def _as_rows(t: torch.Tensor) -> torch.Tensor:
@@ -141,6 +142,45 @@ def static_per_tensor_quantize(tensor: torch.Tensor, scale) -> torch.Tensor:
         x.data_ptr(), _abi.dtype_code(x.dtype), M, K, x.stride(0) if M > 1 else K, q.data_ptr(),
         sdev.data_ptr(), int(promote), _abi.stream_of(x)), "llmq_quant_fp8_static")
     return q.view(*tensor.shape)
+
+
+@torch.no_grad()
+def per_group_quantize(tensor: torch.Tensor):
+    """One scale per token and 128 channels (the last group of a row may be short), the activations of a block-scaled product:
+    scale = max(absmax, 1e-12) / 448 and codes = e4m3fn(tensor / scale), in fp32.
+    -> (float8_e4m3fn tensor like `tensor`, fp32 scales [.., ceil(K / 128)]).  No counterpart in the reference."""
+    out = host().quant_groups(tensor)
+    if out is not None:
+        return out
+    if tensor.dim() < 1:
+        raise RuntimeError("per_group_quantize needs a tensor with a last dimension")
+    groups = (tensor.shape[-1] + 127) // 128
+    if tensor.numel() == 0:
+        return (torch.empty(tensor.shape, dtype=torch.float8_e4m3fn, device=tensor.device),
+                torch.empty((*tensor.shape[:-1], groups), dtype=torch.float32, device=tensor.device))
+    x = _as_rows(tensor)
+    M, K = x.shape
+    q = torch.empty((M, K), dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty((M, groups), dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        _abi.check(_abi.lib().llmq_quant_fp8_per_group(
+            x.data_ptr(), _abi.dtype_code(x.dtype), M, K, x.stride(0) if M > 1 else K, q.data_ptr(), scale.data_ptr(),
+            _abi.stream_of(x)), "llmq_quant_fp8_per_group")
+    return q.view(tensor.shape), scale.view(*tensor.shape[:-1], groups)
+
+
+def quantize_weight_per_block(w: torch.Tensor):
+    """Weights of a block-scaled product, an offline step in plain torch: w [.., N, K] -> (float8_e4m3fn [.., N, K], fp32 scales
+    [.., ceil(N / 128), ceil(K / 128)]) with scale = max(absmax of the 128 x 128 block, 1e-12) / 448."""
+    if w.dim() < 2 or not w.is_floating_point():
+        raise RuntimeError("quantize_weight_per_block needs a floating-point weight [.., N, K]")
+    n, k = w.shape[-2:]
+    nb, kb = (n + 127) // 128, (k + 127) // 128
+    full = torch.nn.functional.pad(w.detach().float(), (0, kb * 128 - k, 0, nb * 128 - n))
+    blocks = full.view(*w.shape[:-2], nb, 128, kb, 128)
+    scale = blocks.abs().amax(dim=(-3, -1)).clamp_min(1e-12) / 448.0
+    q = (blocks / scale[..., :, None, :, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+    return q.view(*w.shape[:-2], nb * 128, kb * 128)[..., :n, :k].contiguous(), scale
 
 
 def _alpha_operands(t: torch.Tensor, w_scale: torch.Tensor):

@@ -14,6 +14,7 @@ from typing import Optional
 import torch
 
 from . import _abi
+from ._native import host
 
 _FP8_FORMATS = {torch.float8_e4m3fn: _abi.E4M3, torch.float8_e5m2: _abi.E5M2}
 _STR_TO_DTYPE = {"bfloat16": torch.bfloat16, "float16": torch.float16}
@@ -190,6 +191,92 @@ def cutlass_f8f8bf16_rowwise_sm89(XQ: torch.Tensor, WQ: torch.Tensor, bias: Opti
     _check(N <= 1 or w_scale.stride(1) == 1, f"{what}: w_scale must be contiguous")
     _check_bias(bias, WQ, N, (torch.bfloat16, torch.float32), what)
     return _run(True, XQ, WQ, x_scale, w_scale, 1.0, None, bias, 1.0, torch.bfloat16, _acc_dump)
+
+
+# ---- block-scaled fp8 (no counterpart among the reference's ops) ------------------------------------------------
+
+def _blocks(n: int) -> int:
+    return (n + 127) // 128
+
+
+def _block_scale(t, shape, dev, what: str, name: str) -> torch.Tensor:
+    _check(isinstance(t, torch.Tensor) and t.device == dev and t.dtype == torch.float32, f"{what}: {name} must be an fp32 tensor on the GPU of the input")
+    _check(tuple(t.shape) == shape, f"{what}: {name} must be {list(shape)}, got {list(t.shape)}")
+    return t.detach().contiguous()
+
+
+def _block_out_dtype(dtype_str, what: str) -> torch.dtype:
+    _check(dtype_str in _STR_TO_DTYPE, f"{what}: currently only support bf16 or fp16 output dtype, the passed dtype is {dtype_str}")
+    return _STR_TO_DTYPE[dtype_str]
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """Rows of a contiguous 16-byte aligned tensor, copied only if they are not."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+@torch.no_grad()
+def f8f8_blockwise(XQ: torch.Tensor, WQ: torch.Tensor, bias: Optional[torch.Tensor], x_scale: torch.Tensor, w_scale: torch.Tensor,
+                   dtype_str: str = "bfloat16") -> torch.Tensor:
+    """out[m, n] = dtype( sum_b x_scale[m, b] * w_scale[n // 128, b] * sum_{k in block b of 128} XQ[m, k] * WQ[k, n] + bias[n] ), fp32 sums.
+
+    ``XQ``: e4m3fn [M, K] with fp32 scales [M, ceil(K / 128)] (quantize.per_group_quantize); ``WQ``: the .t() view of an e4m3fn
+    [N, K] row-major tensor with fp32 scales [ceil(N / 128), ceil(K / 128)] (quantize.quantize_weight_per_block); ``bias``: [N] bf16, fp16 or
+    fp32; ``dtype_str``: "bfloat16" or "float16".  Sums are taken in a fixed order that follows from the sizes."""
+    what = "f8f8_blockwise"
+    out_dtype = _block_out_dtype(dtype_str, what)
+    if XQ.dim() == 2 and WQ.dim() == 2 and x_scale.shape == (XQ.shape[0], _blocks(XQ.shape[1])) and w_scale.shape == (_blocks(WQ.shape[1]), _blocks(WQ.shape[0])):
+        y = host().fp8_block(XQ, x_scale, WQ.t(), w_scale, bias, out_dtype)
+        if y is not None:
+            return y
+    _check(XQ.dtype == torch.float8_e4m3fn and WQ.dtype == torch.float8_e4m3fn, f"{what}: XQ and WQ must be float8_e4m3fn")
+    M, N, K = _check_operands(XQ, WQ, what)
+    _check_bias(bias, WQ, N, (torch.bfloat16, torch.float16, torch.float32), what)
+    xs = _block_scale(x_scale, (M, _blocks(K)), XQ.device, what, "x_scale")
+    ws = _block_scale(w_scale, (_blocks(N), _blocks(K)), XQ.device, what, "w_scale")
+    if M == 0 or N == 0:
+        return torch.empty((M, N), dtype=out_dtype, device=XQ.device)
+    _check(K > 0, f"{what}: K must be positive")
+    y = host().fp8_block(_rows16(XQ), xs, _rows16(WQ.t()), ws, None if bias is None else bias.detach().contiguous(), out_dtype)
+    _check(y is not None, f"{what}: unsupported operands")
+    return y
+
+
+@torch.no_grad()
+def f8f8_blockwise_grouped(XQ: torch.Tensor, WQ: torch.Tensor, bias: Optional[torch.Tensor], x_scale: torch.Tensor, w_scale: torch.Tensor,
+                           offsets: torch.Tensor, dtype_str: str = "bfloat16", out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """f8f8_blockwise by experts: rows offsets[e] .. offsets[e + 1] - 1 of ``XQ`` [M, K] (sorted by expert) with the weights of expert e.
+
+    ``WQ``: e4m3fn [E, N, K] row-major; ``w_scale``: fp32 [E, ceil(N / 128), ceil(K / 128)]; ``bias``: [E, N]; ``offsets``: int32 [E + 1]
+    on the GPU, ascending (values outside [0, M] are taken as the nearest inside).  An expert may have no rows.  Nothing is read back by
+    the host, so a captured call follows the offsets of its replay.  Rows that belong to no expert are not written: they keep what ``out`` [M, N] holds,
+    and are undefined in a new tensor."""
+    what = "f8f8_blockwise_grouped"
+    out_dtype = _block_out_dtype(dtype_str, what)
+    _check(XQ.is_cuda, f"{what}: XQ must be a GPU tensor")
+    _check(XQ.dim() == 2 and WQ.dim() == 3, f"{what}: XQ must be [M, K] and WQ [E, N, K]")
+    (M, K), (E, N) = XQ.shape, WQ.shape[:2]
+    _check(XQ.dtype == torch.float8_e4m3fn and WQ.dtype == torch.float8_e4m3fn, f"{what}: XQ and WQ must be float8_e4m3fn")
+    _check(WQ.shape[2] == K and WQ.device == XQ.device, f"{what}: WQ must be [E, N, K] with the K and device of XQ")
+    _check(K % 16 == 0, f"{what}: K must be a multiple of 16")
+    _check(isinstance(offsets, torch.Tensor) and offsets.dtype == torch.int32 and offsets.device == XQ.device and tuple(offsets.shape) == (E + 1,),
+           f"{what}: offsets must be int32 [E + 1] on the GPU of the input")
+    xs = _block_scale(x_scale, (M, _blocks(K)), XQ.device, what, "x_scale")
+    ws = _block_scale(w_scale, (E, _blocks(N), _blocks(K)), XQ.device, what, "w_scale")
+    if bias is not None:
+        _check(bias.device == XQ.device and tuple(bias.shape) == (E, N) and bias.dtype in (torch.bfloat16, torch.float16, torch.float32),
+               f"{what}: bias must be [E, N] in bf16, fp16 or fp32 on the GPU of the input")
+        bias = bias.detach().contiguous()
+    if out is not None:
+        _check(out.dtype == out_dtype and out.device == XQ.device and tuple(out.shape) == (M, N) and out.is_contiguous(),
+               f"{what}: out must be a contiguous [M, N] tensor of the output dtype on the GPU of the input")
+    if M == 0 or N == 0 or E == 0:
+        return torch.empty((M, N), dtype=out_dtype, device=XQ.device) if out is None else out
+    _check(K > 0, f"{what}: K must be positive")
+    y = host().fp8_block_grouped(_rows16(XQ), xs, _rows16(WQ), ws, bias, offsets.contiguous(), out_dtype, out)
+    _check(y is not None, f"{what}: unsupported operands")
+    return y
 
 
 # ---- one-launch linears for a few tokens (no counterpart among the reference's ops: they fuse the
