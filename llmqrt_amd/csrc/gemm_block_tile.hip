@@ -158,7 +158,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     // ---- LDS -> operands
     const int a_row = wm * C::WTM + l16, b_row = C::BM + wn * C::WTN + l16;
     auto fragment = [&](const uint8_t* st, int row) __attribute__((always_inline)) {
-        const uint4 lo = *reinterpret_cast<const uint4*>(st + chunk_at(row, 2 * kq)), hi = *reinterpret_cast<const uint4*>(st + chunk_at(row, 2 * kq + 1));
+        const uint4 lo = *reinterpret_cast<const uint4*>(st + chunk_at(row, kq)), hi = *reinterpret_cast<const uint4*>(st + chunk_at(row, kq + 4));
         return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
     };
     v8i a[2], b[TN];
@@ -187,32 +187,37 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
 
-    // One block of K.  A product's results are scaled in two MFMAs later, so that the matrix cores never wait for the vector unit; the operands of
+    // One block of K, kt.  A product's results are scaled in two MFMAs later, so that the matrix cores never wait for the vector unit; the operands of
     // the next row of tiles are read under the MFMAs of this one, and those of the next block under the last row, behind the barrier that
-    // publishes its stage and frees this one.
-    auto k_block = [&](const uint8_t* st, const uint8_t* next, int to, int younger, auto load_c, auto next_c) __attribute__((always_inline)) {
-        constexpr bool LOAD = decltype(load_c)::value, NEXT = decltype(next_c)::value;
-        constexpr int PER = (C::LPT + TT - TN - 1) / (TT - TN);  // loads requested behind an MFMA
+    // publishes its stage and frees this one.  REST: the pieces of block kt + NS - 1 that the last call did not request (FIRST: this one requests
+    // the others of kt + NS, into the stage that it frees).
+    constexpr int PER = (C::LPT + TT - 1) / TT, EARLY = TN * PER < C::LPT ? TN * PER : C::LPT;
+    static_assert(EARLY + (TT - TN) * PER >= C::LPT, "all of a block is requested before the wait that counts it");
+    auto k_block = [&](const uint8_t* st, const uint8_t* next, int stage, int prev, int younger, auto rest_c, auto first_c, auto next_c) __attribute__((always_inline)) {
+        constexpr bool REST = decltype(rest_c)::value, FIRST = decltype(first_c)::value, NEXT = decltype(next_c)::value;
         s_last = s[TM - 1];
 #pragma unroll
         for (int i = 0; i < TM; i++) s[i] = s_next[i] * w_next;
         unrolled<0, TT>([&](auto t_c) __attribute__((always_inline)) {
             constexpr int t = decltype(t_c)::value, i = t / TN, j = t % TN;
             if constexpr (NEXT && i == TM - 1 && j == 0) {
+                if constexpr (REST) ld_kb++;
                 wait_loads(younger);
                 lds_barrier();
             }
             p[t & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i & 1], v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
             if constexpr (j == 0 && i + 1 < TM) a[(i + 1) & 1] = fragment(st, a_row + (i + 1) * 16);
             if constexpr (NEXT && i == TM - 1) {
+                if constexpr (j == 0) a[0] = fragment(next, a_row);
                 b[j] = fragment(next, b_row + j * 16);
-                if constexpr (j == 0) a[0] = fragment(next, a_row), read_scales(next);
+                if constexpr (j == TN - 1) read_scales(next);
             }
             if constexpr (t >= 2) scale_in(std::integral_constant<int, t - 2>{}, s[(t - 2) / TN]);
             else scale_in(std::integral_constant<int, TT - 2 + t>{}, s_last);
-            if constexpr (LOAD)  // all before the last row, whose wait counts them
-                unrolled<(t * PER < C::LPT ? t * PER : C::LPT), ((t + 1) * PER < C::LPT ? (t + 1) * PER : C::LPT)>(
-                    [&](auto d) __attribute__((always_inline)) { issue(to, d); });
+            constexpr int D = i == TM - 1 ? j * PER : EARLY + t * PER;
+            if constexpr (i == TM - 1 ? FIRST : REST)
+                unrolled<(D < C::LPT ? D : C::LPT), (D + PER < C::LPT ? D + PER : C::LPT)>(
+                    [&](auto d) __attribute__((always_inline)) { issue(i == TM - 1 ? stage : prev, d); });
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -237,18 +242,21 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         lds_barrier();
         first_operands(smem);
     }
+    if (NS - 1 < kfull) unrolled<0, EARLY>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
     int stage = 0, kt = 0;
-    auto step = [&](auto load_c, auto next_c, int younger) __attribute__((always_inline)) {
+    auto step = [&](auto rest_c, auto first_c, auto next_c, int younger) __attribute__((always_inline)) {
         const int next = stage == NS - 1 ? 0 : stage + 1, prev = stage == 0 ? NS - 1 : stage - 1;
-        k_block(smem + stage * C::STAGE, smem + next * C::STAGE, prev, younger, load_c, next_c);
-        if (decltype(load_c)::value) ld_kb++;
+        k_block(smem + stage * C::STAGE, smem + next * C::STAGE, stage, prev, younger, rest_c, first_c, next_c);
         stage = next, kt++;
     };
+    const std::true_type yes;
+    const std::false_type no;
 #pragma unroll 1
-    while (kt + NS - 1 < kfull) step(std::true_type{}, std::true_type{}, NS - 2);
+    while (kt + NS < kfull) step(yes, yes, yes, NS - 2);
+    if (kt + NS == kfull) step(yes, no, yes, NS - 2);
 #pragma unroll 1
-    while (kt + 1 < kfull) step(std::false_type{}, std::true_type{}, kfull - 2 - kt);
-    if (kt < kfull) step(std::false_type{}, std::false_type{}, 0);
+    while (kt + 1 < kfull) step(no, no, yes, kfull - 2 - kt);
+    if (kt < kfull) step(no, no, no, 0);
     if (kb0 + kfull < kb1) {  // block-uniform: the ragged block, whose missing chunks are zeros, through registers
         lds_barrier();
         const int left = g.K - (kb0 + kfull) * kScaleBlock;
@@ -262,7 +270,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         *reinterpret_cast<float*>(smem + C::DATA + tid * 4) = s_ptr[kb0 + kfull];
         lds_barrier();
         first_operands(smem);
-        k_block(smem, smem, 0, 0, std::false_type{}, std::false_type{});
+        k_block(smem, smem, 0, 0, 0, no, no, no);
     }
     scale_in(std::integral_constant<int, TT - 2>{}, s[TM - 1]);
     scale_in(std::integral_constant<int, TT - 1>{}, s[TM - 1]);
@@ -287,28 +295,55 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         }
     } else {
         const bool bf16 = g.out_dtype == LLMQ_BF16;
-        const bool wide = (g.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 7u) == 0;
+        const int wm0 = row0 + wm * C::WTM, wn0 = n0 + wn * C::WTN;
+        float bb[TN][4];
 #pragma unroll
-        for (int j = 0; j < TN; j++) {
-            const int n = n0 + wn * C::WTN + j * 16 + kq * 4;
-            float bb[4] = {0, 0, 0, 0};
-            if (g.bias) {
+        for (int j = 0; j < TN; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) bb[e] = load_as_f32(g.bias, g.bias_dtype, (int64_t)expert * g.N + min(n + e, g.N - 1));
+            for (int e = 0; e < 4; e++)
+                bb[j][e] = g.bias ? load_as_f32(g.bias, g.bias_dtype, (int64_t)expert * g.N + min(wn0 + j * 16 + kq * 4 + e, g.N - 1)) : 0.f;
+        auto finished = [&](int i, int j) __attribute__((always_inline)) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = acc[i][j][e] + bb[j][e];
+            return bf16 ? make_uint2(Lo<LLMQ_BF16>::pack2(v[0], v[1]), Lo<LLMQ_BF16>::pack2(v[2], v[3]))
+                        : make_uint2(Lo<LLMQ_F16>::pack2(v[0], v[1]), Lo<LLMQ_F16>::pack2(v[2], v[3]));
+        };
+        if ((g.N & 7) == 0 && (g.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15u) == 0) {  // uniform
+            // Through LDS, so that a store covers whole lines of a row: a wavefront's outputs go to a region of its own, 16-byte chunk c of row r at
+            // chunk c ^ (r % CH), and come back 16 bytes per lane, CH lanes a row.
+            constexpr int CH = C::WTN / 8, RPI = kWave / CH;
+            static_assert(C::WTM * C::WTN * 2 * (NT / kWave) <= C::LDS_BYTES, "outputs fit in the ring");
+            lds_barrier();  // every wavefront has read its last operands
+            uint8_t* mine = smem + wave * (C::WTM * C::WTN * 2);
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+#pragma unroll
+                for (int j = 0; j < TN; j++) {
+                    const int r = i * 16 + l16;
+                    *reinterpret_cast<uint2*>(mine + (r * CH + ((2 * j + (kq >> 1)) ^ (r % CH))) * 16 + (kq & 1) * 8) = finished(i, j);
+                }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+            const int c = lane % CH, n = wn0 + c * 8;
+#pragma unroll
+            for (int k = 0; k < C::WTM / RPI; k++) {
+                const int r = k * RPI + lane / CH;
+                const uint4 v = *reinterpret_cast<const uint4*>(mine + (r * CH + (c ^ (r % CH))) * 16);
+                if (wm0 + r < row_end && n < g.N) store_streaming(reinterpret_cast<uint16_t*>(g.out) + (int64_t)(wm0 + r) * g.ldo + n, v);
             }
+        } else {
 #pragma unroll
             for (int i = 0; i < TM; i++) {
-                const int m = row0 + wm * C::WTM + i * 16 + l16;
-                if (m >= row_end || n >= g.N) continue;
-                float v[4];
+                const int m = wm0 + i * 16 + l16;
+                if (m >= row_end) continue;
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = acc[i][j][e] + bb[e];
-                const uint2 h = bf16 ? make_uint2(Lo<LLMQ_BF16>::pack2(v[0], v[1]), Lo<LLMQ_BF16>::pack2(v[2], v[3]))
-                                     : make_uint2(Lo<LLMQ_F16>::pack2(v[0], v[1]), Lo<LLMQ_F16>::pack2(v[2], v[3]));
-                uint16_t* to = reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n;
-                if (wide && n + 3 < g.N) *reinterpret_cast<uint2*>(to) = h;
-                else {
+                for (int j = 0; j < TN; j++) {
+                    const int n = wn0 + j * 16 + kq * 4;
+                    const uint2 h = finished(i, j);
                     const uint32_t w[2] = {h.x, h.y};
+                    uint16_t* to = reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n;
 #pragma unroll
                     for (int e = 0; e < 4; e++)
                         if (n + e < g.N) to[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
