@@ -38,6 +38,23 @@ constexpr BlockTile kBlockTiles[] = {
 };
 constexpr int kNumBlockTiles = sizeof(kBlockTiles) / sizeof(kBlockTiles[0]);
 
+// Variants of gemm_block_rows.hip: 16-channel and 16-token tiles of a block, blocks of K per wavefront and stage, stages; several jobs per block; by
+// experts.  Alone they take up to 16 MT tokens, by experts any number in slabs of 16 MT.
+#define LLMQ_BLOCK_ROWS(V)                                                                                                      \
+    V(0, 1, 1, 1, 4, false, false) V(1, 1, 1, 2, 4, false, false) V(2, 2, 1, 1, 4, false, false) V(3, 1, 2, 1, 3, false, false)   \
+    V(4, 2, 2, 1, 3, false, false) V(5, 4, 2, 1, 3, false, false) V(6, 1, 4, 1, 3, false, false) V(7, 2, 4, 1, 3, false, false)   \
+    V(8, 4, 1, 1, 3, true, false) V(9, 2, 1, 1, 3, true, false) V(10, 2, 3, 1, 3, false, false) V(11, 4, 3, 1, 2, false, false)     \
+    V(12, 1, 1, 1, 4, true, true) V(13, 2, 1, 1, 3, true, true) V(14, 4, 1, 1, 3, true, true) V(15, 2, 2, 1, 3, true, true)       \
+    V(16, 4, 2, 1, 2, true, true) V(17, 2, 4, 1, 2, true, true)
+struct BlockRows { int t, mt; bool jobs, grouped; };
+constexpr BlockRows kBlockRows[] = {
+#define LLMQ_BLOCK_ROWS_SHAPE(I, T, MT, STEPS, NS, JOBS, GROUPED) {T, MT, JOBS, GROUPED},
+    LLMQ_BLOCK_ROWS(LLMQ_BLOCK_ROWS_SHAPE)
+#undef LLMQ_BLOCK_ROWS_SHAPE
+};
+constexpr int kNumBlockRows = sizeof(kBlockRows) / sizeof(kBlockRows[0]);
+
+int launch_block_rows(int variant, const BlockArgs& g, hipStream_t st);
 int launch_block_tile(int cfg, int splits, const BlockArgs& g, hipStream_t st);
 
 }  // namespace llmq

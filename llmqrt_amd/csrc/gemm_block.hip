@@ -1,4 +1,4 @@
-// Block-scaled fp8 products: argument checks, plan and entry points (kernels: gemm_block_tile.hip).
+// Block-scaled fp8 products: argument checks, plan and entry points (kernels: gemm_block_tile.hip, gemm_block_rows.hip).
 #include <algorithm>
 
 #include "gemm_block.h"
@@ -14,9 +14,21 @@ BlockPlan split_plan(int cfg, int splits, int KB) {
     return {cfg, (KB + per - 1) / per, per};
 }
 
+// cfg: a tile configuration, or kRowsCfg + a variant of the row-streaming kernel
+constexpr int kRowsCfg = kNumBlockTiles;
+bool rows_take(int cfg, int64_t M, bool grouped) {
+    const BlockRows& r = kBlockRows[cfg - kRowsCfg];
+    return r.grouped == grouped && (grouped || M <= 16 * r.mt);
+}
+
 BlockPlan plan(int64_t M, int64_t N, int64_t K) {
     const int KB = (int)((K + kScaleBlock - 1) / kScaleBlock);
-    if (forced_cfg >= 0) return split_plan(forced_cfg, std::max(1, std::min(forced_splits, KB)), KB);
+    if (forced_cfg >= 0 && (forced_cfg < kRowsCfg || rows_take(forced_cfg, M, false)))
+        return forced_cfg >= kRowsCfg ? BlockPlan{forced_cfg, 1, KB} : split_plan(forced_cfg, std::max(1, std::min(forced_splits, KB)), KB);
+    if (M <= 16) return {kRowsCfg + (N > 8192 ? 8 : 0), 1, KB};
+    if (M <= 32) return {kRowsCfg + (N > 8192 ? 5 : 3), 1, KB};
+    if (M <= 48) return {kRowsCfg + (N > 8192 ? 11 : 10), 1, KB};
+    if (M <= 64) return {kRowsCfg + (N > 8192 ? 7 : 6), 1, KB};
     const int cfg = M <= 32 ? 4 : M <= 64 ? 3 : M <= 1024 ? 2 : 0;
     const BlockTile t = kBlockTiles[cfg];
     const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
@@ -25,8 +37,9 @@ BlockPlan plan(int64_t M, int64_t N, int64_t K) {
 }
 
 int plan_grouped(int64_t rows, int64_t experts) {
-    if (forced_cfg >= 0) return forced_cfg;
+    if (forced_cfg >= 0 && (forced_cfg < kRowsCfg || rows_take(forced_cfg, rows, true))) return forced_cfg;
     const int64_t each = rows / experts;
+    if (each <= 8) return kRowsCfg + 13;
     return each <= 32 ? 4 : each <= 64 ? 3 : each <= 256 ? 2 : 0;
 }
 
@@ -72,6 +85,7 @@ extern "C" int llmq_gemm_fp8_block(const uint8_t* A, int64_t lda, const float* a
     g.lda = lda, g.ldb = ldb, g.ldo = ldo, g.M = (int)M, g.N = (int)N, g.K = (int)K;
     g.KB = (int)((K + kScaleBlock - 1) / kScaleBlock), g.NB = (int)((N + kScaleBlock - 1) / kScaleBlock), g.experts = 1;
     g.blocks_per_split = p.blocks_per_split, g.bias_dtype = bias_dtype, g.out_dtype = out_dtype;
+    if (p.cfg >= kRowsCfg) return launch_block_rows(p.cfg - kRowsCfg, g, (hipStream_t)stream);
     return launch_block_tile(p.cfg, p.splits, g, (hipStream_t)stream);
 }
 
@@ -87,11 +101,13 @@ extern "C" int llmq_gemm_fp8_block_grouped(const uint8_t* A, int64_t lda, const 
     g.lda = lda, g.ldb = K, g.ldo = ldo, g.M = (int)M, g.N = (int)N, g.K = (int)K;
     g.KB = (int)((K + kScaleBlock - 1) / kScaleBlock), g.NB = (int)((N + kScaleBlock - 1) / kScaleBlock), g.experts = (int)experts;
     g.bias_dtype = bias_dtype, g.out_dtype = out_dtype;
-    return launch_block_tile(plan_grouped(M, experts), 1, g, (hipStream_t)stream);
+    const int cfg = plan_grouped(M, experts);
+    if (cfg >= kRowsCfg) return launch_block_rows(cfg - kRowsCfg, g, (hipStream_t)stream);
+    return launch_block_tile(cfg, 1, g, (hipStream_t)stream);
 }
 
 extern "C" int llmq_gemm_fp8_block_force_plan(int cfg, int splits) {
-    if (cfg >= kNumBlockTiles || splits < 0) return LLMQ_ERR_SHAPE;
+    if (cfg >= kNumBlockTiles + kNumBlockRows || splits < 0) return LLMQ_ERR_SHAPE;
     forced_cfg = cfg < 0 ? -1 : cfg;
     forced_splits = splits;
     return LLMQ_OK;

@@ -163,7 +163,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     };
     v8i a[2], b[TN];
     v4f acc[TM][TN], p[4];
-    float s[TM], s_next[TM], w_next, s_last = 0.f;
+    float s[TM], s_next[TM], w_next;
     auto read_scales = [&](const uint8_t* st) __attribute__((always_inline)) {
         const float* f = reinterpret_cast<const float*>(st + C::DATA);
 #pragma unroll
@@ -195,9 +195,6 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     static_assert(EARLY + (TT - TN) * PER >= C::LPT, "all of a block is requested before the wait that counts it");
     auto k_block = [&](const uint8_t* st, const uint8_t* next, int stage, int prev, int younger, auto rest_c, auto first_c, auto next_c) __attribute__((always_inline)) {
         constexpr bool REST = decltype(rest_c)::value, FIRST = decltype(first_c)::value, NEXT = decltype(next_c)::value;
-        s_last = s[TM - 1];
-#pragma unroll
-        for (int i = 0; i < TM; i++) s[i] = s_next[i] * w_next;
         unrolled<0, TT>([&](auto t_c) __attribute__((always_inline)) {
             constexpr int t = decltype(t_c)::value, i = t / TN, j = t % TN;
             if constexpr (NEXT && i == TM - 1 && j == 0) {
@@ -206,14 +203,18 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
                 lds_barrier();
             }
             p[t & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i & 1], v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+            if constexpr (t == 2) {  // until here s[TM - 1] is the last block's; from the last row on s_next is the next one's
+#pragma unroll
+                for (int k = 0; k < TM; k++) s[k] = s_next[k] * w_next;
+            }
             if constexpr (j == 0 && i + 1 < TM) a[(i + 1) & 1] = fragment(st, a_row + (i + 1) * 16);
             if constexpr (NEXT && i == TM - 1) {
                 if constexpr (j == 0) a[0] = fragment(next, a_row);
                 b[j] = fragment(next, b_row + j * 16);
-                if constexpr (j == TN - 1) read_scales(next);
+                if constexpr (j == 0) read_scales(next);
             }
             if constexpr (t >= 2) scale_in(std::integral_constant<int, t - 2>{}, s[(t - 2) / TN]);
-            else scale_in(std::integral_constant<int, TT - 2 + t>{}, s_last);
+            else scale_in(std::integral_constant<int, TT - 2 + t>{}, s[TM - 1]);
             constexpr int D = i == TM - 1 ? j * PER : EARLY + t * PER;
             if constexpr (i == TM - 1 ? FIRST : REST)
                 unrolled<(D < C::LPT ? D : C::LPT), (D + PER < C::LPT ? D + PER : C::LPT)>(

@@ -13,6 +13,10 @@ E4M3 = torch.float8_e4m3fn
 NAMES = {torch.bfloat16: "bfloat16", torch.float16: "float16"}
 
 
+def same(a, b):
+    return bool(torch.equal(a, b))  # (a plain bool: a failed assertion prints no tensors)
+
+
 def blocks(n):
     return (n + 127) // 128
 
@@ -120,7 +124,7 @@ SIZES = [(1, 1, 16), (1, 128, 128), (2, 3, 144), (7, 130, 256), (16, 512, 384), 
 def test_product_exact(cuda, M, N, K, dtype):
     a, w, sa, sw = exact_operands(M, N, K, M * 3 + N * 5 + K, cuda)
     ref, _ = product64(a, w, sa, sw)
-    assert torch.equal(gemm(a, w, sa, sw, None, dtype), ref.to(dtype))
+    assert same(gemm(a, w, sa, sw, None, dtype), ref.to(dtype))
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
@@ -159,7 +163,7 @@ def test_every_plan_exact(cuda, force, M, N, K, splits):
     for cfg in all_configs():
         print("plan", cfg, splits, M, N, K, flush=True)
         assert force(cfg, splits) == 0
-        assert torch.equal(gemm(a, w, sa, sw, bias), ref.bfloat16()), f"configuration {cfg}, {splits} splits"
+        assert same(gemm(a, w, sa, sw, bias), ref.bfloat16()), f"configuration {cfg}, {splits} splits"
 
 
 def test_product_strides(cuda):
@@ -171,9 +175,9 @@ def test_product_strides(cuda):
     for at in (0, 16, 5):
         va, vw = wide_a[:, at:at + 512], wide_w[:, min(at, 16):min(at, 16) + 512]
         va.copy_(a), vw.copy_(w)
-        assert torch.equal(gemm(va, vw, sa, sw), ref)
-    assert torch.equal(gemm(a, w, sa.t().contiguous().t(), sw), ref)
-    assert torch.equal(gemm(a[3:4], w[:1], sa[3:4], sw[:1]), product64(a[3:4], w[:1], sa[3:4], sw[:1])[0].bfloat16())
+        assert same(gemm(va, vw, sa, sw), ref)
+    assert same(gemm(a, w, sa.t().contiguous().t(), sw), ref)
+    assert same(gemm(a[3:4], w[:1], sa[3:4], sw[:1]), product64(a[3:4], w[:1], sa[3:4], sw[:1])[0].bfloat16())
 
 
 def test_product_of_nothing(cuda):
@@ -229,7 +233,7 @@ def test_grouped_exact(cuda, counts, N, K):
         print("grouped", cfg, counts[:6], N, K, flush=True)
         assert _abi.lib().llmq_gemm_fp8_block_force_plan(cfg, 0) == 0
         try:
-            assert torch.equal(grouped(a, w, sa, sw, off), ref.bfloat16()), f"configuration {cfg}"
+            assert same(grouped(a, w, sa, sw, off), ref.bfloat16()), f"configuration {cfg}"
         finally:
             _abi.lib().llmq_gemm_fp8_block_force_plan(-1, 0)
 
