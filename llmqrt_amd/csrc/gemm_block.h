@@ -30,11 +30,19 @@ __device__ __forceinline__ void expert_rows(const BlockArgs& g, int e, int& firs
 
 struct BlockTile { int bm, bn, nt; };
 constexpr BlockTile kBlockTiles[] = {
-    {256, 256, 512},  // 0: 8 wavefronts of 128 x 64
-    {128, 256, 512},  // 1: 8 of 64 x 64
-    {128, 128, 256},  // 2: 4 of 64 x 64
-    {64, 128, 256},   // 3: 4 of 32 x 64
-    {32, 128, 256},   // 4: 4 of 32 x 32
+    {256, 256, 512},  // 0
+    {128, 256, 512},  // 1
+    {64, 128, 256},  // 2
+    {32, 128, 256},  // 3
+    {64, 256, 512},  // 4
+    {64, 64, 256},  // 5
+    {128, 128, 512},  // 6
+    {64, 128, 512},  // 7
+    {64, 64, 512},  // 8
+    {32, 128, 512},  // 9
+    {64, 128, 512},  // 10
+    {64, 128, 768},  // 11
+    {64, 64, 1024},  // 12
 };
 constexpr int kNumBlockTiles = sizeof(kBlockTiles) / sizeof(kBlockTiles[0]);
 

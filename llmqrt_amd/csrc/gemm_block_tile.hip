@@ -25,19 +25,21 @@ __device__ __forceinline__ void unrolled(F&& f) {
     }
 }
 
-// A block of WM x WN wavefronts owns BM tokens x BN channels; a wavefront (16 TM) x (16 TN) of them.
-template <int BM_, int BN_, int WM_, int WN_>
+// A block owns BM tokens x BN channels.  KS groups of WM x WN wavefronts share its blocks of K among them, one each per stage; a wavefront owns
+// (16 TM) x (16 TN) outputs, and the groups' sums are added at the end.
+template <int BM_, int BN_, int WM_, int WN_, int NS_, int KS_>
 struct TileCfg {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
-    static constexpr int NT = WM * WN * kWave;
+    static constexpr int KS = KS_, NG = WM * WN * kWave, NT = NG * KS;  // threads of a group, of the block
     static constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16, TT = TM * TN;
-    static constexpr int A_LOADS = BM * 8 / NT, B_LOADS = BN * 8 / NT, LPT = A_LOADS + B_LOADS + 1;  // per thread and stage, one of scales
-    static constexpr int DATA = (BM + BN) * 128, STAGE = DATA + NT * 4;  // bytes; the scales' slots are one per thread
-    static constexpr int NS = 4 * STAGE <= 80 * 1024 ? 4 : 3 * STAGE <= 160 * 1024 ? 3 : 2;
+    static constexpr int A_LOADS = BM * 8 / NG, B_LOADS = BN * 8 / NG, LPT = A_LOADS + B_LOADS + 1;  // per thread and stage, one of scales
+    static constexpr int DATA = (BM + BN) * 128, SUB = DATA + NG * 4, STAGE = KS * SUB;  // bytes; a group's part: its operands, a slot for a scale per thread
+    static constexpr int NS = NS_;  // LDS stages
     static constexpr int LDS_BYTES = NS * STAGE;
     static_assert(TM % 2 == 0 && TN >= 2 && TT % 4 == 0, "fragment parity, pending products");
-    static_assert(BM + (BN + 127) / 128 <= NT && 128 % WTN == 0 && (NT / 8) % 16 == 0, "scale slots, a wavefront's channels in one block, swizzle");
-    static_assert(A_LOADS * NT == BM * 8 && B_LOADS * NT == BN * 8 && (NS - 2) * LPT < 64, "even pieces, vmcnt");
+    static_assert(BM + (BN + 127) / 128 <= NG && 128 % WTN == 0 && (NG / 8) % 16 == 0, "scale slots, a wavefront's channels in one block, swizzle");
+    static_assert(A_LOADS * NG == BM * 8 && B_LOADS * NG == BN * 8 && (NS - 2) * LPT < 64, "even pieces, vmcnt");
+    static_assert(LDS_BYTES <= 160 * 1024 && (KS - 1) * BM * BN * 4 <= LDS_BYTES, "stages, the groups' sums");
 };
 
 // LDS place of 16-byte chunk c of row r: 16 rows of one chunk fall on 16 places
@@ -66,8 +68,9 @@ __device__ __forceinline__ void tile_of(int bid, int nblk, int tiles_m, int tile
 template <class C, bool GROUPED, bool SPLIT>
 __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    constexpr int TM = C::TM, TN = C::TN, NT = C::NT, NS = C::NS, TT = C::TT;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    constexpr int TM = C::TM, TN = C::TN, NG = C::NG, NS = C::NS, TT = C::TT, KS = C::KS;
+    const int group = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NG) : 0, tid = threadIdx.x - group * NG;
+    const int lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);  // of the group
     const int wm = wave / C::WN, wn = wave % C::WN, l16 = lane & 15, kq = lane >> 4;
     const int tiles_n = (g.N + C::BN - 1) / C::BN;
 
@@ -112,18 +115,18 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     }
     const int n0 = tn * C::BN;
     const int kb0 = SPLIT ? blockIdx.y * g.blocks_per_split : 0, kb1 = SPLIT ? min(g.KB, kb0 + g.blocks_per_split) : g.KB;
-    const int kfull = min(kb1, g.K / kScaleBlock) - kb0;  // whole blocks of this split; a ragged last one comes after them
+    const int kfull = (min(kb1, g.K / kScaleBlock) - kb0) / KS;  // whole blocks of each group; what is left of this split comes after them
     const uint8_t* B = g.B + (int64_t)expert * g.N * g.ldb;
     const float* sw = g.sw + (int64_t)expert * g.NB * g.KB;
 
-    // ---- global -> LDS.  A thread's pieces are row tid / 8 + i NT / 8 of the tile, LDS slot tid % 8, which holds the row's chunk
+    // ---- global -> LDS.  A thread's pieces are row tid / 8 + i NG / 8 of the tile, LDS slot tid % 8, which holds the row's chunk
     // slot ^ swizzle.  Rows past the end are the last row again.
     const int ld_row = tid / 8, ld_chunk = (tid % 8) ^ ((ld_row >> 1) & 7);
     uint32_t off[C::A_LOADS + C::B_LOADS];
 #pragma unroll
-    for (int i = 0; i < C::A_LOADS; i++) off[i] = (uint32_t)min(ld_row + i * (NT / 8), row_end - 1 - row0) * (uint32_t)g.lda + ld_chunk * 16;
+    for (int i = 0; i < C::A_LOADS; i++) off[i] = (uint32_t)min(ld_row + i * (NG / 8), row_end - 1 - row0) * (uint32_t)g.lda + ld_chunk * 16;
 #pragma unroll
-    for (int i = 0; i < C::B_LOADS; i++) off[C::A_LOADS + i] = (uint32_t)min(ld_row + i * (NT / 8), g.N - 1 - n0) * (uint32_t)g.ldb + ld_chunk * 16;
+    for (int i = 0; i < C::B_LOADS; i++) off[C::A_LOADS + i] = (uint32_t)min(ld_row + i * (NG / 8), g.N - 1 - n0) * (uint32_t)g.ldb + ld_chunk * 16;
     const uint8_t* a_base = g.A + (int64_t)row0 * g.lda;
     const uint8_t* b_base = B + (int64_t)n0 * g.ldb;
     // scale slot tid: tokens in the order in which a lane reads them (its TM tokens together), then the blocks of channels
@@ -134,14 +137,15 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     } else {
         s_ptr = sw + (int64_t)min(n0 / kScaleBlock + min(tid - C::BM, (C::BN - 1) / kScaleBlock), g.NB - 1) * g.KB;
     }
-    const uint32_t lds_base = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) void*)smem);
-    int ld_kb = kb0;
+    const uint8_t* sub = smem + group * C::SUB;  // the group's part of stage 0
+    const uint32_t lds_base = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) void*)smem) + (uint32_t)group * C::SUB;
+    int ld_kb = kb0 + group;
     auto issue = [&](int stage, auto d_c) __attribute__((always_inline)) {  // piece d of block ld_kb
         constexpr int d = decltype(d_c)::value;
         const uint32_t to = lds_base + (uint32_t)stage * C::STAGE;
         if constexpr (d < C::A_LOADS + C::B_LOADS) {
             const uint8_t* base = (d < C::A_LOADS ? a_base : b_base) + (int64_t)ld_kb * kScaleBlock;
-            const uint32_t m0v = to + (uint32_t)d * (NT * 16) + (uint32_t)wave * 1024;
+            const uint32_t m0v = to + (uint32_t)d * (NG * 16) + (uint32_t)wave * 1024;
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(off[d]), "s"(base) : "memory", "m0");
         } else {
             const float* p = s_ptr + ld_kb;
@@ -198,7 +202,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         unrolled<0, TT>([&](auto t_c) __attribute__((always_inline)) {
             constexpr int t = decltype(t_c)::value, i = t / TN, j = t % TN;
             if constexpr (NEXT && i == TM - 1 && j == 0) {
-                if constexpr (REST) ld_kb++;
+                if constexpr (REST) ld_kb += KS;
                 wait_loads(younger);
                 lds_barrier();
             }
@@ -235,19 +239,19 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         constexpr int n = decltype(n_c)::value;
         if (n < kfull) {
             unrolled<0, C::LPT>([&](auto d) __attribute__((always_inline)) { issue(n, d); });
-            ld_kb++;
+            ld_kb += KS;
         }
     });
     if (kfull > 0) {
         wait_loads(min(kfull, NS - 1) - 1);
         lds_barrier();
-        first_operands(smem);
+        first_operands(sub);
     }
     if (NS - 1 < kfull) unrolled<0, EARLY>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
     int stage = 0, kt = 0;
     auto step = [&](auto rest_c, auto first_c, auto next_c, int younger) __attribute__((always_inline)) {
         const int next = stage == NS - 1 ? 0 : stage + 1, prev = stage == 0 ? NS - 1 : stage - 1;
-        k_block(smem + stage * C::STAGE, smem + next * C::STAGE, stage, prev, younger, rest_c, first_c, next_c);
+        k_block(sub + stage * C::STAGE, sub + next * C::STAGE, stage, prev, younger, rest_c, first_c, next_c);
         stage = next, kt++;
     };
     const std::true_type yes;
@@ -258,23 +262,38 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
 #pragma unroll 1
     while (kt + 1 < kfull) step(no, no, yes, kfull - 2 - kt);
     if (kt < kfull) step(no, no, no, 0);
-    if (kb0 + kfull < kb1) {  // block-uniform: the ragged block, whose missing chunks are zeros, through registers
+    if (kb0 + kfull * KS < kb1) {  // block-uniform: at most a block for each group, one of them ragged, through registers; what is missing is zeros
         lds_barrier();
-        const int left = g.K - (kb0 + kfull) * kScaleBlock;
-        const int64_t at = (int64_t)(kb0 + kfull) * kScaleBlock;
+        const int kb = kb0 + kfull * KS + group, left = kb < kb1 ? g.K - kb * kScaleBlock : 0;
+        uint8_t* to = smem + group * C::SUB;
 #pragma unroll
         for (int i = 0; i < C::A_LOADS + C::B_LOADS; i++) {
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (ld_chunk * 16 < left) v = *reinterpret_cast<const uint4*>((i < C::A_LOADS ? a_base : b_base) + at + off[i]);
-            *reinterpret_cast<uint4*>(smem + i * (NT * 16) + tid * 16) = v;
+            if (ld_chunk * 16 < left) v = *reinterpret_cast<const uint4*>((i < C::A_LOADS ? a_base : b_base) + (int64_t)kb * kScaleBlock + off[i]);
+            *reinterpret_cast<uint4*>(to + i * (NG * 16) + tid * 16) = v;
         }
-        *reinterpret_cast<float*>(smem + C::DATA + tid * 4) = s_ptr[kb0 + kfull];
+        *reinterpret_cast<float*>(to + C::DATA + tid * 4) = left > 0 ? s_ptr[kb] : 0.f;
         lds_barrier();
-        first_operands(smem);
-        k_block(smem, smem, 0, 0, 0, no, no, no);
+        first_operands(sub);
+        k_block(sub, sub, 0, 0, 0, no, no, no);
     }
     scale_in(std::integral_constant<int, TT - 2>{}, s[TM - 1]);
     scale_in(std::integral_constant<int, TT - 1>{}, s[TM - 1]);
+    if constexpr (KS > 1) {  // the groups' sums, in order
+        v4f* sums = reinterpret_cast<v4f*>(smem) + ((group - 1) * (NG / kWave) + wave) * TT * kWave + lane;
+        lds_barrier();  // every wavefront has read its last operands
+        if (group > 0)
+#pragma unroll
+            for (int t = 0; t < TT; t++) sums[t * kWave] = acc[t / TN][t % TN];
+        lds_barrier();
+        if (group == 0)
+#pragma unroll
+            for (int k = 1; k < KS; k++)
+#pragma unroll
+                for (int t = 0; t < TT; t++) acc[t / TN][t % TN] += sums[(k * (NG / kWave) * TT + t) * kWave];
+        lds_barrier();  // and their sums: the outputs take their place
+        if (group > 0) return;
+    }
 
     // ---- a lane holds token l16 of each tile of tokens and channels 4 kq .. + 3 of each tile of channels
     if constexpr (SPLIT) {
@@ -314,8 +333,8 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
             // Through LDS, so that a store covers whole lines of a row: a wavefront's outputs go to a region of its own, 16-byte chunk c of row r at
             // chunk c ^ (r % CH), and come back 16 bytes per lane, CH lanes a row.
             constexpr int CH = C::WTN / 8, RPI = kWave / CH;
-            static_assert(C::WTM * C::WTN * 2 * (NT / kWave) <= C::LDS_BYTES, "outputs fit in the ring");
-            lds_barrier();  // every wavefront has read its last operands
+            static_assert(C::WTM * C::WTN * 2 * (NG / kWave) <= C::LDS_BYTES, "outputs fit in the ring");
+            if constexpr (KS == 1) lds_barrier();  // every wavefront has read its last operands
             uint8_t* mine = smem + wave * (C::WTM * C::WTN * 2);
 #pragma unroll
             for (int i = 0; i < TM; i++)
@@ -421,11 +440,19 @@ int launch_cfg(const BlockArgs& g, int splits, hipStream_t st) {
 
 int launch_block_tile(int cfg, int splits, const BlockArgs& g, hipStream_t st) {
     switch (cfg) {
-        case 0: return launch_cfg<TileCfg<256, 256, 2, 4>>(g, splits, st);
-        case 1: return launch_cfg<TileCfg<128, 256, 2, 4>>(g, splits, st);
-        case 2: return launch_cfg<TileCfg<128, 128, 2, 2>>(g, splits, st);
-        case 3: return launch_cfg<TileCfg<64, 128, 2, 2>>(g, splits, st);
-        case 4: return launch_cfg<TileCfg<32, 128, 1, 4>>(g, splits, st);
+        case 0: return launch_cfg<TileCfg<256, 256, 2, 4, 2, 1>>(g, splits, st);
+        case 1: return launch_cfg<TileCfg<128, 256, 2, 4, 3, 1>>(g, splits, st);
+        case 2: return launch_cfg<TileCfg<64, 128, 2, 2, 3, 1>>(g, splits, st);
+        case 3: return launch_cfg<TileCfg<32, 128, 1, 4, 3, 1>>(g, splits, st);
+        case 4: return launch_cfg<TileCfg<64, 256, 2, 4, 3, 1>>(g, splits, st);
+        case 5: return launch_cfg<TileCfg<64, 64, 2, 2, 4, 1>>(g, splits, st);
+        case 6: return launch_cfg<TileCfg<128, 128, 2, 2, 2, 2>>(g, splits, st);
+        case 7: return launch_cfg<TileCfg<64, 128, 2, 2, 3, 2>>(g, splits, st);
+        case 8: return launch_cfg<TileCfg<64, 64, 2, 2, 4, 2>>(g, splits, st);
+        case 9: return launch_cfg<TileCfg<32, 128, 1, 4, 3, 2>>(g, splits, st);
+        case 10: return launch_cfg<TileCfg<64, 128, 2, 2, 2, 2>>(g, splits, st);
+        case 11: return launch_cfg<TileCfg<64, 128, 2, 2, 2, 3>>(g, splits, st);
+        case 12: return launch_cfg<TileCfg<64, 64, 2, 2, 2, 4>>(g, splits, st);
     }
     return LLMQ_ERR_SHAPE;
 }
