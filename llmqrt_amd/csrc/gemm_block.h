@@ -28,35 +28,28 @@ __device__ __forceinline__ void expert_rows(const BlockArgs& g, int e, int& firs
     last = min(max(g.offsets[e + 1], first), g.M);
 }
 
-struct BlockTile { int bm, bn, nt; };
+struct BlockTile { int bm, bn; };  // tokens, channels of a block
 constexpr BlockTile kBlockTiles[] = {
-    {256, 256, 512},  // 0
-    {128, 256, 512},  // 1
-    {64, 128, 256},  // 2
-    {32, 128, 256},  // 3
-    {64, 256, 512},  // 4
-    {64, 64, 256},  // 5
-    {128, 128, 512},  // 6
-    {64, 128, 512},  // 7
-    {64, 64, 512},  // 8
-    {32, 128, 512},  // 9
-    {64, 128, 512},  // 10
-    {64, 128, 768},  // 11
-    {64, 64, 1024},  // 12
+    {256, 256},  // 0: 8 wavefronts of 128 x 64
+    {128, 256},  // 1: 8 wavefronts of 64 x 64
+    {64, 256},  // 2: 8 wavefronts of 32 x 64
+    {64, 128},  // 3: 4 wavefronts of 32 x 64
+    {32, 128},  // 4: 4 wavefronts of 32 x 32
+    {64, 64},  // 5: 4 wavefronts of 32 x 32
+    {64, 128},  // 6: 2 groups of 4 wavefronts of 32 x 64
+    {64, 64},  // 7: 2 groups of 4 wavefronts of 32 x 32
 };
 constexpr int kNumBlockTiles = sizeof(kBlockTiles) / sizeof(kBlockTiles[0]);
 
-// Variants of gemm_block_rows.hip: 16-channel and 16-token tiles of a block, blocks of K per wavefront and stage, stages; several jobs per block; by
-// experts.  Alone they take up to 16 MT tokens, by experts any number in slabs of 16 MT.
-#define LLMQ_BLOCK_ROWS(V)                                                                                                      \
-    V(0, 1, 1, 1, 4, false, false) V(1, 1, 1, 2, 4, false, false) V(2, 2, 1, 1, 4, false, false) V(3, 1, 2, 1, 3, false, false)   \
-    V(4, 2, 2, 1, 3, false, false) V(5, 4, 2, 1, 3, false, false) V(6, 1, 4, 1, 3, false, false) V(7, 2, 4, 1, 3, false, false)   \
-    V(8, 4, 1, 1, 3, true, false) V(9, 2, 1, 1, 3, true, false) V(10, 2, 3, 1, 3, false, false) V(11, 4, 3, 1, 2, false, false)     \
-    V(12, 1, 1, 1, 4, true, true) V(13, 2, 1, 1, 3, true, true) V(14, 4, 1, 1, 3, true, true) V(15, 2, 2, 1, 3, true, true)       \
-    V(16, 4, 2, 1, 2, true, true) V(17, 2, 4, 1, 2, true, true)
-struct BlockRows { int t, mt; bool jobs, grouped; };
+// Variants of gemm_block_rows.hip: 16-channel and 16-token tiles of a block, blocks of K per wavefront and stage, stages; several groups of channels
+// per block.  They take up to 16 MT tokens.
+#define LLMQ_BLOCK_ROWS(V)                                                                                 \
+    V(0, 1, 1, 1, 4, false) V(1, 1, 1, 2, 4, false) V(2, 2, 1, 1, 4, false) V(3, 1, 2, 1, 3, false)         \
+    V(4, 2, 2, 1, 3, false) V(5, 4, 2, 1, 3, false) V(6, 1, 4, 1, 3, false) V(7, 2, 4, 1, 3, false)         \
+    V(8, 4, 1, 1, 3, true) V(9, 2, 1, 1, 3, true) V(10, 1, 3, 1, 4, false) V(11, 2, 3, 1, 3, false)
+struct BlockRows { int t, mt; };
 constexpr BlockRows kBlockRows[] = {
-#define LLMQ_BLOCK_ROWS_SHAPE(I, T, MT, STEPS, NS, JOBS, GROUPED) {T, MT, JOBS, GROUPED},
+#define LLMQ_BLOCK_ROWS_SHAPE(I, T, MT, STEPS, NS, MANY) {T, MT},
     LLMQ_BLOCK_ROWS(LLMQ_BLOCK_ROWS_SHAPE)
 #undef LLMQ_BLOCK_ROWS_SHAPE
 };

@@ -16,14 +16,11 @@ BlockPlan split_plan(int cfg, int splits, int KB) {
 
 // cfg: a tile configuration, or kRowsCfg + a variant of the row-streaming kernel
 constexpr int kRowsCfg = kNumBlockTiles;
-bool rows_take(int cfg, int64_t M, bool grouped) {
-    const BlockRows& r = kBlockRows[cfg - kRowsCfg];
-    return r.grouped == grouped && (grouped || M <= 16 * r.mt);
-}
+bool rows_take(int cfg, int64_t M) { return M <= 16 * kBlockRows[cfg - kRowsCfg].mt; }
 
 BlockPlan plan(int64_t M, int64_t N, int64_t K) {
     const int KB = (int)((K + kScaleBlock - 1) / kScaleBlock);
-    if (forced_cfg >= 0 && (forced_cfg < kRowsCfg || rows_take(forced_cfg, M, false)))
+    if (forced_cfg >= 0 && (forced_cfg < kRowsCfg || rows_take(forced_cfg, M)))
         return forced_cfg >= kRowsCfg ? BlockPlan{forced_cfg, 1, KB} : split_plan(forced_cfg, std::max(1, std::min(forced_splits, KB)), KB);
     if (M <= 16) return {kRowsCfg + (N > 8192 ? 8 : 0), 1, KB};
     if (M <= 32) return {kRowsCfg + (N > 8192 ? 5 : 3), 1, KB};
@@ -37,9 +34,8 @@ BlockPlan plan(int64_t M, int64_t N, int64_t K) {
 }
 
 int plan_grouped(int64_t rows, int64_t experts) {
-    if (forced_cfg >= 0 && (forced_cfg < kRowsCfg || rows_take(forced_cfg, rows, true))) return forced_cfg;
+    if (forced_cfg >= 0 && forced_cfg < kRowsCfg) return forced_cfg;
     const int64_t each = rows / experts;
-    if (each <= 8) return kRowsCfg + 13;
     return each <= 32 ? 4 : each <= 64 ? 3 : each <= 256 ? 2 : 0;
 }
 
@@ -101,9 +97,7 @@ extern "C" int llmq_gemm_fp8_block_grouped(const uint8_t* A, int64_t lda, const 
     g.lda = lda, g.ldb = K, g.ldo = ldo, g.M = (int)M, g.N = (int)N, g.K = (int)K;
     g.KB = (int)((K + kScaleBlock - 1) / kScaleBlock), g.NB = (int)((N + kScaleBlock - 1) / kScaleBlock), g.experts = (int)experts;
     g.bias_dtype = bias_dtype, g.out_dtype = out_dtype;
-    const int cfg = plan_grouped(M, experts);
-    if (cfg >= kRowsCfg) return launch_block_rows(cfg - kRowsCfg, g, (hipStream_t)stream);
-    return launch_block_tile(cfg, 1, g, (hipStream_t)stream);
+    return launch_block_tile(plan_grouped(M, experts), 1, g, (hipStream_t)stream);
 }
 
 extern "C" int llmq_gemm_fp8_block_force_plan(int cfg, int splits) {

@@ -1,4 +1,4 @@
-// Block-scaled fp8 product for a few tokens (alone: up to 64; by experts: a few each): weight rows streamed through LDS in long pieces.
+// Block-scaled fp8 product for up to 64 tokens: weight rows streamed through LDS in long pieces.
 //
 //   out[m, n] = sum_b sa[m, b] sw[n / 128, b] sum_{k in block b} A[m, k] B[n, k]   (+ bias[n])
 //
@@ -6,8 +6,8 @@
 // 512 STEPS bytes of K of every weight and activation row, loaded straight into LDS, NS - 1 stages in flight beside the one that is
 // multiplied; each wavefront takes STEPS blocks of 128 of a stage, one MFMA each, and scales the results into its own fp32 sums with the scales that
 // it loaded with the stage.  The four sums are added in wavefront order at the end: no K split, no second launch, a fixed order.
-// JOBS: a block takes several pieces of work, one after the other, and the ring runs on from one to the next while the sums are added beside it:
-// groups of channels (alone: as many blocks as are resident share them), or slabs of 16 MT rows of its expert (by experts).
+// MANY: for many channels as many blocks as are resident take one group of 16 T channels after the other; the ring runs on into the next group while the
+// last one's sums are added beside it.
 #include <algorithm>
 #include <type_traits>
 
@@ -20,21 +20,20 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int kMostJobs = 16;  // groups of channels of a block (alone)
+constexpr int kMostGroups = 16;  // groups of channels that a block takes
 
-template <int T_, int MT_, int STEPS_, int NS_, bool JOBS_, bool GROUPED_>
+template <int T_, int MT_, int STEPS_, int NS_, bool MANY_>
 struct RowsCfg {
     static constexpr int T = T_, MT = MT_, STEPS = STEPS_, NS = NS_;
-    static constexpr bool JOBS = JOBS_, GROUPED = GROUPED_;
+    static constexpr bool MANY = MANY_;
     static constexpr int NW = 4, NT = NW * kWave, SEG = 512 * STEPS, CPR = SEG / 16;
     static constexpr int ROWS = 16 * (T + MT), DATA = ROWS * SEG;
     static constexpr int SLOADS = 16 * MT + 1 > kWave ? 2 : 1, SWAVE = STEPS * SLOADS * kWave * 4;  // scale loads per block of K; bytes of a wavefront's
     static constexpr int STAGE = DATA + NW * SWAVE, LPT = DATA / (NT * 16), LOADS = LPT + STEPS * SLOADS;
     static constexpr int RING = NS * STAGE, SUMS = NW * T * MT * kWave * 16;
-    static constexpr int BIAS = (JOBS && !GROUPED ? kMostJobs : 1) * 16 * T * 4;
-    static constexpr int LDS_BYTES = (JOBS ? RING + SUMS : (RING > SUMS ? RING : SUMS)) + BIAS;
+    static constexpr int BIAS = (MANY ? kMostGroups : 1) * 16 * T * 4;
+    static constexpr int LDS_BYTES = (MANY ? RING + SUMS : (RING > SUMS ? RING : SUMS)) + BIAS;
     static_assert(DATA % (NT * 16) == 0 && LDS_BYTES <= 160 * 1024 && (NS - 1) * LOADS < 64 && 128 % (16 * T) == 0, "even stages, LDS, vmcnt, one block of channels");
-    static_assert(JOBS || !GROUPED, "an expert's slabs are jobs");
 };
 
 template <class C>
@@ -43,43 +42,31 @@ __global__ __launch_bounds__(C::NT) void block_rows_kernel(BlockArgs g) {
     constexpr int T = C::T, MT = C::MT, NS = C::NS, SEG = C::SEG;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int l16 = lane & 15, kq = lane >> 4;
-    int n0 = blockIdx.x * (16 * T), m0 = 0, row_end = g.M;
-    const int nst = (g.K + SEG - 1) / SEG;
-    const int step_n = C::JOBS && !C::GROUPED ? gridDim.x * (16 * T) : 0, step_m = C::GROUPED ? 16 * MT : 0;
-    const uint8_t* B = g.B;
-    const float* sw = g.sw;
-    int64_t bias0 = 0;
-    if (C::GROUPED) {
-        const int e = blockIdx.y;
-        expert_rows(g, e, m0, row_end);
-        m0 = __builtin_amdgcn_readfirstlane(m0), row_end = __builtin_amdgcn_readfirstlane(row_end);
-        if (m0 >= row_end) return;  // block-uniform
-        B += (int64_t)e * g.N * g.ldb, sw += (int64_t)e * g.NB * g.KB, bias0 = (int64_t)e * g.N;
-    }
-    const int jobs = !C::JOBS ? 1 : C::GROUPED ? (row_end - m0 + 16 * MT - 1) / (16 * MT) : (g.N - n0 + step_n - 1) / max(step_n, 1);
-    const int total = jobs * nst;
+    int n0 = blockIdx.x * (16 * T);
+    const int nst = (g.K + SEG - 1) / SEG, step_n = C::MANY ? gridDim.x * (16 * T) : 0;
+    const int groups = C::MANY ? (g.N - n0 + step_n - 1) / max(step_n, 1) : 1, total = groups * nst;  // of channels; stages of the block
 
     // ---- direct loads: piece p of a stage is row p / CPR (weights, then activations), LDS chunk p % CPR, which holds chunk (p % CPR) ^ (row & 15)
     // of the row, so that the operand reads of 16 rows hit 16 places; rows past the end are the last one again
     uint32_t off[C::LPT], chunk[C::LPT];
-    const uint8_t *a_base, *b_base;
+    const uint8_t* b_base;
     const float *sa_row, *sw_row;
-    auto aim = [&](int n, int m) __attribute__((always_inline)) {  // the loads of a job
-        b_base = B + (int64_t)n * g.ldb, a_base = g.A + (int64_t)m * g.lda;
+    auto aim = [&](int n) __attribute__((always_inline)) {  // the loads of a group
+        b_base = g.B + (int64_t)n * g.ldb;
 #pragma unroll
         for (int i = 0; i < C::LPT; i++) {
             const int row = ((wave * C::LPT + i) * kWave + lane) / C::CPR;
-            off[i] = row < 16 * T ? (uint32_t)min(row, g.N - 1 - n) * (uint32_t)g.ldb : (uint32_t)min(row - 16 * T, row_end - 1 - m) * (uint32_t)g.lda;
+            off[i] = row < 16 * T ? (uint32_t)min(row, g.N - 1 - n) * (uint32_t)g.ldb : (uint32_t)min(row - 16 * T, g.M - 1) * (uint32_t)g.lda;
         }
-        sw_row = sw + (int64_t)(n / kScaleBlock) * g.KB;
-        sa_row = lane < 16 * MT ? g.sa + (int64_t)min(m + lane, row_end - 1) * g.KB : sw_row;  // the lane behind the tokens fetches the weights' scale
+        sw_row = g.sw + (int64_t)(n / kScaleBlock) * g.KB;
+        sa_row = lane < 16 * MT ? g.sa + (int64_t)min(lane, g.M - 1) * g.KB : sw_row;  // the lane behind the tokens fetches the weights' scale
     };
 #pragma unroll
     for (int i = 0; i < C::LPT; i++) {
         const int p = (wave * C::LPT + i) * kWave + lane;
         chunk[i] = 16u * (uint32_t)((p % C::CPR) ^ ((p / C::CPR) & 15));
     }
-    aim(n0, m0);
+    aim(n0);
     const uint32_t lds_base = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) void*)smem);
     auto issue = [&](int s, int slot) __attribute__((always_inline)) {
         const bool tail = (s + 1) * SEG > g.K;  // uniform: chunks past the end re-read the last one of the row, masked when used
@@ -87,7 +74,7 @@ __global__ __launch_bounds__(C::NT) void block_rows_kernel(BlockArgs g) {
 #pragma unroll
         for (int i = 0; i < C::LPT; i++) {
             const bool w = (wave * C::LPT + i) * kWave < 16 * T * C::CPR;  // wavefront-uniform
-            const uint8_t* src = (w ? b_base : a_base) + (int64_t)s * SEG;
+            const uint8_t* src = (w ? b_base : g.A) + (int64_t)s * SEG;
             uint32_t voff = off[i] + chunk[i];
             if (tail) voff = off[i] + min(chunk[i], (uint32_t)(g.K - 16 - s * SEG));
             const uint32_t m0v = to + (uint32_t)(wave * C::LPT + i) * 1024;
@@ -159,15 +146,14 @@ __global__ __launch_bounds__(C::NT) void block_rows_kernel(BlockArgs g) {
     };
     static_assert(NS <= 4, "wait_stage");
 
-    // the bias of all the block's channels waits in LDS: a load at the end of a job would wait behind the ring
+    // the bias of all the block's channels waits in LDS: a load at the end of a group would wait behind the ring
     float* s_bias = reinterpret_cast<float*>(smem + C::LDS_BYTES - C::BIAS);
     if (g.bias) {
-        const int n_jobs = C::GROUPED ? 1 : jobs;
-        for (int i = tid; i < n_jobs * 16 * T; i += C::NT)
-            s_bias[i] = load_as_f32(g.bias, g.bias_dtype, bias0 + min(n0 + i / (16 * T) * step_n + i % (16 * T), g.N - 1));
+        for (int i = tid; i < groups * 16 * T; i += C::NT)
+            s_bias[i] = load_as_f32(g.bias, g.bias_dtype, min(n0 + i / (16 * T) * step_n + i % (16 * T), g.N - 1));
     }
-    v4f (*red)[MT * T][kWave] = reinterpret_cast<v4f (*)[MT * T][kWave]>(smem + (C::JOBS ? C::RING : 0));
-    auto finish = [&](int job) __attribute__((always_inline)) {
+    v4f (*red)[MT * T][kWave] = reinterpret_cast<v4f (*)[MT * T][kWave]>(smem + (C::MANY ? C::RING : 0));
+    auto finish = [&](int group) __attribute__((always_inline)) {
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -179,12 +165,12 @@ __global__ __launch_bounds__(C::NT) void block_rows_kernel(BlockArgs g) {
 #pragma unroll
             for (int w = 1; w < C::NW; w++) sum += red[w][q][l];
             // lane l: token 16 mt + l % 16, channels 16 t + 4 (l / 16) .. + 3
-            const int m = m0 + 16 * mt + (l & 15), c = 16 * t + 4 * (l >> 4), n = n0 + c;
-            if (m >= row_end || n >= g.N) continue;
+            const int m = 16 * mt + (l & 15), c = 16 * t + 4 * (l >> 4), n = n0 + c;
+            if (m >= g.M || n >= g.N) continue;
             uint16_t h[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float v = sum[e] + (g.bias ? s_bias[(C::GROUPED ? 0 : job) * 16 * T + c + e] : 0.f);
+                const float v = sum[e] + (g.bias ? s_bias[group * 16 * T + c + e] : 0.f);
                 h[e] = g.out_dtype == LLMQ_BF16 ? Lo<LLMQ_BF16>::from_f32(v) : Lo<LLMQ_F16>::from_f32(v);
             }
             uint16_t* to = reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n;
@@ -197,19 +183,16 @@ __global__ __launch_bounds__(C::NT) void block_rows_kernel(BlockArgs g) {
         }
     };
 
-    int issued = 0, issue_s = 0, issue_n = n0, issue_m = m0;  // stages requested; the next one within its job
+    int issued = 0, issue_s = 0, issue_n = n0;  // stages requested; the next one within its group
     auto issue_next = [&](int slot) __attribute__((always_inline)) {
         if (issued == total) return;
-        if (C::JOBS && issue_s == nst) {
-            issue_s = 0, issue_n += step_n, issue_m += step_m;
-            aim(issue_n, issue_m);
-        }
+        if (C::MANY && issue_s == nst) issue_s = 0, issue_n += step_n, aim(issue_n);
         issue(issue_s++, slot);
         issued++;
     };
 #pragma unroll
     for (int t = 0; t < NS - 1; t++) issue_next(t);
-    int slot = 0, s = 0, job = 0;
+    int slot = 0, s = 0, group = 0;
 #pragma unroll 1
     for (int f = 0; f < total; f++) {
         wait_stage(min(total - 1, f + NS - 2) - f);
@@ -219,13 +202,13 @@ __global__ __launch_bounds__(C::NT) void block_rows_kernel(BlockArgs g) {
         else compute(slot, false, 0);
         slot = slot == NS - 1 ? 0 : slot + 1;
         s++;
-        if (C::JOBS && s == nst) {
-            finish(job);  // its reads of the sums are done in every wavefront before the barrier of the next stage
+        if (C::MANY && s == nst) {
+            finish(group);  // its reads of the sums are done in every wavefront before the barrier of the next stage
             clear();
-            n0 += step_n, m0 += step_m, job++, s = 0;
+            n0 += step_n, group++, s = 0;
         }
     }
-    if constexpr (!C::JOBS) {
+    if constexpr (!C::MANY) {
         lds_barrier();  // every wavefront is done reading the stages
         finish(0);
     }
@@ -245,12 +228,12 @@ int launch_rows(const BlockArgs& g, hipStream_t st) {
         }
     }
     int64_t blocks = ((int64_t)g.N + 16 * C::T - 1) / (16 * C::T);
-    if (C::JOBS && !C::GROUPED) {  // as many as are resident at once, or fewer so that all take as many groups
-        const int64_t slots = 256 * (160 * 1024 / C::LDS_BYTES), each = std::min<int64_t>(kMostJobs, (blocks + slots - 1) / slots);
+    if (C::MANY) {  // as many as are resident at once, or fewer so that all take as many groups
+        const int64_t slots = 256 * (160 * 1024 / C::LDS_BYTES), each = std::min<int64_t>(kMostGroups, (blocks + slots - 1) / slots);
         blocks = (blocks + each - 1) / each;
     }
     if (blocks * C::NT > 0xffffffffLL) return LLMQ_ERR_SHAPE;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, C::GROUPED ? g.experts : 1), dim3(C::NT), C::LDS_BYTES, st, g);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(C::NT), C::LDS_BYTES, st, g);
     return launch_status();
 }
 
@@ -258,8 +241,8 @@ int launch_rows(const BlockArgs& g, hipStream_t st) {
 
 int launch_block_rows(int variant, const BlockArgs& g, hipStream_t st) {
     switch (variant) {
-#define LLMQ_BLOCK_ROWS_CASE(I, T, MT, STEPS, NS, JOBS, GROUPED) \
-    case I: return launch_rows<RowsCfg<T, MT, STEPS, NS, JOBS, GROUPED>>(g, st);
+#define LLMQ_BLOCK_ROWS_CASE(I, T, MT, STEPS, NS, MANY) \
+    case I: return launch_rows<RowsCfg<T, MT, STEPS, NS, MANY>>(g, st);
         LLMQ_BLOCK_ROWS(LLMQ_BLOCK_ROWS_CASE)
 #undef LLMQ_BLOCK_ROWS_CASE
     }

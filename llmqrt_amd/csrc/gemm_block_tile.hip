@@ -191,10 +191,13 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
 
-    // One block of K, kt.  A product's results are scaled in two MFMAs later, so that the matrix cores never wait for the vector unit; the operands of
+    // One block of K, kt.  A product's results are scaled in DELAY MFMAs later, so that the matrix cores never wait for the vector unit; the operands of
     // the next row of tiles are read under the MFMAs of this one, and those of the next block under the last row, behind the barrier that
-    // publishes its stage and frees this one.  REST: the pieces of block kt + NS - 1 that the last call did not request (FIRST: this one requests
+    // publishes its stage and frees this one.  The priority alternates every two MFMAs, so that the two wavefronts of a SIMD take turns at its
+    // matrix core and vector unit.  REST: the pieces of block kt + NS - 1 that the last call did not request (FIRST: this one requests
     // the others of kt + NS, into the stage that it frees).
+    // (us, 2 MFMAs later without priorities / 3 with: 8192 x 37888 x 3584 951 / 930, 4096 x 3584 x 18944 228 / 222, 777 x 3584 x 18944 on 128 x 256 tiles 104 / 97)
+    constexpr int DELAY = TT > 4 ? 3 : 2;  // (four tiles: s_next is the next block's from the third on)
     constexpr int PER = (C::LPT + TT - 1) / TT, EARLY = TN * PER < C::LPT ? TN * PER : C::LPT;
     static_assert(EARLY + (TT - TN) * PER >= C::LPT, "all of a block is requested before the wait that counts it");
     auto k_block = [&](const uint8_t* st, const uint8_t* next, int stage, int prev, int younger, auto rest_c, auto first_c, auto next_c) __attribute__((always_inline)) {
@@ -206,8 +209,9 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
                 wait_loads(younger);
                 lds_barrier();
             }
+            if constexpr (t % 2 == 0) __builtin_amdgcn_s_setprio(t % 4 == 0);
             p[t & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i & 1], v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
-            if constexpr (t == 2) {  // until here s[TM - 1] is the last block's; from the last row on s_next is the next one's
+            if constexpr (t == DELAY) {  // until here s is the last block's; from the last row on s_next is the next one's
 #pragma unroll
                 for (int k = 0; k < TM; k++) s[k] = s_next[k] * w_next;
             }
@@ -217,8 +221,8 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
                 b[j] = fragment(next, b_row + j * 16);
                 if constexpr (j == 0) read_scales(next);
             }
-            if constexpr (t >= 2) scale_in(std::integral_constant<int, t - 2>{}, s[(t - 2) / TN]);
-            else scale_in(std::integral_constant<int, TT - 2 + t>{}, s[TM - 1]);
+            if constexpr (t >= DELAY) scale_in(std::integral_constant<int, t - DELAY>{}, s[(t - DELAY) / TN]);
+            else scale_in(std::integral_constant<int, TT - DELAY + t>{}, s[(TT - DELAY + t) / TN]);
             constexpr int D = i == TM - 1 ? j * PER : EARLY + t * PER;
             if constexpr (i == TM - 1 ? FIRST : REST)
                 unrolled<(D < C::LPT ? D : C::LPT), (D + PER < C::LPT ? D + PER : C::LPT)>(
@@ -277,8 +281,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         first_operands(sub);
         k_block(sub, sub, 0, 0, 0, no, no, no);
     }
-    scale_in(std::integral_constant<int, TT - 2>{}, s[TM - 1]);
-    scale_in(std::integral_constant<int, TT - 1>{}, s[TM - 1]);
+    unrolled<TT - DELAY, TT>([&](auto t_c) __attribute__((always_inline)) { scale_in(t_c, s[decltype(t_c)::value / TN]); });
     if constexpr (KS > 1) {  // the groups' sums, in order
         v4f* sums = reinterpret_cast<v4f*>(smem) + ((group - 1) * (NG / kWave) + wave) * TT * kWave + lane;
         lds_barrier();  // every wavefront has read its last operands
@@ -442,17 +445,12 @@ int launch_block_tile(int cfg, int splits, const BlockArgs& g, hipStream_t st) {
     switch (cfg) {
         case 0: return launch_cfg<TileCfg<256, 256, 2, 4, 2, 1>>(g, splits, st);
         case 1: return launch_cfg<TileCfg<128, 256, 2, 4, 3, 1>>(g, splits, st);
-        case 2: return launch_cfg<TileCfg<64, 128, 2, 2, 3, 1>>(g, splits, st);
-        case 3: return launch_cfg<TileCfg<32, 128, 1, 4, 3, 1>>(g, splits, st);
-        case 4: return launch_cfg<TileCfg<64, 256, 2, 4, 3, 1>>(g, splits, st);
+        case 2: return launch_cfg<TileCfg<64, 256, 2, 4, 3, 1>>(g, splits, st);
+        case 3: return launch_cfg<TileCfg<64, 128, 2, 2, 3, 1>>(g, splits, st);
+        case 4: return launch_cfg<TileCfg<32, 128, 1, 4, 3, 1>>(g, splits, st);
         case 5: return launch_cfg<TileCfg<64, 64, 2, 2, 4, 1>>(g, splits, st);
-        case 6: return launch_cfg<TileCfg<128, 128, 2, 2, 2, 2>>(g, splits, st);
-        case 7: return launch_cfg<TileCfg<64, 128, 2, 2, 3, 2>>(g, splits, st);
-        case 8: return launch_cfg<TileCfg<64, 64, 2, 2, 4, 2>>(g, splits, st);
-        case 9: return launch_cfg<TileCfg<32, 128, 1, 4, 3, 2>>(g, splits, st);
-        case 10: return launch_cfg<TileCfg<64, 128, 2, 2, 2, 2>>(g, splits, st);
-        case 11: return launch_cfg<TileCfg<64, 128, 2, 2, 2, 3>>(g, splits, st);
-        case 12: return launch_cfg<TileCfg<64, 64, 2, 2, 2, 4>>(g, splits, st);
+        case 6: return launch_cfg<TileCfg<64, 128, 2, 2, 3, 2>>(g, splits, st);
+        case 7: return launch_cfg<TileCfg<64, 64, 2, 2, 4, 2>>(g, splits, st);
     }
     return LLMQ_ERR_SHAPE;
 }

@@ -489,6 +489,8 @@ void block_gemm(const void* q, const float* a_scale, const Tensor& w, const Tens
                               bytes ? ws.data_ptr() : nullptr, (size_t)bytes, l.stream),
           "llmq_gemm_fp8_block");
 }
+bool is_matrix(const Tensor& t, int64_t rows, int64_t cols) { return t.dim() == 2 && t.size(0) == rows && t.size(1) == cols; }
+// codes and scales of any rows, weights [N, K]
 std::optional<Tensor> fp8_block(const Tensor& q, const Tensor& a_scale, const Tensor& w, const Tensor& w_scale, const std::optional<Tensor>& bias,
                                 at::ScalarType odt) {
     const Rows r = rows_of(q);
@@ -499,6 +501,15 @@ std::optional<Tensor> fp8_block(const Tensor& q, const Tensor& a_scale, const Te
     Tensor out = make(out_size(q, w.size(0)), odt, q.device());
     block_gemm(q.data_ptr(), (const float*)a_scale.data_ptr(), w, w_scale, bias, r.M, r.K, out, l);
     return out;
+}
+// the op: matrices only, the weight as the [K, N] view of [N, K] rows
+std::optional<Tensor> fp8_blockwise(const Tensor& q, const Tensor& wt, const std::optional<Tensor>& bias, const Tensor& a_scale, const Tensor& w_scale,
+                                    at::ScalarType odt) {
+    if (!wt.defined() || wt.layout() != at::kStrided || wt.dim() != 2 || wt.stride(0) != 1 || q.dim() != 2 ||
+        !is_matrix(a_scale, q.size(0), blocks128(q.size(1))) || !is_matrix(w_scale, blocks128(wt.size(1)), blocks128(wt.size(0))) ||
+        (bias && bias->dim() != 1))
+        return std::nullopt;
+    return fp8_block(q, a_scale, wt.t(), w_scale, bias, odt);
 }
 // activations not quantized yet; out has their dtype
 std::optional<Tensor> fp8_block_linear(const Tensor& x, const Tensor& w, const Tensor& w_scale, const std::optional<Tensor>& bias) {
@@ -525,7 +536,8 @@ std::optional<Tensor> fp8_block_grouped(const Tensor& x, const std::optional<Ten
         !plain_on(w, dev) || !aligned(w))
         return std::nullopt;
     const int64_t E = w.size(0), N = w.size(1);
-    if (!scale_ok(w_scale, dev, E * blocks128(N) * blocks128(r.K)) || !block_bias_ok(bias, dev, E * N) || offsets.dim() != 1 ||
+    if (w_scale.dim() != 3 || w_scale.size(0) != E || w_scale.size(1) != blocks128(N) || !scale_ok(w_scale, dev, E * blocks128(N) * blocks128(r.K)) ||
+        (bias && !is_matrix(*bias, E, N)) || (a_scale && !is_matrix(*a_scale, r.M, blocks128(r.K))) || !block_bias_ok(bias, dev, E * N) || offsets.dim() != 1 ||
         offsets.numel() != E + 1 || offsets.scalar_type() != at::kInt || !plain_on(offsets, dev) ||
         (given && (given->scalar_type() != odt || given->dim() != 2 || given->size(0) != r.M || given->size(1) != N || !plain_on(*given, dev))))
         return std::nullopt;
@@ -738,6 +750,16 @@ LLMQ_PY(py_fp8_block, 6)
     return wrap(std::move(y));
 LLMQ_PY_END
 
+LLMQ_PY(py_fp8_blockwise, 6)
+    const Tensor &q = in.tensor(0), &w = in.tensor(1), &a = in.tensor(3), &s = in.tensor(4);
+    const auto bias = in.optional(2);
+    const at::ScalarType odt = in.dtype(5);
+    LLMQ_PY_TENSORS;
+    std::optional<Tensor> y;
+    { NoGil g; y = fp8_blockwise(q, w, bias, a, s, odt); }
+    return wrap(std::move(y));
+LLMQ_PY_END
+
 LLMQ_PY(py_fp8_block_linear, 4)
     const Tensor &x = in.tensor(0), &w = in.tensor(1), &s = in.tensor(2);
     const auto bias = in.optional(3);
@@ -794,6 +816,7 @@ PyMethodDef methods[] = {LLMQ_FAST("sq_tensor", py_sq_tensor),
                          LLMQ_FAST("quant_groups", py_quant_groups),
                          LLMQ_FAST("add_norm", py_add_norm),
                          LLMQ_FAST("fp8_block", py_fp8_block),
+                         LLMQ_FAST("fp8_blockwise", py_fp8_blockwise),
                          LLMQ_FAST("fp8_block_linear", py_fp8_block_linear),
                          LLMQ_FAST("fp8_block_grouped", py_fp8_block_grouped),
                          LLMQ_FAST("awq_counters", py_awq_counters),

@@ -85,11 +85,13 @@ def _same_rows(t: torch.Tensor, x: torch.Tensor, what: str) -> torch.Tensor:
     return _as_rows(t)
 
 
-@torch.no_grad()
 def _add_norm(x, residual, weight, eps, out, return_normed=False, inplace=False):
     y = host().add_norm(x, residual, weight, eps, out, return_normed, inplace)
-    if y is not None:
-        return y
+    return _add_norm_general(x, residual, weight, eps, out, return_normed, inplace) if y is None else y
+
+
+@torch.no_grad()
+def _add_norm_general(x, residual, weight, eps, out, return_normed, inplace):
     if inplace and residual is None:
         raise RuntimeError("inplace needs a residual")
     rows = _as_rows(x)

@@ -144,14 +144,16 @@ def static_per_tensor_quantize(tensor: torch.Tensor, scale) -> torch.Tensor:
     return q.view(*tensor.shape)
 
 
-@torch.no_grad()
 def per_group_quantize(tensor: torch.Tensor):
     """One scale per token and 128 channels (the last group of a row may be short), the activations of a block-scaled product:
     scale = max(absmax, 1e-12) / 448 and codes = e4m3fn(tensor / scale), in fp32.
     -> (float8_e4m3fn tensor like `tensor`, fp32 scales [.., ceil(K / 128)]).  No counterpart in the reference."""
     out = host().quant_groups(tensor)
-    if out is not None:
-        return out
+    return _per_group_quantize_general(tensor) if out is None else out
+
+
+@torch.no_grad()
+def _per_group_quantize_general(tensor):
     if tensor.dim() < 1:
         raise RuntimeError("per_group_quantize needs a tensor with a last dimension")
     groups = (tensor.shape[-1] + 127) // 128

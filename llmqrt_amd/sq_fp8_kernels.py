@@ -216,7 +216,6 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     return t.clone() if t.data_ptr() % 16 else t
 
 
-@torch.no_grad()
 def f8f8_blockwise(XQ: torch.Tensor, WQ: torch.Tensor, bias: Optional[torch.Tensor], x_scale: torch.Tensor, w_scale: torch.Tensor,
                    dtype_str: str = "bfloat16") -> torch.Tensor:
     """out[m, n] = dtype( sum_b x_scale[m, b] * w_scale[n // 128, b] * sum_{k in block b of 128} XQ[m, k] * WQ[k, n] + bias[n] ), fp32 sums.
@@ -224,12 +223,14 @@ def f8f8_blockwise(XQ: torch.Tensor, WQ: torch.Tensor, bias: Optional[torch.Tens
     ``XQ``: e4m3fn [M, K] with fp32 scales [M, ceil(K / 128)] (quantize.per_group_quantize); ``WQ``: the .t() view of an e4m3fn
     [N, K] row-major tensor with fp32 scales [ceil(N / 128), ceil(K / 128)] (quantize.quantize_weight_per_block); ``bias``: [N] bf16, fp16 or
     fp32; ``dtype_str``: "bfloat16" or "float16".  Sums are taken in a fixed order that follows from the sizes."""
+    y = host().fp8_blockwise(XQ, WQ, bias, x_scale, w_scale, _STR_TO_DTYPE.get(dtype_str))
+    return _f8f8_blockwise_general(XQ, WQ, bias, x_scale, w_scale, dtype_str) if y is None else y
+
+
+@torch.no_grad()
+def _f8f8_blockwise_general(XQ, WQ, bias, x_scale, w_scale, dtype_str):
     what = "f8f8_blockwise"
     out_dtype = _block_out_dtype(dtype_str, what)
-    if XQ.dim() == 2 and WQ.dim() == 2 and x_scale.shape == (XQ.shape[0], _blocks(XQ.shape[1])) and w_scale.shape == (_blocks(WQ.shape[1]), _blocks(WQ.shape[0])):
-        y = host().fp8_block(XQ, x_scale, WQ.t(), w_scale, bias, out_dtype)
-        if y is not None:
-            return y
     _check(XQ.dtype == torch.float8_e4m3fn and WQ.dtype == torch.float8_e4m3fn, f"{what}: XQ and WQ must be float8_e4m3fn")
     M, N, K = _check_operands(XQ, WQ, what)
     _check_bias(bias, WQ, N, (torch.bfloat16, torch.float16, torch.float32), what)
@@ -243,7 +244,6 @@ def f8f8_blockwise(XQ: torch.Tensor, WQ: torch.Tensor, bias: Optional[torch.Tens
     return y
 
 
-@torch.no_grad()
 def f8f8_blockwise_grouped(XQ: torch.Tensor, WQ: torch.Tensor, bias: Optional[torch.Tensor], x_scale: torch.Tensor, w_scale: torch.Tensor,
                            offsets: torch.Tensor, dtype_str: str = "bfloat16", out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """f8f8_blockwise by experts: rows offsets[e] .. offsets[e + 1] - 1 of ``XQ`` [M, K] (sorted by expert) with the weights of expert e.
@@ -252,6 +252,12 @@ def f8f8_blockwise_grouped(XQ: torch.Tensor, WQ: torch.Tensor, bias: Optional[to
     on the GPU, ascending (values outside [0, M] are taken as the nearest inside).  An expert may have no rows.  Nothing is read back by
     the host, so a captured call follows the offsets of its replay.  Rows that belong to no expert are not written: they keep what ``out`` [M, N] holds,
     and are undefined in a new tensor."""
+    y = None if x_scale is None else host().fp8_block_grouped(XQ, x_scale, WQ, w_scale, bias, offsets, _STR_TO_DTYPE.get(dtype_str), out)
+    return _f8f8_blockwise_grouped_general(XQ, WQ, bias, x_scale, w_scale, offsets, dtype_str, out) if y is None else y
+
+
+@torch.no_grad()
+def _f8f8_blockwise_grouped_general(XQ, WQ, bias, x_scale, w_scale, offsets, dtype_str, out):
     what = "f8f8_blockwise_grouped"
     out_dtype = _block_out_dtype(dtype_str, what)
     _check(XQ.is_cuda, f"{what}: XQ must be a GPU tensor")
