@@ -28,28 +28,27 @@ __device__ __forceinline__ void expert_rows(const BlockArgs& g, int e, int& firs
     last = min(max(g.offsets[e + 1], first), g.M);
 }
 
-struct BlockTile { int bm, bn; };  // tokens, channels of a block
+struct BlockTile { int bm, bn, ks; };  // tokens, channels, groups of wavefronts of a block
 constexpr BlockTile kBlockTiles[] = {
-    {256, 256},  // 0: 8 wavefronts of 128 x 64
-    {128, 256},  // 1: 8 wavefronts of 64 x 64
-    {64, 256},  // 2: 8 wavefronts of 32 x 64
-    {64, 128},  // 3: 4 wavefronts of 32 x 64
-    {32, 128},  // 4: 4 wavefronts of 32 x 32
-    {64, 64},  // 5: 4 wavefronts of 32 x 32
-    {64, 128},  // 6: 2 groups of 4 wavefronts of 32 x 64
-    {64, 64},  // 7: 2 groups of 4 wavefronts of 32 x 32
+    {256, 256, 1},  // 0: 8 wavefronts of 128 x 64
+    {128, 256, 1},  // 1: 8 wavefronts of 64 x 64
+    {64, 256, 1},  // 2: 8 wavefronts of 32 x 64
+    {64, 128, 1},  // 3: 4 wavefronts of 32 x 64
+    {32, 128, 1},  // 4: 4 wavefronts of 32 x 32
+    {64, 64, 1},  // 5: 4 wavefronts of 32 x 32
+    {64, 128, 2},  // 6: 2 groups of 4 wavefronts of 32 x 64
+    {64, 64, 2},  // 7: 2 groups of 4 wavefronts of 32 x 32
 };
 constexpr int kNumBlockTiles = sizeof(kBlockTiles) / sizeof(kBlockTiles[0]);
 
 // Variants of gemm_block_rows.hip: 16-channel and 16-token tiles of a block, blocks of K per wavefront and stage, stages; several groups of channels
 // per block.  They take up to 16 MT tokens.
-#define LLMQ_BLOCK_ROWS(V)                                                                                 \
-    V(0, 1, 1, 1, 4, false) V(1, 1, 1, 2, 4, false) V(2, 2, 1, 1, 4, false) V(3, 1, 2, 1, 3, false)         \
-    V(4, 2, 2, 1, 3, false) V(5, 4, 2, 1, 3, false) V(6, 1, 4, 1, 3, false) V(7, 2, 4, 1, 3, false)         \
-    V(8, 4, 1, 1, 3, true) V(9, 2, 1, 1, 3, true) V(10, 1, 3, 1, 4, false) V(11, 2, 3, 1, 3, false)
-struct BlockRows { int t, mt; };
+#define LLMQ_BLOCK_ROWS(V)                                                                              \
+    V(0, 1, 1, 1, 4, false) V(1, 1, 1, 2, 4, false) V(2, 1, 2, 1, 3, false) V(3, 1, 3, 1, 4, false)      \
+    V(4, 2, 3, 1, 3, false) V(5, 1, 4, 1, 3, false) V(6, 4, 1, 1, 3, true)
+struct BlockRows { int t, mt, steps; };
 constexpr BlockRows kBlockRows[] = {
-#define LLMQ_BLOCK_ROWS_SHAPE(I, T, MT, STEPS, NS, MANY) {T, MT},
+#define LLMQ_BLOCK_ROWS_SHAPE(I, T, MT, STEPS, NS, MANY) {T, MT, STEPS},
     LLMQ_BLOCK_ROWS(LLMQ_BLOCK_ROWS_SHAPE)
 #undef LLMQ_BLOCK_ROWS_SHAPE
 };

@@ -1,42 +1,89 @@
 // Block-scaled fp8 products: argument checks, plan and entry points (kernels: gemm_block_tile.hip, gemm_block_rows.hip).
 #include <algorithm>
+#include <cmath>
 
 #include "gemm_block.h"
 
 namespace llmq {
 namespace {
 
+// cfg: a tile configuration, or kRowsCfg + a variant of the row-streaming kernel
 struct BlockPlan { int cfg, splits, blocks_per_split; };
+constexpr int kRowsCfg = kNumBlockTiles;
 thread_local int forced_cfg = -1, forced_splits = 0;
 
-BlockPlan split_plan(int cfg, int splits, int KB) {
-    const int per = (KB + splits - 1) / splits;
-    return {cfg, (KB + per - 1) / per, per};
+// What a launch takes, in us, as a rule of the sizes alone:
+//   start + max(stream, loop) + min(stream, loop) / 4 + what a K split adds
+// stream: the operands once at 5.6 TB/s.  loop: steps along K times what one takes, from `alone` (a few blocks on the chip) to `alone` + `crowd` (one
+// on every CU), or `full` per block of a CU where there are more: a last round that is not full costs as the fourth root of what it holds.  A split
+// adds a launch and its sums' way out and back.  Fitted to 3300 random sizes (1-8192 tokens, 128-37888 channels, K 512-18944), every
+// configuration and split timed with the weights out of HBM: the choice is 2.2 % (2.9 % up to 64 tokens) slower than the fastest of the
+// size on average, 12 % (17 %) in the worst 5 % of the sizes.  By experts, 700 sizes, the same constants: 2.3 %, 11 %.
+struct Cost { float start, alone, full, crowd; };
+constexpr Cost kTileCost[kNumBlockTiles] = {{5.84, 0.008, 1.97, 1.66}, {5.08, 0.774, 1.12, 0.151}, {4.39, 0.402, 0.765, 0.367}, {4.13, 0.375, 0.437, 0.087}, {3.47, 0.273, 0.346, 0.109}, {3.92, 0.241, 0.298, 0.046}, {5.65, 0.311, 0.861, 0.181}, {4.41, 0.318, 0.603, 0.1}};
+constexpr Cost kRowsCost[kNumBlockRows] = {{2.75, 0.34, 0.298, 0}, {3.02, 0.475, 0.589, 0.164}, {2.92, 0.401, 0.357, 0.016}, {3.09, 0, 0.559, 0.507}, {3.29, 0.176, 0.749, 0.586}, {3.19, 0, 0.686, 0.622}, {3.37, 0.022, 0.633, 0.029}};
+
+float cost_us(const Cost& c, double blocks, double steps, double bytes) {
+    const float rounds = (float)(blocks / 256.0), whole = floorf(rounds), rest = rounds - whole;
+    const float loop = (float)steps * std::max(c.alone + c.crowd * std::min(rounds, 1.f), c.full * (whole + sqrtf(sqrtf(rest))));
+    const float stream = (float)(bytes / 5.6e6);
+    return c.start + std::max(stream, loop) + 0.25f * std::min(stream, loop);
 }
 
-// cfg: a tile configuration, or kRowsCfg + a variant of the row-streaming kernel
-constexpr int kRowsCfg = kNumBlockTiles;
-bool rows_take(int cfg, int64_t M) { return M <= 16 * kBlockRows[cfg - kRowsCfg].mt; }
+BlockPlan search(int64_t M, int64_t N, int64_t K) {
+    const int KB = (int)((K + kScaleBlock - 1) / kScaleBlock);
+    BlockPlan best = {0, 1, KB};
+    float least = 3e38f;
+    for (int c = 0; c < kNumBlockTiles; c++) {
+        const BlockTile& t = kBlockTiles[c];
+        const double tiles = (double)((M + t.bm - 1) / t.bm) * (double)((N + t.bn - 1) / t.bn);
+        for (int s : {1, 2, 3, 4, 6, 8}) {
+            if (s > 1 && (KB / s < 4 || tiles * s > (t.bm * t.bn > 64 * 128 ? 300 : 600))) break;
+            const int per = (KB + s - 1) / s, splits = (KB + per - 1) / per;
+            float us = cost_us(kTileCost[c], tiles * splits, (per + t.ks - 1) / t.ks, (double)N * K + (double)M * K);
+            if (splits > 1) us += 3.f + (float)(splits * (double)M * N * 8 / 6e6);
+            if (us < least) least = us, best = {c, splits, per};
+        }
+    }
+    for (int v = 0; v < kNumBlockRows; v++) {
+        const BlockRows& r = kBlockRows[v];
+        if (M > 16 * r.mt) continue;
+        const float us = cost_us(kRowsCost[v], (double)((N + 16 * r.t - 1) / (16 * r.t)), (KB + 4 * r.steps - 1) / (4 * r.steps), (double)N * K);
+        if (us < least) least = us, best = {kRowsCfg + v, 1, KB};
+    }
+    return best;
+}
 
 BlockPlan plan(int64_t M, int64_t N, int64_t K) {
     const int KB = (int)((K + kScaleBlock - 1) / kScaleBlock);
-    if (forced_cfg >= 0 && (forced_cfg < kRowsCfg || rows_take(forced_cfg, M)))
-        return forced_cfg >= kRowsCfg ? BlockPlan{forced_cfg, 1, KB} : split_plan(forced_cfg, std::max(1, std::min(forced_splits, KB)), KB);
-    if (M <= 16) return {kRowsCfg + (N > 8192 ? 8 : 0), 1, KB};
-    if (M <= 32) return {kRowsCfg + (N > 8192 ? 5 : 3), 1, KB};
-    if (M <= 48) return {kRowsCfg + (N > 8192 ? 11 : 10), 1, KB};
-    if (M <= 64) return {kRowsCfg + (N > 8192 ? 7 : 6), 1, KB};
-    const int cfg = M <= 32 ? 4 : M <= 64 ? 3 : M <= 1024 ? 2 : 0;
-    const BlockTile t = kBlockTiles[cfg];
-    const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
-    const int splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / tiles, KB / 8));
-    return split_plan(cfg, splits, KB);
+    if (forced_cfg >= kRowsCfg && M <= 16 * kBlockRows[forced_cfg - kRowsCfg].mt) return {forced_cfg, 1, KB};
+    if (forced_cfg >= 0 && forced_cfg < kRowsCfg) {
+        const int per = (KB + std::max(1, std::min(forced_splits, KB)) - 1) / std::max(1, std::min(forced_splits, KB));
+        return {forced_cfg, (KB + per - 1) / per, per};
+    }
+    thread_local int64_t of[3] = {0, 0, 0};  // the last size
+    thread_local BlockPlan last;
+    if (of[0] != M || of[1] != N || of[2] != K) last = search(M, N, K), of[0] = M, of[1] = N, of[2] = K;
+    return last;
 }
 
-int plan_grouped(int64_t rows, int64_t experts) {
+// The host knows the rows of all experts together, not each one's: every expert that may have rows is taken to end with half a tile.
+int plan_grouped(int64_t rows, int64_t experts, int64_t N, int64_t K) {
     if (forced_cfg >= 0 && forced_cfg < kRowsCfg) return forced_cfg;
-    const int64_t each = rows / experts;
-    return each <= 32 ? 4 : each <= 64 ? 3 : each <= 256 ? 2 : 0;
+    thread_local int64_t of[4] = {0, 0, 0, 0};
+    thread_local int last;
+    if (of[0] == rows && of[1] == experts && of[2] == N && of[3] == K) return last;
+    const int KB = (int)((K + kScaleBlock - 1) / kScaleBlock);
+    const double used = (double)std::min(rows, experts);
+    float least = 3e38f;
+    for (int c = 0; c < kNumBlockTiles; c++) {
+        const BlockTile& t = kBlockTiles[c];
+        const double tiles = std::max(used, (double)rows / t.bm + 0.5 * used) * (double)((N + t.bn - 1) / t.bn);
+        const float us = cost_us(kTileCost[c], tiles, (KB + t.ks - 1) / t.ks, used * (double)N * K + (double)rows * K);
+        if (us < least) least = us, last = c;
+    }
+    of[0] = rows, of[1] = experts, of[2] = N, of[3] = K;
+    return last;
 }
 
 size_t partial_bytes(const BlockPlan& p, int64_t M, int64_t N) { return p.splits > 1 ? (size_t)p.splits * (size_t)M * (size_t)N * 4 : 0; }
@@ -97,7 +144,7 @@ extern "C" int llmq_gemm_fp8_block_grouped(const uint8_t* A, int64_t lda, const 
     g.lda = lda, g.ldb = K, g.ldo = ldo, g.M = (int)M, g.N = (int)N, g.K = (int)K;
     g.KB = (int)((K + kScaleBlock - 1) / kScaleBlock), g.NB = (int)((N + kScaleBlock - 1) / kScaleBlock), g.experts = (int)experts;
     g.bias_dtype = bias_dtype, g.out_dtype = out_dtype;
-    return launch_block_tile(plan_grouped(M, experts), 1, g, (hipStream_t)stream);
+    return launch_block_tile(plan_grouped(M, experts, N, K), 1, g, (hipStream_t)stream);
 }
 
 extern "C" int llmq_gemm_fp8_block_force_plan(int cfg, int splits) {
