@@ -24,7 +24,7 @@ from typing import Iterable
 import torch
 from torch import nn
 
-from .linear import SqW8A8BBF16OBF16PerChannel, method_to_linear
+from .linear import FP8BlockLinear, SqW8A8BBF16OBF16PerChannel, method_to_linear
 
 
 @dataclass
@@ -86,10 +86,13 @@ def replace_linears(model: nn.Module, cfg: QuantConfig, dtype=torch.bfloat16) ->
     module of the configured kind (buffers allocated, not filled).  -> the names that were replaced.
 
     ``quant_method == "sq"`` with ``per_tensor == False`` selects the per-token x per-channel SmoothQuant module,
-    which the reference declares but does not implement."""
+    which the reference declares but does not implement; ``quant_method == "fp8_dynamic_quant"`` with ``q_group_size == 128`` the block-scaled FP8
+    module, whose weight is stored in e4m3fn with a scale per 128 x 128 block (the reference's FP8 modules refuse any group size but 0)."""
     kind = method_to_linear[cfg.quant_method]
     if cfg.quant_method == "sq" and not cfg.per_tensor:
         kind = SqW8A8BBF16OBF16PerChannel
+    if cfg.quant_method == "fp8_dynamic_quant" and cfg.q_group_size == 128:
+        kind = FP8BlockLinear
     skip = cfg.modules_to_not_convert or []
     targets = [(n, m) for n, m in model.named_modules()
                if isinstance(m, nn.Linear) and n and not any(key in n for key in skip)]
@@ -148,5 +151,5 @@ def load_quantized_weights(model: nn.Module, path: str, device=None) -> tuple[li
 
 
 def named_quantized_linears(model: nn.Module) -> Iterable[tuple[str, nn.Module]]:
-    kinds = tuple(set(method_to_linear.values()) | {SqW8A8BBF16OBF16PerChannel})
+    kinds = tuple(set(method_to_linear.values()) | {SqW8A8BBF16OBF16PerChannel, FP8BlockLinear})
     return ((n, m) for n, m in model.named_modules() if isinstance(m, kinds))

@@ -14,19 +14,19 @@ thread_local int forced_cfg = -1, forced_splits = 0;
 
 // What a launch takes, in us, as a rule of the sizes alone:
 //   start + max(stream, loop) + min(stream, loop) / 4 + what a K split adds
-// stream: the operands once at 5.6 TB/s.  loop: steps along K times what one takes, from `alone` (a few blocks on the chip) to `alone` + `crowd` (one
-// on every CU), or `full` per block of a CU where there are more: a last round that is not full costs as the fourth root of what it holds.  A split
-// adds a launch and its sums' way out and back.  Fitted to 3300 random sizes (1-8192 tokens, 128-37888 channels, K 512-18944), every
-// configuration and split timed with the weights out of HBM: the choice is 2.2 % (2.9 % up to 64 tokens) slower than the fastest of the
-// size on average, 12 % (17 %) in the worst 5 % of the sizes.  By experts, 700 sizes, the same constants: 2.3 %, 11 %.
+// stream: the operands once at 5.8 TB/s.  loop: steps along K times what one takes, from `alone` (a few blocks on the chip) to `alone` + `crowd` (one
+// on every CU), or `full` per block of a CU where there are more: a last round that is not full costs as the fourth root of what it holds (rows: all of it).  A split
+// adds a launch and its sums' way out and back.  Fitted to 4300 random sizes (1-8192 tokens, 128-37888 channels, K 512-18944), every
+// configuration and split timed with the weights out of HBM: the choice is 2.0 % (2.5 % up to 64 tokens) slower than the fastest of the
+// size on average, 11 % (16 %) in the worst 5 % of the sizes.  By experts, 1200 sizes, the same constants: 2.8 %, 12 %.
 struct Cost { float start, alone, full, crowd; };
-constexpr Cost kTileCost[kNumBlockTiles] = {{5.84, 0.008, 1.97, 1.66}, {5.08, 0.774, 1.12, 0.151}, {4.39, 0.402, 0.765, 0.367}, {4.13, 0.375, 0.437, 0.087}, {3.47, 0.273, 0.346, 0.109}, {3.92, 0.241, 0.298, 0.046}, {5.65, 0.311, 0.861, 0.181}, {4.41, 0.318, 0.603, 0.1}};
-constexpr Cost kRowsCost[kNumBlockRows] = {{2.75, 0.34, 0.298, 0}, {3.02, 0.475, 0.589, 0.164}, {2.92, 0.401, 0.357, 0.016}, {3.09, 0, 0.559, 0.507}, {3.29, 0.176, 0.749, 0.586}, {3.19, 0, 0.686, 0.622}, {3.37, 0.022, 0.633, 0.029}};
+constexpr Cost kTileCost[kNumBlockTiles] = {{4.99, 0, 1.95, 1.56}, {4.74, 0.755, 1.11, 0.187}, {4.49, 0.333, 0.742, 0.41}, {4.19, 0.347, 0.427, 0.114}, {3.57, 0.279, 0.345, 0.096}, {3.94, 0.233, 0.292, 0.038}, {5.82, 0.368, 0.841, 0.427}, {4.54, 0.292, 0.611, 0.02}};
+constexpr Cost kRowsCost[kNumBlockRows] = {{2.76, 0.34, 0.305, 0}, {3.03, 0.473, 0.595, 0.149}, {2.92, 0.4, 0.364, 0.014}, {3.09, 0, 0.557, 0.545}, {3.25, 0.584, 0.764, 0.205}, {3.17, 0.139, 0.689, 0.15}, {3.29, 0.046, 0.666, 0.081}};
 
-float cost_us(const Cost& c, double blocks, double steps, double bytes) {
+float cost_us(const Cost& c, double blocks, double steps, double bytes, bool rows) {
     const float rounds = (float)(blocks / 256.0), whole = floorf(rounds), rest = rounds - whole;
-    const float loop = (float)steps * std::max(c.alone + c.crowd * std::min(rounds, 1.f), c.full * (whole + sqrtf(sqrtf(rest))));
-    const float stream = (float)(bytes / 5.6e6);
+    const float loop = (float)steps * std::max(c.alone + c.crowd * std::min(rounds, 1.f), c.full * (whole + (rows ? ceilf(rest) : sqrtf(sqrtf(rest)))));
+    const float stream = (float)(bytes / 5.8e6);
     return c.start + std::max(stream, loop) + 0.25f * std::min(stream, loop);
 }
 
@@ -40,15 +40,15 @@ BlockPlan search(int64_t M, int64_t N, int64_t K) {
         for (int s : {1, 2, 3, 4, 6, 8}) {
             if (s > 1 && (KB / s < 4 || tiles * s > (t.bm * t.bn > 64 * 128 ? 300 : 600))) break;
             const int per = (KB + s - 1) / s, splits = (KB + per - 1) / per;
-            float us = cost_us(kTileCost[c], tiles * splits, (per + t.ks - 1) / t.ks, (double)N * K + (double)M * K);
-            if (splits > 1) us += 3.f + (float)(splits * (double)M * N * 8 / 6e6);
+            float us = cost_us(kTileCost[c], tiles * splits, (per + t.ks - 1) / t.ks, (double)N * K + (double)M * K, false);
+            if (splits > 1) us += 3.f + (float)(splits * (double)M * N * 8 / 5e6);
             if (us < least) least = us, best = {c, splits, per};
         }
     }
     for (int v = 0; v < kNumBlockRows; v++) {
         const BlockRows& r = kBlockRows[v];
         if (M > 16 * r.mt) continue;
-        const float us = cost_us(kRowsCost[v], (double)((N + 16 * r.t - 1) / (16 * r.t)), (KB + 4 * r.steps - 1) / (4 * r.steps), (double)N * K);
+        const float us = cost_us(kRowsCost[v], (double)((N + 16 * r.t - 1) / (16 * r.t)), (KB + 4 * r.steps - 1) / (4 * r.steps), (double)N * K, true);
         if (us < least) least = us, best = {kRowsCfg + v, 1, KB};
     }
     return best;
@@ -79,7 +79,7 @@ int plan_grouped(int64_t rows, int64_t experts, int64_t N, int64_t K) {
     for (int c = 0; c < kNumBlockTiles; c++) {
         const BlockTile& t = kBlockTiles[c];
         const double tiles = std::max(used, (double)rows / t.bm + 0.5 * used) * (double)((N + t.bn - 1) / t.bn);
-        const float us = cost_us(kTileCost[c], tiles, (KB + t.ks - 1) / t.ks, used * (double)N * K + (double)rows * K);
+        const float us = cost_us(kTileCost[c], tiles, (KB + t.ks - 1) / t.ks, used * (double)N * K + (double)rows * K, false);
         if (us < least) least = us, last = c;
     }
     of[0] = rows, of[1] = experts, of[2] = N, of[3] = K;

@@ -56,10 +56,13 @@ __device__ __forceinline__ int wave_prefix(int v) {
     return v;
 }
 
-// flat id -> (tile of rows, tile of channels): contiguous ranges per XCD, then groups of kGroupM tiles of rows
-__device__ __forceinline__ void tile_of(int bid, int nblk, int tiles_m, int tiles_n, int& tm, int& tn) {
+// flat block id -> place in the order of tiles: a contiguous range per XCD
+__device__ __forceinline__ int place_of(int bid, int nblk) {
     const int q = nblk / kNumXcd, r = nblk % kNumXcd, xcd = bid % kNumXcd, local = bid / kNumXcd;
-    const int pid = xcd < r ? xcd * (q + 1) + local : r * (q + 1) + (xcd - r) * q + local;
+    return xcd < r ? xcd * (q + 1) + local : r * (q + 1) + (xcd - r) * q + local;
+}
+// place in one matrix's order -> (tile of rows, tile of channels): groups of kGroupM tiles of rows
+__device__ __forceinline__ void tile_of(int pid, int tiles_m, int tiles_n, int& tm, int& tn) {
     const int width = kGroupM * tiles_n, group = pid / width, first = group * kGroupM, size = min(tiles_m - first, kGroupM);
     tm = first + (pid % width) % size;
     tn = (pid % width) / size;
@@ -78,7 +81,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     int tm, tn, row0, row_end, expert = 0;
     if (!GROUPED) {
         const int tiles_m = (g.M + C::BM - 1) / C::BM;
-        tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
+        tile_of(place_of(blockIdx.x, gridDim.x), tiles_m, tiles_n, tm, tn);
         row0 = tm * C::BM, row_end = g.M;
     } else {
         // the experts' tiles of rows, counted by every wavefront for itself: 64 experts at a time
@@ -91,23 +94,25 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         total = __builtin_amdgcn_readfirstlane(total);
         const int64_t nblk = min((int64_t)gridDim.x, (int64_t)total * tiles_n);
         if (blockIdx.x >= nblk) return;  // block-uniform
-        tile_of(blockIdx.x, (int)nblk, total, tiles_n, tm, tn);
-        int before = 0;
+        // one expert's tiles after the other's, so that neighbours share its weights
+        const int pid = place_of(blockIdx.x, (int)nblk), flat = pid / tiles_n;
+        int before = 0, tiles = 1;
         row0 = row_end = 0;
         for (int e0 = 0; e0 < g.experts; e0 += kWave) {
             int first = 0, last = 0;
             if (e0 + lane < g.experts) expert_rows(g, e0 + lane, first, last);
             const int mine = (last - first + C::BM - 1) / C::BM, upto = before + wave_prefix(mine);
-            const uint64_t has = __ballot(tm >= upto - mine && tm < upto);
+            const uint64_t has = __ballot(flat >= upto - mine && flat < upto);
             if (has) {
                 const int at = __ffsll((unsigned long long)has) - 1;
                 expert = e0 + at;
-                row0 = __shfl(first, at) + (tm - __shfl(upto - mine, at)) * C::BM;
-                row_end = __shfl(last, at);
+                row0 = __shfl(first, at), row_end = __shfl(last, at), tiles = __shfl(mine, at), before = __shfl(upto - mine, at);
                 break;
             }
             before = __shfl(upto, kWave - 1);
         }
+        tile_of(pid - __builtin_amdgcn_readfirstlane(before) * tiles_n, __builtin_amdgcn_readfirstlane(tiles), tiles_n, tm, tn);
+        row0 += tm * C::BM;
         expert = __builtin_amdgcn_readfirstlane(expert);
         row0 = __builtin_amdgcn_readfirstlane(row0);
         row_end = __builtin_amdgcn_readfirstlane(row_end);
@@ -239,34 +244,38 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
 #pragma unroll
     for (int i = 0; i < TM; i++) s[i] = 0.f;
 
-    unrolled<0, NS - 1>([&](auto n_c) __attribute__((always_inline)) {
-        constexpr int n = decltype(n_c)::value;
-        if (n < kfull) {
-            unrolled<0, C::LPT>([&](auto d) __attribute__((always_inline)) { issue(n, d); });
-            ld_kb += KS;
-        }
-    });
-    if (kfull > 0) {
-        wait_loads(min(kfull, NS - 1) - 1);
-        lds_barrier();
-        first_operands(sub);
-    }
-    if (NS - 1 < kfull) unrolled<0, EARLY>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
-    int stage = 0, kt = 0;
-    auto step = [&](auto rest_c, auto first_c, auto next_c, int younger) __attribute__((always_inline)) {
-        const int next = stage == NS - 1 ? 0 : stage + 1, prev = stage == 0 ? NS - 1 : stage - 1;
-        k_block(sub + stage * C::STAGE, sub + next * C::STAGE, stage, prev, younger, rest_c, first_c, next_c);
-        stage = next, kt++;
-    };
     const std::true_type yes;
     const std::false_type no;
+    // all of the K loop; step(stage, next, prev, younger, REST, FIRST, NEXT) does a block
+    auto drive = [&](auto&& ready, auto&& step) __attribute__((always_inline)) {
+        unrolled<0, NS - 1>([&](auto n_c) __attribute__((always_inline)) {
+            constexpr int n = decltype(n_c)::value;
+            if (n < kfull) {
+                unrolled<0, C::LPT>([&](auto d) __attribute__((always_inline)) { issue(n, d); });
+                ld_kb += KS;
+            }
+        });
+        if (kfull > 0) {
+            wait_loads(min(kfull, NS - 1) - 1);
+            lds_barrier();
+            ready();
+        }
+        if (NS - 1 < kfull) unrolled<0, EARLY>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
+        int stage = 0, kt = 0;
+        auto one = [&](auto rest_c, auto first_c, auto next_c, int younger) __attribute__((always_inline)) {
+            const int next = stage == NS - 1 ? 0 : stage + 1, prev = stage == 0 ? NS - 1 : stage - 1;
+            step(stage, next, prev, younger, rest_c, first_c, next_c);
+            stage = next, kt++;
+        };
 #pragma unroll 1
-    while (kt + NS < kfull) step(yes, yes, yes, NS - 2);
-    if (kt + NS == kfull) step(yes, no, yes, NS - 2);
+        while (kt + NS < kfull) one(yes, yes, yes, NS - 2);
+        if (kt + NS == kfull) one(yes, no, yes, NS - 2);
 #pragma unroll 1
-    while (kt + 1 < kfull) step(no, no, yes, kfull - 2 - kt);
-    if (kt < kfull) step(no, no, no, 0);
-    if (kb0 + kfull * KS < kb1) {  // block-uniform: at most a block for each group, one of them ragged, through registers; what is missing is zeros
+        while (kt + 1 < kfull) one(no, no, yes, kfull - 2 - kt);
+        if (kt < kfull) one(no, no, no, 0);
+    };
+    const bool ragged = kb0 + kfull * KS < kb1;  // block-uniform
+    auto load_ragged = [&]() __attribute__((always_inline)) {  // at most a block for each group, one of them ragged, through registers; what is missing is zeros
         lds_barrier();
         const int kb = kb0 + kfull * KS + group, left = kb < kb1 ? g.K - kb * kScaleBlock : 0;
         uint8_t* to = smem + group * C::SUB;
@@ -278,6 +287,34 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         }
         *reinterpret_cast<float*>(to + C::DATA + tid * 4) = left > 0 ? s_ptr[kb] : 0.f;
         lds_barrier();
+    };
+    // outputs go through LDS where they are whole 16-byte pieces
+    const bool wide = !SPLIT && (g.N & 7) == 0 && (g.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15u) == 0;
+    if (row0 + wm * C::WTM >= row_end || n0 + wn * C::WTN >= g.N) {
+        // a wavefront whose rows or channels all lie behind the last one loads its pieces and waits with the others, and multiplies nothing
+        // (32768 rows on 28 of 32 experts, 4864 x 3584, 256-row tiles: 672 us multiplying, 606 not)
+        drive([] {}, [&](int stage, int, int prev, int younger, auto rest_c, auto first_c, auto next_c) __attribute__((always_inline)) {
+            if constexpr (decltype(rest_c)::value) {
+                unrolled<EARLY, C::LPT>([&](auto d) __attribute__((always_inline)) { issue(prev, d); });
+                ld_kb += KS;
+            }
+            if constexpr (decltype(next_c)::value) {
+                wait_loads(younger);
+                lds_barrier();
+            }
+            if constexpr (decltype(first_c)::value) unrolled<0, EARLY>([&](auto d) __attribute__((always_inline)) { issue(stage, d); });
+        });
+        if (ragged) load_ragged();
+        if constexpr (KS > 1) lds_barrier(), lds_barrier(), lds_barrier();
+        else if (wide) lds_barrier();
+        return;
+    }
+    drive([&]() __attribute__((always_inline)) { first_operands(sub); },
+          [&](int stage, int next, int prev, int younger, auto rest_c, auto first_c, auto next_c) __attribute__((always_inline)) {
+              k_block(sub + stage * C::STAGE, sub + next * C::STAGE, stage, prev, younger, rest_c, first_c, next_c);
+          });
+    if (ragged) {
+        load_ragged();
         first_operands(sub);
         k_block(sub, sub, 0, 0, 0, no, no, no);
     }
@@ -332,7 +369,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
             return bf16 ? make_uint2(Lo<LLMQ_BF16>::pack2(v[0], v[1]), Lo<LLMQ_BF16>::pack2(v[2], v[3]))
                         : make_uint2(Lo<LLMQ_F16>::pack2(v[0], v[1]), Lo<LLMQ_F16>::pack2(v[2], v[3]));
         };
-        if ((g.N & 7) == 0 && (g.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15u) == 0) {  // uniform
+        if (wide) {
             // Through LDS, so that a store covers whole lines of a row: a wavefront's outputs go to a region of its own, 16-byte chunk c of row r at
             // chunk c ^ (r % CH), and come back 16 bytes per lane, CH lanes a row.
             constexpr int CH = C::WTN / 8, RPI = kWave / CH;

@@ -13,7 +13,8 @@ from __future__ import annotations
 
 import torch
 
-from .linear import FP8DynamicLinear, FP8StaticLinear, SqW8A8BBF16OBF16PerChannel, SqW8A8BBF16OBF16PerTensor, WQLinear_GEMM
+from .linear import (FP8BlockLinear, FP8DynamicLinear, FP8StaticLinear, SqW8A8BBF16OBF16PerChannel, SqW8A8BBF16OBF16PerTensor,
+                     WQLinear_GEMM)
 
 
 def _cat_bias(linears):
@@ -61,6 +62,17 @@ def fuse_linears(linears):
         fused.weight_scale.data = torch.cat([l.weight_scale.data.reshape(-1, 1) for l in linears], dim=0).contiguous()
         if first.bias is not None:
             fused.bias.data = _cat_bias(linears)
+        return fused
+    if kind is FP8BlockLinear:
+        if any(l.out_features % 128 for l in linears[:-1]):
+            return list(linears)  # a block of 128 channels would straddle two modules, whose scales differ
+        if any(l.dtype != first.dtype for l in linears):
+            raise RuntimeError("FP8 modules with different dtypes cannot be fused")
+        fused = FP8BlockLinear(first.in_features, n_out, first.bias is not None, dev=first.weight.device, dtype=first.dtype)
+        fused.weight = torch.cat([l.weight for l in linears], dim=0).contiguous()
+        fused.weight_scale = torch.cat([l.weight_scale for l in linears], dim=0).contiguous()
+        if first.bias is not None:
+            fused.bias = _cat_bias(linears)
         return fused
     if kind in (SqW8A8BBF16OBF16PerTensor, FP8StaticLinear):
         return list(linears)  # per-module stored activation scales: not fusable without changing results

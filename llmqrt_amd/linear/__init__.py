@@ -2,6 +2,7 @@
 from .linear_awq import WQLinear_GEMM
 from .linear_base import LinearBase
 from .linear_fp8 import FP8DynamicLinear, FP8StaticLinear
+from .linear_fp8_block import FP8BlockGroupedLinear, FP8BlockLinear
 from .linear_sq import SqW8A8BBF16OBF16PerChannel, SqW8A8BBF16OBF16PerTensor
 
 method_to_linear: dict[str, type[LinearBase]] = {

@@ -178,6 +178,14 @@ class RMSNorm(nn.Module):
         y = host().rmsnorm(hidden_states, self.weight, self.variance_epsilon)
         return rmsnorm(hidden_states, self.weight, self.variance_epsilon) if y is None else y
 
+    def forward_add(self, hidden_states, residual, quantize: str | None = None, return_normed: bool = False, inplace: bool = False):
+        """The residual's addition in front of the norm, in the same pass: add_rmsnorm (``quantize`` None) or its form for the Linear that follows:
+        "int8" (SqW8A8BBF16OBF16PerChannel), "fp8" (FP8DynamicLinear per token), "fp8_block" (FP8BlockLinear)."""
+        kinds = {None: _SAME, "int8": _I8_TOKEN, "fp8": _FP8_TOKEN, "fp8_block": _FP8_GROUP}
+        if quantize not in kinds or residual is None:
+            raise RuntimeError(f"forward_add needs a residual, and quantize one of {list(kinds)}")
+        return _add_norm(hidden_states, residual, self.weight, self.variance_epsilon, kinds[quantize], return_normed and quantize is not None, inplace)
+
     def forward_quantized(self, hidden_states, fp8: bool = False, return_normed: bool = False):
         """Normalise and quantize per token in one pass, for a W8A8 / FP8 Linear that accepts (q, scale)."""
         if not return_normed:
