@@ -61,11 +61,13 @@ __device__ __forceinline__ int place_of(int bid, int nblk) {
     const int q = nblk / kNumXcd, r = nblk % kNumXcd, xcd = bid % kNumXcd, local = bid / kNumXcd;
     return xcd < r ? xcd * (q + 1) + local : r * (q + 1) + (xcd - r) * q + local;
 }
-// place in one matrix's order -> (tile of rows, tile of channels): groups of kGroupM tiles of rows
+// place in one matrix's order -> (tile of rows, tile of channels): groups of kGroupM tiles of rows, each of which starts its walk over the weights at
+// another place, so that the XCDs do not all wait for the same weights from HBM (us, all from the first channel / so: 8192 x 37888 x 3584 1008 / 988,
+// on 128 x 256 tiles 1175 / 1097, 8192 x 4608 x 3584 157 / 146)
 __device__ __forceinline__ void tile_of(int pid, int tiles_m, int tiles_n, int& tm, int& tn) {
     const int width = kGroupM * tiles_n, group = pid / width, first = group * kGroupM, size = min(tiles_m - first, kGroupM);
     tm = first + (pid % width) % size;
-    tn = (pid % width) / size;
+    tn = (pid % width / size + group * tiles_n / ((tiles_m + kGroupM - 1) / kGroupM)) % tiles_n;
 }
 
 template <class C, bool GROUPED, bool SPLIT>
@@ -144,7 +146,14 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     }
     const uint8_t* sub = smem + group * C::SUB;  // the group's part of stage 0
     const uint32_t lds_base = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) void*)smem) + (uint32_t)group * C::SUB;
-    int ld_kb = kb0 + group;
+    // The walk over K starts at an eighth that follows from the tile of channels and wraps around: the XCDs work on different channels, and so do not
+    // all ask for the same part of the rows at once, which lie the same distance apart and fall on few memory channels (us, from 0 / so: 777 x 3584 x
+    // 18944 on 128 x 256 tiles 130 / 115, in two splits 82 / 76).  A channel's sums have one order for every token of a call.
+    int ld_kb = kb0 + group + tn * kNumXcd / tiles_n * kfull / kNumXcd * KS;
+    auto next_kb = [&]() __attribute__((always_inline)) {
+        ld_kb += KS;
+        if (ld_kb >= kb0 + kfull * KS) ld_kb -= kfull * KS;
+    };
     auto issue = [&](int stage, auto d_c) __attribute__((always_inline)) {  // piece d of block ld_kb
         constexpr int d = decltype(d_c)::value;
         const uint32_t to = lds_base + (uint32_t)stage * C::STAGE;
@@ -210,7 +219,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         unrolled<0, TT>([&](auto t_c) __attribute__((always_inline)) {
             constexpr int t = decltype(t_c)::value, i = t / TN, j = t % TN;
             if constexpr (NEXT && i == TM - 1 && j == 0) {
-                if constexpr (REST) ld_kb += KS;
+                if constexpr (REST) next_kb();
                 wait_loads(younger);
                 lds_barrier();
             }
@@ -252,7 +261,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
             constexpr int n = decltype(n_c)::value;
             if (n < kfull) {
                 unrolled<0, C::LPT>([&](auto d) __attribute__((always_inline)) { issue(n, d); });
-                ld_kb += KS;
+                next_kb();
             }
         });
         if (kfull > 0) {
@@ -296,7 +305,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         drive([] {}, [&](int stage, int, int prev, int younger, auto rest_c, auto first_c, auto next_c) __attribute__((always_inline)) {
             if constexpr (decltype(rest_c)::value) {
                 unrolled<EARLY, C::LPT>([&](auto d) __attribute__((always_inline)) { issue(prev, d); });
-                ld_kb += KS;
+                next_kb();
             }
             if constexpr (decltype(next_c)::value) {
                 wait_loads(younger);
@@ -371,7 +380,8 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         };
         if (wide) {
             // Through LDS, so that a store covers whole lines of a row: a wavefront's outputs go to a region of its own, 16-byte chunk c of row r at
-            // chunk c ^ (r % CH), and come back 16 bytes per lane, CH lanes a row.
+            // chunk c ^ (r % CH), and come back 16 bytes per lane, CH lanes a row.  (8 bytes per lane from the registers: 8192 x 37888 x 3584 1403 us,
+            // so 1130.)
             constexpr int CH = C::WTN / 8, RPI = kWave / CH;
             static_assert(C::WTM * C::WTN * 2 * (NG / kWave) <= C::LDS_BYTES, "outputs fit in the ring");
             if constexpr (KS == 1) lds_barrier();  // every wavefront has read its last operands
