@@ -390,6 +390,7 @@ int llmq_quant_fp8_per_group(const void* x, int x_dtype, int64_t M, int64_t K, i
  *   LLMQ_NORM_I8_TOKEN   q = clamp(rint(y / s), -128, 127), s = max(max |y|, 1e-5) / 127          scale: fp32 [M]
  *   LLMQ_NORM_FP8_TOKEN  q = e4m3(y / s),                   s = max(max |y|, 1e-12) / 448         scale: fp32 [M]
  *   LLMQ_NORM_FP8_GROUP  as llmq_quant_fp8_per_group of the fp32 y                                scale: fp32 [M, ceil(K / 128)]
+ * The quotients y / s are formed as (h * weight) / (s / inv), whose operands are exact but for the scale; h * weight has to be finite in fp32.
  * The 8-bit forms write x_dtype(y) too where y is not null.  Unlike llmq_rmsnorm_quant_*, which round h * inv and y to x_dtype as the
  * reference does, y is not rounded before it is quantized.  residual null: h = x, and h is not written.  h may be the residual itself (the
  * addition in place) or x; otherwise nothing may overlap.  K % 8 == 0, row strides % 8 == 0, 16-byte aligned (q: 8). */

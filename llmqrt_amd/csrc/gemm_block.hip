@@ -13,21 +13,26 @@ constexpr int kRowsCfg = kNumBlockTiles;
 thread_local int forced_cfg = -1, forced_splits = 0;
 
 // What a launch takes, in us, as a rule of the sizes alone:
-//   start + max(stream, loop) + min(stream, loop) / 4 + what a K split adds
-// stream: the operands once at 5.8 TB/s.  loop: steps along K times what one takes, from `alone` (a few blocks on the chip) to `alone` + `crowd` (one
-// on every CU), or `full` per block of a CU where there are more: a last round that is not full costs as the fourth root of what it holds (rows: all of it).  A split
-// adds a launch and its sums' way out and back.  Fitted to 4300 random sizes (1-8192 tokens, 128-37888 channels, K 512-18944), every
-// configuration and split timed with the weights out of HBM: the choice is 2.0 % (2.5 % up to 64 tokens) slower than the fastest of the
-// size on average, 11 % (16 %) in the worst 5 % of the sizes.  By experts, 1200 sizes, the same constants: 2.8 %, 12 %.
+//   start + max(stream, loop) + 0.15 min(stream, loop) + what a K split adds
+// stream: the operands once at 6.6 TB/s, longer where some CUs have a block more than others.  loop: steps along K times what one takes, from
+// `alone` (a few blocks on the chip) to `alone` + `crowd` (one on every CU); with more blocks than CUs `full` for each of a CU's, and a last round that is
+// not full costs as the fourth root of what it holds (row-streaming kernel: all of it).  A split adds a launch and its sums' way out and back.
+// Fitted to 4300 random sizes (1-8192 tokens, 128-37888 channels, K 512-18944), every configuration and split timed with the weights out of
+// HBM: the choice is 1.8 % (2.2 % up to 64 tokens) slower than the fastest of the size on average, 10 % (14 %) in the worst 5 % of the sizes.  By
+// experts, 1200 sizes, the same constants: 2.9 %, 13 %.
 struct Cost { float start, alone, full, crowd; };
-constexpr Cost kTileCost[kNumBlockTiles] = {{4.99, 0, 1.95, 1.56}, {4.74, 0.755, 1.11, 0.187}, {4.49, 0.333, 0.742, 0.41}, {4.19, 0.347, 0.427, 0.114}, {3.57, 0.279, 0.345, 0.096}, {3.94, 0.233, 0.292, 0.038}, {5.82, 0.368, 0.841, 0.427}, {4.54, 0.292, 0.611, 0.02}};
-constexpr Cost kRowsCost[kNumBlockRows] = {{2.76, 0.34, 0.305, 0}, {3.03, 0.473, 0.595, 0.149}, {2.92, 0.4, 0.364, 0.014}, {3.09, 0, 0.557, 0.545}, {3.25, 0.584, 0.764, 0.205}, {3.17, 0.139, 0.689, 0.15}, {3.29, 0.046, 0.666, 0.081}};
+constexpr Cost kTileCost[kNumBlockTiles] = {{6.86, 1.15, 2.21, 0.615}, {5.85, 0.757, 1.25, 0.232}, {5.28, 0.349, 0.809, 0.424}, {4.51, 0.354, 0.441, 0.152}, {3.78, 0.311, 0.364, 0.098}, {4.09, 0.278, 0.316, 0.044}, {6.15, 0.495, 0.906, 0.311}, {5.03, 0.329, 0.686, 0.235}};
+constexpr Cost kRowsCost[kNumBlockRows] = {{2.76, 0.34, 0.336, 0.026}, {3.05, 0.548, 0.764, 0.116}, {2.93, 0.4, 0.392, 0.055}, {3.08, 0.531, 0.712, 0.055}, {3.29, 0.704, 0.82, 0.114}, {3.18, 0.645, 1, 0.091}, {3.36, 0.551, 0.935, 0.557}};
 
 float cost_us(const Cost& c, double blocks, double steps, double bytes, bool rows) {
-    const float rounds = (float)(blocks / 256.0), whole = floorf(rounds), rest = rounds - whole;
-    const float loop = (float)steps * std::max(c.alone + c.crowd * std::min(rounds, 1.f), c.full * (whole + (rows ? ceilf(rest) : sqrtf(sqrtf(rest)))));
-    const float stream = (float)(bytes / 5.8e6);
-    return c.start + std::max(stream, loop) + 0.25f * std::min(stream, loop);
+    const float r = (float)(blocks / 256.0), whole = floorf(r), rest = r - whole;
+    float step = c.alone + c.crowd * std::min(r, 1.f), stream = (float)(bytes / 6.6e6);
+    if (r > 1.f) {
+        step = std::max(step, c.full * (whole + (rows ? ceilf(rest) : sqrtf(sqrtf(rest)))));
+        stream *= 1.f + 0.3f * (ceilf(r) / r - 1.f);
+    }
+    const float loop = (float)steps * step;
+    return c.start + std::max(stream, loop) + 0.15f * std::min(stream, loop);
 }
 
 BlockPlan search(int64_t M, int64_t N, int64_t K) {
@@ -41,7 +46,7 @@ BlockPlan search(int64_t M, int64_t N, int64_t K) {
             if (s > 1 && (KB / s < 4 || tiles * s > (t.bm * t.bn > 64 * 128 ? 300 : 600))) break;
             const int per = (KB + s - 1) / s, splits = (KB + per - 1) / per;
             float us = cost_us(kTileCost[c], tiles * splits, (per + t.ks - 1) / t.ks, (double)N * K + (double)M * K, false);
-            if (splits > 1) us += 3.f + (float)(splits * (double)M * N * 8 / 5e6);
+            if (splits > 1) us += 3.f + (float)(splits * (double)M * N * 8 / 5.5e6);
             if (us < least) least = us, best = {c, splits, per};
         }
     }

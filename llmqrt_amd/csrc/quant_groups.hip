@@ -204,13 +204,31 @@ __global__ __launch_bounds__(NT * RPB) void add_norm_kernel(NormArgs a) {
     ss = RPB > 1 ? wave_sum(ss) : block_sum<NT / kWave>(ss, smem);
     const float inv = 1.0f / sqrtf(ss / (float)a.K + a.eps);
 
-    // y of chunk i; a row that is not in registers is read again, by the thread that wrote it
-    auto values = [&](int c, int i, float* v) __attribute__((always_inline)) {
-        float w[8];
-        if (NC > 0) widen8<DT>(hc[c], v), widen8<DT>(wc[c], w);
-        else widen8<DT>(rr ? hr[i] : xr[i], v), widen8<DT>(wr[i], w);
+    // h and w of chunk i; a row that is not in registers is read again, by the thread that wrote it
+    auto operands = [&](int c, int i, float* h, float* w) __attribute__((always_inline)) {
+        if (NC > 0) widen8<DT>(hc[c], h), widen8<DT>(wc[c], w);
+        else widen8<DT>(rr ? hr[i] : xr[i], h), widen8<DT>(wr[i], w);
+    };
+    auto store_y = [&](int c, int i) __attribute__((always_inline)) {
+        float h[8], w[8];
+        operands(c, i, h, w);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = (v[e] * inv) * w[e];
+        for (int e = 0; e < 8; e++) h[e] = (h[e] * inv) * w[e];
+        yr[i] = narrow8<DT>(h);
+    };
+    // What is quantized is y / s = (h w) / (s / inv): h w is exact (two 16-bit floats), and inv, the same for scale and value, leaves the quotient, so that
+    // a code depends on the rounding of s / inv = max |h w| / qmax alone.
+    auto products = [&](int c, int i, float* v) __attribute__((always_inline)) {
+        float w[8];
+        operands(c, i, v, w);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] *= w[e];
+    };
+    // scale of y, and of h w, from max |h w|
+    auto scales = [&](float amax, float& s, float& sp) __attribute__((always_inline)) {
+        sp = amax / QP<MODE>::qmax;
+        s = sp * inv;
+        if (!(amax * inv > QP<MODE>::floor_ && amax < __builtin_inff())) s = scale32<MODE>(amax * inv), sp = s / inv;  // the floor; NaN and infinity
     };
     auto each = [&](auto&& f) __attribute__((always_inline)) {  // f(register, chunk, whether it is in the row), all lanes of a wavefront together
         if (NC > 0) {
@@ -223,24 +241,24 @@ __global__ __launch_bounds__(NT * RPB) void add_norm_kernel(NormArgs a) {
 
     if (OUT == OUT_SAME) {
         each([&](int c, int i, bool in) __attribute__((always_inline)) {
-            if (!in) return;
-            float v[8];
-            values(c, i, v);
-            yr[i] = narrow8<DT>(v);
+            if (in) store_y(c, i);
         });
         return;
     }
     if (OUT == OUT_GROUP) {
         each([&](int c, int i, bool in) __attribute__((always_inline)) {
             float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (in) values(c, i, v);
-            const float amax = team_max(absmax8f(v)), s = scale32<MODE>(amax), inv_s = 1.0f / s;
+            if (in) products(c, i, v);
+            float s, sp;
+            const float amax = team_max(absmax8f(v));
+            scales(amax, s, sp);
+            const float inv_s = 1.0f / sp;
             uint2 code;
-            if (__all(near_ok(amax, s))) code = codes8<MODE, true>(v, s, inv_s);
-            else code = codes8<MODE, false>(v, s, inv_s);
+            if (__all(near_ok(amax, sp))) code = codes8<MODE, true>(v, sp, inv_s);
+            else code = codes8<MODE, false>(v, sp, inv_s);
             if (!in) return;
             qr[i] = code;
-            if (yr) yr[i] = narrow8<DT>(v);
+            if (yr) store_y(c, i);
             if (i % kTeam == 0) a.scale[row * groups + i / kTeam] = s;
         });
         return;
@@ -249,20 +267,22 @@ __global__ __launch_bounds__(NT * RPB) void add_norm_kernel(NormArgs a) {
     each([&](int c, int i, bool in) __attribute__((always_inline)) {
         if (!in) return;
         float v[8];
-        values(c, i, v);
+        products(c, i, v);
         amax = max_nonneg(amax, absmax8f(v));
-        if (yr) yr[i] = narrow8<DT>(v);
+        if (yr) store_y(c, i);
     });
     amax = RPB > 1 ? wave_max(amax) : block_max<NT / kWave>(amax, smem);
-    const float s = scale32<MODE>(amax), inv_s = 1.0f / s;
+    float s, sp;
+    scales(amax, s, sp);
+    const float inv_s = 1.0f / sp;
     if (tid == 0) a.scale[row] = s;
-    const bool fast = near_ok(amax, s);  // of the row
+    const bool fast = near_ok(amax, sp);  // of the row
     each([&](int c, int i, bool in) __attribute__((always_inline)) {
         if (!in) return;
         float v[8];
-        values(c, i, v);
-        if (fast) qr[i] = codes8<MODE, true>(v, s, inv_s);
-        else qr[i] = codes8<MODE, false>(v, s, inv_s);
+        products(c, i, v);
+        if (fast) qr[i] = codes8<MODE, true>(v, sp, inv_s);
+        else qr[i] = codes8<MODE, false>(v, sp, inv_s);
     });
 }
 
