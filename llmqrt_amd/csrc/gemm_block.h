@@ -6,6 +6,7 @@
 namespace llmq {
 
 constexpr int kScaleBlock = 128;
+constexpr int kMostSplits = 8;  // of K
 
 struct BlockArgs {
     const uint8_t* A;      // [M, K] e4m3

@@ -63,7 +63,7 @@ BlockPlan plan(int64_t M, int64_t N, int64_t K) {
     const int KB = (int)((K + kScaleBlock - 1) / kScaleBlock);
     if (forced_cfg >= kRowsCfg && M <= 16 * kBlockRows[forced_cfg - kRowsCfg].mt) return {forced_cfg, 1, KB};
     if (forced_cfg >= 0 && forced_cfg < kRowsCfg) {
-        const int per = (KB + std::max(1, std::min(forced_splits, KB)) - 1) / std::max(1, std::min(forced_splits, KB));
+        const int want = std::max(1, std::min({forced_splits, KB, kMostSplits})), per = (KB + want - 1) / want;
         return {forced_cfg, (KB + per - 1) / per, per};
     }
     thread_local int64_t of[3] = {0, 0, 0};  // the last size

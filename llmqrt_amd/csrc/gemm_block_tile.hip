@@ -423,32 +423,51 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     }
 }
 
-// the splits' sums in order, bias, rounding; 4 channels per thread
+// The splits' sums in order, bias, rounding; 8 channels per thread, all splits requested before the first is used.  WIDE: rows of whole 16-byte
+// pieces.  (us with two splits of 777 x 3584: 4 channels per thread 7.9, so 6.2; partial sums stored past
+// the L2: products 2-10 % slower.)
+template <bool WIDE>
 __global__ __launch_bounds__(256) void block_reduce_kernel(BlockArgs g, int splits) {
-    const int64_t per_row = (g.N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t per_row = (g.N + 7) / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= per_row * g.M) return;
-    const int m = (int)(i / per_row), n = (int)(i - (int64_t)m * per_row) * 4;
+    const int m = (int)((uint64_t)i <= 0xffffffffu ? (uint32_t)i / (uint32_t)per_row : i / per_row), n = (int)(i - (int64_t)m * per_row) * 8;
     const int64_t plane = (int64_t)g.M * g.N;
     const float* p = g.partials + (int64_t)m * g.N + n;
     uint16_t* to = reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n;
-    float v[4] = {0, 0, 0, 0};
-    if ((g.N & 3) == 0) {
-        for (int k = 0; k < splits; k++) {
-            const v4f q = *reinterpret_cast<const v4f*>(p + k * plane);
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (WIDE) {
+        v4f q[kMostSplits][2];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] += q[e];
-        }
+        for (int k = 0; k < kMostSplits; k++)
+            if (k < splits) {  // uniform
+                q[k][0] = *reinterpret_cast<const v4f*>(p + k * plane);
+                q[k][1] = *(reinterpret_cast<const v4f*>(p + k * plane) + 1);
+            }
+#pragma unroll
+        for (int k = 0; k < kMostSplits; k++)
+            if (k < splits)
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] += q[k][e / 4][e % 4];
     } else {
         for (int k = 0; k < splits; k++)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
+            for (int e = 0; e < 8; e++)
                 if (n + e < g.N) v[e] += p[k * plane + e];
     }
+    if (g.bias)
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        if (n + e >= g.N) continue;
-        const float f = v[e] + (g.bias ? load_as_f32(g.bias, g.bias_dtype, n + e) : 0.f);
-        to[e] = g.out_dtype == LLMQ_BF16 ? Lo<LLMQ_BF16>::from_f32(f) : Lo<LLMQ_F16>::from_f32(f);
+        for (int e = 0; e < 8; e++) v[e] += load_as_f32(g.bias, g.bias_dtype, min(n + e, g.N - 1));
+    const bool bf16 = g.out_dtype == LLMQ_BF16;
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        w[e] = bf16 ? Lo<LLMQ_BF16>::pack2(v[2 * e], v[2 * e + 1]) : Lo<LLMQ_F16>::pack2(v[2 * e], v[2 * e + 1]);
+    if (WIDE) {
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (n + e < g.N) to[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
     }
 }
 
@@ -472,9 +491,11 @@ int launch_tile(const BlockArgs& g, int splits, hipStream_t st) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * tiles_n), SPLIT ? splits : 1), dim3(C::NT), C::LDS_BYTES, st, g);
     if (launch_status() != LLMQ_OK) return LLMQ_ERR_LAUNCH;
     if (SPLIT) {
-        const int64_t n = (int64_t)((g.N + 3) / 4) * g.M;
-        if (n > 0xffffff00LL) return LLMQ_ERR_SHAPE;
-        hipLaunchKernelGGL(block_reduce_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g, splits);
+        const int64_t n = (int64_t)((g.N + 7) / 8) * g.M;
+        if (n > 0xffffff00LL || splits > kMostSplits) return LLMQ_ERR_SHAPE;
+        const bool wide = (g.N & 7) == 0 && (g.ldo & 7) == 0 && aligned16(g.out);
+        if (wide) hipLaunchKernelGGL(block_reduce_kernel<true>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g, splits);
+        else hipLaunchKernelGGL(block_reduce_kernel<false>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g, splits);
         return launch_status();
     }
     return LLMQ_OK;

@@ -96,6 +96,8 @@ class FP8BlockLinear(_FP8BlockBase):
         by the fused norm; the result is in the module's dtype."""
         b = self._buffers
         y = host().fp8_block(qinput, x_scale, b["weight"], b["weight_scale"], b["bias"], self.dtype)
+        if y is None and x_scale.shape[:-1] != qinput.shape[:-1]:
+            raise RuntimeError("x_scale must hold one scale per token and 128 channels, [.., ceil(K / 128)]")
         if y is None:
             y = f8f8_blockwise(qinput.reshape(-1, qinput.shape[-1]), self.weight.t(), self.bias, x_scale.reshape(-1, x_scale.shape[-1]), self.weight_scale,
                                _NAMES[self.dtype]).view(*qinput.shape[:-1], self.out_features)

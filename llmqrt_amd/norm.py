@@ -12,7 +12,7 @@ from torch import nn
 
 from . import _abi
 from ._native import host
-from .quantize import _as_rows
+from .quantize import _apart, _as_rows
 
 
 def _check_weight(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
@@ -82,7 +82,7 @@ _SAME, _I8_TOKEN, _FP8_TOKEN, _FP8_GROUP = range(4)
 def _same_rows(t: torch.Tensor, x: torch.Tensor, what: str) -> torch.Tensor:
     if t.dtype != x.dtype or t.device != x.device or t.shape != x.shape:
         raise RuntimeError(f"{what} must have the shape, dtype and device of the activations")
-    return _as_rows(t)
+    return _apart(_as_rows(t))
 
 
 def _add_norm(x, residual, weight, eps, out, return_normed=False, inplace=False):
@@ -94,7 +94,7 @@ def _add_norm(x, residual, weight, eps, out, return_normed=False, inplace=False)
 def _add_norm_general(x, residual, weight, eps, out, return_normed, inplace):
     if inplace and residual is None:
         raise RuntimeError("inplace needs a residual")
-    rows = _as_rows(x)
+    rows = _apart(_as_rows(x))
     w = _check_weight(rows, weight)
     M, K = rows.shape
     dev = rows.device

@@ -145,11 +145,16 @@ def static_per_tensor_quantize(tensor: torch.Tensor, scale) -> torch.Tensor:
 
 
 def per_group_quantize(tensor: torch.Tensor):
-    """One scale per token and 128 channels (the last group of a row may be short), the activations of a block-scaled product:
+    """One scale per token and 128 channels (a multiple of 8; the last group of a row may be short), the activations of a block-scaled product:
     scale = max(absmax, 1e-12) / 448 and codes = e4m3fn(tensor / scale), in fp32.
     -> (float8_e4m3fn tensor like `tensor`, fp32 scales [.., ceil(K / 128)]).  No counterpart in the reference."""
     out = host().quant_groups(tensor)
     return _per_group_quantize_general(tensor) if out is None else out
+
+
+def _apart(x: torch.Tensor) -> torch.Tensor:
+    """Rows that do not overlap: an expanded tensor, whose rows are one, is copied."""
+    return x.contiguous() if x.shape[0] > 1 and x.stride(0) < x.shape[1] else x
 
 
 @torch.no_grad()
@@ -160,7 +165,7 @@ def _per_group_quantize_general(tensor):
     if tensor.numel() == 0:
         return (torch.empty(tensor.shape, dtype=torch.float8_e4m3fn, device=tensor.device),
                 torch.empty((*tensor.shape[:-1], groups), dtype=torch.float32, device=tensor.device))
-    x = _as_rows(tensor)
+    x = _apart(_as_rows(tensor))
     M, K = x.shape
     q = torch.empty((M, K), dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty((M, groups), dtype=torch.float32, device=x.device)

@@ -177,3 +177,47 @@ def test_captured(cuda):
         q1, s1, h3 = add_rmsnorm_quantize_activation_per_token_absmax(y1, h1, w)
         torch.cuda.synchronize()
         assert torch.equal(y, y1) and torch.equal(h, h1) and torch.equal(q, q1) and torch.equal(s, s1) and torch.equal(h2, h3)
+
+
+def test_no_rows_one_row_and_more_dimensions(cuda):
+    from llmqrt_amd.norm import RMSNorm, add_rmsnorm, add_rmsnorm_per_group_quantize
+    x, r, w = (t.to(cuda) for t in inputs(12, 904, torch.float16, 3))
+    y, h = add_rmsnorm(x[:0], r[:0], w)
+    assert y.shape == h.shape == (0, 904)
+    q, s, h = add_rmsnorm_per_group_quantize(x[:0], r[:0], w)
+    assert q.shape == (0, 904) and s.shape == (0, 8)
+    want = add_rmsnorm(x, r, w)
+    one = add_rmsnorm(x[5], r[5], w)
+    assert all(torch.equal(a, b[5]) for a, b in zip(one, want))
+    cube = add_rmsnorm_per_group_quantize(x.view(3, 4, 904), r.view(3, 4, 904), w)
+    flat = add_rmsnorm_per_group_quantize(x, r, w)
+    assert cube[1].shape == (3, 4, 8) and all(torch.equal(a.view(torch.uint8).flatten(), b.view(torch.uint8).flatten()) for a, b in zip(cube, flat))
+    m = RMSNorm(w, 1e-6)
+    assert all(torch.equal(a, b) for a, b in zip(m.forward_add(x, r), want))
+    # the same row for every token, and x as its own residual
+    assert torch.equal(add_rmsnorm(x, r[:1].expand(12, 904), w)[1], x + r[:1])
+    with pytest.raises(RuntimeError):
+        add_rmsnorm(x, r[:1].expand(12, 904), w, inplace=True)
+    twice = x.clone()
+    y2, h2 = add_rmsnorm(twice, twice, w, inplace=True)
+    y3, h3 = add_rmsnorm(x, x, w)
+    assert torch.equal(y2, y3) and torch.equal(twice, h3)
+
+
+def test_many_rows(cuda):
+    """2.2 million short rows: more than one grid's, and offsets past 2^32 bytes."""
+    from llmqrt_amd.norm import add_rmsnorm_quantize_activation_per_token_absmax as f
+    M, K = 2_200_000, 1032
+    g = torch.Generator(device=cuda).manual_seed(1)
+    x = torch.empty(M, K, dtype=torch.bfloat16, device=cuda)
+    for part in x.split(200_000):
+        part.copy_(torch.randn(part.shape, generator=g, device=cuda))
+    r = x.flip(0)
+    w = torch.ones(K, dtype=torch.bfloat16, device=cuda)
+    q, s, h = f(x, r, w)
+    for rows in (slice(0, 50), slice(2_097_100, 2_097_200), slice(M - 50, M)):
+        q1, s1, h1 = f(x[rows].contiguous(), r[rows].contiguous(), w)
+        href = x[rows] + r[rows]
+        assert torch.equal(h[rows], href) and torch.equal(h1, href)
+        check_codes(q[rows].cpu(), s[rows].cpu(), norm64(href.cpu(), w.cpu(), 1e-6), "int8")
+        check_codes(q1.cpu(), s1.cpu(), norm64(href.cpu(), w.cpu(), 1e-6), "int8")

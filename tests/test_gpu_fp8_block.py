@@ -1,9 +1,11 @@
 """GPU: block-scaled fp8 - the group quantizer, the product, the product by experts - against plain forms in 64 bits.
 
 Two kinds of comparison.  Exact: codes that are small whole numbers and scales that are powers of two, so that every sum is exact in fp32 and the
-only rounding is the output's; results have to be the same bits.  General: |error| <= (eps(out) / 2) |y| + c S with S = sum |a b| of the dequantized
-operands; c = 2 u (K + 3 KB + 2), u = 2^-24: each of the K additions of a sum, each scale product, each scaled addition and the bias
-loses at most u of what it adds, doubled for matrix cores that cut instead of rounding."""
+only rounding is the output's; results have to be the same bits.  (The matrix instruction adds each run of 8 products in fixed point and keeps those down
+to 2^-13 of the largest, test_gpu_gemm.py; products of whole numbers up to 3 lie closer together.)  General: |error| <= (eps(out) / 2) |y| +
+c S with S = sum |a b| of the dequantized operands; c = 7 2^-14 for the other seven products of a run, each cut by at most 2^-14 of the largest, and
+2 u (K + 3 KB + 2), u = 2^-24: each of the K additions of a sum, each scale product, each scaled addition and the bias loses at most u
+of what it adds, doubled for matrix cores that cut instead of rounding."""
 import pytest
 import torch
 
@@ -52,7 +54,7 @@ def product64(a, w, sa, sw, bias=None):
 
 
 def check_general(y, ref, s, k):
-    c = 2.0 ** -23 * (k + 3 * blocks(k) + 2)
+    c = 7 * 2.0 ** -14 + 2.0 ** -23 * (k + 3 * blocks(k) + 2)
     err = (y.double() - ref).abs()
     bound = torch.finfo(y.dtype).eps / 2 * ref.abs() * (1 + 1e-6) + c * s + 2.0 ** -25  # the last: fp16 results below the normal range
     assert torch.isfinite(y).all()
@@ -312,3 +314,89 @@ def test_two_streams_at_once(cuda):
     for i in range(2):
         for y in got[i]:
             assert torch.equal(y, want[i])
+
+
+def test_captured_split(cuda):
+    """A K split inside a graph: its partial sums are the graph's own, beside eager calls of the same size."""
+    from llmqrt_amd import _abi
+    a, w, sa, sw = general_operands(200, 512, 18944, 3, cuda)
+    assert _abi.lib().llmq_gemm_fp8_block_workspace_bytes(200, 512, 18944) > 0
+    gemm(a, w, sa, sw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = gemm(a, w, sa, sw)
+        z = gemm(a[:150], w, sa[:150], sw)
+    for k in range(3):
+        sa.mul_(1.25)
+        graph.replay()
+        y1, z1 = gemm(a, w, sa, sw), gemm(a[:150], w, sa[:150], sw)
+        torch.cuda.synchronize()
+        assert same(y, y1) and same(z, z1)
+
+
+# ---- offsets past 32 bits
+
+def test_many_rows(cuda):
+    """1.25 million rows: 4.5 GB of codes, whose scales and products start past 2^32 bytes; compared on the last rows, and a block of rows in between."""
+    from llmqrt_amd.quantize import per_group_quantize
+    M, N, K = 1_250_000, 136, 3600
+    x = torch.empty(M, K, dtype=torch.bfloat16, device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    for part in x.split(100_000):
+        part.copy_(torch.randn(part.shape, generator=g, device=cuda))
+    q, s = per_group_quantize(x)
+    _, w, _, sw = general_operands(1, N, K, 2, cuda)
+    y = gemm(q, w, s, sw)
+    off = torch.tensor([0, 5, M - 40, M], dtype=torch.int32, device=cuda)
+    z = grouped(q, torch.stack([w, w, w]), s, torch.stack([sw, sw, sw]), off)
+    for lo, hi in ((M - 300, M), (1_193_000, 1_193_300)):
+        qr, sr = groups_ref(x[lo:hi].cpu())
+        assert same(s[lo:hi].cpu(), sr) and same(q[lo:hi].cpu().view(torch.uint8), qr.view(torch.uint8))
+        ref, r = product64(q[lo:hi], w, s[lo:hi], sw)
+        check_general(y[lo:hi], ref, r, K)
+        check_general(z[lo:hi], ref, r, K)
+
+
+def test_many_experts(cuda):
+    """600 experts, 4.7 GB of weights: the last ones' lie past 2^32 bytes; more experts than a wavefront counts at once."""
+    E, N, K = 600, 2200, 3584
+    _, w1, _, sw1 = general_operands(1, N, K, 3, cuda)
+    w, sw = torch.zeros(E, N, K, dtype=E4M3, device=cuda), torch.ones(E, blocks(N), blocks(K), device=cuda)
+    for e in (0, 299, 598, 599):
+        w[e].copy_(w1.view(torch.uint8).roll(e, 0).view(E4M3)), sw[e].copy_(sw1 * (1 + e / E))
+    a, _, sa, _ = general_operands(50, 1, K, 4, cuda)
+    counts = [0] * E
+    counts[0], counts[299], counts[598], counts[599] = 3, 17, 1, 29
+    at = [0]
+    for c in counts:
+        at.append(at[-1] + c)
+    y = grouped(a, w, sa, sw, torch.tensor(at, dtype=torch.int32, device=cuda))
+    for e in (0, 299, 598, 599):
+        lo, hi = at[e], at[e + 1]
+        check_general(y[lo:hi], *product64(a[lo:hi], w[e], sa[lo:hi], sw[e]), K)
+
+
+def test_refusals_of_gpu_tensors(cuda):
+    from llmqrt_amd.linear import FP8BlockLinear
+    from llmqrt_amd.sq_fp8_kernels import f8f8_blockwise, f8f8_blockwise_grouped
+    a, w, sa, sw = exact_operands(4, 130, 384, 1, cuda, lead=(2,))  # scales of [2, 3]: a transposed one shows
+    off = torch.tensor([0, 2, 4], dtype=torch.int32, device=cuda)
+    bad = [dict(x_scale=sa.t().contiguous()), dict(x_scale=sa.half()), dict(x_scale=sa.cpu()), dict(w_scale=sw[0].t().contiguous()), dict(XQ=a.float()), dict(XQ=a[:, :128]),
+           dict(WQ=w[0]), dict(bias=torch.zeros(129, device=cuda)), dict(bias=torch.zeros(130, dtype=torch.int32, device=cuda)), dict(dtype_str="float32")]
+    for b in bad:
+        with pytest.raises(RuntimeError):
+            f8f8_blockwise(**{**dict(XQ=a, WQ=w[0].t(), bias=None, x_scale=sa, w_scale=sw[0]), **b})
+    bad = [dict(x_scale=sa.t().contiguous()), dict(w_scale=sw[0]), dict(w_scale=sw.transpose(1, 2).contiguous()), dict(WQ=w[:1]), dict(offsets=off[:2]), dict(offsets=off.long()),
+           dict(offsets=off.cpu()), dict(bias=torch.zeros(130, device=cuda)), dict(out=torch.zeros(4, 130, dtype=torch.float16, device=cuda)),
+           dict(out=torch.zeros(130, 4, dtype=torch.bfloat16, device=cuda).t()), dict(out=torch.zeros(3, 130, dtype=torch.bfloat16, device=cuda))]
+    for b in bad:
+        with pytest.raises(RuntimeError):
+            f8f8_blockwise_grouped(**{**dict(XQ=a, WQ=w, bias=None, x_scale=sa, w_scale=sw, offsets=off), **b})
+    m = FP8BlockLinear(384, 130, False)
+    for args in ((a, sa.t().contiguous()), (a.float(), sa), (a[:, :128], sa)):
+        with pytest.raises(RuntimeError):
+            m.forward_quantized(*args)
+    for x in (torch.zeros(2, 128, dtype=torch.bfloat16, device=cuda), torch.zeros(2, 384, device=cuda)):
+        with pytest.raises(RuntimeError):
+            m(x)

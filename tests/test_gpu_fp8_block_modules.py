@@ -49,6 +49,27 @@ def test_module(cuda, M, K, N, bias, dtype):
     assert m(x[:0]).shape == (0, N)
 
 
+def test_outputs_of_one_call_are_apart(cuda):
+    """Small outputs of a call share an allocation: writing one changes no other, and each counts its own versions."""
+    from llmqrt_amd.norm import add_rmsnorm_per_group_quantize
+    from llmqrt_amd.quantize import per_group_quantize
+    x = torch.randn(3, 904).bfloat16().cuda()
+    w = torch.ones(904, dtype=torch.bfloat16, device=cuda)
+    for f in (lambda: add_rmsnorm_per_group_quantize(x, x, w, return_normed=True), lambda: per_group_quantize(x)):
+        outs, ref = f(), f()
+        assert all(t.data_ptr() % 256 == 0 and t.is_contiguous() and t._base is None for t in outs)
+        for i, t in enumerate(outs):
+            t.view(torch.uint8).fill_(255)
+            assert t._version == 1 and all(same(a.view(torch.uint8), b.view(torch.uint8)) for a, b in list(zip(outs, ref))[i + 1:])
+    with torch.inference_mode():
+        q, s, y, h = add_rmsnorm_per_group_quantize(x, x, w, return_normed=True)
+        assert h.is_inference() and same(h, x + x)
+    h = add_rmsnorm_per_group_quantize(x, x, w)[-1]
+    h.requires_grad_(True)
+    (h.float() * 2).sum().backward()
+    assert bool((h.grad == 2).all())
+
+
 def test_module_moves_and_converts(cuda):
     from llmqrt_amd.linear import FP8BlockLinear
     m = FP8BlockLinear.from_linear(linear(256, 384, True, 1), init_only=False)
@@ -106,7 +127,8 @@ def test_grouped_module(cuda):
         lo, hi = at[e], at[e + 1]
         w = dequantized(m.weight[e], m.weight_scale[e])
         want = a[lo:hi] @ w.t() + m.bias[e].double()
-        room = 2.0 ** -8 * want.abs() + 2.0 ** -23 * 420 * (a[lo:hi].abs() @ w.abs().t() + m.bias[e].double().abs()) + 1e-30
+        # bf16's half step; 7 products of a run of 8 cut by 2^-14 of the largest each; 400 sums, 4 blocks (as in test_gpu_fp8_block.py)
+        room = 2.0 ** -8 * want.abs() + (7 * 2.0 ** -14 + 2.0 ** -23 * 420) * (a[lo:hi].abs() @ w.abs().t() + m.bias[e].double().abs()) + 1e-30
         assert ((y[lo:hi].double() - want).abs() <= room * (1 + 1e-6)).all()
         one = FP8BlockLinear.from_linear(mods[e], init_only=False)
         assert same(one.weight.view(torch.uint8), m.weight[e].view(torch.uint8)) and same(one.weight_scale, m.weight_scale[e])
