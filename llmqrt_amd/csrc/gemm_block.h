@@ -8,6 +8,8 @@ namespace llmq {
 constexpr int kScaleBlock = 128;
 constexpr int kMostSplits = 8;  // of K
 
+__host__ __device__ inline int64_t partial_ld(int64_t N) { return (N + 7) & ~(int64_t)7; }
+
 struct BlockArgs {
     const uint8_t* A;      // [M, K] e4m3
     const float* sa;       // [M, KB]
@@ -16,7 +18,7 @@ struct BlockArgs {
     const void* bias;      // [N] of expert 0, or null
     void* out;             // [M, N]
     const int32_t* offsets;  // experts + 1 first rows, or null: one matrix for all rows
-    float* partials;       // K split: [splits, M, N]
+    float* partials;       // K split: [splits, M, partial_ld(N)]
     int64_t lda, ldb, ldo;
     int M, N, K, KB, NB, experts;
     int blocks_per_split;  // of 128 of K

@@ -91,7 +91,7 @@ int plan_grouped(int64_t rows, int64_t experts, int64_t N, int64_t K) {
     return last;
 }
 
-size_t partial_bytes(const BlockPlan& p, int64_t M, int64_t N) { return p.splits > 1 ? (size_t)p.splits * (size_t)M * (size_t)N * 4 : 0; }
+size_t partial_bytes(const BlockPlan& p, int64_t M, int64_t N) { return p.splits > 1 ? (size_t)p.splits * (size_t)M * (size_t)partial_ld(N) * 4 : 0; }
 
 constexpr int64_t kMaxLd = 1 << 23;  // 256 rows stay within 32-bit offsets
 

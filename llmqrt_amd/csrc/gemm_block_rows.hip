@@ -174,8 +174,10 @@ __global__ __launch_bounds__(C::NT) void block_rows_kernel(BlockArgs g) {
                 h[e] = g.out_dtype == LLMQ_BF16 ? Lo<LLMQ_BF16>::from_f32(v) : Lo<LLMQ_F16>::from_f32(v);
             }
             uint16_t* to = reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n;
-            if (n + 3 < g.N && (reinterpret_cast<uintptr_t>(to) & 7u) == 0)
-                *reinterpret_cast<uint2*>(to) = make_uint2((uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16));
+            typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+            typedef u2v u2any __attribute__((aligned(2)));  // (rows of an odd number of channels start at any even address)
+            if (n + 3 < g.N)
+                *reinterpret_cast<u2any*>(to) = u2v{(uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16)};
             else
 #pragma unroll
                 for (int e = 0; e < 4; e++)

@@ -45,6 +45,20 @@ struct TileCfg {
 // LDS place of 16-byte chunk c of row r: 16 rows of one chunk fall on 16 places
 __device__ __forceinline__ int chunk_at(int r, int c) { return (r * 8 + (c ^ ((r >> 1) & 7))) * 16; }
 
+// the first `left` of eight 16-bit outputs, to any even address
+__device__ __forceinline__ void store8(uint16_t* to, uint4 v, int left) {
+    typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+    typedef u4v u4any __attribute__((aligned(2)));
+    if (left >= 8) {
+        __builtin_nontemporal_store(u4v{v.x, v.y, v.z, v.w}, reinterpret_cast<u4any*>(to));
+    } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 7; e++)
+            if (e < left) to[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+    }
+}
+
 // sum over lanes 0 .. lane
 __device__ __forceinline__ int wave_prefix(int v) {
     const int lane = threadIdx.x & (kWave - 1);
@@ -297,8 +311,6 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         *reinterpret_cast<float*>(to + C::DATA + tid * 4) = left > 0 ? s_ptr[kb] : 0.f;
         lds_barrier();
     };
-    // outputs go through LDS where they are whole 16-byte pieces
-    const bool wide = !SPLIT && (g.N & 7) == 0 && (g.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15u) == 0;
     if (row0 + wm * C::WTM >= row_end || n0 + wn * C::WTN >= g.N) {
         // a wavefront whose rows or channels all lie behind the last one loads its pieces and waits with the others, and multiplies nothing
         // (32768 rows on 28 of 32 experts, 4864 x 3584, 256-row tiles: 672 us multiplying, 606 not)
@@ -315,7 +327,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         });
         if (ragged) load_ragged();
         if constexpr (KS > 1) lds_barrier(), lds_barrier(), lds_barrier();
-        else if (wide) lds_barrier();
+        else if (!SPLIT) lds_barrier();
         return;
     }
     drive([&]() __attribute__((always_inline)) { first_operands(sub); },
@@ -345,130 +357,90 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     }
 
     // ---- a lane holds token l16 of each tile of tokens and channels 4 kq .. + 3 of each tile of channels
+    const int wm0 = row0 + wm * C::WTM, wn0 = n0 + wn * C::WTN;
     if constexpr (SPLIT) {
-        float* part = g.partials + (int64_t)blockIdx.y * g.M * g.N;
+        const int64_t ldp = partial_ld(g.N);  // whole 32-byte pieces: a piece that starts in the row ends in its padding
+        float* part = g.partials + (int64_t)blockIdx.y * g.M * ldp;
 #pragma unroll
         for (int i = 0; i < TM; i++) {
-            const int m = row0 + wm * C::WTM + i * 16 + l16;
+            const int m = wm0 + i * 16 + l16;
             if (m >= row_end) continue;
 #pragma unroll
             for (int j = 0; j < TN; j++) {
-                const int n = n0 + wn * C::WTN + j * 16 + kq * 4;
-                float* to = part + (int64_t)m * g.N + n;
-                if ((g.N & 3) == 0 && n < g.N) *reinterpret_cast<v4f*>(to) = acc[i][j];
-                else
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (n + e < g.N) to[e] = acc[i][j][e];
+                const int n = wn0 + j * 16 + kq * 4;
+                if (n < g.N) *reinterpret_cast<v4f*>(part + (int64_t)m * ldp + n) = acc[i][j];
             }
         }
     } else {
         const bool bf16 = g.out_dtype == LLMQ_BF16;
-        const int wm0 = row0 + wm * C::WTM, wn0 = n0 + wn * C::WTN;
         float bb[TN][4];
 #pragma unroll
         for (int j = 0; j < TN; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 bb[j][e] = g.bias ? load_as_f32(g.bias, g.bias_dtype, (int64_t)expert * g.N + min(wn0 + j * 16 + kq * 4 + e, g.N - 1)) : 0.f;
-        auto finished = [&](int i, int j) __attribute__((always_inline)) {
-            float v[4];
+        // Through LDS, so that a store covers whole lines of a row: a wavefront's outputs go to a region of its own, 16-byte chunk c of row r at
+        // chunk c ^ (r % CH), and come back 16 bytes per lane, CH lanes a row.  (8 bytes per lane from the registers: 8192 x 37888 x 3584 1403 us,
+        // so 1130.)  Rows of an odd number of channels start at any even address; the stores are as wide there (2 bytes at a time from the
+        // registers: 4138 x 2847 x 944 40.6 us, so ODD).
+        constexpr int CH = C::WTN / 8, RPI = kWave / CH;
+        static_assert(C::WTM * C::WTN * 2 * (NG / kWave) <= C::LDS_BYTES, "outputs fit in the ring");
+        if constexpr (KS == 1) lds_barrier();  // every wavefront has read its last operands
+        uint8_t* mine = smem + wave * (C::WTM * C::WTN * 2);
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = acc[i][j][e] + bb[j][e];
-            return bf16 ? make_uint2(Lo<LLMQ_BF16>::pack2(v[0], v[1]), Lo<LLMQ_BF16>::pack2(v[2], v[3]))
-                        : make_uint2(Lo<LLMQ_F16>::pack2(v[0], v[1]), Lo<LLMQ_F16>::pack2(v[2], v[3]));
-        };
-        if (wide) {
-            // Through LDS, so that a store covers whole lines of a row: a wavefront's outputs go to a region of its own, 16-byte chunk c of row r at
-            // chunk c ^ (r % CH), and come back 16 bytes per lane, CH lanes a row.  (8 bytes per lane from the registers: 8192 x 37888 x 3584 1403 us,
-            // so 1130.)
-            constexpr int CH = C::WTN / 8, RPI = kWave / CH;
-            static_assert(C::WTM * C::WTN * 2 * (NG / kWave) <= C::LDS_BYTES, "outputs fit in the ring");
-            if constexpr (KS == 1) lds_barrier();  // every wavefront has read its last operands
-            uint8_t* mine = smem + wave * (C::WTM * C::WTN * 2);
+        for (int i = 0; i < TM; i++)
 #pragma unroll
-            for (int i = 0; i < TM; i++)
+            for (int j = 0; j < TN; j++) {
+                const int r = i * 16 + l16;
+                float v[4];
 #pragma unroll
-                for (int j = 0; j < TN; j++) {
-                    const int r = i * 16 + l16;
-                    *reinterpret_cast<uint2*>(mine + (r * CH + ((2 * j + (kq >> 1)) ^ (r % CH))) * 16 + (kq & 1) * 8) = finished(i, j);
-                }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-            const int c = lane % CH, n = wn0 + c * 8;
-#pragma unroll
-            for (int k = 0; k < C::WTM / RPI; k++) {
-                const int r = k * RPI + lane / CH;
-                const uint4 v = *reinterpret_cast<const uint4*>(mine + (r * CH + (c ^ (r % CH))) * 16);
-                if (wm0 + r < row_end && n < g.N) store_streaming(reinterpret_cast<uint16_t*>(g.out) + (int64_t)(wm0 + r) * g.ldo + n, v);
+                for (int e = 0; e < 4; e++) v[e] = acc[i][j][e] + bb[j][e];
+                *reinterpret_cast<uint2*>(mine + (r * CH + ((2 * j + (kq >> 1)) ^ (r % CH))) * 16 + (kq & 1) * 8) =
+                    bf16 ? make_uint2(Lo<LLMQ_BF16>::pack2(v[0], v[1]), Lo<LLMQ_BF16>::pack2(v[2], v[3]))
+                         : make_uint2(Lo<LLMQ_F16>::pack2(v[0], v[1]), Lo<LLMQ_F16>::pack2(v[2], v[3]));
             }
-        } else {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+        const int c = lane % CH, n = wn0 + c * 8;
 #pragma unroll
-            for (int i = 0; i < TM; i++) {
-                const int m = wm0 + i * 16 + l16;
-                if (m >= row_end) continue;
-#pragma unroll
-                for (int j = 0; j < TN; j++) {
-                    const int n = wn0 + j * 16 + kq * 4;
-                    const uint2 h = finished(i, j);
-                    const uint32_t w[2] = {h.x, h.y};
-                    uint16_t* to = reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n;
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (n + e < g.N) to[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
-                }
-            }
+        for (int k = 0; k < C::WTM / RPI; k++) {
+            const int r = k * RPI + lane / CH;
+            const uint4 v = *reinterpret_cast<const uint4*>(mine + (r * CH + (c ^ (r % CH))) * 16);
+            if (wm0 + r < row_end) store8(reinterpret_cast<uint16_t*>(g.out) + (int64_t)(wm0 + r) * g.ldo + n, v, g.N - n);
         }
     }
 }
 
-// The splits' sums in order, bias, rounding; 8 channels per thread, all splits requested before the first is used.  WIDE: rows of whole 16-byte
-// pieces.  (us with two splits of 777 x 3584: 4 channels per thread 7.9, so 6.2; partial sums stored past
-// the L2: products 2-10 % slower.)
-template <bool WIDE>
+// The splits' sums in order, bias, rounding; 8 channels per thread, all splits requested before the first is used.  (us with two splits of 777 x 3584: 4
+// channels per thread 7.9, so 6.2; partial sums stored past the L2: products 2-10 % slower.)
 __global__ __launch_bounds__(256) void block_reduce_kernel(BlockArgs g, int splits) {
-    const int64_t per_row = (g.N + 7) / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t ldp = partial_ld(g.N), per_row = ldp / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= per_row * g.M) return;
     const int m = (int)((uint64_t)i <= 0xffffffffu ? (uint32_t)i / (uint32_t)per_row : i / per_row), n = (int)(i - (int64_t)m * per_row) * 8;
-    const int64_t plane = (int64_t)g.M * g.N;
-    const float* p = g.partials + (int64_t)m * g.N + n;
-    uint16_t* to = reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n;
+    const int64_t plane = (int64_t)g.M * ldp;
+    const float* p = g.partials + (int64_t)m * ldp + n;
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (WIDE) {
-        v4f q[kMostSplits][2];
+    v4f q[kMostSplits][2];  // (past the last channel: padding that nobody wrote, and nobody keeps)
 #pragma unroll
-        for (int k = 0; k < kMostSplits; k++)
-            if (k < splits) {  // uniform
-                q[k][0] = *reinterpret_cast<const v4f*>(p + k * plane);
-                q[k][1] = *(reinterpret_cast<const v4f*>(p + k * plane) + 1);
-            }
+    for (int k = 0; k < kMostSplits; k++)
+        if (k < splits) {  // uniform
+            q[k][0] = *reinterpret_cast<const v4f*>(p + k * plane);
+            q[k][1] = *(reinterpret_cast<const v4f*>(p + k * plane) + 1);
+        }
 #pragma unroll
-        for (int k = 0; k < kMostSplits; k++)
-            if (k < splits)
+    for (int k = 0; k < kMostSplits; k++)
+        if (k < splits)
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] += q[k][e / 4][e % 4];
-    } else {
-        for (int k = 0; k < splits; k++)
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (n + e < g.N) v[e] += p[k * plane + e];
-    }
+            for (int e = 0; e < 8; e++) v[e] += q[k][e / 4][e % 4];
     if (g.bias)
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] += load_as_f32(g.bias, g.bias_dtype, min(n + e, g.N - 1));
     const bool bf16 = g.out_dtype == LLMQ_BF16;
     uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-        w[e] = bf16 ? Lo<LLMQ_BF16>::pack2(v[2 * e], v[2 * e + 1]) : Lo<LLMQ_F16>::pack2(v[2 * e], v[2 * e + 1]);
-    if (WIDE) {
-        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (n + e < g.N) to[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
-    }
+    for (int e = 0; e < 4; e++) w[e] = bf16 ? Lo<LLMQ_BF16>::pack2(v[2 * e], v[2 * e + 1]) : Lo<LLMQ_F16>::pack2(v[2 * e], v[2 * e + 1]);
+    store8(reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n, make_uint4(w[0], w[1], w[2], w[3]), g.N - n);
 }
 
 template <class C, bool GROUPED, bool SPLIT>
@@ -491,11 +463,9 @@ int launch_tile(const BlockArgs& g, int splits, hipStream_t st) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * tiles_n), SPLIT ? splits : 1), dim3(C::NT), C::LDS_BYTES, st, g);
     if (launch_status() != LLMQ_OK) return LLMQ_ERR_LAUNCH;
     if (SPLIT) {
-        const int64_t n = (int64_t)((g.N + 7) / 8) * g.M;
+        const int64_t n = partial_ld(g.N) / 8 * g.M;
         if (n > 0xffffff00LL || splits > kMostSplits) return LLMQ_ERR_SHAPE;
-        const bool wide = (g.N & 7) == 0 && (g.ldo & 7) == 0 && aligned16(g.out);
-        if (wide) hipLaunchKernelGGL(block_reduce_kernel<true>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g, splits);
-        else hipLaunchKernelGGL(block_reduce_kernel<false>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g, splits);
+        hipLaunchKernelGGL(block_reduce_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g, splits);
         return launch_status();
     }
     return LLMQ_OK;

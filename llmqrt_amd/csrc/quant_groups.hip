@@ -286,6 +286,10 @@ __global__ __launch_bounds__(NT * RPB) void add_norm_kernel(NormArgs a) {
     });
 }
 
+// Threads per row and chunks per thread, by the length of a row and how many rows fill the chip: a few rows are a chain of latencies (load, reduction,
+// codes), which more threads with less each shorten; many are arithmetic that every wavefront repeats per row.  A group's scale costs two
+// divisions per chunk, which favours fewer chunks per thread.  us, K = 8192, 1024 x 1 / 512 x 2: 1 row int8 3.83 / 3.67, group 3.61 / 3.87; 128 rows 5.15 /
+// 4.99, 5.09 / 5.36; 333 rows 7.59 / 7.20, 7.34 / 7.54.  A wavefront per row at K = 896, 8192 rows: int8 13.1 us (0.95 of a copy's rate).
 template <int DT, int OUT>
 int launch_add_norm(const NormArgs& a, hipStream_t st) {
     const int64_t chunks = a.K >> 3;
@@ -297,7 +301,8 @@ int launch_add_norm(const NormArgs& a, hipStream_t st) {
         if (a.M < 400) LLMQ_NORM(1, 512, 1);
         else LLMQ_NORM(2, 256, 1);
     } else if (chunks <= 1024) {
-        if (a.M < 400) LLMQ_NORM(1, 1024, 1);
+        if (a.M < 400 && OUT == OUT_GROUP) LLMQ_NORM(1, 1024, 1);
+        else if (a.M < 400) LLMQ_NORM(2, 512, 1);
         else LLMQ_NORM(4, 256, 1);
     } else if (chunks <= 2560) LLMQ_NORM(5, 512, 1);
     else LLMQ_NORM(0, 512, 1);
