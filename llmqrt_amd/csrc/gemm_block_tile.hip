@@ -136,7 +136,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     }
     const int n0 = tn * C::BN;
     const int kb0 = SPLIT ? blockIdx.y * g.blocks_per_split : 0, kb1 = SPLIT ? min(g.KB, kb0 + g.blocks_per_split) : g.KB;
-    const int kfull = (min(kb1, g.K / kScaleBlock) - kb0) / KS;  // whole blocks of each group; what is left of this split comes after them
+    const int kfull = (min(kb1, g.K / kScaleBlock) - kb0) / KS;  // whole blocks of each group
     const uint8_t* B = g.B + (int64_t)expert * g.N * g.ldb;
     const float* sw = g.sw + (int64_t)expert * g.NB * g.KB;
 
@@ -163,10 +163,24 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     // The walk over K starts at an eighth that follows from the tile of channels and wraps around: the XCDs work on different channels, and so do not
     // all ask for the same part of the rows at once, which lie the same distance apart and fall on few memory channels (us, from 0 / so: 777 x 3584 x
     // 18944 on 128 x 256 tiles 130 / 115, in two splits 82 / 76).  A channel's sums have one order for every token of a call.
-    int ld_kb = kb0 + group + tn * kNumXcd / tiles_n * kfull / kNumXcd * KS;
+    int ld_kb = kb0 + group + tn * kNumXcd / tiles_n * kfull / kNumXcd * KS, ld_it = 0;
+    // What the groups' whole blocks leave of this split comes last: at most a block for each group, one of them ragged.  Its missing chunks are read as
+    // the block's first one (a group without a block: of any), and zeros take their place in the weights' operand.  What the tokens and the scales
+    // have there belongs to the same row and channels, so where it is not finite the result is not either.
+    const bool rest = kb0 + kfull * KS < kb1;  // block-uniform
+    const int kall = kfull + (rest ? 1 : 0), tail_kb = min(kb0 + kfull * KS + group, g.KB - 1);
+    const int left = kb0 + kfull * KS + group < kb1 ? min(g.K - (kb0 + kfull * KS + group) * kScaleBlock, kScaleBlock) : 0;
+    uint32_t back = 0;  // of the lane's chunk, in the block that is requested
+    auto at_tail = [&]() __attribute__((always_inline)) {
+        if (ld_it != kfull) return;
+        ld_kb = tail_kb;
+        if (ld_chunk * 16 >= min(left, g.K - tail_kb * kScaleBlock)) back = ld_chunk * 16;
+    };
+    at_tail();
     auto next_kb = [&]() __attribute__((always_inline)) {
-        ld_kb += KS;
+        ld_kb += KS, ld_it++;
         if (ld_kb >= kb0 + kfull * KS) ld_kb -= kfull * KS;
+        at_tail();
     };
     auto issue = [&](int stage, auto d_c) __attribute__((always_inline)) {  // piece d of block ld_kb
         constexpr int d = decltype(d_c)::value;
@@ -174,7 +188,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         if constexpr (d < C::A_LOADS + C::B_LOADS) {
             const uint8_t* base = (d < C::A_LOADS ? a_base : b_base) + (int64_t)ld_kb * kScaleBlock;
             const uint32_t m0v = to + (uint32_t)d * (NG * 16) + (uint32_t)wave * 1024;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(off[d]), "s"(base) : "memory", "m0");
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(off[d] - back), "s"(base) : "memory", "m0");
         } else {
             const float* p = s_ptr + ld_kb;
             const uint32_t m0v = to + C::DATA + (uint32_t)wave * 256;
@@ -273,17 +287,17 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     auto drive = [&](auto&& ready, auto&& step) __attribute__((always_inline)) {
         unrolled<0, NS - 1>([&](auto n_c) __attribute__((always_inline)) {
             constexpr int n = decltype(n_c)::value;
-            if (n < kfull) {
+            if (n < kall) {
                 unrolled<0, C::LPT>([&](auto d) __attribute__((always_inline)) { issue(n, d); });
                 next_kb();
             }
         });
-        if (kfull > 0) {
-            wait_loads(min(kfull, NS - 1) - 1);
+        if (kall > 0) {
+            wait_loads(min(kall, NS - 1) - 1);
             lds_barrier();
             ready();
         }
-        if (NS - 1 < kfull) unrolled<0, EARLY>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
+        if (NS - 1 < kall) unrolled<0, EARLY>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
         int stage = 0, kt = 0;
         auto one = [&](auto rest_c, auto first_c, auto next_c, int younger) __attribute__((always_inline)) {
             const int next = stage == NS - 1 ? 0 : stage + 1, prev = stage == 0 ? NS - 1 : stage - 1;
@@ -291,25 +305,11 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
             stage = next, kt++;
         };
 #pragma unroll 1
-        while (kt + NS < kfull) one(yes, yes, yes, NS - 2);
-        if (kt + NS == kfull) one(yes, no, yes, NS - 2);
+        while (kt + NS < kall) one(yes, yes, yes, NS - 2);
+        if (kt + NS == kall) one(yes, no, yes, NS - 2);
 #pragma unroll 1
-        while (kt + 1 < kfull) one(no, no, yes, kfull - 2 - kt);
-        if (kt < kfull) one(no, no, no, 0);
-    };
-    const bool ragged = kb0 + kfull * KS < kb1;  // block-uniform
-    auto load_ragged = [&]() __attribute__((always_inline)) {  // at most a block for each group, one of them ragged, through registers; what is missing is zeros
-        lds_barrier();
-        const int kb = kb0 + kfull * KS + group, left = kb < kb1 ? g.K - kb * kScaleBlock : 0;
-        uint8_t* to = smem + group * C::SUB;
-#pragma unroll
-        for (int i = 0; i < C::A_LOADS + C::B_LOADS; i++) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (ld_chunk * 16 < left) v = *reinterpret_cast<const uint4*>((i < C::A_LOADS ? a_base : b_base) + (int64_t)kb * kScaleBlock + off[i]);
-            *reinterpret_cast<uint4*>(to + i * (NG * 16) + tid * 16) = v;
-        }
-        *reinterpret_cast<float*>(to + C::DATA + tid * 4) = left > 0 ? s_ptr[kb] : 0.f;
-        lds_barrier();
+        while (kt + 1 < kall) one(no, no, yes, kall - 2 - kt);
+        if (kt < kall) one(no, no, no, 0);
     };
     if (row0 + wm * C::WTM >= row_end || n0 + wn * C::WTN >= g.N) {
         // a wavefront whose rows or channels all lie behind the last one loads its pieces and waits with the others, and multiplies nothing
@@ -325,20 +325,21 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
             }
             if constexpr (decltype(first_c)::value) unrolled<0, EARLY>([&](auto d) __attribute__((always_inline)) { issue(stage, d); });
         });
-        if (ragged) load_ragged();
         if constexpr (KS > 1) lds_barrier(), lds_barrier(), lds_barrier();
         else if (!SPLIT) lds_barrier();
         return;
     }
     drive([&]() __attribute__((always_inline)) { first_operands(sub); },
           [&](int stage, int next, int prev, int younger, auto rest_c, auto first_c, auto next_c) __attribute__((always_inline)) {
+              if (!decltype(next_c)::value && rest) {  // the last block: a lane's chunks kq and kq + 4 of it
+                  const int lo = kq * 16 < left ? -1 : 0, hi = (kq + 4) * 16 < left ? -1 : 0;
+#pragma unroll
+                  for (int j = 0; j < TN; j++)
+#pragma unroll
+                      for (int e = 0; e < 8; e++) b[j][e] &= e < 4 ? lo : hi;
+              }
               k_block(sub + stage * C::STAGE, sub + next * C::STAGE, stage, prev, younger, rest_c, first_c, next_c);
           });
-    if (ragged) {
-        load_ragged();
-        first_operands(sub);
-        k_block(sub, sub, 0, 0, 0, no, no, no);
-    }
     unrolled<TT - DELAY, TT>([&](auto t_c) __attribute__((always_inline)) { scale_in(t_c, s[decltype(t_c)::value / TN]); });
     if constexpr (KS > 1) {  // the groups' sums, in order
         v4f* sums = reinterpret_cast<v4f*>(smem) + ((group - 1) * (NG / kWave) + wave) * TT * kWave + lane;
@@ -382,7 +383,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         // Through LDS, so that a store covers whole lines of a row: a wavefront's outputs go to a region of its own, 16-byte chunk c of row r at
         // chunk c ^ (r % CH), and come back 16 bytes per lane, CH lanes a row.  (8 bytes per lane from the registers: 8192 x 37888 x 3584 1403 us,
         // so 1130.)  Rows of an odd number of channels start at any even address; the stores are as wide there (2 bytes at a time from the
-        // registers: 4138 x 2847 x 944 40.6 us, so ODD).
+        // registers: 4138 x 2847 x 944 40.6 us, so 25.8).
         constexpr int CH = C::WTN / 8, RPI = kWave / CH;
         static_assert(C::WTM * C::WTN * 2 * (NG / kWave) <= C::LDS_BYTES, "outputs fit in the ring");
         if constexpr (KS == 1) lds_barrier();  // every wavefront has read its last operands
