@@ -6,7 +6,7 @@
  *  - The caller owns every buffer (inputs, outputs, workspaces); the library allocates
  *    nothing, never synchronises with the host and launches on the stream it is given
  *    (0 = the null stream).  Calls are asynchronous.  State kept between calls, all of
- *    it per host thread: the *_force_plan tuning hooks, and the last GEMM and AWQ plans (a function of
+ *    it per host thread: the *_force_plan tuning hooks, and the last GEMM, AWQ and block-scaled plans (a function of
  *    sizes and format alone).  llmq_gemm_w8a8_static has a scratch array per GPU.
  *  - Matrices are row-major; `ld*` is the row stride in ELEMENTS.
  *  - Return value: LLMQ_OK (0) or a negative llmq_status; llmq_status_string() names it.
@@ -400,8 +400,8 @@ int llmq_add_rmsnorm(int out, const void* x, int x_dtype, int64_t M, int64_t K, 
 
 /* out[m, n] = out_dtype( sum_b a_scale[m, b] w_scale[n / 128, b] sum_{k in block b} A[m, k] B[n, k]  + bias[n] ), blocks of 128 of K, fp32.
  * A: e4m3fn [M, K] (lda >= K), B: e4m3fn [N, K] (ldb >= K), 16-byte aligned, K, lda, ldb multiples of 16 and at most 2^23; a_scale: fp32
- * [M, ceil(K / 128)], w_scale: fp32 [ceil(N / 128), ceil(K / 128)], contiguous; bias: [N] bf16 / f16 / f32 or null; out: bf16 / f16, ldo >= N.
- * workspace: >= llmq_gemm_fp8_block_workspace_bytes(M, N, K) bytes, 16-byte aligned (may be NULL when that is 0). */
+ * [M, ceil(K / 128)], w_scale: fp32 [ceil(N / 128), ceil(K / 128)], contiguous; bias: [N] bf16 / f16 / f32 or null; out: bf16 / f16, ldo >= N, any
+ * even address.  workspace: >= llmq_gemm_fp8_block_workspace_bytes(M, N, K) bytes, 16-byte aligned (may be NULL when that is 0). */
 int llmq_gemm_fp8_block(const uint8_t* A, int64_t lda, const float* a_scale, const uint8_t* B, int64_t ldb, const float* w_scale,
                         const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K,
                         void* workspace, size_t workspace_bytes, llmq_stream_t stream);
@@ -414,7 +414,8 @@ size_t llmq_gemm_fp8_block_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int llmq_gemm_fp8_block_grouped(const uint8_t* A, int64_t lda, const float* a_scale, const uint8_t* B, const float* w_scale,
                                 const int32_t* offsets, int64_t experts, const void* bias, int bias_dtype, void* out, int out_dtype,
                                 int64_t ldo, int64_t M, int64_t N, int64_t K, llmq_stream_t stream);
-/* Tuning / test hook: tile configuration `cfg` (-1: the built-in choice) and K split of later calls of the two products.  Per host thread. */
+/* Tuning / test hook: configuration `cfg` (0-7: tiles, 8-14: the row-streaming kernel where the tokens fit it, -1: the built-in choice) and K split of
+ * later calls of the two products (by experts: tiles only, no split).  Per host thread. */
 int llmq_gemm_fp8_block_force_plan(int cfg, int splits);
 
 #ifdef __cplusplus

@@ -3,9 +3,9 @@
 Layout:
   csrc/            HIP kernels + C ABI (include/llmq.h) -> lib/libllmq_gfx950.so
   _abi.py          ctypes loader (no fallback: a missing library raises)
-  quantize.py      activation quantizers (reference names)
-  norm.py          RMSNorm, alone or fused with the per-token quantizer
-  sq_fp8_kernels   drop-in for runtime.sq_fp8_kernels
+  quantize.py      activation quantizers (reference names), fp8 per token and 128 channels, block-scaled weights
+  norm.py          RMSNorm, alone, behind the residual's addition, and with an output in 8 bits
+  sq_fp8_kernels   drop-in for runtime.sq_fp8_kernels; block-scaled fp8 products, alone and by experts
   awq_kernels      drop-in for runtime.triton_kernels.awq_kernels
   linear/          quantized Linear modules + registry
   fused_utils.py   fuse q/k/v or gate/up sibling modules into one

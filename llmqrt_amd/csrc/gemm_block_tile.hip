@@ -101,12 +101,13 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         row0 = tm * C::BM, row_end = g.M;
     } else {
         // the experts' tiles of rows, counted by every wavefront for itself: 64 experts at a time
-        int total = 0;
-        for (int e0 = 0; e0 < g.experts; e0 += kWave) {
-            int first = 0, last = 0;
+        int total = 0, first, last, mine, upto;
+        auto count = [&](int e0, int before) __attribute__((always_inline)) {
+            first = last = 0;
             if (e0 + lane < g.experts) expert_rows(g, e0 + lane, first, last);
-            total += __shfl(wave_prefix((last - first + C::BM - 1) / C::BM), kWave - 1);
-        }
+            mine = (last - first + C::BM - 1) / C::BM, upto = before + wave_prefix(mine);
+        };
+        for (int e0 = 0; e0 < g.experts; e0 += kWave) count(e0, total), total = __shfl(upto, kWave - 1);
         total = __builtin_amdgcn_readfirstlane(total);
         const int64_t nblk = min((int64_t)gridDim.x, (int64_t)total * tiles_n);
         if (blockIdx.x >= nblk) return;  // block-uniform
@@ -115,9 +116,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         int before = 0, tiles = 1;
         row0 = row_end = 0;
         for (int e0 = 0; e0 < g.experts; e0 += kWave) {
-            int first = 0, last = 0;
-            if (e0 + lane < g.experts) expert_rows(g, e0 + lane, first, last);
-            const int mine = (last - first + C::BM - 1) / C::BM, upto = before + wave_prefix(mine);
+            if (g.experts > kWave) count(e0, before);  // (not again what is still there)
             const uint64_t has = __ballot(flat >= upto - mine && flat < upto);
             if (has) {
                 const int at = __ffsll((unsigned long long)has) - 1;
