@@ -15,23 +15,27 @@ thread_local int forced_cfg = -1, forced_splits = 0;
 // What a launch takes, in us, as a rule of the sizes alone:
 //   start + max(stream, loop) + 0.15 min(stream, loop) + what a K split adds
 // stream: the operands once at 6.6 TB/s, longer where some CUs have a block more than others.  loop: steps along K times what one takes, from
-// `alone` (a few blocks on the chip) to `alone` + `crowd` (one on every CU); with more blocks than CUs `full` for each of a CU's, and a last round that is
-// not full costs as the fourth root of what it holds (row-streaming kernel: all of it).  A split adds a launch and its sums' way out and back.
-// Fitted to 4300 random sizes (1-8192 tokens, 128-37888 channels, K 512-18944), every configuration and split timed with the weights out of
-// HBM: the choice is 1.8 % (2.2 % up to 64 tokens) slower than the fastest of the size on average, 10 % (14 %) in the worst 5 % of the sizes.  By
-// experts, 1200 sizes, the same constants: 2.9 %, 13 %.
-struct Cost { float start, alone, full, crowd; };
-constexpr Cost kTileCost[kNumBlockTiles] = {{6.86, 1.15, 2.21, 0.615}, {5.85, 0.757, 1.25, 0.232}, {5.28, 0.349, 0.809, 0.424}, {4.51, 0.354, 0.441, 0.152}, {3.78, 0.311, 0.364, 0.098}, {4.09, 0.278, 0.316, 0.044}, {6.15, 0.495, 0.906, 0.311}, {5.03, 0.329, 0.686, 0.235}};
-constexpr Cost kRowsCost[kNumBlockRows] = {{2.76, 0.34, 0.336, 0.026}, {3.05, 0.548, 0.764, 0.116}, {2.93, 0.4, 0.392, 0.055}, {3.08, 0.531, 0.712, 0.055}, {3.29, 0.704, 0.82, 0.114}, {3.18, 0.645, 1, 0.091}, {3.36, 0.551, 0.935, 0.557}};
+// `alone` (a few blocks on the chip) to `alone` + `crowd` (one on every CU); with more blocks than CUs `full` for each of a CU's, and `turn` from one to the next
+// (outputs out, first operands in); a last round that is not full costs as the fourth root of what it holds (row-streaming kernel: all of it).  A split
+// adds a launch and its sums' way out and back.
+// Fitted to random sizes (1-8192 tokens, 128-37888 channels, K 512-18944; up to 128 experts), every configuration and split timed with the weights out of
+// HBM.  The choice is slower than the fastest of the size by, on average and in the worst 5 % of the sizes: 1.4 % and 9 % (3900 sizes of more than 64
+// tokens), 2.0 % and 12 % (2000 of fewer), 1.9 % and 10 % (4000 by experts).  Without `turn` it was 1.8, 2.2 and 2.7 % on average.
+struct Cost { float start, alone, full, crowd, turn; };
+constexpr Cost kTileCost[kNumBlockTiles] = {{7.27, 1.27, 1.86, 0.544, 8.63}, {5.63, 0.639, 1.05, 0.417, 4.86}, {5.37, 0.325, 0.676, 0.411, 2.65}, {4.55, 0.363, 0.405, 0.124, 0.823},
+                                            {3.75, 0.319, 0.313, 0.043, 0.559}, {4.05, 0.281, 0.286, 0.049, 0.621}, {5.4, 0.466, 0.792, 0.29, 2.17}, {4.76, 0.344, 0.575, 0.182, 2.49}};
+constexpr Cost kRowsCost[kNumBlockRows] = {{2.74, 0.343, 0.298, 0.025, 0.417}, {3.04, 0.55, 0.655, 0.119, 1.52}, {2.9, 0.402, 0.356, 0.057, 0.402}, {3.07, 0.532, 0.605, 0.057, 1.59},
+                                           {3.28, 0.706, 0.714, 0.116, 2.61}, {3.18, 0.646, 0.794, 0.092, 1.39}, {3.34, 0.56, 0.888, 0.545, 0.384}};
 
 float cost_us(const Cost& c, double blocks, double steps, double bytes, bool rows) {
     const float r = (float)(blocks / 256.0), whole = floorf(r), rest = r - whole;
-    float step = c.alone + c.crowd * std::min(r, 1.f), stream = (float)(bytes / 6.6e6);
+    const float step = c.alone + c.crowd * std::min(r, 1.f);
+    float rounds = 1.f, stream = (float)(bytes / 6.6e6);
     if (r > 1.f) {
-        step = std::max(step, c.full * (whole + (rows ? ceilf(rest) : sqrtf(sqrtf(rest)))));
+        rounds = whole + (rows ? ceilf(rest) : sqrtf(sqrtf(rest)));
         stream *= 1.f + 0.3f * (ceilf(r) / r - 1.f);
     }
-    const float loop = (float)steps * step;
+    const float loop = std::max((float)steps * step, rounds > 1.f ? (float)steps * c.full * rounds + c.turn * (rounds - 1.f) : 0.f);
     return c.start + std::max(stream, loop) + 0.15f * std::min(stream, loop);
 }
 
@@ -46,7 +50,7 @@ BlockPlan search(int64_t M, int64_t N, int64_t K) {
             if (s > 1 && (KB / s < 4 || tiles * s > (t.bm * t.bn > 64 * 128 ? 300 : 600))) break;
             const int per = (KB + s - 1) / s, splits = (KB + per - 1) / per;
             float us = cost_us(kTileCost[c], tiles * splits, (per + t.ks - 1) / t.ks, (double)N * K + (double)M * K, false);
-            if (splits > 1) us += 3.f + (float)(splits * (double)M * N * 8 / 5.5e6);
+            if (splits > 1) us += 3.f + (float)(splits * (double)M * N * 8 / 7e6);
             if (us < least) least = us, best = {c, splits, per};
         }
     }
@@ -72,7 +76,7 @@ BlockPlan plan(int64_t M, int64_t N, int64_t K) {
     return last;
 }
 
-// The host knows the rows of all experts together, not each one's: every expert that may have rows is taken to end with half a tile.
+// The host knows the rows of all experts together, not each one's: every expert that may have rows is taken to end with about half a tile.
 int plan_grouped(int64_t rows, int64_t experts, int64_t N, int64_t K) {
     if (forced_cfg >= 0 && forced_cfg < kRowsCfg) return forced_cfg;
     thread_local int64_t of[4] = {0, 0, 0, 0};
@@ -83,7 +87,7 @@ int plan_grouped(int64_t rows, int64_t experts, int64_t N, int64_t K) {
     float least = 3e38f;
     for (int c = 0; c < kNumBlockTiles; c++) {
         const BlockTile& t = kBlockTiles[c];
-        const double tiles = std::max(used, (double)rows / t.bm + 0.5 * used) * (double)((N + t.bn - 1) / t.bn);
+        const double tiles = std::max(used, (double)rows / t.bm + 0.45 * used) * (double)((N + t.bn - 1) / t.bn);
         const float us = cost_us(kTileCost[c], tiles, (KB + t.ks - 1) / t.ks, used * (double)N * K + (double)rows * K, false);
         if (us < least) least = us, last = c;
     }
