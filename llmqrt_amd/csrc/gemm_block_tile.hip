@@ -87,7 +87,8 @@ __device__ __forceinline__ void tile_of(int pid, int tiles_m, int tiles_n, int& 
     tn = (pid % width / size + group * tiles_n / ((tiles_m + kGroupM - 1) / kGroupM)) % tiles_n;
 }
 
-template <class C, bool GROUPED, bool SPLIT>
+// TAIL: K, or a split's share of it, is not made of whole blocks for every group
+template <class C, bool GROUPED, bool SPLIT, bool TAIL>
 __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     constexpr int TM = C::TM, TN = C::TN, NG = C::NG, NS = C::NS, TT = C::TT, KS = C::KS;
@@ -165,24 +166,25 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     // The walk over K starts at an eighth that follows from the tile of channels and wraps around: the XCDs work on different channels, and so do not
     // all ask for the same part of the rows at once, which lie the same distance apart and fall on few memory channels (us, from 0 / so: 777 x 3584 x
     // 18944 on 128 x 256 tiles 130 / 115, in two splits 82 / 76).  A channel's sums have one order for every token of a call.
-    int ld_kb = kb0 + group + tn * kNumXcd / tiles_n * kfull / kNumXcd * KS, ld_it = 0;
+    int ld_kb = kb0 + group + tn * kNumXcd / tiles_n * kfull / kNumXcd * KS;
     // What the groups' whole blocks leave of this split comes last: at most a block for each group, one of them ragged.  Its missing chunks are read as
     // the block's first one (a group without a block: of any), and zeros take their place in the weights' operand.  What the tokens and the scales
     // have there belongs to the same row and channels, so where it is not finite the result is not either.
-    const bool rest = kb0 + kfull * KS < kb1;  // block-uniform
+    // It has a place of its own behind the loop below, so that the others' loads have no part in it (us, each load's offset corrected in the loop / so: 8192 x
+    // 37888 x 3584 1055 / 990, 1000 x 4608 x 3584 26.2 / 25.4).
+    const bool rest = TAIL && kb0 + kfull * KS < kb1;  // block-uniform
     const int kall = kfull + (rest ? 1 : 0), tail_kb = min(kb0 + kfull * KS + group, g.KB - 1);
     const int left = kb0 + kfull * KS + group < kb1 ? min(g.K - (kb0 + kfull * KS + group) * kScaleBlock, kScaleBlock) : 0;
-    uint32_t back = 0;  // of the lane's chunk, in the block that is requested
-    auto at_tail = [&]() __attribute__((always_inline)) {
-        if (ld_it != kfull) return;
-        ld_kb = tail_kb;
-        if (ld_chunk * 16 >= min(left, g.K - tail_kb * kScaleBlock)) back = ld_chunk * 16;
-    };
-    at_tail();
     auto next_kb = [&]() __attribute__((always_inline)) {
-        ld_kb += KS, ld_it++;
+        ld_kb += KS;
         if (ld_kb >= kb0 + kfull * KS) ld_kb -= kfull * KS;
-        at_tail();
+    };
+    auto last_kb = [&]() __attribute__((always_inline)) {  // the last block of all is requested next
+        if (!TAIL) return;
+        ld_kb = rest ? tail_kb : ld_kb;
+        const uint32_t back = rest && ld_chunk * 16 >= min(left, g.K - tail_kb * kScaleBlock) ? ld_chunk * 16 : 0;
+#pragma unroll
+        for (int i = 0; i < C::A_LOADS + C::B_LOADS; i++) off[i] -= back;
     };
     auto issue = [&](int stage, auto d_c) __attribute__((always_inline)) {  // piece d of block ld_kb
         constexpr int d = decltype(d_c)::value;
@@ -190,7 +192,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         if constexpr (d < C::A_LOADS + C::B_LOADS) {
             const uint8_t* base = (d < C::A_LOADS ? a_base : b_base) + (int64_t)ld_kb * kScaleBlock;
             const uint32_t m0v = to + (uint32_t)d * (NG * 16) + (uint32_t)wave * 1024;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(off[d] - back), "s"(base) : "memory", "m0");
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(off[d]), "s"(base) : "memory", "m0");
         } else {
             const float* p = s_ptr + ld_kb;
             const uint32_t m0v = to + C::DATA + (uint32_t)wave * 256;
@@ -244,12 +246,13 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     constexpr int DELAY = TT > 4 ? 3 : 2;  // (four tiles: s_next is the next block's from the third on)
     constexpr int PER = (C::LPT + TT - 1) / TT, EARLY = TN * PER < C::LPT ? TN * PER : C::LPT;
     static_assert(EARLY + (TT - TN) * PER >= C::LPT, "all of a block is requested before the wait that counts it");
-    auto k_block = [&](const uint8_t* st, const uint8_t* next, int stage, int prev, int younger, auto rest_c, auto first_c, auto next_c) __attribute__((always_inline)) {
-        constexpr bool REST = decltype(rest_c)::value, FIRST = decltype(first_c)::value, NEXT = decltype(next_c)::value;
+    auto k_block = [&](const uint8_t* st, const uint8_t* next, int stage, int prev, int younger, auto rest_c, auto first_c, auto next_c, auto last_c) __attribute__((always_inline)) {
+        constexpr bool REST = decltype(rest_c)::value, FIRST = decltype(first_c)::value, NEXT = decltype(next_c)::value, LAST = decltype(last_c)::value;
         unrolled<0, TT>([&](auto t_c) __attribute__((always_inline)) {
             constexpr int t = decltype(t_c)::value, i = t / TN, j = t % TN;
             if constexpr (NEXT && i == TM - 1 && j == 0) {
                 if constexpr (REST) next_kb();
+                if constexpr (LAST) last_kb();
                 wait_loads(younger);
                 lds_barrier();
             }
@@ -285,11 +288,12 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
 
     const std::true_type yes;
     const std::false_type no;
-    // all of the K loop; step(stage, next, prev, younger, REST, FIRST, NEXT) does a block
+    // all of the K loop; step(stage, next, prev, younger, REST, FIRST, NEXT, LAST) does a block
     auto drive = [&](auto&& ready, auto&& step) __attribute__((always_inline)) {
         unrolled<0, NS - 1>([&](auto n_c) __attribute__((always_inline)) {
             constexpr int n = decltype(n_c)::value;
             if (n < kall) {
+                if (n == kall - 1) last_kb();
                 unrolled<0, C::LPT>([&](auto d) __attribute__((always_inline)) { issue(n, d); });
                 next_kb();
             }
@@ -299,27 +303,34 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
             lds_barrier();
             ready();
         }
-        if (NS - 1 < kall) unrolled<0, EARLY>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
+        if (NS - 1 < kall) {
+            if (NS == kall) last_kb();
+            unrolled<0, EARLY>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
+        }
         int stage = 0, kt = 0;
-        auto one = [&](auto rest_c, auto first_c, auto next_c, int younger) __attribute__((always_inline)) {
+        auto one = [&](auto rest_c, auto first_c, auto next_c, auto last_c, int younger) __attribute__((always_inline)) {
             const int next = stage == NS - 1 ? 0 : stage + 1, prev = stage == 0 ? NS - 1 : stage - 1;
-            step(stage, next, prev, younger, rest_c, first_c, next_c);
+            step(stage, next, prev, younger, rest_c, first_c, next_c, last_c);
             stage = next, kt++;
         };
 #pragma unroll 1
-        while (kt + NS < kall) one(yes, yes, yes, NS - 2);
-        if (kt + NS == kall) one(yes, no, yes, NS - 2);
+        while (kt + NS + (TAIL ? 1 : 0) < kall) one(yes, yes, yes, no, NS - 2);
+        if constexpr (TAIL) {
+            if (kt + NS < kall) one(yes, yes, yes, yes, NS - 2);
+        }
+        if (kt + NS == kall) one(yes, no, yes, no, NS - 2);
 #pragma unroll 1
-        while (kt + 1 < kall) one(no, no, yes, kall - 2 - kt);
-        if (kt < kall) one(no, no, no, 0);
+        while (kt + 1 < kall) one(no, no, yes, no, kall - 2 - kt);
+        if (kt < kall) one(no, no, no, no, 0);
     };
     if (row0 + wm * C::WTM >= row_end || n0 + wn * C::WTN >= g.N) {
         // a wavefront whose rows or channels all lie behind the last one loads its pieces and waits with the others, and multiplies nothing
         // (32768 rows on 28 of 32 experts, 4864 x 3584, 256-row tiles: 672 us multiplying, 606 not)
-        drive([] {}, [&](int stage, int, int prev, int younger, auto rest_c, auto first_c, auto next_c) __attribute__((always_inline)) {
+        drive([] {}, [&](int stage, int, int prev, int younger, auto rest_c, auto first_c, auto next_c, auto last_c) __attribute__((always_inline)) {
             if constexpr (decltype(rest_c)::value) {
                 unrolled<EARLY, C::LPT>([&](auto d) __attribute__((always_inline)) { issue(prev, d); });
                 next_kb();
+                if constexpr (decltype(last_c)::value) last_kb();
             }
             if constexpr (decltype(next_c)::value) {
                 wait_loads(younger);
@@ -332,15 +343,15 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         return;
     }
     drive([&]() __attribute__((always_inline)) { first_operands(sub); },
-          [&](int stage, int next, int prev, int younger, auto rest_c, auto first_c, auto next_c) __attribute__((always_inline)) {
-              if (!decltype(next_c)::value && rest) {  // the last block: a lane's chunks kq and kq + 4 of it
+          [&](int stage, int next, int prev, int younger, auto rest_c, auto first_c, auto next_c, auto last_c) __attribute__((always_inline)) {
+              if (TAIL && !decltype(next_c)::value && rest) {  // the last block: a lane's chunks kq and kq + 4 of it
                   const int lo = kq * 16 < left ? -1 : 0, hi = (kq + 4) * 16 < left ? -1 : 0;
 #pragma unroll
                   for (int j = 0; j < TN; j++)
 #pragma unroll
                       for (int e = 0; e < 8; e++) b[j][e] &= e < 4 ? lo : hi;
               }
-              k_block(sub + stage * C::STAGE, sub + next * C::STAGE, stage, prev, younger, rest_c, first_c, next_c);
+              k_block(sub + stage * C::STAGE, sub + next * C::STAGE, stage, prev, younger, rest_c, first_c, next_c, last_c);
           });
     unrolled<TT - DELAY, TT>([&](auto t_c) __attribute__((always_inline)) { scale_in(t_c, s[decltype(t_c)::value / TN]); });
     if constexpr (KS > 1) {  // the groups' sums, in order
@@ -446,9 +457,9 @@ __global__ __launch_bounds__(256) void block_reduce_kernel(BlockArgs g, int spli
     store8(reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n, make_uint4(w[0], w[1], w[2], w[3]), g.N - n);
 }
 
-template <class C, bool GROUPED, bool SPLIT>
+template <class C, bool GROUPED, bool SPLIT, bool TAIL>
 int launch_tile(const BlockArgs& g, int splits, hipStream_t st) {
-    auto kernel = block_tile_kernel<C, GROUPED, SPLIT>;
+    auto kernel = block_tile_kernel<C, GROUPED, SPLIT, TAIL>;
     if (C::LDS_BYTES > 64 * 1024) {
         static bool raised[64] = {};  // per device: the attribute belongs to the loaded code object of the current device
         int dev = 0;
@@ -474,10 +485,16 @@ int launch_tile(const BlockArgs& g, int splits, hipStream_t st) {
     return LLMQ_OK;
 }
 
+template <class C, bool TAIL>
+int launch_kind(const BlockArgs& g, int splits, hipStream_t st) {
+    if (g.offsets) return launch_tile<C, true, false, TAIL>(g, 1, st);
+    return splits > 1 ? launch_tile<C, false, true, TAIL>(g, splits, st) : launch_tile<C, false, false, TAIL>(g, 1, st);
+}
+
 template <class C>
 int launch_cfg(const BlockArgs& g, int splits, hipStream_t st) {
-    if (g.offsets) return launch_tile<C, true, false>(g, 1, st);
-    return splits > 1 ? launch_tile<C, false, true>(g, splits, st) : launch_tile<C, false, false>(g, 1, st);
+    const bool whole = g.K % kScaleBlock == 0 && g.KB % C::KS == 0 && (splits == 1 || g.blocks_per_split % C::KS == 0);
+    return whole ? launch_kind<C, false>(g, splits, st) : launch_kind<C, true>(g, splits, st);
 }
 
 }  // namespace
