@@ -168,6 +168,22 @@ def test_every_plan_exact(cuda, force, M, N, K, splits):
         assert same(gemm(a, w, sa, sw, bias), ref.bfloat16()), f"configuration {cfg}, {splits} splits"
 
 
+@pytest.mark.parametrize("K", [16, 112, 144, 256, 272, 400, 512, 528, 656, 784, 896, 912, 1040, 1280, 1424])
+def test_every_plan_at_the_end_of_k(cuda, force, K):
+    """Every number of blocks around the stages of a ring, whole ones and with a partial last one, shared by groups of wavefronts and by splits."""
+    for M, N in ((130, 200), (33, 72)):
+        a, w, sa, sw = exact_operands(M, N, K, K, cuda)
+        ref = product64(a, w, sa, sw)[0].bfloat16()
+        off = torch.tensor([0, 1, M - 20, M - 20, M], dtype=torch.int32, device=cuda)
+        wg, swg = w.expand(4, N, K).contiguous(), sw.expand(4, *sw.shape).contiguous()
+        for cfg in all_configs():
+            for splits in (1, 2, 4):
+                print("plan", cfg, splits, M, N, K, flush=True)
+                assert force(cfg, splits) == 0
+                assert same(gemm(a, w, sa, sw), ref), f"configuration {cfg}, {splits} splits"
+            assert same(grouped(a, wg, sa, swg, off), ref), f"configuration {cfg}, by experts"
+
+
 def test_product_strides(cuda):
     """Operands inside larger tensors, 16-byte aligned or not, and outputs of odd widths."""
     a, w, sa, sw = exact_operands(20, 50, 512, 9, cuda)
