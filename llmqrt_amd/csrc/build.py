@@ -18,9 +18,9 @@ LIB = OUT_DIR / "libllmq_gfx950.so"
 HOST_LIB = OUT_DIR / "_llmq_host.so"  # native forward passes of the modules (host code against torch and the C ABI)
 MICROBENCH_LIB = OUT_DIR / "libllmq_microbench_gfx950.so"  # hardware microbenchmarks for `bench.py --micro`; not the product
 # the tile GEMM is instantiated per operand format in four translation units (the long poles of the build), listed first
-SOURCES = ["gemm_tile_i8.hip", "gemm_tile_fp8.hip", "gemm_tile_fp8_e5m2.hip", "gemm_tile_f16.hip", "awq_stream.hip", "gemm_block_tile.hip", "gemm_block_rows.hip", "gemm_rows.hip", "gemm_mfma.hip", "abi.hip",
-           "quant.hip", "gemm_skinny.hip", "linear_fused.hip", "awq.hip", "awq_decode.hip", "awq_tile.hip", "gemm_block.hip",
-           "quant_groups.hip"]
+SOURCES = ["gemm_tile_i8.hip", "gemm_tile_fp8.hip", "gemm_tile_fp8_e5m2.hip", "gemm_tile_f16.hip", "gemm_block_tile.hip", "awq_stream.hip",
+           "gemm_block_rows.hip", "gemm_rows.hip", "gemm_mfma.hip", "abi.hip", "quant.hip", "gemm_skinny.hip", "linear_fused.hip", "awq.hip", "awq_decode.hip",
+           "awq_tile.hip", "gemm_block.hip", "quant_groups.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
