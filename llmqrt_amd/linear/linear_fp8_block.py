@@ -38,12 +38,15 @@ class _FP8BlockBase(LinearBase):
         self.register_buffer("bias", torch.zeros((*lead, out_features), dtype=dtype, device=dev) if bias else None)
 
     def _apply(self, fn, *args, **kwargs):
-        def moved(t):  # .half() and .bfloat16() are for the bias: codes and scales keep their types
+        kept = self.weight, self.weight_scale
+
+        def moved(t):  # .half() and .bfloat16() are for the bias and the outputs: codes and scales keep their types
             u = fn(t)
-            return u if u.dtype == t.dtype or t.dtype in _NAMES else t.to(u.device)
+            return t.to(u.device) if u.dtype != t.dtype and any(t is k for k in kept) else u
+        like = fn(torch.empty(0, dtype=self.dtype, device=self.weight.device))  # the type that a module without a bias is converted to
         out = super()._apply(moved, *args, **kwargs)
-        if self.bias is not None and self.bias.dtype in _NAMES:
-            self.dtype = self.bias.dtype
+        if like.dtype in _NAMES:
+            self.dtype = like.dtype
         return out
 
     @torch.no_grad()

@@ -1,0 +1,44 @@
+"""CPU-only checks of the block-scaled FP8 modules: conversions, and what a module may be made from."""
+import copy
+
+import pytest
+import torch
+
+E4M3 = torch.float8_e4m3fn
+
+
+def module(grouped, bias):
+    from llmqrt_amd.linear import FP8BlockGroupedLinear, FP8BlockLinear
+    g = torch.Generator().manual_seed(1)
+    m = FP8BlockGroupedLinear(3, 256, 200, bias, dev="cpu") if grouped else FP8BlockLinear(256, 200, bias, dev="cpu")
+    m.set_weight(torch.randn(m.weight.shape, generator=g), torch.randn(m.bias.shape, generator=g) if bias else None)
+    return m
+
+
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("grouped", [True, False])
+def test_conversions(grouped, bias):
+    """A conversion changes the type of the bias and of the outputs, whether there is a bias or not; codes and scales keep theirs."""
+    m = module(grouped, bias)
+    w, s = m.weight.clone(), m.weight_scale.clone()
+
+    def holds(dtype, bias_dtype=None):
+        assert m.dtype == dtype
+        assert m.weight.dtype == E4M3 and torch.equal(m.weight.view(torch.uint8), w.view(torch.uint8))
+        assert m.weight_scale.dtype == torch.float32 and torch.equal(m.weight_scale, s)
+        assert m.bias is None if not bias else m.bias.dtype == (bias_dtype or dtype)
+    holds(torch.bfloat16)
+    assert m.half() is m
+    holds(torch.float16)
+    m.to(torch.bfloat16)
+    holds(torch.bfloat16)
+    m.to("cpu")
+    holds(torch.bfloat16)
+    m.float()  # outputs are bf16 or fp16; an fp32 bias is one that the products take
+    holds(torch.bfloat16, torch.float32)
+    m.half()
+    holds(torch.float16)
+    m = copy.deepcopy(torch.nn.Sequential(m)).to(torch.bfloat16)[0]
+    holds(torch.bfloat16)
+    m.to("meta")
+    assert m.weight.device.type == "meta" and m.weight.dtype == E4M3 and m.weight_scale.dtype == torch.float32 and m.dtype == torch.bfloat16
