@@ -132,6 +132,15 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def check_writable(t: torch.Tensor, what: str) -> None:
+    """Whether a kernel may write a caller's tensor, as torch's own in-place operations see it.  These calls record no backward pass, so a tensor that
+    requires grad is written under no_grad only."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} requires grad and would be written in place without a backward pass: call under torch.no_grad()")
+    if t.is_inference() and not torch.is_inference_mode_enabled():
+        raise RuntimeError(f"{what} is an inference tensor, which is written in inference mode only")
+
+
 def capturing(device: torch.device) -> bool:
     """Whether the current stream of `device` is being captured into a graph."""
     if device.index == torch.cuda.current_device():

@@ -16,6 +16,8 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
@@ -44,6 +46,15 @@ bool is16(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
 int code(at::ScalarType t) { return t == at::kBFloat16 ? LLMQ_BF16 : t == at::kHalf ? LLMQ_F16 : LLMQ_F32; }
 bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
 bool plain_on(const Tensor& t, const at::Device& dev) { return t.layout() == at::kStrided && t.device() == dev && t.is_contiguous(); }
+
+// A caller's tensor that a kernel writes: as torch's own in-place operations see it.  None of these calls records a backward pass, so one that requires
+// grad is written under no_grad only (otherwise the Python path refuses it).
+bool writable(const Tensor& t) {
+    return !(t.requires_grad() && c10::GradMode::is_enabled()) && (!t.is_inference() || c10::InferenceMode::is_enabled());
+}
+void written(const Tensor& t) {  // whoever saved t for a backward pass finds out
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 
 Tensor make(at::IntArrayRef size, at::ScalarType dtype, const at::Device& dev) {
     return Tensor(at::detail::empty_cuda(size, dtype, dev, std::nullopt));
@@ -497,7 +508,8 @@ struct NormOut {
 NormOut add_norm(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& w, double eps, int out, bool normed, bool inplace) {
     NormOut o;
     const Rows r = rows_of(x);
-    if (out < LLMQ_NORM_SAME || out > LLMQ_NORM_FP8_GROUP || !norm_ok(x, w, r) || (inplace && !residual)) return o;
+    if (out < LLMQ_NORM_SAME || out > LLMQ_NORM_FP8_GROUP || !norm_ok(x, w, r) || (inplace && (!residual || !writable(*residual))))
+        return o;
     if (residual && (residual->scalar_type() != x.scalar_type() || residual->sizes() != x.sizes() || !plain_on(*residual, x.device()) || !aligned(*residual)))
         return o;
     const Launch l(x.device());
@@ -515,6 +527,7 @@ NormOut add_norm(const Tensor& x, const std::optional<Tensor>& residual, const T
                            w.data_ptr(), (float)eps, y.defined() ? y.data_ptr() : nullptr, q.defined() ? q.data_ptr() : nullptr,
                            s.defined() ? (float*)s.data_ptr() : nullptr, l.stream),
           "llmq_add_rmsnorm");
+    if (inplace) written(h);
     for (const Tensor* t : {&q, &s, &y, &h})
         if (t->defined()) o.t[o.n++] = *t;
     o.ok = true;
@@ -591,7 +604,8 @@ std::optional<Tensor> fp8_block_grouped(const Tensor& x, const std::optional<Ten
     if (w_scale.dim() != 3 || w_scale.size(0) != E || w_scale.size(1) != blocks128(N) || !scale_ok(w_scale, dev, E * blocks128(N) * blocks128(r.K)) ||
         (bias && !is_matrix(*bias, E, N)) || (a_scale && !is_matrix(*a_scale, r.M, blocks128(r.K))) || !block_bias_ok(bias, dev, E * N) || offsets.dim() != 1 ||
         offsets.numel() != E + 1 || offsets.scalar_type() != at::kInt || !plain_on(offsets, dev) ||
-        (given && (given->scalar_type() != odt || given->dim() != 2 || given->size(0) != r.M || given->size(1) != N || !plain_on(*given, dev))))
+        (given && (given->scalar_type() != odt || given->dim() != 2 || given->size(0) != r.M || given->size(1) != N || !plain_on(*given, dev) ||
+                   !writable(*given))))
         return std::nullopt;
     if (a_scale ? (x.scalar_type() != at::kFloat8_e4m3fn || !scale_ok(*a_scale, dev, r.M * blocks128(r.K))) : !is16(x.scalar_type()))
         return std::nullopt;
@@ -611,6 +625,7 @@ std::optional<Tensor> fp8_block_grouped(const Tensor& x, const std::optional<Ten
                                       (const int32_t*)offsets.data_ptr(), E, ptr(bias), bias ? code(bias->scalar_type()) : LLMQ_BF16, out.data_ptr(),
                                       code(odt), N, r.M, N, r.K, l.stream),
           "llmq_gemm_fp8_block_grouped");
+    if (given) written(out);
     return out;
 }
 

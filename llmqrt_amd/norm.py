@@ -87,7 +87,11 @@ def _same_rows(t: torch.Tensor, x: torch.Tensor, what: str) -> torch.Tensor:
 
 def _add_norm(x, residual, weight, eps, out, return_normed=False, inplace=False):
     y = host().add_norm(x, residual, weight, eps, out, return_normed, inplace)
-    return _add_norm_general(x, residual, weight, eps, out, return_normed, inplace) if y is None else y
+    if y is not None:
+        return y
+    if inplace and residual is not None:
+        _abi.check_writable(residual, "the residual")
+    return _add_norm_general(x, residual, weight, eps, out, return_normed, inplace)
 
 
 @torch.no_grad()
@@ -120,6 +124,8 @@ def _add_norm_general(x, residual, weight, eps, out, return_normed, inplace):
                 out, rows.data_ptr(), _abi.dtype_code(rows.dtype), M, K, rows.stride(0) if M > 1 else K, _abi.ptr(res),
                 res.stride(0) if res is not None and M > 1 else K, _abi.ptr(h), h.stride(0) if h is not None and M > 1 else K, w.data_ptr(), float(eps),
                 _abi.ptr(y), _abi.ptr(q), _abi.ptr(scale), _abi.stream_of(rows)), "llmq_add_rmsnorm")
+        if inplace:
+            torch.autograd.graph.increment_version(residual)
     result = [] if q is None else [q.view(x.shape), scale.view(*x.shape[:-1], scale.shape[-1])]
     if y is not None:
         result.append(y.view(x.shape))
@@ -130,7 +136,8 @@ def _add_norm_general(x, residual, weight, eps, out, return_normed, inplace):
 
 def add_rmsnorm(x, residual, weight, eps: float = 1e-6, inplace: bool = False):
     """The residual's addition and RMSNorm in one pass: h = (x + residual).to(x.dtype), y = (h * rsqrt(mean(h^2) + eps) * weight) in fp32,
-    rounded once to x.dtype.  -> (y, h).  ``inplace`` writes h over the residual (and returns it)."""
+    rounded once to x.dtype.  -> (y, h).  ``inplace`` writes h over the residual (and returns it), as torch's in-place operations do: its version is
+    raised, and a residual that requires grad is refused outside no_grad."""
     if residual is None:
         raise RuntimeError("add_rmsnorm needs a residual (rmsnorm is the form without)")
     return _add_norm(x, residual, weight, eps, _SAME, inplace=inplace)

@@ -251,9 +251,14 @@ def f8f8_blockwise_grouped(XQ: torch.Tensor, WQ: torch.Tensor, bias: Optional[to
     ``WQ``: e4m3fn [E, N, K] row-major; ``w_scale``: fp32 [E, ceil(N / 128), ceil(K / 128)]; ``bias``: [E, N]; ``offsets``: int32 [E + 1]
     on the GPU, ascending (values outside [0, M] are taken as the nearest inside).  An expert may have no rows.  Nothing is read back by
     the host, so a captured call follows the offsets of its replay.  Rows that belong to no expert are not written: they keep what ``out`` [M, N] holds,
-    and are undefined in a new tensor."""
+    and are undefined in a new tensor.  ``out`` is written as torch's in-place operations do: its version is raised, and one that requires grad is refused
+    outside no_grad."""
     y = None if x_scale is None else host().fp8_block_grouped(XQ, x_scale, WQ, w_scale, bias, offsets, _STR_TO_DTYPE.get(dtype_str), out)
-    return _f8f8_blockwise_grouped_general(XQ, WQ, bias, x_scale, w_scale, offsets, dtype_str, out) if y is None else y
+    if y is not None:
+        return y
+    if out is not None:
+        _abi.check_writable(out, "out")
+    return _f8f8_blockwise_grouped_general(XQ, WQ, bias, x_scale, w_scale, offsets, dtype_str, out)
 
 
 @torch.no_grad()

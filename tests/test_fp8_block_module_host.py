@@ -42,3 +42,29 @@ def test_conversions(grouped, bias):
     holds(torch.bfloat16)
     m.to("meta")
     assert m.weight.device.type == "meta" and m.weight.dtype == E4M3 and m.weight_scale.dtype == torch.float32 and m.dtype == torch.bfloat16
+
+
+def test_tensors_that_require_grad_are_not_written():
+    """(Refused before anything else is looked at, so also without a GPU.)"""
+    from llmqrt_amd import norm as N
+    from llmqrt_amd.linear import FP8BlockGroupedLinear
+    from llmqrt_amd.sq_fp8_kernels import f8f8_blockwise_grouped
+    x, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.ones(64, dtype=torch.bfloat16)
+    leaf = torch.zeros(4, 64, dtype=torch.bfloat16, requires_grad=True)
+    for r in (leaf, leaf * 2, (leaf * 2)[:]):
+        for f in (N.add_rmsnorm, N.add_rmsnorm_quantize_activation_per_token_absmax, N.add_rmsnorm_per_token_quantize, N.add_rmsnorm_per_group_quantize):
+            with pytest.raises(RuntimeError, match="requires grad"):
+                f(x, r, w, inplace=True)
+        with pytest.raises(RuntimeError, match="requires grad"):
+            N.RMSNorm(w).forward_add(x, r, inplace=True)
+    with torch.inference_mode():
+        made = torch.zeros(4, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="inference"):
+        N.add_rmsnorm(x, made, w, inplace=True)
+    out = torch.zeros(4, 200, dtype=torch.bfloat16, requires_grad=True)
+    m, off = FP8BlockGroupedLinear(1, 64, 200, dev="cpu"), torch.tensor([0, 4], dtype=torch.int32)
+    q, s = torch.zeros(4, 64, dtype=E4M3), torch.ones(4, 1)
+    with pytest.raises(RuntimeError, match="requires grad"):
+        f8f8_blockwise_grouped(q, m.weight, None, s, m.weight_scale, off, out=out)
+    with pytest.raises(RuntimeError, match="requires grad"):
+        m.forward_quantized(q, s, off, out)

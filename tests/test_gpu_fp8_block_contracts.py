@@ -27,3 +27,76 @@ def test_converted_modules_agree_on_their_type(cuda, bias):
         m = torch.nn.Sequential(m).half()[0]
         y = m.forward_quantized(q, s, *args)
         assert y.dtype == torch.float16 and same(m(x, *args), y)
+
+
+def norm_calls():
+    from llmqrt_amd import norm as N
+    return [N.add_rmsnorm, N.add_rmsnorm_quantize_activation_per_token_absmax, N.add_rmsnorm_per_token_quantize, N.add_rmsnorm_per_group_quantize]
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_autograd_sees_a_residual_written_in_place(cuda, strided):
+    """Both the native path (contiguous rows) and the general one (rows inside a wider tensor)."""
+    x = torch.randn(5, 256, generator=torch.Generator().manual_seed(3)).bfloat16().to(cuda)
+    w = torch.ones(256, dtype=torch.bfloat16, device=cuda)
+    for f in norm_calls():
+        room = torch.zeros(5, 512 if strided else 256, dtype=torch.bfloat16, device=cuda)
+        r = room[:, :256]
+        r.fill_(2)
+        before = r._version
+        scale = torch.ones(5, 256, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+        saved = (scale * r).float().sum()  # keeps r for its backward pass
+        f(x, r, w)
+        assert r._version == before
+        f(x, r, w, inplace=True)
+        assert r._version > before and room._version == r._version and same(r, x + 2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            saved.backward()
+        # one that requires grad: left as it is, and written under no_grad
+        leaf = torch.full((5, 512 if strided else 256), 2.0, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+        for t in (leaf, leaf * 1):
+            with pytest.raises(RuntimeError, match="requires grad"):
+                f(x, t[:, :256] if strided else t, w, inplace=True)
+            assert (t == 2).all()
+        with torch.no_grad():
+            part = leaf[:, :256] if strided else leaf
+            before = leaf._version
+            f(x, part, w, inplace=True)
+            assert leaf._version > before and same(part, x + 2)
+        with torch.inference_mode():
+            made = torch.full((5, 512 if strided else 256), 2.0, dtype=torch.bfloat16, device=cuda)
+            part = made[:, :256]
+            assert f(x, part, w, inplace=True)[-1].data_ptr() == made.data_ptr() and same(part, x + 2)
+        with pytest.raises(RuntimeError, match="inference"):
+            f(x, part, w, inplace=True)
+
+
+def test_autograd_sees_out_of_a_product_by_experts(cuda):
+    from llmqrt_amd.linear import FP8BlockGroupedLinear
+    from llmqrt_amd.quantize import per_group_quantize
+    from llmqrt_amd.sq_fp8_kernels import f8f8_blockwise_grouped
+    g = torch.Generator().manual_seed(4)
+    m = FP8BlockGroupedLinear(2, 256, 200, dev=cuda)
+    m.set_weight(torch.randn(2, 200, 256, generator=g))
+    x = torch.randn(6, 256, generator=g).bfloat16().to(cuda)
+    wide = torch.cat([x, x], 1)[:, :256]  # rows inside a wider tensor: the general path
+    off = torch.tensor([0, 2, 6], dtype=torch.int32, device=cuda)
+    q, s = per_group_quantize(x)
+    calls = [lambda o: m(x, off, o), lambda o: m(wide, off, o), lambda o: m.forward_quantized(q, s, off, o),
+             lambda o: f8f8_blockwise_grouped(q, m.weight, None, s.t().contiguous().t(), m.weight_scale, off, out=o)]
+    want = m(x, off)
+    for call in calls:
+        out = torch.ones(6, 200, dtype=torch.bfloat16, device=cuda)
+        scale = torch.ones(6, 200, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+        saved = (scale * out).float().sum()
+        assert call(out) is out or same(out, want)
+        assert same(out, want) and out._version > 0
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            saved.backward()
+        leaf = torch.ones(6, 200, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+        with pytest.raises(RuntimeError, match="requires grad"):
+            call(leaf)
+        assert (leaf == 1).all()
+        with torch.no_grad():
+            call(leaf)
+        assert same(leaf, want) and leaf._version > 0
