@@ -24,6 +24,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cstdlib>
 #include <mutex>
 #include <optional>
 #include <stdexcept>
@@ -512,6 +513,10 @@ NormOut add_norm(const Tensor& x, const std::optional<Tensor>& residual, const T
         return o;
     if (residual && (residual->scalar_type() != x.scalar_type() || residual->sizes() != x.sizes() || !plain_on(*residual, x.device()) || !aligned(*residual)))
         return o;
+    if (inplace) {  // a row would be read after another had been written there
+        const int64_t apart = (const char*)residual->data_ptr() - (const char*)x.data_ptr();
+        if (apart != 0 && std::abs(apart) < 2 * r.M * r.K) return o;
+    }
     const Launch l(x.device());
     Tensor q, s, y, h;
     Outputs all(x.device());

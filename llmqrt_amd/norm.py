@@ -85,6 +85,21 @@ def _same_rows(t: torch.Tensor, x: torch.Tensor, what: str) -> torch.Tensor:
     return _apart(_as_rows(t))
 
 
+def _partly_over(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two sets of rows of one shape and type share elements without being the same (different strides: whether their ranges meet)."""
+    if a.data_ptr() < b.data_ptr():
+        a, b = b, a
+    M, K = a.shape
+    apart = (a.data_ptr() - b.data_ptr()) // a.element_size()
+    if M == 1:
+        return 0 < apart < K
+    ld = b.stride(0)
+    if a.stride(0) != ld:
+        return apart < (M - 1) * ld + K
+    rows, columns = divmod(apart, ld)  # how many a lies behind b
+    return apart > 0 and (columns < K and rows < M or ld - columns < K and rows + 1 < M)
+
+
 def _add_norm(x, residual, weight, eps, out, return_normed=False, inplace=False):
     y = host().add_norm(x, residual, weight, eps, out, return_normed, inplace)
     if y is not None:
@@ -109,6 +124,8 @@ def _add_norm_general(x, residual, weight, eps, out, return_normed, inplace):
             h = torch.empty((M, K), dtype=rows.dtype, device=dev)
         elif res.data_ptr() != residual.data_ptr():
             raise RuntimeError("a residual that is updated in place needs rows of one stride that is a multiple of 16 bytes, 16-byte aligned")
+        elif M and _partly_over(rows, res):
+            raise RuntimeError("a residual that is updated in place must be the activations or lie apart from them")
         else:
             h = res
     groups = (K + 127) // 128
@@ -137,7 +154,7 @@ def _add_norm_general(x, residual, weight, eps, out, return_normed, inplace):
 def add_rmsnorm(x, residual, weight, eps: float = 1e-6, inplace: bool = False):
     """The residual's addition and RMSNorm in one pass: h = (x + residual).to(x.dtype), y = (h * rsqrt(mean(h^2) + eps) * weight) in fp32,
     rounded once to x.dtype.  -> (y, h).  ``inplace`` writes h over the residual (and returns it), as torch's in-place operations do: its version is
-    raised, and a residual that requires grad is refused outside no_grad."""
+    raised, and a residual that requires grad is refused outside no_grad.  There the residual may be x itself, and may not overlap it otherwise."""
     if residual is None:
         raise RuntimeError("add_rmsnorm needs a residual (rmsnorm is the form without)")
     return _add_norm(x, residual, weight, eps, _SAME, inplace=inplace)

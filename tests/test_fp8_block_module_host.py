@@ -68,3 +68,20 @@ def test_tensors_that_require_grad_are_not_written():
         f8f8_blockwise_grouped(q, m.weight, None, s, m.weight_scale, off, out=out)
     with pytest.raises(RuntimeError, match="requires grad"):
         m.forward_quantized(q, s, off, out)
+
+
+def test_rows_that_partly_overlap():
+    """The rule on addresses against the sets of elements, for rows anywhere in one buffer."""
+    from llmqrt_amd.norm import _partly_over
+    buf = torch.arange(200, dtype=torch.int16)
+    for m in (1, 2, 5):
+        for k in (1, 4, 7):
+            for ld in (k, k + 1, 2 * k, 2 * k + 3):
+                b = buf.as_strided((m, k), (ld, 1), 40)
+                mine = set(b.flatten().tolist())
+                for at in range(0, 120):
+                    a = buf.as_strided((m, k), (ld, 1), at)
+                    want = a.data_ptr() != b.data_ptr() and bool(mine & set(a.flatten().tolist()))
+                    assert _partly_over(a, b) == want and _partly_over(b, a) == want, (m, k, ld, at)
+    a, b = buf.as_strided((3, 4), (8, 1), 0), buf.as_strided((3, 4), (12, 1), 0)
+    assert _partly_over(a, b) and not _partly_over(a, buf.as_strided((3, 4), (12, 1), 20))

@@ -100,3 +100,26 @@ def test_autograd_sees_out_of_a_product_by_experts(cuda):
         with torch.no_grad():
             call(leaf)
         assert same(leaf, want) and leaf._version > 0
+
+
+def test_a_residual_over_part_of_the_activations(cuda):
+    """Refused in place, and left as it was; halves of the same rows, neighbours, and the activations themselves are fine, and so is any overlap otherwise."""
+    w = torch.ones(64, dtype=torch.bfloat16, device=cuda)
+    buf = torch.randn(12, 128, generator=torch.Generator().manual_seed(5)).bfloat16().to(cuda)
+    flat = buf.view(24, 64)
+    bad = [(flat[1:9], flat[0:8]), (flat[0:8], flat[1:9]), (buf[1:9, :64], buf[0:8, :64]), (buf[:8, :64], buf[:8, 8:72]), (flat[:5], buf[:5, :64]),
+           (buf.view(-1)[:64], buf.view(-1)[8:72])]
+    for f in norm_calls():
+        for x, r in bad:
+            was = buf.clone()
+            want = f(x.clone(), r.clone(), w)
+            assert all(same(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(f(x, r, w), want))
+            with pytest.raises(RuntimeError, match="apart"):
+                f(x, r, w, inplace=True)
+            assert same(buf, was)
+        for x, r in ((flat[:8], flat[8:16]), (buf[:, :64], buf[:, 64:]), (buf[:, 64:], buf[:, :64]), (flat[:8], flat[:8]), (buf[:, :64], buf[:, :64])):
+            was = buf.clone()
+            want = f(x.clone(), r.clone(), w)
+            got = f(x, r, w, inplace=True)
+            assert got[-1].data_ptr() == r.data_ptr() and all(same(a.contiguous().view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+            buf.copy_(was)
