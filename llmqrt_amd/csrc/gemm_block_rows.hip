@@ -119,6 +119,7 @@ __global__ __launch_bounds__(C::NT) void block_rows_kernel(BlockArgs g) {
         const uint8_t* st = smem + slot * C::STAGE;
 #pragma unroll
         for (int step = 0; step < C::STEPS; step++) {
+            if (tail && (wave * C::STEPS + step) * kScaleBlock >= left) continue;  // no block (the scales loaded for it are the last one's); wavefront-uniform
             const float* sc = reinterpret_cast<const float*>(st + C::DATA + wave * C::SWAVE + step * C::SLOADS * kWave * 4);
             v8i b[T], a[MT];
 #pragma unroll
