@@ -44,7 +44,7 @@ __global__ __launch_bounds__(C::NT) void block_rows_kernel(BlockArgs g) {
     const int l16 = lane & 15, kq = lane >> 4;
     int n0 = blockIdx.x * (16 * T);
     const int nst = (g.K + SEG - 1) / SEG, step_n = C::MANY ? gridDim.x * (16 * T) : 0;
-    const int groups = C::MANY ? (g.N - n0 + step_n - 1) / max(step_n, 1) : 1, total = groups * nst;  // of channels; stages of the block
+    const int groups = C::MANY ? (g.N - 1 - n0) / max(step_n, 1) + 1 : 1, total = groups * nst;  // of channels; stages of the block
 
     // ---- direct loads: piece p of a stage is row p / CPR (weights, then activations), LDS chunk p % CPR, which holds chunk (p % CPR) ^ (row & 15)
     // of the row, so that the operand reads of 16 rows hit 16 places; rows past the end are the last one again
@@ -208,7 +208,8 @@ __global__ __launch_bounds__(C::NT) void block_rows_kernel(BlockArgs g) {
         if (C::MANY && s == nst) {
             finish(group);  // its reads of the sums are done in every wavefront before the barrier of the next stage
             clear();
-            n0 += step_n, group++, s = 0;
+            group++, s = 0;
+            if (group < groups) n0 += step_n;
         }
     }
     if constexpr (!C::MANY) {
