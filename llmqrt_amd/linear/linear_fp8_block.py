@@ -23,6 +23,12 @@ def _blocks(n: int) -> int:
     return (n + BLOCK - 1) // BLOCK
 
 
+def _check_plain(module) -> None:
+    """A module whose weight is codes has scales beside it, which a quantizer of the codes would lose."""
+    if getattr(module, "weight_scale", None) is not None or module.weight.dtype.itemsize < 2:
+        raise RuntimeError(f"{type(module).__name__} is quantized already: a weight to be quantized must be a floating-point one without scales")
+
+
 class _FP8BlockBase(LinearBase):
     def _init_block(self, lead, in_features, out_features, bias, dev, dtype):
         if in_features % 16:
@@ -54,6 +60,8 @@ class _FP8BlockBase(LinearBase):
         """Quantize a floating-point weight (and take a bias) of the module's shape."""
         if weight.shape != self.weight.shape or (bias is not None) != (self.bias is not None):
             raise RuntimeError(f"weight must be {list(self.weight.shape)}, with a bias if the module has one")
+        if weight.dtype.itemsize < 2 or (bias is not None and bias.shape != self.bias.shape):
+            raise RuntimeError("a weight to be quantized must have 16 bits or more, and a bias the module's shape")
         q, s = quantize_weight_per_block(weight.to(self.weight.device))
         self.weight.copy_(q)
         self.weight_scale.copy_(s)
@@ -73,6 +81,8 @@ class FP8BlockLinear(_FP8BlockBase):
     def from_linear(cls, module: torch.nn.Linear, w_bit=8, group_size=BLOCK, init_only=True, dtype=torch.bfloat16, per_tensor=False):
         if w_bit != 8 or group_size != BLOCK:
             raise RuntimeError(f"block-scaled fp8 has 8 bits and groups of {BLOCK}, got {w_bit} and {group_size}")
+        if not init_only:
+            _check_plain(module)
         lin = cls(module.in_features, module.out_features, module.bias is not None, module.weight.device, dtype)
         if not init_only:
             lin.set_weight(module.weight.data, None if module.bias is None else module.bias.data)
@@ -116,11 +126,29 @@ class FP8BlockGroupedLinear(_FP8BlockBase):
         self._init_block((num_experts,), in_features, out_features, bias, dev, dtype)
 
     @classmethod
-    def from_linears(cls, modules, dtype=torch.bfloat16):
+    def from_linears(cls, modules, dtype=None):
+        """The experts' nn.Linear modules, whose weights are quantized here (``dtype`` of the outputs: bf16 unless given), or their FP8BlockLinear
+        modules, as a checkpoint fills them, whose codes and scales are taken as they are (``dtype``: theirs unless given)."""
+        modules = list(modules)
+        if not modules:
+            raise RuntimeError("from_linears needs the modules of one expert or more")
         first = modules[0]
+        codes = isinstance(first, FP8BlockLinear)
+        if any(isinstance(m, FP8BlockLinear) != codes or (codes and dtype is None and m.dtype != first.dtype) for m in modules):
+            raise RuntimeError("the experts must be modules of one kind and type")
         if any(m.weight.shape != first.weight.shape or (m.bias is None) != (first.bias is None) for m in modules):
             raise RuntimeError("the experts must have the same shape, and all or none of them a bias")
-        lin = cls(len(modules), first.in_features, first.out_features, first.bias is not None, first.weight.device, dtype)
+        if not codes:
+            for m in modules:
+                _check_plain(m)
+        lin = cls(len(modules), first.in_features, first.out_features, first.bias is not None, first.weight.device,
+                  dtype or (first.dtype if codes else torch.bfloat16))
+        if codes:
+            for e, m in enumerate(modules):
+                for name in ("weight", "weight_scale", "bias"):
+                    if m._buffers[name] is not None:
+                        lin._buffers[name][e].copy_(m._buffers[name])
+            return lin
         lin.set_weight(torch.stack([m.weight.data for m in modules]), None if first.bias is None else torch.stack([m.bias.data for m in modules]))
         return lin
 

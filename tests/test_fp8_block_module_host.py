@@ -85,3 +85,46 @@ def test_rows_that_partly_overlap():
                     assert _partly_over(a, b) == want and _partly_over(b, a) == want, (m, k, ld, at)
     a, b = buf.as_strided((3, 4), (8, 1), 0), buf.as_strided((3, 4), (12, 1), 0)
     assert _partly_over(a, b) and not _partly_over(a, buf.as_strided((3, 4), (12, 1), 20))
+
+
+@pytest.mark.parametrize("bias", [True, False])
+def test_experts_of_quantized_modules(bias):
+    """The codes, scales and biases of FP8BlockLinear modules, as they are."""
+    from llmqrt_amd.linear import FP8BlockGroupedLinear, FP8BlockLinear
+    g = torch.Generator().manual_seed(3)
+    plain = [torch.nn.Linear(144, 200, bias=bias) for _ in range(3)]
+    for p in plain:
+        p.weight.data = torch.randn(200, 144, generator=g)
+    parts = [FP8BlockLinear.from_linear(p, init_only=False, dtype=torch.float16) for p in plain]
+    m = FP8BlockGroupedLinear.from_linears(torch.nn.ModuleList(parts))
+    assert m.dtype == torch.float16 and m.num_experts == 3
+    for e, p in enumerate(parts):
+        assert torch.equal(m.weight[e].view(torch.uint8), p.weight.view(torch.uint8)) and torch.equal(m.weight_scale[e], p.weight_scale)
+        assert m.bias is None if not bias else torch.equal(m.bias[e], p.bias)
+    quantized_here = FP8BlockGroupedLinear.from_linears(plain)
+    assert quantized_here.dtype == torch.bfloat16 and torch.equal(quantized_here.weight.view(torch.uint8), m.weight.view(torch.uint8))
+    assert FP8BlockGroupedLinear.from_linears(parts, torch.bfloat16).dtype == torch.bfloat16
+    other = FP8BlockLinear.from_linear(plain[0], init_only=False)
+    for bad in ([], [parts[0], plain[1]], [plain[0], parts[1]], [parts[0], other], [parts[0], FP8BlockLinear(144, 72, bias, dev="cpu", dtype=torch.float16)],
+                [parts[0], FP8BlockLinear(144, 200, not bias, dev="cpu", dtype=torch.float16)]):
+        with pytest.raises(RuntimeError):
+            FP8BlockGroupedLinear.from_linears(bad)
+
+
+def test_codes_are_not_quantized_again():
+    """Codes without their scales are no weight: the result would be right but for factors that nobody sees."""
+    from llmqrt_amd.linear import FP8BlockGroupedLinear, FP8BlockLinear, FP8DynamicLinear
+    lin = torch.nn.Linear(64, 72)
+    block, token = FP8BlockLinear.from_linear(lin, init_only=False), FP8DynamicLinear.from_linear(lin, init_only=False, per_tensor=False)
+    for m in (block, token):
+        with pytest.raises(RuntimeError, match="quantized already"):
+            FP8BlockLinear.from_linear(m, init_only=False)
+    with pytest.raises(RuntimeError, match="quantized already"):
+        FP8BlockGroupedLinear.from_linears([token, token])
+    with pytest.raises(RuntimeError):
+        block.set_weight(block.weight, block.bias)
+    for bias in (torch.zeros(1), torch.zeros(1, 72), torch.zeros(())):
+        with pytest.raises(RuntimeError):
+            block.set_weight(lin.weight, bias)
+    empty = FP8BlockLinear.from_linear(token)  # sizes only
+    assert empty.weight.shape == (72, 64)
