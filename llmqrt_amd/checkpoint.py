@@ -24,7 +24,7 @@ from typing import Iterable
 import torch
 from torch import nn
 
-from .linear import FP8BlockLinear, SqW8A8BBF16OBF16PerChannel, method_to_linear
+from .linear import FP8BlockGroupedLinear, FP8BlockLinear, SqW8A8BBF16OBF16PerChannel, method_to_linear
 
 
 @dataclass
@@ -119,7 +119,9 @@ def _checkpoint_files(path: str) -> list[str]:
 def load_quantized_weights(model: nn.Module, path: str, device=None) -> tuple[list[str], list[str]]:
     """Fill parameters and buffers by name from the ``.safetensors`` file(s) at ``path`` (a file, a directory,
     or a directory with a ``model.safetensors.index.json``).  Shapes and dtypes must match what the modules
-    allocated (scalars may come as 0-dim or 1-element tensors).  -> (missing names, unexpected names)."""
+    allocated (scalars may come as 0-dim or 1-element tensors).  Floating-point values are converted; what becomes 8 bits must be such values already
+    (codes that are stored in a wider type), since an unquantized weight would lose most of its bits unseen.  A directory that holds a block-scaled
+    module's weight must hold its scales too.  -> (missing names, unexpected names)."""
     from safetensors import safe_open
 
     own = dict(model.named_parameters())
@@ -139,9 +141,16 @@ def load_quantized_weights(model: nn.Module, path: str, device=None) -> tuple[li
                     raise RuntimeError(f"{key}: checkpoint shape {tuple(src.shape)} != module shape {tuple(dst.shape)}")
                 if src.dtype != dst.dtype and not (src.is_floating_point() and dst.is_floating_point()):
                     raise RuntimeError(f"{key}: checkpoint dtype {src.dtype} != module dtype {dst.dtype}")
+                cast = src.to(dst.dtype)
+                if dst.dtype.itemsize == 1 and src.dtype != dst.dtype and not torch.equal(cast.float(), src.float()):
+                    raise RuntimeError(f"{key}: values in {src.dtype} that are no {dst.dtype} codes; an unquantized weight must be quantized first")
                 with torch.no_grad():
-                    dst.copy_(src.to(dst.dtype))
+                    dst.copy_(cast)
                 seen.add(key)
+    for name, m in model.named_modules():
+        weight, scale = (f"{name}.{t}" if name else t for t in ("weight", "weight_scale"))
+        if not os.path.isfile(path) and isinstance(m, (FP8BlockLinear, FP8BlockGroupedLinear)) and weight in seen and scale not in seen:
+            raise RuntimeError(f"{scale}: the checkpoint holds the codes of {weight} and no scales for them")
     for m in model.modules():   # cached fp8 casts of weights that were just overwritten
         if hasattr(m, "invalidate_cache"):
             m.invalidate_cache()
