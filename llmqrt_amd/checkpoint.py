@@ -160,5 +160,5 @@ def load_quantized_weights(model: nn.Module, path: str, device=None) -> tuple[li
 
 
 def named_quantized_linears(model: nn.Module) -> Iterable[tuple[str, nn.Module]]:
-    kinds = tuple(set(method_to_linear.values()) | {SqW8A8BBF16OBF16PerChannel, FP8BlockLinear})
+    kinds = tuple(set(method_to_linear.values()) | {SqW8A8BBF16OBF16PerChannel, FP8BlockLinear, FP8BlockGroupedLinear})
     return ((n, m) for n, m in model.named_modules() if isinstance(m, kinds))

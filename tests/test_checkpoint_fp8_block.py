@@ -54,3 +54,9 @@ def test_codes_without_scales(tmp_path, experts):
     save_file({"weight": weight}, str(tmp_path / "c" / "m.safetensors"))
     with pytest.raises(RuntimeError, match="weight_scale"):
         load_quantized_weights(one, str(tmp_path / "c"))
+
+
+def test_experts_are_named(tmp_path):
+    from llmqrt_amd.checkpoint import named_quantized_linears
+    m = torch.nn.ModuleDict({"a": model("up", experts=2), "b": model("up"), "c": torch.nn.Linear(16, 16)})
+    assert [n for n, _ in named_quantized_linears(m)] == ["a.up", "b.up"]
