@@ -39,6 +39,7 @@ class QuantConfig:
     fp8_static_quant: bool = False
     kv_cache_quant_layers: list = field(default_factory=list)
     per_tensor: bool = True
+    skip_whole_names: bool = False     # modules_to_not_convert lists whole parts of names (published fp8 checkpoints), not any piece of one
 
     @classmethod
     def from_dict(cls, d: dict | None = None) -> "QuantConfig":
@@ -48,11 +49,15 @@ class QuantConfig:
 
     @classmethod
     def from_transformers_dict(cls, d: dict) -> "QuantConfig":
-        """The key names used inside config.json (core/config.py:88-112): group_size, bits."""
+        """The key names used inside config.json (core/config.py:88-112): group_size, bits.  Block-scaled fp8 checkpoints as published have names of their
+        own, quant_method "fp8" with a weight_block_size: of 128 x 128 with dynamic scales of the activations, they are this package's
+        "fp8_dynamic_quant" with groups of 128; of any other kind they keep their quant_method, which replace_linears refuses."""
+        if d.get("quant_method") == "fp8" and list(d.get("weight_block_size") or ()) == [128, 128] and d.get("activation_scheme", "dynamic") == "dynamic":
+            d = {**d, "quant_method": "fp8_dynamic_quant", "group_size": 128, "bits": 8, "skip_whole_names": True}
         known = {"quant_method": "quant_method", "zero_point": "zero_point", "group_size": "q_group_size",
                  "bits": "w_bit", "fp8_static_quant": "fp8_static_quant",
                  "kv_cache_quant_layers": "kv_cache_quant_layers",
-                 "modules_to_not_convert": "modules_to_not_convert", "per_tensor": "per_tensor"}
+                 "modules_to_not_convert": "modules_to_not_convert", "per_tensor": "per_tensor", "skip_whole_names": "skip_whole_names"}
         kwargs = {ours: d[theirs] for theirs, ours in known.items() if d.get(theirs) is not None}
         return cls.from_dict(kwargs)
 
@@ -67,10 +72,11 @@ class QuantConfig:
         return cls.from_transformers_dict(q) if q else cls()
 
     def to_transformers_dict(self) -> dict:
-        return {"quant_method": self.quant_method, "zero_point": self.zero_point, "group_size": self.q_group_size,
-                "bits": self.w_bit, "fp8_static_quant": self.fp8_static_quant,
-                "kv_cache_quant_layers": self.kv_cache_quant_layers,
-                "modules_to_not_convert": self.modules_to_not_convert, "per_tensor": self.per_tensor}
+        d = {"quant_method": self.quant_method, "zero_point": self.zero_point, "group_size": self.q_group_size,
+             "bits": self.w_bit, "fp8_static_quant": self.fp8_static_quant,
+             "kv_cache_quant_layers": self.kv_cache_quant_layers,
+             "modules_to_not_convert": self.modules_to_not_convert, "per_tensor": self.per_tensor}
+        return {**d, "skip_whole_names": True} if self.skip_whole_names else d
 
 
 def _set_submodule(root: nn.Module, name: str, new: nn.Module) -> None:
@@ -87,15 +93,21 @@ def replace_linears(model: nn.Module, cfg: QuantConfig, dtype=torch.bfloat16) ->
 
     ``quant_method == "sq"`` with ``per_tensor == False`` selects the per-token x per-channel SmoothQuant module,
     which the reference declares but does not implement; ``quant_method == "fp8_dynamic_quant"`` with ``q_group_size == 128`` the block-scaled FP8
-    module, whose weight is stored in e4m3fn with a scale per 128 x 128 block (the reference's FP8 modules refuse any group size but 0)."""
+    module, whose weight is stored in e4m3fn with a scale per 128 x 128 block (the reference's FP8 modules refuse any group size but 0).  With
+    ``skip_whole_names`` a name is skipped only where whole parts of it are listed ("mlp.gate" is no part of "mlp.gate_proj").  The modules of a list of experts are replaced one by
+    one; FP8BlockGroupedLinear.from_linears joins them once they are filled."""
+    if cfg.quant_method not in method_to_linear:
+        raise RuntimeError(f"quant_method {cfg.quant_method!r} is not supported: {sorted(method_to_linear)}, or \"fp8\" with a weight_block_size of 128 x 128 "
+                           "and dynamic activation scales")
     kind = method_to_linear[cfg.quant_method]
     if cfg.quant_method == "sq" and not cfg.per_tensor:
         kind = SqW8A8BBF16OBF16PerChannel
     if cfg.quant_method == "fp8_dynamic_quant" and cfg.q_group_size == 128:
         kind = FP8BlockLinear
     skip = cfg.modules_to_not_convert or []
+    skipped = (lambda n: any(f".{key}." in f".{n}." for key in skip)) if cfg.skip_whole_names else (lambda n: any(key in n for key in skip))
     targets = [(n, m) for n, m in model.named_modules()
-               if isinstance(m, nn.Linear) and n and not any(key in n for key in skip)]
+               if isinstance(m, nn.Linear) and n and not skipped(n)]
     for name, lin in targets:
         q = kind.from_linear(lin, cfg.w_bit, cfg.q_group_size, True, dtype=dtype, per_tensor=cfg.per_tensor)
         _set_submodule(model, name, q)
@@ -121,35 +133,43 @@ def load_quantized_weights(model: nn.Module, path: str, device=None) -> tuple[li
     or a directory with a ``model.safetensors.index.json``).  Shapes and dtypes must match what the modules
     allocated (scalars may come as 0-dim or 1-element tensors).  Floating-point values are converted; what becomes 8 bits must be such values already
     (codes that are stored in a wider type), since an unquantized weight would lose most of its bits unseen.  A directory that holds a block-scaled
-    module's weight must hold its scales too.  -> (missing names, unexpected names)."""
+    module's weight must hold its scales too, which may be named ``weight_scale_inv`` (the factor of the codes all the same).  Codes are not loaded as the
+    weight of an nn.Linear.  -> (missing names, unexpected names)."""
     from safetensors import safe_open
 
     own = dict(model.named_parameters())
     own.update(dict(model.named_buffers()))
+    modules = dict(model.named_modules())
+    block_scaled = (FP8BlockLinear, FP8BlockGroupedLinear)
     seen, unexpected = set(), []
     for file in _checkpoint_files(path):
         with safe_open(file, framework="pt", device="cpu") as f:
             for key in f.keys():
+                stored, owner = key, modules.get(key.rpartition(".")[0])
+                if isinstance(owner, block_scaled) and key.endswith("weight_scale_inv"):
+                    key = key.removesuffix("_inv")
                 dst = own.get(key)
                 if dst is None:
                     unexpected.append(key)
                     continue
-                src = f.get_tensor(key)
+                src = f.get_tensor(stored)
                 if src.numel() == dst.numel() and src.shape != dst.shape and dst.numel() == 1:
                     src = src.reshape(dst.shape)
                 if src.shape != dst.shape:
                     raise RuntimeError(f"{key}: checkpoint shape {tuple(src.shape)} != module shape {tuple(dst.shape)}")
                 if src.dtype != dst.dtype and not (src.is_floating_point() and dst.is_floating_point()):
                     raise RuntimeError(f"{key}: checkpoint dtype {src.dtype} != module dtype {dst.dtype}")
+                if type(owner) is nn.Linear and src.dtype.itemsize == 1 and src.is_floating_point():
+                    raise RuntimeError(f"{key}: the checkpoint holds codes in {src.dtype} for a module that is not quantized")
                 cast = src.to(dst.dtype)
                 if dst.dtype.itemsize == 1 and src.dtype != dst.dtype and not torch.equal(cast.float(), src.float()):
                     raise RuntimeError(f"{key}: values in {src.dtype} that are no {dst.dtype} codes; an unquantized weight must be quantized first")
                 with torch.no_grad():
                     dst.copy_(cast)
                 seen.add(key)
-    for name, m in model.named_modules():
+    for name, m in modules.items():
         weight, scale = (f"{name}.{t}" if name else t for t in ("weight", "weight_scale"))
-        if not os.path.isfile(path) and isinstance(m, (FP8BlockLinear, FP8BlockGroupedLinear)) and weight in seen and scale not in seen:
+        if not os.path.isfile(path) and isinstance(m, block_scaled) and weight in seen and scale not in seen:
             raise RuntimeError(f"{scale}: the checkpoint holds the codes of {weight} and no scales for them")
     for m in model.modules():   # cached fp8 casts of weights that were just overwritten
         if hasattr(m, "invalidate_cache"):

@@ -2,7 +2,7 @@
 128 x 128 block of the weight.
 
 The reference refuses group-wise FP8 (``group_size`` must be 0, nn_models/modules/linear/linear_fp8.py:160-163); buffer names follow its FP8
-modules.  The weight is kept in e4m3fn, as checkpoints of this format store it.
+modules.  The weight is kept in e4m3fn, as checkpoints of this format store it (checkpoint.py reads their names).
 """
 from __future__ import annotations
 
