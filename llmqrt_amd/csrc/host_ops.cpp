@@ -546,8 +546,10 @@ bool block_weight_ok(const Tensor& w, const Tensor& w_scale, const std::optional
     return weight_ok(w, at::kFloat8_e4m3fn, dev, K) && scale_ok(w_scale, dev, blocks128(w.size(0)) * blocks128(K)) && w_scale.dim() == 2 &&
            w_scale.size(1) == blocks128(K) && block_bias_ok(bias, dev, w.size(0));
 }
-bool groups_ok(const Tensor& a_scale, const at::Device& dev, const Rows& r) {  // [.., ceil(K / 128)]
-    return scale_ok(a_scale, dev, r.M * blocks128(r.K)) && a_scale.dim() >= 1 && a_scale.size(-1) == blocks128(r.K);
+// [.., ceil(K / 128)] with the rows' own dimensions, or those in one
+bool groups_ok(const Tensor& a_scale, const Tensor& q, const Rows& r) {
+    if (!scale_ok(a_scale, q.device(), r.M * blocks128(r.K)) || a_scale.dim() < 1 || a_scale.size(-1) != blocks128(r.K)) return false;
+    return a_scale.dim() == 2 || (a_scale.dim() == q.dim() && a_scale.sizes().slice(0, a_scale.dim() - 1) == q.sizes().slice(0, q.dim() - 1));
 }
 void block_gemm(const void* q, const float* a_scale, const Tensor& w, const Tensor& w_scale, const std::optional<Tensor>& bias, int64_t M, int64_t K,
                 Tensor& out, const Launch& l) {
@@ -565,7 +567,7 @@ std::optional<Tensor> fp8_block(const Tensor& q, const Tensor& a_scale, const Te
                                 at::ScalarType odt) {
     const Rows r = rows_of(q);
     if (!r.ok || !is16(odt) || q.scalar_type() != at::kFloat8_e4m3fn || !block_weight_ok(w, w_scale, bias, q.device(), r.K) ||
-        !groups_ok(a_scale, q.device(), r))
+        !groups_ok(a_scale, q, r))
         return std::nullopt;
     const Launch l(q.device());
     Tensor out = make(out_size(q, w.size(0)), odt, q.device());

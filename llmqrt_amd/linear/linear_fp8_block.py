@@ -105,13 +105,13 @@ class FP8BlockLinear(_FP8BlockBase):
         return f8f8_blockwise(q, self.weight.t(), self.bias, s, self.weight_scale, _NAMES[x.dtype]).view(out_shape)
 
     def forward_quantized(self, qinput, x_scale):
-        """Forward for activations already quantized per token and 128 channels (e4m3fn qinput [.., K], fp32 scales [.., ceil(K / 128)]), e.g.
-        by the fused norm; the result is in the module's dtype."""
+        """Forward for activations already quantized per token and 128 channels (e4m3fn qinput [.., K], fp32 scales [.., ceil(K / 128)] or
+        [tokens, ceil(K / 128)]), e.g. by the fused norm; the result is in the module's dtype."""
         b = self._buffers
         y = host().fp8_block(qinput, x_scale, b["weight"], b["weight_scale"], b["bias"], self.dtype)
-        if y is None and x_scale.shape[:-1] != qinput.shape[:-1]:
-            raise RuntimeError("x_scale must hold one scale per token and 128 channels, [.., ceil(K / 128)]")
         if y is None:
+            if x_scale.dim() != 2 and x_scale.shape[:-1] != qinput.shape[:-1]:
+                raise RuntimeError("x_scale must hold one scale per token and 128 channels, [.., ceil(K / 128)]")
             y = f8f8_blockwise(qinput.reshape(-1, qinput.shape[-1]), self.weight.t(), self.bias, x_scale.reshape(-1, x_scale.shape[-1]), self.weight_scale,
                                _NAMES[self.dtype]).view(*qinput.shape[:-1], self.out_features)
         return y

@@ -123,3 +123,25 @@ def test_a_residual_over_part_of_the_activations(cuda):
             got = f(x, r, w, inplace=True)
             assert got[-1].data_ptr() == r.data_ptr() and all(same(a.contiguous().view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
             buf.copy_(was)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_scales_in_the_tokens_order(cuda, wide):
+    """Scales with the dimensions of the codes, or one row per token; other dimensions of as many scales are refused.  Contiguous codes (the native path) and
+    codes inside a wider tensor."""
+    from llmqrt_amd.linear import FP8BlockLinear
+    from llmqrt_amd.quantize import per_group_quantize
+    g = torch.Generator().manual_seed(6)
+    m = FP8BlockLinear(256, 72, False, dev=cuda)
+    m.set_weight(torch.randn(72, 256, generator=g))
+    x = torch.randn(2, 3, 256, generator=g).bfloat16().to(cuda)
+    q, s = per_group_quantize(x)
+    want = m(x)
+    if wide:
+        room = torch.zeros(2, 3, 512, dtype=torch.uint8, device=cuda)
+        room[..., :256] = q.view(torch.uint8)
+        q = room.view(E4M3)[..., :256]
+    assert same(m.forward_quantized(q, s), want) and same(m.forward_quantized(q, s.view(6, 2)), want)
+    for bad in (s.transpose(0, 1).contiguous(), s.view(3, 2, 2), s.view(1, 6, 2), s.view(1, 2, 3, 2), s.view(12), s.view(4, 3), s.view(6, 2)[:5]):
+        with pytest.raises(RuntimeError):
+            m.forward_quantized(q, bad)
