@@ -169,7 +169,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     int ld_kb = kb0 + group + tn * kNumXcd / tiles_n * kfull / kNumXcd * KS;
     // What the groups' whole blocks leave of this split comes last: at most a block for each group, one of them ragged.  Its missing chunks are read as
     // the block's first one (a group without a block: of any), and zeros take their place in the weights' operand; what the tokens have there belongs to the
-    // same row, so where it is NaN the result is too.  A group without a block has zeros for scales as well: those it read may be infinite.
+    // same row, so where it is NaN the result is too.  A group without a block multiplies nothing: the scales that it read may be infinite.
     // It has a place of its own behind the loop below, so that the others' loads have no part in it (us, each load's offset corrected in the loop / so: 8192 x
     // 37888 x 3584 1055 / 990, 1000 x 4608 x 3584 26.2 / 25.4).
     const bool rest = TAIL && kb0 + kfull * KS < kb1;  // block-uniform
@@ -344,12 +344,8 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     }
     drive([&]() __attribute__((always_inline)) { first_operands(sub); },
           [&](int stage, int next, int prev, int younger, auto rest_c, auto first_c, auto next_c, auto last_c) __attribute__((always_inline)) {
-              if (TAIL && !decltype(next_c)::value && rest) {  // the last block: a lane's chunks kq and kq + 4 of it, its scales
-                  if (left == 0) {
-                      w_next = 0.f;
-#pragma unroll
-                      for (int i = 0; i < TM; i++) s_next[i] = 0.f;
-                  }
+              if (TAIL && !decltype(next_c)::value && rest) {  // the last block: a lane's chunks kq and kq + 4 of it
+                  if (KS > 1 && left == 0) return;  // (one group always has a block here); the products before are scaled in behind the loop
                   const int lo = kq * 16 < left ? -1 : 0, hi = (kq + 4) * 16 < left ? -1 : 0;
 #pragma unroll
                   for (int j = 0; j < TN; j++)
