@@ -29,7 +29,7 @@ from .linear import FP8BlockGroupedLinear, FP8BlockLinear, SqW8A8BBF16OBF16PerCh
 
 @dataclass
 class QuantConfig:
-    """Field names and defaults of the reference's QuantConfig (core/config.py:9-20)."""
+    """Field names and defaults of the reference's QuantConfig (core/config.py:9-20), and one for block-scaled checkpoints."""
     quant_method: str = "awq"          # "awq" | "sq" | "fp8_static_quant" | "fp8_dynamic_quant"
     zero_point: bool = False
     q_group_size: int = 0
