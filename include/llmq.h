@@ -401,7 +401,8 @@ int llmq_add_rmsnorm(int out, const void* x, int x_dtype, int64_t M, int64_t K, 
 /* out[m, n] = out_dtype( sum_b a_scale[m, b] w_scale[n / 128, b] sum_{k in block b} A[m, k] B[n, k]  + bias[n] ), blocks of 128 of K, sums in fp32.
  * Not every bit of an fp32 sum is there: the matrix instruction adds each run of 8 consecutive products (k = 8 i .. 8 i + 7) in fixed point and cuts each of
  * them off below 2^-13 of the run's largest.  A run loses less than 7 * 2^-13 of its largest product, so where large products cancel, small ones beside them
- * may be gone.
+ * may be gone.  Sizes that take 2^32 threads or more in one launch, which can happen from 2^28 channels, 2^28 rows or 2^35 outputs on, are refused
+ * (LLMQ_ERR_SHAPE).
  * A: e4m3fn [M, K] (lda >= K), B: e4m3fn [N, K] (ldb >= K), 16-byte aligned, K, lda, ldb multiples of 16 and at most 2^23; a_scale: fp32
  * [M, ceil(K / 128)], w_scale: fp32 [ceil(N / 128), ceil(K / 128)], contiguous; bias: [N] bf16 / f16 / f32 or null; out: bf16 / f16, ldo >= N, any
  * even address.  workspace: >= llmq_gemm_fp8_block_workspace_bytes(M, N, K) bytes, 16-byte aligned (may be NULL when that is 0). */

@@ -133,24 +133,25 @@ def load_quantized_weights(model: nn.Module, path: str, device=None) -> tuple[li
     or a directory with a ``model.safetensors.index.json``).  Shapes and dtypes must match what the modules
     allocated (scalars may come as 0-dim or 1-element tensors).  Floating-point values are converted; what becomes 8 bits must be such values already
     (codes that are stored in a wider type), since an unquantized weight would lose most of its bits unseen.  A directory that holds a block-scaled
-    module's weight must hold its scales too, which may be named ``weight_scale_inv`` (the factor of the codes all the same).  Codes are not loaded as the
-    weight of an nn.Linear.  -> (missing names, unexpected names)."""
+    module's weight must hold its scales too, which may be named ``weight_scale_inv`` (the factor of the codes all the same).  Codes with
+    scales are refused for an nn.Linear.  -> (missing names, unexpected names)."""
     from safetensors import safe_open
 
     own = dict(model.named_parameters())
     own.update(dict(model.named_buffers()))
     modules = dict(model.named_modules())
     block_scaled = (FP8BlockLinear, FP8BlockGroupedLinear)
-    seen, unexpected = set(), []
+    seen, unexpected, plain = set(), [], []
     for file in _checkpoint_files(path):
         with safe_open(file, framework="pt", device="cpu") as f:
             for key in f.keys():
-                stored, owner = key, modules.get(key.rpartition(".")[0])
-                if isinstance(owner, block_scaled) and key.endswith("weight_scale_inv"):
+                stored, (prefix, _, last) = key, key.rpartition(".")
+                owner = modules.get(prefix)
+                if isinstance(owner, block_scaled) and last == "weight_scale_inv":
                     key = key.removesuffix("_inv")
                 dst = own.get(key)
                 if dst is None:
-                    unexpected.append(key)
+                    unexpected.append(stored)
                     continue
                 src = f.get_tensor(stored)
                 if src.numel() == dst.numel() and src.shape != dst.shape and dst.numel() == 1:
@@ -160,13 +161,16 @@ def load_quantized_weights(model: nn.Module, path: str, device=None) -> tuple[li
                 if src.dtype != dst.dtype and not (src.is_floating_point() and dst.is_floating_point()):
                     raise RuntimeError(f"{key}: checkpoint dtype {src.dtype} != module dtype {dst.dtype}")
                 if type(owner) is nn.Linear and src.dtype.itemsize == 1 and src.is_floating_point():
-                    raise RuntimeError(f"{key}: the checkpoint holds codes in {src.dtype} for a module that is not quantized")
+                    plain.append(key)
                 cast = src.to(dst.dtype)
                 if dst.dtype.itemsize == 1 and src.dtype != dst.dtype and not torch.equal(cast.float(), src.float()):
                     raise RuntimeError(f"{key}: values in {src.dtype} that are no {dst.dtype} codes; an unquantized weight must be quantized first")
                 with torch.no_grad():
                     dst.copy_(cast)
                 seen.add(key)
+    for key in plain:
+        if f"{key}_scale" in unexpected or f"{key}_scale_inv" in unexpected:
+            raise RuntimeError(f"{key}: the checkpoint holds codes and scales for a module that is not quantized")
     for name, m in modules.items():
         weight, scale = (f"{name}.{t}" if name else t for t in ("weight", "weight_scale"))
         if not os.path.isfile(path) and isinstance(m, block_scaled) and weight in seen and scale not in seen:

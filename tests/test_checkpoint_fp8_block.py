@@ -121,8 +121,17 @@ def test_other_fp8_checkpoints_are_refused(tmp_path, config):
 def test_codes_do_not_become_plain_weights(tmp_path):
     from llmqrt_amd.checkpoint import load_quantized_weights
     m = Layer()
-    was = m.mlp.gate.weight.clone()
-    save_file({"mlp.gate.weight": codes((2, 144), 1)}, str(tmp_path / "m.safetensors"))
-    with pytest.raises(RuntimeError, match="not quantized"):
-        load_quantized_weights(m, str(tmp_path))
-    assert torch.equal(m.mlp.gate.weight, was)
+    q = codes((2, 144), 1)
+    for name in ("weight_scale_inv", "weight_scale"):
+        save_file({"mlp.gate.weight": q, f"mlp.gate.{name}": torch.ones(1, 2)}, str(tmp_path / "m.safetensors"))
+        with pytest.raises(RuntimeError, match="not quantized"):
+            load_quantized_weights(m, str(tmp_path))
+    save_file({"mlp.gate.weight": q}, str(tmp_path / "m.safetensors"))  # 8-bit values as they are, without scales
+    assert "mlp.gate.weight" not in load_quantized_weights(m, str(tmp_path))[0] and torch.equal(m.mlp.gate.weight, q.float())
+
+
+def test_other_names_stay_unexpected(tmp_path):
+    from llmqrt_amd.checkpoint import load_quantized_weights
+    m = model("up")
+    save_file({"up.my_weight_scale_inv": torch.ones(2, 2)}, str(tmp_path / "m.safetensors"))
+    assert load_quantized_weights(m, str(tmp_path)) == (["up.weight", "up.weight_scale"], ["up.my_weight_scale_inv"])
