@@ -145,3 +145,58 @@ def test_scales_in_the_tokens_order(cuda, wide):
     for bad in (s.transpose(0, 1).contiguous(), s.view(3, 2, 2), s.view(1, 6, 2), s.view(1, 2, 3, 2), s.view(12), s.view(4, 3), s.view(6, 2)[:5]):
         with pytest.raises(RuntimeError):
             m.forward_quantized(q, bad)
+
+
+def test_threads(cuda):
+    """Four threads with a stream each, every one with its own sizes (split products among them): what each gets alone."""
+    import threading
+    from llmqrt_amd.norm import add_rmsnorm_per_group_quantize
+    from llmqrt_amd.sq_fp8_kernels import f8f8_blockwise, f8f8_blockwise_grouped
+    g = torch.Generator().manual_seed(7)
+    cases = []
+    for rows, n, k in ((1, 640, 896), (70, 256, 8192), (200, 512, 4096), (17, 1000, 400)):
+        x, r = [torch.randn(rows, k, generator=g).bfloat16().to(cuda) for _ in range(2)]
+        w = (torch.randn(2, n, k, generator=g) * 90).clamp(-448, 448).to(E4M3).to(cuda)
+        sw = (torch.rand(2, -(-n // 128), -(-k // 128), generator=g) * 1e-3).to(cuda)
+        off = torch.tensor([0, rows // 2, rows], dtype=torch.int32, device=cuda)
+        cases.append((x, r, torch.ones(k, dtype=torch.bfloat16, device=cuda), w, sw, off))
+
+    def run(x, r, weight, w, sw, off):
+        q, s, h = add_rmsnorm_per_group_quantize(x, r, weight)
+        return q.view(torch.uint8), s, h, f8f8_blockwise(q, w[0].t(), None, s, sw[0]), f8f8_blockwise_grouped(q, w, None, s, sw, off)
+    want = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = run(*cases[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(same(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not wrong and not any(t.is_alive() for t in threads)
+
+
+def test_a_captured_residual_in_place(cuda):
+    """Each replay adds the activations to the residual as it then is, beside eager calls on another one."""
+    for f in norm_calls():
+        x = torch.ones(6, 256, dtype=torch.bfloat16, device=cuda)
+        w = torch.ones(256, dtype=torch.bfloat16, device=cuda)
+        r, other = torch.zeros_like(x), torch.zeros_like(x)
+        f(x, r, w, inplace=True)
+        r.zero_()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = f(x, r, w, inplace=True)
+        for k in range(1, 4):
+            graph.replay()
+            eager = f(x, other, w, inplace=True)
+            torch.cuda.synchronize()
+            assert (r == k).all() and all(same(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(outs, eager))
