@@ -422,6 +422,63 @@ int llmq_gemm_fp8_block_grouped(const uint8_t* A, int64_t lda, const float* a_sc
  * later calls of the two products (by experts: tiles only, no split).  Per host thread. */
 int llmq_gemm_fp8_block_force_plan(int cfg, int splits);
 
+/* ------------------------------------------------------------------------------------
+ * Around products by experts (no counterpart in the reference): a token's experts, its rows' way to them and back, the W8A8 product by experts, and the
+ * gated activation between two products.  Nothing is read back by the host, so captured calls follow the routing of their replay.
+ * ------------------------------------------------------------------------------------ */
+
+/* experts[t, :] = the top_k experts with the largest c = s + bias, largest first, ties to the lowest expert; weights[t, :] = their s, divided by
+ * their sum where renormalize != 0, times scale;  s = softmax(logits[t, :]) or 1 / (1 + exp(-logits)).  bias: fp32 [experts] or null; it takes part in the choice
+ * alone.  With groups > 1 (it divides experts; at most 64) only the experts of the top_groups groups of neighbours with the largest score are
+ * chosen from: the largest c of the group, or the sum of its two largest.
+ * An expert whose logit or bias is -inf is never chosen; a place that is left over has expert -1 and weight 0.  The order is that of the exact scores: without a
+ * bias the logits' own, otherwise that of scores in 64 bits.  A token with a NaN among its logits gets experts of that range, none twice, and for
+ * softmax weights that are NaN.
+ * logits: bf16 / f16 / f32 [tokens, experts], row stride ld, at any address of its type; at most 1024 experts, top_k at most 64 and at most experts /
+ * groups * top_groups.  weights: fp32 [tokens, top_k]; experts: int32 [tokens, top_k]. */
+enum { LLMQ_ROUTE_SOFTMAX = 0, LLMQ_ROUTE_SIGMOID = 1 };
+enum { LLMQ_ROUTE_GROUP_MAX = 0, LLMQ_ROUTE_GROUP_TOP2 = 1 };
+int llmq_route_experts(int scoring, const void* logits, int logits_dtype, int64_t tokens, int64_t experts, int64_t ld, const float* bias,
+                       int64_t groups, int64_t top_groups, int group_score, int64_t top_k, int renormalize, float scale, float* weights,
+                       int32_t* ids, llmq_stream_t stream);
+
+/* The rows of products by experts: a row for each of a token's top_k experts, sorted by expert and within an expert as the ids lie.
+ *   ids: int32 [tokens, top_k], counted from first_expert; those outside [first_expert, first_expert + experts) go nowhere
+ *   offsets: int32 [experts + 1], the experts' first rows and the end of the last; places: int32 [tokens, top_k], the row of a token's copy, -1: none
+ *   rows: [tokens * top_k, K]; rows from offsets[experts] on are left as they are.  out (of llmq_add_rmsnorm's):
+ *     LLMQ_NORM_SAME       x_dtype, 16-byte aligned
+ *     LLMQ_NORM_I8_TOKEN   the codes of llmq_quant_i8_per_token, 8-byte aligned; scale: fp32 [tokens * top_k]
+ *     LLMQ_NORM_FP8_GROUP  the codes of llmq_quant_fp8_per_group, 8-byte aligned; scale: fp32 [tokens * top_k, ceil(K / 128)]
+ * x: [tokens, K] bf16 / f16, K % 8 == 0, ldx % 8 == 0, 16-byte aligned.  At most 4096 experts, top_k at most 64, fewer than 2^31 - 255 rows.
+ * workspace: >= llmq_dispatch_workspace_bytes(tokens, top_k, experts) bytes, 4-byte aligned, contents irrelevant (may be NULL when that is 0). */
+int llmq_dispatch_experts(int out, const void* x, int x_dtype, int64_t tokens, int64_t K, int64_t ldx, const int32_t* ids, int64_t top_k,
+                          int64_t first_expert, int64_t experts, void* rows, float* scale, int32_t* offsets, int32_t* places,
+                          void* workspace, size_t workspace_bytes, llmq_stream_t stream);
+size_t llmq_dispatch_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts);
+
+/* out[t, :] = dtype( sum_j weights[t, j] y[places[t, j], :]  (+ shared[t, :]) ), fp32 sums in the order of j, the shared row last.  Places outside
+ * [0, rows) add nothing, whatever their weight.  y: bf16 / f16 [rows, N], shared: [tokens, N] or null, out: [tokens, N] contiguous, all of one type; N % 8 == 0,
+ * row strides % 8 == 0, 16-byte aligned; top_k at most 64.  out must not overlap y or shared. */
+int llmq_combine_experts(const void* y, int dtype, int64_t rows, int64_t N, int64_t ldy, const int32_t* places, const float* weights,
+                         int64_t tokens, int64_t top_k, const void* shared, int64_t ld_shared, void* out, llmq_stream_t stream);
+
+/* out[m, n] = out_dtype( (acc * a_scale[m]) * w_scale[e, n] + bias[e, n] ), acc = sum_k A[m, k] B[e, n, k] exact, for the rows m of expert e: offsets[e] ..
+ * offsets[e + 1] - 1.  A: int8 [M, K] (lda >= K), B: int8 [experts, N, K], 16-byte aligned, K and lda multiples of 16, K < 131072 (the sums stay in int32),
+ * lda at most 2^23; a_scale: fp32 [M], w_scale: fp32 [experts, N]; bias: [experts, N] bf16 / f16 / f32 or null; all but A contiguous; out: bf16 / f16, ldo >= N.
+ * offsets: int32 [experts + 1] on the device, ascending; values outside [0, M] are taken as the nearest inside,
+ * and one below an earlier one as that, so that no row has two experts.  Rows of no expert are not written.
+ * At most 65536 experts.  No workspace.  Sizes that take 2^32 threads or more in one launch are refused (LLMQ_ERR_SHAPE). */
+int llmq_gemm_w8a8_grouped(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, const float* w_scale, const int32_t* offsets,
+                           int64_t experts, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N,
+                           int64_t K, llmq_stream_t stream);
+/* Tuning / test hook: tile configuration 4 .. 10 of later calls (numbered as llmq_gemm_force_plan's), -1: the built-in choice.  Per host thread. */
+int llmq_gemm_w8a8_grouped_force_plan(int cfg);
+
+/* y[m, n] = g / (1 + exp(-g)) * u with g = x[m, n], u = x[m, N + n], in fp32; out as llmq_add_rmsnorm's:
+ *   LLMQ_NORM_SAME y = x_dtype(y) (16-byte aligned); otherwise codes of the fp32 y (8-byte aligned) and scale: fp32 [M] or [M, ceil(N / 128)]
+ * x: [M, 2 N] bf16 / f16, N % 8 == 0, ldx % 8 == 0, 16-byte aligned; y: [M, N] contiguous, must not overlap x. */
+int llmq_silu_mul(int out, const void* x, int x_dtype, int64_t M, int64_t N, int64_t ldx, void* y, float* scale, llmq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

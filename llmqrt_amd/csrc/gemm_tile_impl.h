@@ -102,11 +102,16 @@ __device__ __forceinline__ void unrolled(F&& f) {
     }
 }
 
-template <class C, bool KFULL>
+// What a launch multiplies: one matrix, or the experts' (gemm_tile_i8_grouped.hip)
+struct OneMatrix { static constexpr bool GROUPED = false; };
+
+// EX::GROUPED: A's rows are sorted by expert; B, the channels' scales and the bias are expert 0's, the others' follow.  No K split and no dump.
+template <class C, bool KFULL, class EX = OneMatrix>
 __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
     const uint8_t* __restrict__ A, int64_t lda, const uint8_t* __restrict__ B, int64_t ldb,
     int M, int N, int K, int k_per_split, Epilogue ep, void* __restrict__ out, int64_t ldo,
-    void* __restrict__ acc_dump, void* __restrict__ partials) {
+    void* __restrict__ acc_dump, void* __restrict__ partials, EX ex = {}) {
+    constexpr bool GROUPED = EX::GROUPED;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem_raw[];
     uint4* lds = reinterpret_cast<uint4*>(smem_raw);
     using acc_t = typename std::conditional<C::FACC, v16f, v16i>::type;
@@ -114,9 +119,19 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
     const int wm = wave / C::WN, wn = wave % C::WN;
     const int tiles_m = (M + C::BM - 1) / C::BM, tiles_n = (N + C::BN - 1) / C::BN;
-    int tile_m, tile_n;
-    tile_coords(blockIdx.x, gridDim.x, tiles_m, tiles_n, tile_m, tile_n);
-    const int m0 = tile_m * C::BM, n0 = tile_n * C::BN;
+    int tile_m, tile_n, row0;
+    if constexpr (GROUPED) {
+        int expert, row_end;
+        if (!ex.template tile<C::BM>(M, tiles_n, expert, row0, row_end, tile_n)) return;  // block-uniform
+        M = row_end;  // the tile's rows end where the expert's do
+        B += (int64_t)expert * N * ldb;
+        ep.w_scale += (int64_t)expert * N;
+        if (ep.bias) ep.bias = (const uint8_t*)ep.bias + (int64_t)expert * N * (ep.bias_dtype == LLMQ_F32 ? 4 : 2);
+    } else {
+        tile_coords(blockIdx.x, gridDim.x, tiles_m, tiles_n, tile_m, tile_n);
+        row0 = tile_m * C::BM;
+    }
+    const int m0 = row0, n0 = tile_n * C::BN;
     const int k_begin = blockIdx.y * k_per_split;
     const int k_end = min(K, k_begin + k_per_split);
     const int ktiles = (k_end - k_begin + C::BK - 1) / C::BK;
@@ -360,23 +375,27 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
         // tiles not requested, weights out of HBM, int8 1000 x 4608 x 3584 32.1 / 30.0, 2048 x 4608 x 3584 50.8 / 44.1, 8192 x
         // 37888 x 3584 996 / 975, fp8 512 x 37888 x 3584 93.0 / 88.7, 4096 x 3584 x 18944 249 / 226, fp16 777 x 3584 x 18944 140 / 132.
         // (Level or slower: two requests behind an MFMA, s_setprio around the MFMAs, all fragment reads first.)
-        auto sub_step = [&](int rd, int ks_rd, auto par_c, auto d0_c, auto load_c, int ld_stage) __attribute__((always_inline)) {
+        auto sub_step = [&](auto work_c, int rd, int ks_rd, auto par_c, auto d0_c, auto load_c, int ld_stage) __attribute__((always_inline)) {
             constexpr int par = decltype(par_c)::value, D0 = decltype(d0_c)::value;
             constexpr bool LOAD = decltype(load_c)::value && D0 < LPT;
+            constexpr bool WORK = decltype(work_c)::value;
             unrolled<0, SLOTS>([&](auto m_c) __attribute__((always_inline)) {
                 constexpr int m = decltype(m_c)::value, FR = C::TM + C::TN, RPS = (FR + SLOTS - 1) / SLOTS;
-                unrolled<(m * RPS < FR ? m * RPS : FR), ((m + 1) * RPS < FR ? (m + 1) * RPS : FR)>([&](auto r_c) __attribute__((always_inline)) {
+                if constexpr (WORK) unrolled<(m * RPS < FR ? m * RPS : FR), ((m + 1) * RPS < FR ? (m + 1) * RPS : FR)>([&](auto r_c) __attribute__((always_inline)) {
                     constexpr int r = decltype(r_c)::value;  // the order of first use: A 0, B 0 .. TN - 1, A 1 ..
                     if constexpr (r >= 1 && r <= C::TN) read_frag_b(rd, ks_rd, r - 1, fb[par ^ 1][r - 1]);
                     else read_frag_a(rd, ks_rd, r ? r - C::TN : 0, fa[par ^ 1][r ? r - C::TN : 0]);
                 });
-                mfma_one(m / C::TN, m % C::TN, fa[par], fb[par]);
+                if constexpr (WORK) mfma_one(m / C::TN, m % C::TN, fa[par], fb[par]);
                 if constexpr (LOAD)
                     unrolled<(D0 + m * PER < LPT ? D0 + m * PER : LPT), (D0 + (m + 1) * PER < LPT ? D0 + (m + 1) * PER : LPT)>(
                         [&](auto d) __attribute__((always_inline)) { issue(ld_stage, d); });
                 __builtin_amdgcn_sched_barrier(0);
             });
         };
+        // WORK: the wavefront has rows and channels; otherwise it loads its pieces and waits with the others, and multiplies nothing
+        auto all_tiles = [&](auto work_c) __attribute__((always_inline)) {
+        constexpr bool WORK = decltype(work_c)::value;
         unrolled<0, NS - 1>([&](auto t_c) __attribute__((always_inline)) {
             constexpr int t = decltype(t_c)::value;
             if (t < kfull) {
@@ -386,7 +405,7 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
         });
         wait_next_tile(min(kfull, NS - 1) - 1);
         lds_barrier();
-        read_frags(0, 0, fa[0], fb[0]);
+        if constexpr (WORK) read_frags(0, 0, fa[0], fb[0]);
         // the stage NS - 1 is free from the start: the part of its tile that the loop requests behind a barrier comes first
         if (NS - 1 < kfull)
             unrolled<0, (STEP < LPT ? STEP : LPT)>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
@@ -396,7 +415,7 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
             const int prev = stage == 0 ? NS - 1 : stage - 1, next = stage == NS - 1 ? 0 : stage + 1;
             unrolled<0, C::KSUB - 1>([&](auto ks_c) __attribute__((always_inline)) {
                 constexpr int ks = decltype(ks_c)::value;
-                sub_step(stage, ks + 1, std::integral_constant<int, ks & 1>{}, std::integral_constant<int, (ks + 1) * STEP>{}, rest_c, prev);
+                sub_step(work_c, stage, ks + 1, std::integral_constant<int, ks & 1>{}, std::integral_constant<int, (ks + 1) * STEP>{}, rest_c, prev);
             });
             if constexpr (decltype(rest_c)::value) {
                 next_kt();
@@ -406,7 +425,7 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
             }
             lds_barrier();
             // every wavefront has read the whole of stage kt: it takes tile kt + NS
-            sub_step(next, 0, std::integral_constant<int, (C::KSUB - 1) & 1>{}, std::integral_constant<int, 0>{}, first_c, stage);
+            sub_step(work_c, next, 0, std::integral_constant<int, (C::KSUB - 1) & 1>{}, std::integral_constant<int, 0>{}, first_c, stage);
             stage = next;
             kt++;
         };
@@ -416,6 +435,11 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
         // Past the last request nothing is fetched: a block that ends waits for no load that nobody reads.
 #pragma unroll 1
         while (kt < kfull) k_tile(std::false_type{}, std::false_type{});
+        };
+        bool idle = false;  // wavefront-uniform
+        if constexpr (GROUPED) idle = m0 + __builtin_amdgcn_readfirstlane(wm) * C::WTM >= M || n0 + __builtin_amdgcn_readfirstlane(wn) * C::WTN >= N;
+        if (idle) all_tiles(std::false_type{});
+        else all_tiles(std::true_type{});
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing may still be landing in LDS when it is reused or released
         lds_barrier();
         if constexpr (!KFULL) {
@@ -423,10 +447,12 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
                 load_tile(kfull, ra[0], rb[0]);
                 store_tile(0, kfull, ra[0], rb[0]);
                 lds_barrier();
+                if (!idle) {
 #pragma unroll
-                for (int ks = 0; ks < C::KSUB; ks++) {
-                    read_frags(0, ks, fa[0], fb[0]);
-                    mfma_step(fa[0], fb[0]);
+                    for (int ks = 0; ks < C::KSUB; ks++) {
+                        read_frags(0, ks, fa[0], fb[0]);
+                        mfma_step(fa[0], fb[0]);
+                    }
                 }
                 lds_barrier();
             }
@@ -464,7 +490,8 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
     // register quad.  After the dequant math the two half-waves exchange quads (v_permlane32_swap) so
     // that every lane owns 8 consecutive channels of its token and stores them as one 16-byte vector,
     // the two lanes of a token adjacent to each other.
-    const bool split = gridDim.y > 1;
+    const bool split = !GROUPED && gridDim.y > 1;
+    if constexpr (GROUPED) acc_dump = nullptr;
     const float alpha = ep.alpha * (ep.alpha_dev ? *ep.alpha_dev : 1.0f);
     const bool out_vec = ((ldo & 7) == 0) && ((reinterpret_cast<uintptr_t>(out) & 15u) == 0);
     const bool raw_vec = (N & 3) == 0;
@@ -473,8 +500,10 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
 
     // Fast path (block-uniform): interior tile, fused epilogue, vector stores.  No per-element dtype
     // switches or bounds checks: ~5 VALU operations per output instead of several times that.
-    if (!split && !acc_dump && !ep.out_scale && out_vec && m0 + C::BM <= M && n0 + C::BN <= N &&
+    // (By experts: rows past the expert's last are computed from its last and not stored.)
+    if (!split && !acc_dump && !ep.out_scale && out_vec && (GROUPED || m0 + C::BM <= M) && n0 + C::BN <= N &&
         (reinterpret_cast<uintptr_t>(ep.w_scale) & 15u) == 0) {
+        auto row_in = [&](int m) __attribute__((always_inline)) { return GROUPED ? min(m, M - 1) : m; };
         auto fast = [&](auto out_dt_c, auto plain_c) {
             constexpr int ODT = decltype(out_dt_c)::value;
             constexpr bool PLAIN = decltype(plain_c)::value;  // no bias term and alpha = 1: the scaled accumulator is the output
@@ -487,7 +516,7 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
                 // store's completion (microseconds when every CU writes at once).
                 float sa_r[C::TM], sw_r[C::TN][16], bb_r[C::TN][16];
 #pragma unroll
-                for (int i = 0; i < C::TM; i++) sa_r[i] = ep.a_scale ? ep.a_scale[m0 + wm * C::WTM + i * 32 + l32] : 1.f;
+                for (int i = 0; i < C::TM; i++) sa_r[i] = ep.a_scale ? ep.a_scale[row_in(m0 + wm * C::WTM + i * 32 + l32)] : 1.f;
 #pragma unroll
                 for (int j = 0; j < C::TN; j++)
 #pragma unroll
@@ -547,7 +576,7 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
                     for (int it = 0; it < 8; it++) {
                         const int q = it * kWave + lane, row = q >> 3, c = q & 7;
                         const uint4 v = region[row * 8 + (c ^ ((row >> 1) & 7))];
-                        store_streaming(obase + (int64_t)row * ldo + 8 * c, v);
+                        if (!GROUPED || m0 + wm * C::WTM + p * 64 + row < M) store_streaming(obase + (int64_t)row * ldo + 8 * c, v);
                     }
                   }
                 }
@@ -561,7 +590,7 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
             if constexpr (BLOCK_EPI) {
                 float sa_r[C::TM], sw_r[C::TN][16], bb_r[C::TN][16];  // fetched before any store is issued (see above)
 #pragma unroll
-                for (int i = 0; i < C::TM; i++) sa_r[i] = ep.a_scale ? ep.a_scale[m0 + wm * C::WTM + i * 32 + l32] : 1.f;
+                for (int i = 0; i < C::TM; i++) sa_r[i] = ep.a_scale ? ep.a_scale[row_in(m0 + wm * C::WTM + i * 32 + l32)] : 1.f;
 #pragma unroll
                 for (int j = 0; j < C::TN; j++)
 #pragma unroll
@@ -607,13 +636,13 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
 #pragma unroll
                 for (int it = 0; it < C::BM * 16 / C::NT; it++) {
                     const int q = it * C::NT + tid, row = q >> 4, c = q & 15;
-                    store_streaming(obase + (int64_t)row * ldo + 8 * c, lds[row * 16 + (c ^ (row & 15))]);
+                    if (!GROUPED || m0 + row < M) store_streaming(obase + (int64_t)row * ldo + 8 * c, lds[row * 16 + (c ^ (row & 15))]);
                 }
                 return;
             }
             float sa_r[C::TM];  // fetched before any store is issued (see above)
 #pragma unroll
-            for (int i = 0; i < C::TM; i++) sa_r[i] = ep.a_scale ? ep.a_scale[m0 + wm * C::WTM + i * 32 + l32] : 1.f;
+            for (int i = 0; i < C::TM; i++) sa_r[i] = ep.a_scale ? ep.a_scale[row_in(m0 + wm * C::WTM + i * 32 + l32)] : 1.f;
 #pragma unroll
             for (int j = 0; j < C::TN; j++) {
                 const int nb = n0 + wn * C::WTN + j * 32;
@@ -656,7 +685,7 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
                             pk[2 * g][x] = sw2[0];
                             pk[2 * g + 1][x] = sw2[1];
                         }
-                        store_streaming(orow + nb + 16 * g + 8 * khalf, make_uint4(pk[2 * g][0], pk[2 * g][1], pk[2 * g + 1][0], pk[2 * g + 1][1]));
+                        if (!GROUPED || m < M) store_streaming(orow + nb + 16 * g + 8 * khalf, make_uint4(pk[2 * g][0], pk[2 * g][1], pk[2 * g + 1][0], pk[2 * g + 1][1]));
                     }
                 }
             }
@@ -872,13 +901,13 @@ int launch_cfg(const uint8_t* A, int64_t lda, const uint8_t* B, int64_t ldb, int
     if constexpr (C::DMA && C::BK != 128) {
         if (!kfull) return LLMQ_ERR_SHAPE;  // callers route ragged K to the register-staged kernel
         hipLaunchKernelGGL((gemm_tile_kernel<C, true>), dim3(tiles, p.splits), dim3(C::NT), C::LDS_BYTES, st, A, lda, B,
-                           ldb, M, N, K, p.k_per_split, ep, out, ldo, acc_dump, ws);
+                           ldb, M, N, K, p.k_per_split, ep, out, ldo, acc_dump, ws, OneMatrix{});
     } else if (kfull)
         hipLaunchKernelGGL((gemm_tile_kernel<C, true>), dim3(tiles, p.splits), dim3(C::NT), C::LDS_BYTES, st, A, lda, B,
-                           ldb, M, N, K, p.k_per_split, ep, out, ldo, acc_dump, ws);
+                           ldb, M, N, K, p.k_per_split, ep, out, ldo, acc_dump, ws, OneMatrix{});
     else
         hipLaunchKernelGGL((gemm_tile_kernel<C, false>), dim3(tiles, p.splits), dim3(C::NT), C::LDS_BYTES, st, A, lda,
-                           B, ldb, M, N, K, p.k_per_split, ep, out, ldo, acc_dump, ws);
+                           B, ldb, M, N, K, p.k_per_split, ep, out, ldo, acc_dump, ws, OneMatrix{});
     return launch_status();
 }
 

@@ -636,6 +636,130 @@ std::optional<Tensor> fp8_block_grouped(const Tensor& x, const std::optional<Ten
     return out;
 }
 
+// ---- around products by experts ----------------------------------------------------------------------------------
+// A status that a general path explains better
+bool refused(int status) { return status == LLMQ_ERR_SHAPE || status == LLMQ_ERR_DTYPE; }
+bool floats(at::ScalarType t) { return is16(t) || t == at::kFloat; }
+
+std::optional<Pair> route(const Tensor& logits, const std::optional<Tensor>& bias, int64_t top, int scoring, int64_t groups, int64_t top_groups,
+                          int group_score, bool renormalize, double scale) {
+    if (!logits.defined() || !logits.is_cuda() || logits.layout() != at::kStrided || logits.dim() < 1 || logits.numel() == 0 || !logits.is_contiguous() ||
+        !floats(logits.scalar_type()) || top < 1 || top > 64)
+        return std::nullopt;
+    const at::Device dev = logits.device();
+    const int64_t E = logits.size(-1), T = logits.numel() / E;
+    if (bias && (bias->dim() != 1 || !scale_ok(*bias, dev, E))) return std::nullopt;
+    const Launch l(dev);
+    Tensor w, ids;
+    Outputs o(dev);
+    o.add(&w, out_size(logits, top), at::kFloat);
+    o.add(&ids, out_size(logits, top), at::kInt);
+    o.make_all();
+    const int rc = llmq_route_experts(scoring, logits.data_ptr(), code(logits.scalar_type()), T, E, E, (const float*)ptr(bias), groups, top_groups, group_score,
+                                      top, renormalize, (float)scale, (float*)w.data_ptr(), (int32_t*)ids.data_ptr(), l.stream);
+    if (refused(rc)) return std::nullopt;
+    check(rc, "llmq_route_experts");
+    return std::make_pair(w, ids);
+}
+
+// out: LLMQ_NORM_SAME, _I8_TOKEN or _FP8_GROUP.  Results in order: rows, [scales], offsets, places.
+struct Sorted {
+    Tensor t[4];
+    int n = 0;
+};
+std::optional<Sorted> dispatch(const Tensor& x, const Tensor& ids, int64_t experts, int64_t first, int out) {
+    const Rows r = rows_of(x);
+    if (!r.ok || !is16(x.scalar_type()) || r.K % 8 || !ids.defined() || ids.scalar_type() != at::kInt || ids.dim() != x.dim() || !plain_on(ids, x.device()) ||
+        ids.sizes().slice(0, ids.dim() - 1) != x.sizes().slice(0, x.dim() - 1) || experts < 1 || experts > 4096 || ids.numel() > 0x7fffff00LL)
+        return std::nullopt;
+    const int64_t top = ids.size(-1), n = r.M * top;
+    if (top < 1 || top > 64) return std::nullopt;
+    const at::Device dev = x.device();
+    const Launch l(dev);
+    Tensor rows, scale, offsets, places, ws;
+    Outputs o(dev);
+    const bool same = out == LLMQ_NORM_SAME;
+    o.add(&rows, {n, r.K}, same ? x.scalar_type() : out == LLMQ_NORM_I8_TOKEN ? at::kChar : at::kFloat8_e4m3fn);
+    if (!same) o.add(&scale, {n, out == LLMQ_NORM_FP8_GROUP ? blocks128(r.K) : 1}, at::kFloat);
+    o.add(&offsets, {experts + 1}, at::kInt);
+    o.add(&places, ids.sizes(), at::kInt);
+    o.make_all();
+    const int64_t bytes = (int64_t)llmq_dispatch_workspace_bytes(r.M, top, experts);
+    if (bytes) ws = make({bytes}, at::kByte, dev);
+    const int rc = llmq_dispatch_experts(out, x.data_ptr(), code(x.scalar_type()), r.M, r.K, r.K, (const int32_t*)ids.data_ptr(), top, first, experts,
+                                         rows.data_ptr(), same ? nullptr : (float*)scale.data_ptr(), (int32_t*)offsets.data_ptr(),
+                                         (int32_t*)places.data_ptr(), bytes ? ws.data_ptr() : nullptr, (size_t)bytes, l.stream);
+    if (refused(rc)) return std::nullopt;
+    check(rc, "llmq_dispatch_experts");
+    Sorted s;
+    for (const Tensor* t : {&rows, &scale, &offsets, &places})
+        if (t->defined()) s.t[s.n++] = *t;
+    return s;
+}
+
+std::optional<Tensor> combine(const Tensor& y, const Tensor& places, const Tensor& weights, const std::optional<Tensor>& shared) {
+    const Rows r = rows_of(y);
+    if (!r.ok || y.dim() != 2 || !is16(y.scalar_type()) || r.K % 8) return std::nullopt;
+    const at::Device dev = y.device();
+    if (!places.defined() || places.scalar_type() != at::kInt || places.dim() < 1 || places.numel() == 0 || places.numel() > 0x7fffff00LL ||
+        !plain_on(places, dev) || !weights.defined() || weights.scalar_type() != at::kFloat || weights.sizes() != places.sizes() || !plain_on(weights, dev))
+        return std::nullopt;
+    const at::DimVector size = out_size(places, r.K);
+    if (shared && (shared->scalar_type() != y.scalar_type() || shared->sizes() != at::IntArrayRef(size) || !plain_on(*shared, dev) || !aligned(*shared)))
+        return std::nullopt;
+    const int64_t top = places.size(-1);
+    const Launch l(dev);
+    Tensor out = make(size, y.scalar_type(), dev);
+    const int rc = llmq_combine_experts(y.data_ptr(), code(y.scalar_type()), r.M, r.K, r.K, (const int32_t*)places.data_ptr(), (const float*)weights.data_ptr(),
+                                        places.numel() / top, top, ptr(shared), r.K, out.data_ptr(), l.stream);
+    if (refused(rc)) return std::nullopt;
+    check(rc, "llmq_combine_experts");
+    return out;
+}
+
+// int8 rows sorted by expert and their scales, one per row; out: given, or new
+std::optional<Tensor> w8a8_grouped(const Tensor& q, const Tensor& a_scale, const Tensor& w, const Tensor& w_scale, const std::optional<Tensor>& bias,
+                                   const Tensor& offsets, at::ScalarType odt, const std::optional<Tensor>& given) {
+    const Rows r = rows_of(q);
+    const at::Device dev = q.device();
+    if (!r.ok || q.dim() != 2 || q.scalar_type() != at::kChar || !is16(odt) || w.dim() != 3 || w.scalar_type() != at::kChar || w.size(2) != r.K || r.K % 16 ||
+        w.numel() == 0 || !plain_on(w, dev) || !aligned(w))
+        return std::nullopt;
+    const int64_t E = w.size(0), N = w.size(1);
+    if (!scale_ok(a_scale, dev, r.M) || a_scale.dim() < 1 || a_scale.dim() > 2 || a_scale.size(0) != r.M || !scale_ok(w_scale, dev, E * N) ||
+        !is_matrix(w_scale, E, N) || (bias && !is_matrix(*bias, E, N)) || !block_bias_ok(bias, dev, E * N) || offsets.dim() != 1 ||
+        offsets.numel() != E + 1 || offsets.scalar_type() != at::kInt || !plain_on(offsets, dev) ||
+        (given && (given->scalar_type() != odt || given->dim() != 2 || given->size(0) != r.M || given->size(1) != N || !plain_on(*given, dev) ||
+                   !writable(*given))))
+        return std::nullopt;
+    const Launch l(dev);
+    Tensor out = given ? *given : make({r.M, N}, odt, dev);
+    check(llmq_gemm_w8a8_grouped((const int8_t*)q.data_ptr(), r.K, (const float*)a_scale.data_ptr(), (const int8_t*)w.data_ptr(),
+                                 (const float*)w_scale.data_ptr(), (const int32_t*)offsets.data_ptr(), E, ptr(bias),
+                                 bias ? code(bias->scalar_type()) : LLMQ_BF16, out.data_ptr(), code(odt), N, r.M, N, r.K, l.stream),
+          "llmq_gemm_w8a8_grouped");
+    if (given) written(out);
+    return out;
+}
+
+// out: LLMQ_NORM_*.  Results: [y] or [codes, scales].
+std::optional<Sorted> silu_mul(const Tensor& x, int out) {
+    const Rows r = rows_of(x);
+    if (!r.ok || !is16(x.scalar_type()) || r.K % 16) return std::nullopt;
+    const at::Device dev = x.device();
+    const int64_t N = r.K / 2;
+    const Launch l(dev);
+    Sorted s;
+    Outputs o(dev);
+    const bool same = out == LLMQ_NORM_SAME;
+    o.add(&s.t[s.n++], out_size(x, N), same ? x.scalar_type() : out == LLMQ_NORM_I8_TOKEN ? at::kChar : at::kFloat8_e4m3fn);
+    if (!same) o.add(&s.t[s.n++], out_size(x, out == LLMQ_NORM_FP8_GROUP ? blocks128(N) : 1), at::kFloat);
+    o.make_all();
+    check(llmq_silu_mul(out, x.data_ptr(), code(x.scalar_type()), r.M, N, r.K, s.t[0].data_ptr(), same ? nullptr : (float*)s.t[1].data_ptr(), l.stream),
+          "llmq_silu_mul");
+    return s;
+}
+
 // ---- Python ----------------------------------------------------------------------------------------------------
 struct NoGil {
     PyThreadState* state = PyEval_SaveThread();
@@ -853,6 +977,63 @@ LLMQ_PY(py_fp8_block_grouped, 8)
     return wrap(std::move(y));
 LLMQ_PY_END
 
+LLMQ_PY(py_route, 9)
+    const Tensor& x = in.tensor(0);
+    const auto bias = in.optional(1);
+    LLMQ_PY_TENSORS;
+    const long long top = PyLong_AsLongLong(argv[2]), scoring = PyLong_AsLongLong(argv[3]), groups = PyLong_AsLongLong(argv[4]),
+                    top_groups = PyLong_AsLongLong(argv[5]), score = PyLong_AsLongLong(argv[6]);
+    const int renormalize = PyObject_IsTrue(argv[7]);
+    const double scale = PyFloat_AsDouble(argv[8]);
+    if (PyErr_Occurred()) return nullptr;
+    std::optional<Pair> y;
+    { NoGil g; y = route(x, bias, top, (int)scoring, groups, top_groups, (int)score, renormalize != 0, scale); }
+    if (!y) Py_RETURN_NONE;
+    Tensor t[2] = {std::move(y->first), std::move(y->second)};
+    return tuple_of(t, 2);
+LLMQ_PY_END
+
+LLMQ_PY(py_dispatch, 5)
+    const Tensor &x = in.tensor(0), &ids = in.tensor(1);
+    LLMQ_PY_TENSORS;
+    const long long experts = PyLong_AsLongLong(argv[2]), first = PyLong_AsLongLong(argv[3]), out = PyLong_AsLongLong(argv[4]);
+    if (PyErr_Occurred()) return nullptr;
+    std::optional<Sorted> y;
+    { NoGil g; y = dispatch(x, ids, experts, first, (int)out); }
+    if (!y) Py_RETURN_NONE;
+    return tuple_of(y->t, y->n);
+LLMQ_PY_END
+
+LLMQ_PY(py_combine, 4)
+    const Tensor &x = in.tensor(0), &places = in.tensor(1), &weights = in.tensor(2);
+    const auto shared = in.optional(3);
+    LLMQ_PY_TENSORS;
+    std::optional<Tensor> y;
+    { NoGil g; y = combine(x, places, weights, shared); }
+    return wrap(std::move(y));
+LLMQ_PY_END
+
+LLMQ_PY(py_w8a8_grouped, 8)
+    const Tensor &x = in.tensor(0), &a = in.tensor(1), &w = in.tensor(2), &s = in.tensor(3), &offsets = in.tensor(5);
+    const auto bias = in.optional(4), out = in.optional(7);
+    const at::ScalarType odt = in.dtype(6);
+    LLMQ_PY_TENSORS;
+    std::optional<Tensor> y;
+    { NoGil g; y = w8a8_grouped(x, a, w, s, bias, offsets, odt, out); }
+    return wrap(std::move(y));
+LLMQ_PY_END
+
+LLMQ_PY(py_silu_mul, 2)
+    const Tensor& x = in.tensor(0);
+    LLMQ_PY_TENSORS;
+    const long long out = PyLong_AsLongLong(argv[1]);
+    if (PyErr_Occurred()) return nullptr;
+    std::optional<Sorted> y;
+    { NoGil g; y = silu_mul(x, (int)out); }
+    if (!y) Py_RETURN_NONE;
+    return y->n == 1 ? THPVariable_Wrap(std::move(y->t[0])) : tuple_of(y->t, y->n);
+LLMQ_PY_END
+
 // the counters of the current stream of a tensor's device
 LLMQ_PY(py_awq_counters, 1)
     const Tensor& x = in.tensor(0);
@@ -893,6 +1074,11 @@ PyMethodDef methods[] = {LLMQ_FAST("sq_tensor", py_sq_tensor),
                          LLMQ_FAST("fp8_blockwise", py_fp8_blockwise),
                          LLMQ_FAST("fp8_block_linear", py_fp8_block_linear),
                          LLMQ_FAST("fp8_block_grouped", py_fp8_block_grouped),
+                         LLMQ_FAST("route", py_route),
+                         LLMQ_FAST("dispatch", py_dispatch),
+                         LLMQ_FAST("combine", py_combine),
+                         LLMQ_FAST("w8a8_grouped", py_w8a8_grouped),
+                         LLMQ_FAST("silu_mul", py_silu_mul),
                          LLMQ_FAST("awq_counters", py_awq_counters),
                          {"release_tickets", py_release_counters, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

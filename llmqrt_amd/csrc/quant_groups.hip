@@ -14,70 +14,7 @@
 namespace llmq {
 namespace {
 
-constexpr int kTeam = 16;        // lanes that share a group: 16 chunks of 8 elements
 constexpr int kQuantThreads = 256;
-
-// |v| of 8 fp32 values; NaN propagates (max_nonneg)
-__device__ __forceinline__ float absmax8f(const float* v) {
-    float m = fabsf(v[0]);
-#pragma unroll
-    for (int i = 1; i < 8; i++) m = max_nonneg(m, fabsf(v[i]));
-    return m;
-}
-__device__ __forceinline__ float team_max(float v) {  // over 16 lanes in a row
-    v = max_nonneg(v, lane_xor<1>(v));
-    v = max_nonneg(v, lane_xor<2>(v));
-    v = max_nonneg(v, lane_xor<4>(v));
-    return max_nonneg(v, lane_xor<8>(v));
-}
-template <int DT>
-__device__ __forceinline__ void widen8(uint4 r, float* f) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) f[2 * i] = Lo<DT>::lo_f32(w[i]), f[2 * i + 1] = Lo<DT>::hi_f32(w[i]);
-}
-template <int DT>
-__device__ __forceinline__ uint4 narrow8(const float* f) {
-    return make_uint4(Lo<DT>::pack2(f[0], f[1]), Lo<DT>::pack2(f[2], f[3]), Lo<DT>::pack2(f[4], f[5]), Lo<DT>::pack2(f[6], f[7]));
-}
-
-template <int MODE>
-__device__ __forceinline__ float scale32(float amax) { return max_nonneg(amax, QP<MODE>::floor_) / QP<MODE>::qmax; }
-
-// Codes of 8 fp32 values.  NEAR: the scale is in [2^-60, 2^60] and the values are finite, so the quotient comes from a product and one exact
-// correction (near_quotient: three instructions instead of about ten); otherwise divided.  A quotient that is NaN stays NaN in e4m3 and
-// becomes 0 in int8.
-template <int MODE, bool NEAR>
-__device__ __forceinline__ uint2 codes8(const float* v, float s, float inv_s) {
-    float f[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        float q = NEAR ? near_quotient(v[i], v[i] * inv_s, s, inv_s) : v[i] / s;
-        if (MODE == MODE_I8) {
-            q = (!NEAR && q != q) ? 0.f : rintf(q);
-            f[i] = q + 128.f;  // an integer: the conversion below has nothing to round, and saturates
-        } else {
-            const float c = __builtin_amdgcn_fmed3f(q, -448.f, 448.f);
-            f[i] = (!NEAR && q != q) ? q : c;
-        }
-    }
-    uint32_t out[2];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        if (MODE == MODE_I8) {
-            uint32_t w = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) w = __builtin_amdgcn_cvt_pk_u8_f32(f[4 * h + i], i, w);
-            out[h] = w ^ 0x80808080u;
-        } else {
-            int p = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * h], f[4 * h + 1], 0, false);
-            out[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * h + 2], f[4 * h + 3], p, true);
-        }
-    }
-    return make_uint2(out[0], out[1]);
-}
-// finite values under a scale that near_quotient takes
-__device__ __forceinline__ bool near_ok(float amax, float s) { return amax < __builtin_inff() && near_scale(s); }
 
 // ---- group quantizer -------------------------------------------------------------------------------------------------------
 // 16 lanes take a group, 16 bytes each, U groups in flight per lane; the maximum is a butterfly of lane selects.  HBM-bound: 2 bytes read, 1

@@ -1,0 +1,191 @@
+// Gated activation between two products, with an output in 16 or 8 bits.
+//
+//   y[m, k] = g / (1 + exp(-g)) * u,   g = x[m, k], u = x[m, N + k]
+//   and y rounded once to x_dtype, or quantized:  int8 s = max(max_k |y|, 1e-5) / 127,  q = rint(y / s)
+//                                                 e4m3 s = max(max |y|, 1e-12) / 448, per token or per token and group of 128 channels
+// Everything between x and the codes is fp32.  HBM-bound: 4 bytes read and 1 or 2 written per output.
+#include <algorithm>
+
+#include "llmq_common.h"
+#include "quant_math.h"
+
+namespace llmq {
+namespace {
+
+enum { OUT_SAME = LLMQ_NORM_SAME, OUT_I8 = LLMQ_NORM_I8_TOKEN, OUT_F8 = LLMQ_NORM_FP8_TOKEN, OUT_GROUP = LLMQ_NORM_FP8_GROUP };
+constexpr int kSiluThreads = 256;
+
+struct SiluArgs {
+    const uint16_t* x;
+    uint16_t* y;  // OUT_SAME
+    uint8_t* q;   // otherwise
+    float* scale;
+    int64_t ldx, M, N;
+};
+
+// exp by the base-2 instruction: |g| 2^-24 off relative to itself, far below what 16 or 8 bits keep.  g of -inf gives -inf * 0 = NaN, as the formula does.
+__device__ __forceinline__ float silu(float g) {
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896f * g));
+}
+template <int DT>
+__device__ __forceinline__ void gated8(uint4 gv, uint4 uv, float* y) {
+    float g[8], u[8];
+    widen8<DT>(gv, g), widen8<DT>(uv, u);
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = silu(g[i]) * u[i];
+}
+
+// No reduction over the whole row: 16 lanes take 128 channels of a row, U such pieces in flight per lane.
+template <int DT, bool GROUP, int U>
+__global__ __launch_bounds__(kSiluThreads) void silu_groups_kernel(SiluArgs a, uint32_t groups, uint32_t total) {
+    constexpr int TEAMS = kSiluThreads / kTeam;
+    const int l = threadIdx.x % kTeam;
+    const uint32_t g0 = blockIdx.x * (TEAMS * U) + threadIdx.x / kTeam;
+    uint4 gv[U], uv[U];
+    int64_t to[U];  // first element of the lane's chunk in the output; < 0: none
+    uint32_t row = g0 / groups, col = g0 - row * groups;
+    const uint32_t step_rows = TEAMS / groups, step_cols = TEAMS - step_rows * groups;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int64_t k = (int64_t)col * 128 + l * 8;
+        const bool in = g0 + u * TEAMS < total && k < a.N;
+        const uint16_t* xr = a.x + (int64_t)row * a.ldx + k;
+        to[u] = in ? (int64_t)row * a.N + k : -1;
+        gv[u] = in ? *reinterpret_cast<const uint4*>(xr) : make_uint4(0, 0, 0, 0);
+        uv[u] = in ? *reinterpret_cast<const uint4*>(xr + a.N) : make_uint4(0, 0, 0, 0);
+        row += step_rows, col += step_cols;
+        if (col >= groups) col -= groups, row++;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        float y[8];
+        gated8<DT>(gv[u], uv[u], y);
+        if (!GROUP) {
+            if (to[u] >= 0) *reinterpret_cast<uint4*>(a.y + to[u]) = narrow8<DT>(y);
+            continue;
+        }
+        const float amax = team_max(absmax8f(y)), s = scale32<MODE_F8>(amax), inv_s = 1.0f / s;
+        uint2 c;
+        if (__all(near_ok(amax, s))) c = codes8<MODE_F8, true>(y, s, inv_s);
+        else c = codes8<MODE_F8, false>(y, s, inv_s);
+        if (to[u] >= 0) *reinterpret_cast<uint2*>(a.q + to[u]) = c;
+        if (l == 0 && g0 + u * TEAMS < total) a.scale[g0 + u * TEAMS] = s;
+    }
+}
+
+// A scale per row.  NT threads per row, RPB rows per block (more than one: a wavefront each, and no barrier).  NC > 0: a row's outputs stay in 8 NC
+// registers per thread between the maximum and the codes; 0: rows of any length, computed twice.
+template <int DT, int MODE, int NC, int NT, int RPB>
+__global__ __launch_bounds__(NT * RPB) void silu_rows_kernel(SiluArgs a) {
+    static_assert(RPB == 1 || NT == kWave, "several rows per block are a wavefront each");
+    __shared__ float smem[NT / kWave];
+    const int tid = RPB > 1 ? threadIdx.x % kWave : threadIdx.x;
+    const int64_t row = RPB > 1 ? (int64_t)blockIdx.x * RPB + threadIdx.x / kWave : blockIdx.x;
+    if (RPB > 1 && row >= a.M) return;  // wavefront-uniform; no barrier follows
+    const int nchunk = (int)(a.N >> 3);
+    const uint4* gr = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
+    const uint4* ur = reinterpret_cast<const uint4*>(a.x + row * a.ldx + a.N);
+    uint2* qr = reinterpret_cast<uint2*>(a.q + row * a.N);
+    float y[NC > 0 ? NC : 1][8], amax = 0.f;
+    if (NC > 0) {
+        uint4 gv[NC > 0 ? NC : 1], uv[NC > 0 ? NC : 1];
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const int i = tid + c * NT;
+            gv[c] = i < nchunk ? gr[i] : make_uint4(0, 0, 0, 0);
+            uv[c] = i < nchunk ? ur[i] : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            gated8<DT>(gv[c], uv[c], y[c]);
+            amax = max_nonneg(amax, absmax8f(y[c]));
+        }
+    } else {
+        for (int i = tid; i < nchunk; i += NT) {
+            gated8<DT>(gr[i], ur[i], y[0]);
+            amax = max_nonneg(amax, absmax8f(y[0]));
+        }
+    }
+    amax = RPB > 1 ? wave_max(amax) : block_max<NT / kWave>(amax, smem);
+    const float s = scale32<MODE>(amax), inv_s = 1.0f / s;
+    if (tid == 0) a.scale[row] = s;
+    const bool fast = near_ok(amax, s);  // of the row
+    if (NC > 0) {
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const int i = tid + c * NT;
+            if (i < nchunk) qr[i] = fast ? codes8<MODE, true>(y[c], s, inv_s) : codes8<MODE, false>(y[c], s, inv_s);
+        }
+    } else {
+        for (int i = tid; i < nchunk; i += NT) {
+            gated8<DT>(gr[i], ur[i], y[0]);
+            qr[i] = fast ? codes8<MODE, true>(y[0], s, inv_s) : codes8<MODE, false>(y[0], s, inv_s);
+        }
+    }
+}
+
+template <int DT, bool GROUP>
+int launch_groups(const SiluArgs& a, hipStream_t st) {
+    constexpr int TEAMS = kSiluThreads / kTeam;
+    const uint32_t groups = (uint32_t)((a.N + 127) / 128), total = (uint32_t)(a.M * groups);
+    if (total >= 256 * TEAMS * 8)
+        hipLaunchKernelGGL((silu_groups_kernel<DT, GROUP, 2>), dim3((total + TEAMS * 2 - 1) / (TEAMS * 2)), dim3(kSiluThreads), 0, st, a, groups, total);
+    else
+        hipLaunchKernelGGL((silu_groups_kernel<DT, GROUP, 1>), dim3((total + TEAMS - 1) / TEAMS), dim3(kSiluThreads), 0, st, a, groups, total);
+    return launch_status();
+}
+
+// Threads per row and chunks per thread as for the norm with an 8-bit output (quant_groups.hip): a few rows are a chain of latencies, many are bytes.
+template <int DT, int MODE>
+int launch_rows(const SiluArgs& a, hipStream_t st) {
+    const int64_t chunks = a.N >> 3;
+#define LLMQ_SILU(NC, NT, RPB) \
+    hipLaunchKernelGGL((silu_rows_kernel<DT, MODE, NC, NT, RPB>), dim3((unsigned)((a.M + RPB - 1) / RPB)), dim3(NT * RPB), 0, st, a)
+    if (chunks <= 128 && a.M >= 256) LLMQ_SILU(2, 64, 4);
+    else if (chunks <= 256) LLMQ_SILU(1, 256, 1);
+    else if (chunks <= 512) {
+        if (a.M < 400) LLMQ_SILU(1, 512, 1);
+        else LLMQ_SILU(2, 256, 1);
+    } else if (chunks <= 1024) {
+        if (a.M < 400) LLMQ_SILU(1, 1024, 1);
+        else LLMQ_SILU(2, 512, 1);
+    } else if (chunks <= 3072) LLMQ_SILU(3, 1024, 1);
+    else LLMQ_SILU(0, 512, 1);
+#undef LLMQ_SILU
+    return launch_status();
+}
+
+template <int DT>
+int launch_silu(int out, const SiluArgs& a, hipStream_t st) {
+    switch (out) {
+        case OUT_SAME: return launch_groups<DT, false>(a, st);
+        case OUT_GROUP: return launch_groups<DT, true>(a, st);
+        case OUT_I8: return launch_rows<DT, MODE_I8>(a, st);
+        default: return launch_rows<DT, MODE_F8>(a, st);
+    }
+}
+
+}  // namespace
+}  // namespace llmq
+
+using namespace llmq;
+
+extern "C" int llmq_silu_mul(int out, const void* x, int x_dtype, int64_t M, int64_t N, int64_t ldx, void* y, float* scale, llmq_stream_t stream) {
+    if (out < OUT_SAME || out > OUT_GROUP || (x_dtype != LLMQ_BF16 && x_dtype != LLMQ_F16)) return LLMQ_ERR_DTYPE;
+    if (M < 0 || N < 0 || M > 0x7fffffffLL || N > 0x3fffffffLL || ldx < 2 * N || (N & 7) || (ldx & 7)) return LLMQ_ERR_SHAPE;
+    if (M == 0 || N == 0) return LLMQ_OK;
+    if (!x || !y || (out != OUT_SAME && !scale)) return LLMQ_ERR_NULL;
+    if (!aligned16(x) || (out == OUT_SAME ? !aligned16(y) : (reinterpret_cast<uintptr_t>(y) & 7u) != 0)) return LLMQ_ERR_ALIGN;
+    // a grid holds fewer than 2^32 threads: rows beyond that many go to further launches
+    const int64_t groups = (N + 127) / 128, per_row = out == OUT_GROUP ? groups : 1;
+    const int64_t step = out == OUT_SAME || out == OUT_GROUP ? std::max<int64_t>(1, ((int64_t)1 << 27) / groups) : (int64_t)1 << 21;
+    int rc = LLMQ_OK;
+    for (int64_t m = 0; m < M && rc == LLMQ_OK; m += step) {
+        SiluArgs a = {};
+        a.x = (const uint16_t*)x + m * ldx, a.ldx = ldx, a.M = std::min(step, M - m), a.N = N;
+        if (out == OUT_SAME) a.y = (uint16_t*)y + m * N;
+        else a.q = (uint8_t*)y + m * N, a.scale = scale + m * per_row;
+        rc = x_dtype == LLMQ_BF16 ? launch_silu<LLMQ_BF16>(out, a, (hipStream_t)stream) : launch_silu<LLMQ_F16>(out, a, (hipStream_t)stream);
+    }
+    return rc;
+}

@@ -291,6 +291,61 @@ def _f8f8_blockwise_grouped_general(XQ, WQ, bias, x_scale, w_scale, offsets, dty
     return y
 
 
+# ---- W8A8 by experts (no counterpart among the reference's ops) ------------------------------------------------
+
+def w8a8_int8_linear_per_channel_grouped(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], alpha: torch.Tensor,
+                                         beta: torch.Tensor, offsets: torch.Tensor, dtype_str: str = "bfloat16",
+                                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """w8a8_int8_linear_bbf16_obf16_per_channel by experts: rows offsets[e] .. offsets[e + 1] - 1 of ``input`` (sorted by expert) with the weights of expert e,
+    out[m, n] = dtype((acc * alpha[m]) * beta[e, n] + bias[e, n]), acc = sum_k input[m, k] * weight[e, n, k] exact.
+
+    ``input``: int8 [M, K], K a multiple of 16 below 131072; ``weight``: int8 [E, N, K] row-major; ``alpha``: one scale per row, ``beta``: [E, N]; ``bias``: [E, N]
+    in bf16, fp16 or fp32, or None; ``offsets``: int32 [E + 1] on the GPU, ascending (values outside [0, M] are taken as the nearest inside,
+    one below an earlier one as that); ``dtype_str``: "bfloat16" or "float16".  An expert may have no rows.  Nothing is read back by the host, so a captured call follows the offsets of its
+    replay.  Rows that belong to no expert are not written: they keep what ``out`` [M, N] holds, and are undefined in a new tensor.  ``out`` is written as torch's
+    in-place operations do, as f8f8_blockwise_grouped's is."""
+    y = host().w8a8_grouped(input, alpha, weight, beta, bias, offsets, _STR_TO_DTYPE.get(dtype_str), out)
+    if y is not None:
+        return y
+    if out is not None:
+        _abi.check_writable(out, "out")
+    return _w8a8_grouped_general(input, weight, bias, alpha, beta, offsets, dtype_str, out)
+
+
+@torch.no_grad()
+def _w8a8_grouped_general(input, weight, bias, alpha, beta, offsets, dtype_str, out):
+    what = "w8a8_int8_linear_per_channel_grouped"
+    out_dtype = _block_out_dtype(dtype_str, what)
+    _check(input.is_cuda, f"{what}: input must be a GPU tensor")
+    _check(input.dim() == 2 and weight.dim() == 3, f"{what}: input must be [M, K] and weight [E, N, K]")
+    (M, K), (E, N) = input.shape, weight.shape[:2]
+    dev = input.device
+    _check(input.dtype == torch.int8 and weight.dtype == torch.int8, f"{what}: input and weight must be int8")
+    _check(weight.shape[2] == K and weight.device == dev, f"{what}: weight must be [E, N, K] with the K and device of the input")
+    _check(K % 16 == 0 and K < 1 << 17, f"{what}: K must be a multiple of 16 below 131072")
+    _check(isinstance(offsets, torch.Tensor) and offsets.dtype == torch.int32 and offsets.device == dev and tuple(offsets.shape) == (E + 1,),
+           f"{what}: offsets must be int32 [E + 1] on the GPU of the input")
+    _check(isinstance(alpha, torch.Tensor) and alpha.is_floating_point() and alpha.device == dev and tuple(alpha.shape) in ((M,), (M, 1)),
+           f"{what}: alpha must hold one floating-point scale per row, on the GPU of the input")
+    _check(isinstance(beta, torch.Tensor) and beta.is_floating_point() and beta.device == dev and tuple(beta.shape) == (E, N),
+           f"{what}: beta must be [E, N] floating-point scales on the GPU of the input")
+    if bias is not None:
+        _check(bias.device == dev and tuple(bias.shape) == (E, N) and bias.dtype in (torch.bfloat16, torch.float16, torch.float32),
+               f"{what}: bias must be [E, N] in bf16, fp16 or fp32 on the GPU of the input")
+        bias = bias.detach().contiguous()
+    if out is not None:
+        _check(out.dtype == out_dtype and out.device == dev and tuple(out.shape) == (M, N) and out.is_contiguous(),
+               f"{what}: out must be a contiguous [M, N] tensor of the output dtype on the GPU of the input")
+    if M == 0 or N == 0 or E == 0:
+        return torch.empty((M, N), dtype=out_dtype, device=dev) if out is None else out
+    _check(K > 0, f"{what}: K must be positive")
+    _check(E <= 65536, f"{what}: at most 65536 experts")
+    y = host().w8a8_grouped(_rows16(input), alpha.detach().to(torch.float32).contiguous(), _rows16(weight), beta.detach().to(torch.float32).contiguous(), bias,
+                            offsets.contiguous(), out_dtype, out)
+    _check(y is not None, f"{what}: unsupported operands")
+    return y
+
+
 # ---- one-launch linears for a few tokens (no counterpart among the reference's ops: they fuse the
 # quantizer call and the GEMM op of linear_sq.py:97-138 / linear_fp8.py:199-221) ------------------------------
 
