@@ -8,8 +8,11 @@
 // Which experts are chosen has to follow from the scores, not from how they were rounded: without a bias the order of c is that of the logits, which are
 // compared as they are; with one, and where two scores of a group are added, scores are formed and compared in 64 bits.
 //
-// LPT lanes share a token, V neighbouring experts each, in registers.  A choice is the maximum of the lanes' best ones by lane selects; the lane that had it
-// notes it in LDS and looks for its next one.
+// Most tokens take the short form: 16 lanes share a token, at most V neighbouring experts of one group each, in registers, with the scores in 32 bits.  A
+// choice is a maximum over a lane's experts and over the 16 lanes (row rotations, no LDS) and the lowest expert that has it.  Its order is that of the exact
+// scores wherever neighbours in it lie further apart than both scores can be off; a token with two closer ones is done over with scores in 64 bits.  Bound by
+// the vector unit: about 90 instructions for a choice of 4 tokens from 256 experts each.
+// More than 256 experts, 16 groups or 16 choices, and tokens with a NaN, take the long form.
 #include <algorithm>
 #include <type_traits>
 
@@ -18,7 +21,7 @@
 namespace llmq {
 namespace {
 
-constexpr int kThreads = 256, kMaxTop = 64, kMaxExperts = 1024, kMaxGroups = 64;
+constexpr int kThreads = kWave, kMaxTop = 64, kMaxExperts = 1024, kMaxGroups = 64;
 
 struct RouteArgs {
     const void* logits;
@@ -77,15 +80,14 @@ __device__ __forceinline__ void wave_fence() {  // LDS written by other lanes of
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
-template <int DT, bool EXACT, int LPT, int V>
-__global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
-    constexpr int TPB = kThreads / LPT;
-    extern __shared__ uint64_t dyn[];  // with groups: keys of the block's experts, then of its groups
-    __shared__ int32_t s_id[TPB][kMaxTop];
-    __shared__ float s_x[TPB][kMaxTop];
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), team = tid / LPT, l = tid % LPT;
-    const int64_t token = (int64_t)blockIdx.x * TPB + team, t = min(token, a.tokens - 1);  // (a team without a token repeats the last one's)
-    const int e0 = l * V;
+// The long form: a wavefront takes a token, V neighbouring experts each lane; the lane that has a choice notes it in LDS and looks for its next one.
+template <int DT, bool EXACT, int V>
+__device__ __forceinline__ void route_long(const RouteArgs& a, int64_t t) {
+    constexpr int LPT = kWave;
+    extern __shared__ uint64_t dyn[];  // with groups: keys of the experts, then of the groups
+    __shared__ int32_t s_id[kMaxTop];
+    __shared__ float s_x[kMaxTop];
+    const int l = threadIdx.x, e0 = l * V;
 
     float x[V];
 #pragma unroll
@@ -129,8 +131,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
     }
 
     if (a.groups > 1) {
-        uint64_t* mine = dyn + team * a.experts;
-        uint64_t* group = dyn + TPB * a.experts + team * a.groups;
+        uint64_t *mine = dyn, *group = dyn + a.experts;
 #pragma unroll
         for (int v = 0; v < V; v++)
             if (e0 + v < a.experts) mine[e0 + v] = key[v];
@@ -157,7 +158,6 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
         }
     }
 
-    const uint64_t team_lanes = (LPT == 64 ? ~0ull : (1ull << LPT) - 1) << (lane / LPT * LPT);
     for (int j = 0; j < a.top; j++) {
         uint64_t best = key[0];
         int bv = 0;
@@ -165,15 +165,15 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
         for (int v = 1; v < V; v++)
             if (key[v] > best) best = key[v], bv = v;
         const uint64_t most = team_reduce<LPT>(best, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
-        const uint64_t have = __ballot(best == most) & team_lanes;  // the lowest of them has the lowest expert
-        if (lane == __ffsll((unsigned long long)have) - 1) {
+        const uint64_t have = __ballot(best == most);  // the lowest of them has the lowest expert
+        if (l == __ffsll((unsigned long long)have) - 1) {
             float bx = x[0];
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 if (v == bv) bx = x[v], key[v] = 0;
             }
-            s_id[team][j] = most ? e0 + bv : -1;
-            s_x[team][j] = bx;
+            s_id[j] = most ? e0 + bv : -1;
+            s_x[j] = bx;
         }
     }
     wave_fence();
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
     // Weights.  Renormalised ones are ratios of the chosen scores, formed relative to the largest so that none of them underflows.
     float top_x = -__builtin_inff();
     for (int j = 0; j < a.top; j++)
-        if (s_id[team][j] >= 0) top_x = fmaxf(top_x, s_x[team][j]);
+        if (s_id[j] >= 0) top_x = fmaxf(top_x, s_x[j]);
     auto part = [&](float v) __attribute__((always_inline)) {
         if (!a.sigmoid) return expf(v - (a.renormalize ? top_x : m));
         if (!a.renormalize || v > 0.f || top_x > 0.f) return 1.f / (1.f + expf(-v));
@@ -190,29 +190,332 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
     if (a.renormalize) {
         sum = 0.f;
         for (int j = 0; j < a.top; j++)
-            if (s_id[team][j] >= 0) sum += part(s_x[team][j]);
+            if (s_id[j] >= 0) sum += part(s_x[j]);
     } else if (a.sigmoid) {
         sum = 1.f;
     }
     for (int j = l; j < a.top; j += LPT) {
-        if (token >= a.tokens) break;
-        const int id = s_id[team][j];
-        a.ids[token * a.top + j] = id;
-        a.weights[token * a.top + j] = id < 0 ? 0.f : part(s_x[team][j]) / sum * a.scale;
+        const int id = s_id[j];
+        a.ids[t * a.top + j] = id;
+        a.weights[t * a.top + j] = id < 0 ? 0.f : part(s_x[j]) / sum * a.scale;
     }
 }
 
+// ---- the short form
+constexpr int kShortExperts = 256, kShortGroups = 16, kShortTop = 16;
+
+template <int N>
+__device__ __forceinline__ uint32_t rotated(uint32_t v) {  // the value N lanes on, among 16
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x120 + N, 0xf, 0xf, false);
+}
+template <class T, class F>  // f of the 32-bit halves of a value
+__device__ __forceinline__ T by_halves(T v, F&& f) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, f(__builtin_bit_cast(uint32_t, v)));
+    } else {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(T, (uint64_t)f((uint32_t)u) | (uint64_t)f((uint32_t)(u >> 32)) << 32);
+    }
+}
+// over the LPT lanes of a token
+template <int LPT, class T, class F>
+__device__ __forceinline__ T over_token(T v, F&& f) {
+    v = f(v, by_halves(v, [](uint32_t u) { return rotated<1>(u); })), v = f(v, by_halves(v, [](uint32_t u) { return rotated<2>(u); }));
+    v = f(v, by_halves(v, [](uint32_t u) { return rotated<4>(u); })), v = f(v, by_halves(v, [](uint32_t u) { return rotated<8>(u); }));
+    // (both halves of a swap of v with itself: one has the lane's own value, the other its partner's)
+    if constexpr (LPT >= 32)
+        v = f(by_halves(v, [](uint32_t u) { return (uint32_t)__builtin_amdgcn_permlane16_swap(u, u, false, false)[0]; }),
+              by_halves(v, [](uint32_t u) { return (uint32_t)__builtin_amdgcn_permlane16_swap(u, u, false, false)[1]; }));
+    if constexpr (LPT >= 64)
+        v = f(by_halves(v, [](uint32_t u) { return (uint32_t)__builtin_amdgcn_permlane32_swap(u, u, false, false)[0]; }),
+              by_halves(v, [](uint32_t u) { return (uint32_t)__builtin_amdgcn_permlane32_swap(u, u, false, false)[1]; }));
+    return v;
+}
+__device__ __forceinline__ uint32_t larger(uint32_t p, uint32_t q) { return max(p, q); }
+__device__ __forceinline__ float larger(float p, float q) { return fmaxf(p, q); }
+__device__ __forceinline__ double larger(double p, double q) { return __builtin_fmax(p, q); }
+__device__ __forceinline__ float smaller(float p, float q) { return fminf(p, q); }
+__device__ __forceinline__ double smaller(double p, double q) { return __builtin_fmin(p, q); }
+template <int LPT, class T>
+__device__ __forceinline__ T token_max(T v) { return over_token<LPT>(v, [](T p, T q) __attribute__((always_inline)) { return larger(p, q); }); }
+template <int LPT, class T>
+__device__ __forceinline__ T token_sum(T v) { return over_token<LPT>(v, [](T p, T q) __attribute__((always_inline)) { return p + q; }); }
+// the value of lane ^ 1, ^ 2, and of lanes that pair up where 4 or 8 neighbours agree already
+template <int CTRL, class T>
+__device__ __forceinline__ T paired(T v) { return by_halves(v, [](uint32_t u) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)u, CTRL, 0xf, 0xf, true); }); }
+
+__device__ __forceinline__ float exp_fast(float v) { return __builtin_amdgcn_exp2f(1.44269504088896f * v); }
+__device__ __forceinline__ uint32_t key32(float c) { return (uint32_t)(key_of(c) >> 32); }
+__device__ __forceinline__ float value32(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
+
+// What choices go by: the logits; scores in 32 bits, where their neighbours lie far enough apart; scores in 64 bits
+enum { BY_LOGITS, BY_SCORES_32, BY_SCORES_64 };
+
+// How the experts lie: lanes_per_group lanes have a group, per_lane experts each; vec: in whole 16-byte pieces (8-byte ones in 16 bits)
+struct Lay { int lanes_per_group, per_lane, vec; };
+
+// The LPT lanes' token t, the V experts of each lane at most.  -> whether it is done, which with scores in 64 bits it is unless it has a NaN
+template <int DT, int BY, int LPT, int V>
+__device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t t, bool wanted) {
+    using score_t = std::conditional_t<BY == BY_SCORES_64, double, float>;
+    using key_t = std::conditional_t<BY == BY_SCORES_64, double, uint32_t>;
+    constexpr score_t kNone = -(score_t)__builtin_inff();
+    constexpr key_t kNoKey = BY == BY_SCORES_64 ? (key_t)kNone : (key_t)0;
+    __shared__ float stage[kThreads / LPT][LPT * V];
+    const int l = threadIdx.x % LPT, team = threadIdx.x / LPT, lanes_per_group = lay.lanes_per_group, per_lane = lay.per_lane;
+    const uint64_t token_lanes = (LPT == 64 ? ~0ull : (1ull << (LPT & 63)) - 1) << ((threadIdx.x & (kWave - 1)) / LPT * LPT);
+    const int g = l / lanes_per_group, first = l % lanes_per_group * per_lane, e0 = g * a.group_size + first;
+    const int count = g < a.groups ? min(max(a.group_size - first, 0), per_lane) : 0;  // experts of the lane
+
+    float x[V];
+    if (lay.vec) {
+        if constexpr (DT == LLMQ_F32) {
+            const float4* p = reinterpret_cast<const float4*>((const float*)a.logits + t * a.ld + (count ? e0 : 0));
+#pragma unroll
+            for (int v = 0; v < V / 4; v++) {
+                const float4 f = p[v];
+                x[4 * v] = f.x, x[4 * v + 1] = f.y, x[4 * v + 2] = f.z, x[4 * v + 3] = f.w;
+            }
+        } else {
+            const uint2* p = reinterpret_cast<const uint2*>((const uint16_t*)a.logits + t * a.ld + (count ? e0 : 0));
+#pragma unroll
+            for (int v = 0; v < V / 4; v++) {
+                const uint2 f = p[v];
+                x[4 * v] = Lo<DT>::lo_f32(f.x), x[4 * v + 1] = Lo<DT>::hi_f32(f.x), x[4 * v + 2] = Lo<DT>::lo_f32(f.y), x[4 * v + 3] = Lo<DT>::hi_f32(f.y);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const int i = l + v * LPT;
+            if (i < a.experts) stage[team][i] = load_as_f32(a.logits, DT, t * a.ld + i);
+        }
+        wave_fence();
+#pragma unroll
+        for (int v = 0; v < V; v++) x[v] = v < count ? stage[team][e0 + v] : 0.f;
+    }
+#pragma unroll
+    for (int v = 0; v < V; v++) x[v] = v < count ? x[v] : -__builtin_inff();
+
+    float m = 0.f, sum = 1.f;
+    if (!a.sigmoid) {
+        m = x[0];
+#pragma unroll
+        for (int v = 1; v < V; v++) m = fmaxf(m, x[v]);
+        m = token_max<LPT>(m);
+    }
+    key_t key[V];
+    score_t group = kNone, size = 0, off = 0;  // score of the lane's group and what its rounding goes by; what a score can be off, but for its last rounding
+    bool sure = true;
+    if constexpr (BY != BY_LOGITS) {
+        score_t c[V];
+        if constexpr (BY == BY_SCORES_64) {
+            if (a.sigmoid) {
+#pragma unroll
+                for (int v = 0; v < V; v++) c[v] = 1.0 / (1.0 + exp(-(double)x[v]));
+            } else {
+                double all = 0.0;
+#pragma unroll
+                for (int v = 0; v < V; v++) c[v] = exp((double)x[v] - (double)m), all += c[v];
+                all = token_sum<LPT>(all), sum = (float)all;
+                const double r = 1.0 / all;
+#pragma unroll
+                for (int v = 0; v < V; v++) c[v] *= r;
+            }
+        } else if (a.sigmoid) {
+#pragma unroll
+            for (int v = 0; v < V; v++) c[v] = __builtin_amdgcn_rcpf(1.f + exp_fast(-x[v]));
+            // exp takes 2 |x| 2^-24 from its argument and 2^-23 of its own, of which s (1 - s) reaches s: less than 2^-24; the sum and the reciprocal 3 2^-24
+            off = 5 * 0x1p-24f;
+        } else {
+            sum = 0.f;
+#pragma unroll
+            for (int v = 0; v < V; v++) c[v] = exp_fast(x[v] - m), sum += c[v];
+            sum = token_sum<LPT>(sum);
+            const float r = __builtin_amdgcn_rcpf(sum);
+#pragma unroll
+            for (int v = 0; v < V; v++) c[v] *= r;
+            // in 2^-24 of the largest score, which is r: exp takes 2.5 d + 2 with d = m - x, of which less than 3 remain behind exp(-d); the sum's share of that
+            // is at most 2.5 ln 256 + 2 < 16, which all scores have in common but the bias does not; V + 4 additions, the reciprocal 2 and the product 1
+            off = (V + 32) * 0x1p-24f * r;
+        }
+        score_t best = kNone, second = kNone;
+        bool number = true;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const float b = a.bias && v < count ? a.bias[e0 + v] : 0.f;
+            c[v] = x[v] == -__builtin_inff() ? kNone : c[v] + (score_t)b;
+            number &= c[v] == c[v];
+            if constexpr (BY == BY_SCORES_64) key[v] = c[v];
+            else key[v] = c[v] == kNone ? 0 : key32(c[v]);
+            second = larger(second, smaller(best, c[v]));
+            best = larger(best, c[v]);
+        }
+        sure = (__ballot(!number) & token_lanes) == 0;  // (a NaN: the long form knows its place)
+        if (a.groups > 1) {
+            auto merge = [&](score_t b2, score_t s2) __attribute__((always_inline)) {
+                second = larger(smaller(best, b2), larger(second, s2));
+                best = larger(best, b2);
+            };
+            if (lanes_per_group > 1) merge(paired<0xB1>(best), paired<0xB1>(second));   // quad_perm [1,0,3,2]
+            if (lanes_per_group > 2) merge(paired<0x4E>(best), paired<0x4E>(second));   // quad_perm [2,3,0,1]
+            if (lanes_per_group > 4) merge(paired<0x141>(best), paired<0x141>(second));  // row_half_mirror
+            if (LPT > 16 && lanes_per_group > 8) merge(paired<0x140>(best), paired<0x140>(second));  // row_mirror
+            if (LPT > 32 && lanes_per_group > 16) {
+                const auto other = [&](score_t v) __attribute__((always_inline)) {  // of the 16 lanes before or behind
+                    return by_halves(v, [](uint32_t u) __attribute__((always_inline)) {
+                        const auto both = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+                        return (uint32_t)(threadIdx.x & 16 ? both[0] : both[1]);
+                    });
+                };
+                merge(other(best), other(second));
+            }
+            const bool two = a.top2 && second != kNone;
+            group = two ? best + second : best;
+            if constexpr (BY == BY_SCORES_32) size = group == kNone ? 0.f : fabsf(best) + (two ? fabsf(second) : 0.f);
+        }
+    } else {
+        score_t best = kNone;
+        uint32_t top = 0;
+#pragma unroll
+        for (int v = 0; v < V; v++) key[v] = x[v] == -__builtin_inff() ? 0 : key32(x[v]), best = fmaxf(best, x[v]), top = max(top, key[v]);
+        sure = token_max<LPT>(top) != ~0u;  // a NaN's key
+        if (!a.sigmoid && !a.renormalize) {
+            sum = 0.f;
+#pragma unroll
+            for (int v = 0; v < V; v++) sum += x[v] == -__builtin_inff() ? 0.f : expf(x[v] - m);
+            sum = token_sum<LPT>(sum);
+        }
+        if (a.groups > 1) {
+            if (lanes_per_group > 1) best = fmaxf(best, paired<0xB1>(best));
+            if (lanes_per_group > 2) best = fmaxf(best, paired<0x4E>(best));
+            if (lanes_per_group > 4) best = fmaxf(best, paired<0x141>(best));
+            if (LPT > 16 && lanes_per_group > 8) best = fmaxf(best, paired<0x140>(best));
+            if (LPT > 32 && lanes_per_group > 16) {
+                const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(best), __float_as_uint(best), false, false);
+                best = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+            }
+            group = best;
+        }
+    }
+    auto apart = [&](float p, float q, float s) __attribute__((always_inline)) { return p - q > 4 * off + 0x1p-22f * s; };  // (for sums of two as well)
+    if (a.groups > 1) {
+        score_t left = group, least = 0;
+        // the last of as many different scores as groups are asked for, or of fewer where groups are level
+        int room = a.top_groups * lanes_per_group;
+        bool kept = false;
+        for (int i = 0; i < a.top_groups; i++) {
+            least = token_max<LPT>(left);
+            const uint64_t level = __ballot(left == least) & token_lanes, below = ((uint64_t)1 << (threadIdx.x & (kWave - 1))) - 1;
+            if (BY == BY_SCORES_32 && least > kNone && (int)__popcll(level) != lanes_per_group) sure = false;
+            kept |= left == least && (int)__popcll(level & below) < room;  // of level ones, the lowest
+            room -= (int)__popcll(level);
+            left = left == least ? kNone : left;
+        }
+        if constexpr (BY == BY_SCORES_32) {
+            const float next = token_max<LPT>(left);
+            size = token_max<LPT>(size);
+            if (least > kNone && next > kNone && !apart(least, next, 2 * size)) sure = false;
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++) key[v] = kept ? key[v] : kNoKey;
+    }
+
+    // ---- the choices; lane j keeps choice j
+    int id = -1;
+    float before = __builtin_inff();
+    for (int j = 0; j < a.top + (BY == BY_SCORES_32 ? 1 : 0); j++) {
+        key_t best = key[0];
+#pragma unroll
+        for (int v = 1; v < V; v++) best = larger(best, key[v]);
+        best = token_max<LPT>(best);
+        if constexpr (BY == BY_SCORES_32) {
+            const float c = value32(best);
+            if (j > 0 && best != 0 && !apart(before, c, fabsf(before) + fabsf(c))) sure = false;
+            before = c;
+            if (j == a.top) break;
+        }
+        int at = V;  // the lowest of the lane's experts that has it
+#pragma unroll
+        for (int v = V - 1; v >= 0; v--) at = key[v] == best ? v : at;
+        const uint32_t lowest = token_max<LPT>(at < V ? 0xffffu - (uint32_t)(e0 + at) : 0u);
+        const int chosen = 0xffff - (int)lowest;
+        at = chosen - e0;
+#pragma unroll
+        for (int v = 0; v < V; v++) key[v] = v == at && v < count ? kNoKey : key[v];
+        if (l == j) id = best != kNoKey ? chosen : -1;
+    }
+    if (!__any(sure && wanted)) return false;
+
+    // ---- weights, as in the long form
+    const float cx = id >= 0 ? load_as_f32(a.logits, DT, t * a.ld + id) : -__builtin_inff();
+    const float top_x = token_max<LPT>(cx);
+    float w = 0.f;
+    if (id >= 0) {
+        if (!a.sigmoid) w = expf(cx - (a.renormalize ? top_x : m));
+        else if (!a.renormalize || cx > 0.f || top_x > 0.f) w = 1.f / (1.f + expf(-cx));
+        else w = expf(cx - top_x) / (1.f + expf(cx));
+    }
+    if (a.renormalize) sum = token_sum<LPT>(w);
+    else if (a.sigmoid) sum = 1.f;
+    if (sure && wanted && l < a.top) {
+        a.ids[t * a.top + l] = id;
+        a.weights[t * a.top + l] = id < 0 ? 0.f : w / sum * a.scale;
+    }
+    return sure;
+}
+
+// Tokens that are not done at first are taken one after the other by the whole wavefront: there is one of them among thousands, and everything waits for it.  (A
+// token's form depends on its own scores alone.)
+template <int DT, bool EXACT, int LPT, int V>
+__global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a, Lay lay, Lay alone) {
+    const int64_t t0 = (int64_t)blockIdx.x * (kThreads / LPT), t = t0 + threadIdx.x / LPT;
+    const bool mine = t < a.tokens;  // (lanes without a token repeat the last one's work)
+    const bool done = route_short<DT, EXACT ? BY_SCORES_32 : BY_LOGITS, LPT, V>(a, lay, mine ? t : a.tokens - 1, mine);
+    uint64_t left = __ballot(mine && !done);
+    while (left) {
+        const int lane = __ffsll((unsigned long long)left) - 1;
+        const int64_t one = t0 + lane / LPT;
+        left &= LPT == 64 ? 0 : ~(((1ull << (LPT & 63)) - 1) << (lane / LPT * LPT));
+        if (EXACT && route_short<DT, BY_SCORES_64, kWave, kShortExperts / kWave>(a, alone, one, true)) continue;
+        route_long<DT, EXACT, kShortExperts / kWave>(a, one);
+    }
+}
+template <int DT, bool EXACT>
+__global__ __launch_bounds__(kThreads) void route_many_kernel(RouteArgs a) { route_long<DT, EXACT, 16>(a, blockIdx.x); }
+
+// -> whether LPT lanes for a token and V experts for a lane take these sizes
+template <int DT, int LPT, int V>
+bool lay_out(const RouteArgs& a, Lay& lay) {
+    int lanes = LPT;  // of a group
+    while (lanes > 1 && lanes * a.groups > LPT) lanes /= 2;
+    lay.lanes_per_group = lanes, lay.per_lane = (a.group_size + lanes - 1) / lanes;
+    lay.vec = a.group_size == lanes * V && a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.logits) % (DT == LLMQ_F32 ? 16 : 8) == 0;
+    return lanes * a.groups <= LPT && lay.per_lane <= V;
+}
+template <int DT, bool EXACT, int LPT, int V>
+bool try_short(const RouteArgs& a, hipStream_t st) {
+    Lay lay, alone;
+    if (!lay_out<DT, LPT, V>(a, lay) || !lay_out<DT, kWave, kShortExperts / kWave>(a, alone)) return false;
+    constexpr int kTokens = kThreads / LPT;
+    hipLaunchKernelGGL((route_kernel<DT, EXACT, LPT, V>), dim3((unsigned)((a.tokens + kTokens - 1) / kTokens)), dim3(kThreads),
+                       a.groups > 1 ? (a.experts + a.groups) * 8 : 0, st, a, lay, alone);
+    return true;
+}
+
+// A few tokens are a chain of latencies, which fewer experts for a lane shorten; many are instructions, of which more experts for a lane need fewer.
+// us without / with a bias, 16, 32, 64 lanes for a token: 16 tokens of 256 experts 5.6 4.5 4.0 / 7.9 6.0 4.9, 1024 of them 5.8 4.8 4.4 / 8.2 6.4 5.3, 4096 6.2
+// 5.7 7.1, 8192 7.1 8.1 11.3; 16 of 128 4.2 3.8 4.3 / 5.8 4.8 5.0, 8192 5.5 6.6 11.6; 16 of 64 3.5 4.0 4.2 / 4.5 4.9 4.9, 8192 4.4 6.9 11.5.
 template <int DT, bool EXACT>
 int launch_route(const RouteArgs& a, hipStream_t st) {
-    const int64_t per_team = a.groups > 1 ? (int64_t)(a.experts + a.groups) * 8 : 0;
-#define LLMQ_ROUTE(LPT, V)                                                                                                          \
-    hipLaunchKernelGGL((route_kernel<DT, EXACT, LPT, V>), dim3((unsigned)((a.tokens + kThreads / LPT - 1) / (kThreads / LPT))), dim3(kThreads), \
-                       (unsigned)(per_team * (kThreads / LPT)), st, a)
-    if (a.experts <= 64) LLMQ_ROUTE(16, 4);
-    else if (a.experts <= 128) LLMQ_ROUTE(16, 8);
-    else if (a.experts <= 256) LLMQ_ROUTE(32, 8);
-    else LLMQ_ROUTE(64, 16);
-#undef LLMQ_ROUTE
+    bool done = false;
+    if (a.groups <= kShortGroups && a.top <= kShortTop && a.experts <= kShortExperts) {
+        done = try_short<DT, EXACT, 16, 4>(a, st);
+        if (!done && a.tokens <= 3000) done = try_short<DT, EXACT, 32, 4>(a, st) || try_short<DT, EXACT, 64, 4>(a, st);
+        if (!done) done = try_short<DT, EXACT, 16, 8>(a, st) || try_short<DT, EXACT, 16, 16>(a, st) || try_short<DT, EXACT, 64, 4>(a, st);
+    }
+    if (!done)
+        hipLaunchKernelGGL((route_many_kernel<DT, EXACT>), dim3((unsigned)a.tokens), dim3(kThreads), a.groups > 1 ? (a.experts + a.groups) * 8 : 0, st, a);
     return launch_status();
 }
 

@@ -149,7 +149,7 @@ int launch_rows(const SiluArgs& a, hipStream_t st) {
     } else if (chunks <= 1024) {
         if (a.M < 400) LLMQ_SILU(1, 1024, 1);
         else LLMQ_SILU(2, 512, 1);
-    } else if (chunks <= 3072) LLMQ_SILU(3, 1024, 1);
+    } else if (chunks <= 3 * 1024) LLMQ_SILU(3, 1024, 1);
     else LLMQ_SILU(0, 512, 1);
 #undef LLMQ_SILU
     return launch_status();
