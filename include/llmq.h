@@ -471,7 +471,8 @@ int llmq_combine_experts(const void* y, int dtype, int64_t rows, int64_t N, int6
 int llmq_gemm_w8a8_grouped(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, const float* w_scale, const int32_t* offsets,
                            int64_t experts, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N,
                            int64_t K, llmq_stream_t stream);
-/* Tuning / test hook: tile configuration 4 .. 10 of later calls (numbered as llmq_gemm_force_plan's), -1: the built-in choice.  Per host thread. */
+/* Tuning / test hook: configuration of later calls, 4-10: tiles (numbered as llmq_gemm_force_plan's), 11-17: the row-streaming kernel where it takes as many
+ * experts, -1: the built-in choice.  Per host thread. */
 int llmq_gemm_w8a8_grouped_force_plan(int cfg);
 
 /* y[m, n] = g / (1 + exp(-g)) * u with g = x[m, n], u = x[m, N + n], in fp32; out as llmq_add_rmsnorm's:

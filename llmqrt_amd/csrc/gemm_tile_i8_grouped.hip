@@ -5,6 +5,7 @@
 // The host does not know the experts' rows, so the grid is what any distribution can need (each expert may end with a tile that is not full) and a block
 // finds its tile from the offsets.
 #include "expert_tiles.h"
+#include "gemm_grouped.h"
 #include "gemm_tile_impl.h"
 
 namespace llmq {
@@ -18,15 +19,6 @@ struct ManyMatrices {
     __device__ __forceinline__ bool tile(int M, int tiles_n, int& expert, int& row0, int& row_end, int& tn) const {
         return expert_tile<BM>(offsets, experts, M, tiles_n, expert, row0, row_end, tn);
     }
-};
-
-struct GroupedCall {
-    const uint8_t *A, *B;
-    int64_t lda, ldo;
-    int M, N, K;
-    Epilogue ep;
-    void* out;
-    ManyMatrices ex;
 };
 
 template <class C>
@@ -43,10 +35,10 @@ int launch_grouped(const GroupedCall& g, hipStream_t st) {
             if (dev >= 0 && dev < 64) raised[kfull][dev] = true;  // benign if two threads race here: both set the same value
         }
     }
-    const int64_t tiles_n = cdiv(g.N, C::BN), tiles_m = g.M / C::BM + std::min<int64_t>(g.ex.experts, g.M);
+    const int64_t tiles_n = cdiv(g.N, C::BN), tiles_m = g.M / C::BM + std::min(g.experts, g.M);
     if (tiles_m * tiles_n * C::NT > 0xffffffffLL) return LLMQ_ERR_SHAPE;  // threads of a grid
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * tiles_n)), dim3(C::NT), C::LDS_BYTES, st, g.A, g.lda, g.B, (int64_t)g.K, g.M, g.N, g.K, g.K, g.ep,
-                       g.out, g.ldo, (void*)nullptr, (void*)nullptr, g.ex);
+                       g.out, g.ldo, (void*)nullptr, (void*)nullptr, ManyMatrices{g.offsets, g.experts});
     return launch_status();
 }
 
@@ -79,9 +71,11 @@ extern "C" int llmq_gemm_w8a8_grouped(const int8_t* A, int64_t lda, const float*
     g.A = (const uint8_t*)A, g.B = (const uint8_t*)B, g.lda = lda, g.ldo = ldo, g.M = (int)M, g.N = (int)N, g.K = (int)K, g.out = out;
     g.ep.a_scale = a_scale, g.ep.w_scale = w_scale, g.ep.bias = bias, g.ep.alpha = 1.f, g.ep.beta = 1.f;
     g.ep.bias_dtype = bias_dtype, g.ep.out_dtype = out_dtype;
-    g.ex.offsets = offsets, g.ex.experts = (int)experts;
+    g.offsets = offsets, g.experts = (int)experts;
     const hipStream_t st = (hipStream_t)stream;
-    switch (forced >= 0 ? forced : plan(M, experts)) {
+    const int cfg = forced >= 0 && (forced < kNumShapes || experts <= kGroupedRowsExperts) ? forced : plan(M, experts);
+    if (cfg >= kNumShapes) return launch_grouped_rows(cfg - kNumShapes, g, st);
+    switch (cfg) {
         case 4: return launch_grouped<GemmCfg<64, 128, 128, 2, 2, false, 0, 2, true>>(g, st);
         case 5: return launch_grouped<GemmCfg<32, 128, 128, 1, 4, false, 0, 2, true>>(g, st);
         case 6: return launch_grouped<GemmCfg<256, 256, 128, 2, 4, false, 0, 1, true>>(g, st);
@@ -94,7 +88,7 @@ extern "C" int llmq_gemm_w8a8_grouped(const int8_t* A, int64_t lda, const float*
 }
 
 extern "C" int llmq_gemm_w8a8_grouped_force_plan(int cfg) {
-    if (cfg >= 0 && (cfg < 4 || cfg > 10)) return LLMQ_ERR_SHAPE;
+    if (cfg >= 0 && (cfg < 4 || cfg >= kNumShapes + kNumGroupedRows)) return LLMQ_ERR_SHAPE;
     forced = cfg < 0 ? -1 : cfg;
     return LLMQ_OK;
 }
