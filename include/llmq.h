@@ -471,7 +471,7 @@ int llmq_combine_experts(const void* y, int dtype, int64_t rows, int64_t N, int6
 int llmq_gemm_w8a8_grouped(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, const float* w_scale, const int32_t* offsets,
                            int64_t experts, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N,
                            int64_t K, llmq_stream_t stream);
-/* Tuning / test hook: configuration of later calls, 4-10: tiles (numbered as llmq_gemm_force_plan's), 11-17: the row-streaming kernel where it takes as many
+/* Tuning / test hook: configuration of later calls, 4-10: tiles (numbered as llmq_gemm_force_plan's), 11-12: the row-streaming kernel where it takes as many
  * experts, -1: the built-in choice.  Per host thread. */
 int llmq_gemm_w8a8_grouped_force_plan(int cfg);
 

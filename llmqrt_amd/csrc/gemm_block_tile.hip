@@ -45,20 +45,6 @@ struct TileCfg {
 // LDS place of 16-byte chunk c of row r: 16 rows of one chunk fall on 16 places
 __device__ __forceinline__ int chunk_at(int r, int c) { return (r * 8 + (c ^ ((r >> 1) & 7))) * 16; }
 
-// the first `left` of eight 16-bit outputs, to any even address
-__device__ __forceinline__ void store8(uint16_t* to, uint4 v, int left) {
-    typedef uint32_t u4v __attribute__((ext_vector_type(4)));
-    typedef u4v u4any __attribute__((aligned(2)));
-    if (left >= 8) {
-        __builtin_nontemporal_store(u4v{v.x, v.y, v.z, v.w}, reinterpret_cast<u4any*>(to));
-    } else {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 7; e++)
-            if (e < left) to[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
-    }
-}
-
 // sum over lanes 0 .. lane, in registers (us, by lane shuffles through LDS / so: 256 rows of 64 experts 45.5 / 45.0, 700 of 90 8.2 / 7.5)
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int plus_lanes(int v) {  // of the rows of 16 lanes in ROWS; where there is none, plus zero
@@ -422,7 +408,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
         for (int k = 0; k < C::WTM / RPI; k++) {
             const int r = k * RPI + lane / CH;
             const uint4 v = *reinterpret_cast<const uint4*>(mine + (r * CH + (c ^ (r % CH))) * 16);
-            if (wm0 + r < row_end) store8(reinterpret_cast<uint16_t*>(g.out) + (int64_t)(wm0 + r) * g.ldo + n, v, g.N - n);
+            if (wm0 + r < row_end) store_any(reinterpret_cast<uint16_t*>(g.out) + (int64_t)(wm0 + r) * g.ldo + n, v, g.N - n);
         }
     }
 }
@@ -455,7 +441,7 @@ __global__ __launch_bounds__(256) void block_reduce_kernel(BlockArgs g, int spli
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) w[e] = bf16 ? Lo<LLMQ_BF16>::pack2(v[2 * e], v[2 * e + 1]) : Lo<LLMQ_F16>::pack2(v[2 * e], v[2 * e + 1]);
-    store8(reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n, make_uint4(w[0], w[1], w[2], w[3]), g.N - n);
+    store_any(reinterpret_cast<uint16_t*>(g.out) + (int64_t)m * g.ldo + n, make_uint4(w[0], w[1], w[2], w[3]), g.N - n);
 }
 
 template <class C, bool GROUPED, bool SPLIT, bool TAIL>

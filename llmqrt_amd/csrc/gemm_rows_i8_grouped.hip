@@ -231,7 +231,7 @@ __global__ __launch_bounds__(C::NT) void grouped_rows_kernel(GroupedCall g) {
     }
 }
 
-template <class C>
+template <class C, int PER_CU>
 int launch_rows(const GroupedCall& g, hipStream_t st) {
     auto kernel = grouped_rows_kernel<C>;
     if (C::LDS_BYTES > 64 * 1024) {
@@ -246,7 +246,8 @@ int launch_rows(const GroupedCall& g, hipStream_t st) {
     }
     const int64_t slabs = g.M / (16 * C::MT) + std::min(g.experts, g.M), items = slabs * cdiv(g.N, 16 * C::T);
     if (items > 0x7fffffffLL || g.experts > kGroupedRowsExperts) return LLMQ_ERR_SHAPE;
-    const int64_t slots = 256 * (160 * 1024 / C::LDS_BYTES), blocks = (std::min(items, slots) + kExpertXcd - 1) / kExpertXcd * kExpertXcd;
+    static_assert(PER_CU == 160 * 1024 / C::LDS_BYTES, "resident blocks");
+    const int64_t slots = 256 * PER_CU, blocks = (std::min(items, slots) + kExpertXcd - 1) / kExpertXcd * kExpertXcd;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(C::NT), C::LDS_BYTES, st, g);
     return launch_status();
 }
@@ -255,8 +256,8 @@ int launch_rows(const GroupedCall& g, hipStream_t st) {
 
 int launch_grouped_rows(int variant, const GroupedCall& g, hipStream_t st) {
     switch (variant) {
-#define LLMQ_GROUPED_ROWS_CASE(I, T, MT, NS) \
-    case I: return launch_rows<GRowsCfg<T, MT, NS>>(g, st);
+#define LLMQ_GROUPED_ROWS_CASE(I, T, MT, NS, CU) \
+    case I: return launch_rows<GRowsCfg<T, MT, NS>, CU>(g, st);
         LLMQ_GROUPED_ROWS(LLMQ_GROUPED_ROWS_CASE)
 #undef LLMQ_GROUPED_ROWS_CASE
     }

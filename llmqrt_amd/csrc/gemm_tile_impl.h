@@ -331,6 +331,10 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
         // through registers / only its tail, weights out of HBM: int8 1000 x 4608 x 3600 45.0 / 29.3, 4096 x 18944 x 3600 354 / 295, fp8
         // 4096 x 3584 x 3600 72.0 / 63.1, fp16 1000 x 4608 x 3592 77.4 / 59.8; the tiles differ too)
         const int kfull = KFULL ? ktiles : (k_end - k_begin) / C::BK;
+        // By experts the tail comes through the ring as a last tile: its missing chunks are read as the row's first ones of the tile, and zeros take their
+        // place in the weights' operand
+        constexpr bool TAIL = GROUPED && !KFULL;
+        const int kall = TAIL ? ktiles : kfull, left = k_end - k_begin - kfull * C::BK;
         constexpr int NS = C::STAGES, LPT = C::A_LOADS + C::B_LOADS;  // loads per thread and tile
         constexpr int SLOTS = C::TM * C::TN;                          // MFMAs per sub-step
         constexpr int PER = (LPT + C::KSUB * SLOTS - 1) / (C::KSUB * SLOTS);  // loads requested behind one MFMA
@@ -361,6 +365,12 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
         };
         static_assert(C::A_LOADS * C::NT * 16 == C::BM * C::CPR * 16, "the B pieces follow the A pieces in a stage");
         auto next_kt = [&]() __attribute__((always_inline)) { ld_kt = ld_kt + 1 == kfull ? 0 : ld_kt + 1; };
+        auto last_kt = [&]() __attribute__((always_inline)) {  // the last tile of all is requested next
+            ld_kt = kfull;
+            const uint32_t back = (ld_c ^ swz) * 16 >= left ? (uint32_t)((ld_c ^ swz) * 16) : 0u;
+#pragma unroll
+            for (int i = 0; i < LPT; i++) off[i] -= back;
+        };
         // the tile behind the one being computed has landed when at most `younger` later tiles are still in flight
         auto wait_next_tile = [](int younger) __attribute__((always_inline)) {
             static_assert((NS - 2) * LPT < 64, "vmcnt is a 6-bit counter");
@@ -375,10 +385,18 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
         // tiles not requested, weights out of HBM, int8 1000 x 4608 x 3584 32.1 / 30.0, 2048 x 4608 x 3584 50.8 / 44.1, 8192 x
         // 37888 x 3584 996 / 975, fp8 512 x 37888 x 3584 93.0 / 88.7, 4096 x 3584 x 18944 249 / 226, fp16 777 x 3584 x 18944 140 / 132.
         // (Level or slower: two requests behind an MFMA, s_setprio around the MFMAs, all fragment reads first.)
-        auto sub_step = [&](auto work_c, int rd, int ks_rd, auto par_c, auto d0_c, auto load_c, int ld_stage) __attribute__((always_inline)) {
+        // mask: 1 + this sub-step of a ragged tile
+        auto sub_step = [&](auto work_c, auto mask_c, int rd, int ks_rd, auto par_c, auto d0_c, auto load_c, int ld_stage) __attribute__((always_inline)) {
             constexpr int par = decltype(par_c)::value, D0 = decltype(d0_c)::value;
             constexpr bool LOAD = decltype(load_c)::value && D0 < LPT;
             constexpr bool WORK = decltype(work_c)::value;
+            if constexpr (WORK && decltype(mask_c)::value > 0) {
+                const int keep = ((decltype(mask_c)::value - 1) * 2 + khalf) * 16 < left ? -1 : 0;
+#pragma unroll
+                for (int j = 0; j < C::TN; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) fb[par][j][e] &= keep;
+            }
             unrolled<0, SLOTS>([&](auto m_c) __attribute__((always_inline)) {
                 constexpr int m = decltype(m_c)::value, FR = C::TM + C::TN, RPS = (FR + SLOTS - 1) / SLOTS;
                 if constexpr (WORK) unrolled<(m * RPS < FR ? m * RPS : FR), ((m + 1) * RPS < FR ? (m + 1) * RPS : FR)>([&](auto r_c) __attribute__((always_inline)) {
@@ -398,43 +416,57 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
         constexpr bool WORK = decltype(work_c)::value;
         unrolled<0, NS - 1>([&](auto t_c) __attribute__((always_inline)) {
             constexpr int t = decltype(t_c)::value;
-            if (t < kfull) {
+            if (t < kall) {
+                if (TAIL && t == kall - 1) last_kt();
                 unrolled<0, LPT>([&](auto d) __attribute__((always_inline)) { issue(t, d); });
                 next_kt();
             }
         });
-        wait_next_tile(min(kfull, NS - 1) - 1);
+        wait_next_tile(min(kall, NS - 1) - 1);
         lds_barrier();
         if constexpr (WORK) read_frags(0, 0, fa[0], fb[0]);
         // the stage NS - 1 is free from the start: the part of its tile that the loop requests behind a barrier comes first
-        if (NS - 1 < kfull)
+        if (NS - 1 < kall) {
+            if (TAIL && NS == kall) last_kt();
             unrolled<0, (STEP < LPT ? STEP : LPT)>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
+        }
         int stage = 0, kt = 0;
-        // rest: the part of tile kt + NS - 1 that the last iteration did not request; first: tile kt + NS exists
-        auto k_tile = [&](auto rest_c, auto first_c) __attribute__((always_inline)) {
+        // rest: the part of tile kt + NS - 1 that the last iteration did not request; first: tile kt + NS exists; last: it is the last one; mask: tile kt is
+        // ragged
+        auto k_tile = [&](auto rest_c, auto first_c, auto last_c, auto mask_c) __attribute__((always_inline)) {
             const int prev = stage == 0 ? NS - 1 : stage - 1, next = stage == NS - 1 ? 0 : stage + 1;
+            constexpr int MASK = decltype(mask_c)::value;
             unrolled<0, C::KSUB - 1>([&](auto ks_c) __attribute__((always_inline)) {
                 constexpr int ks = decltype(ks_c)::value;
-                sub_step(work_c, stage, ks + 1, std::integral_constant<int, ks & 1>{}, std::integral_constant<int, (ks + 1) * STEP>{}, rest_c, prev);
+                sub_step(work_c, std::integral_constant<int, MASK ? 1 + ks : 0>{}, stage, ks + 1, std::integral_constant<int, ks & 1>{},
+                         std::integral_constant<int, (ks + 1) * STEP>{}, rest_c, prev);
             });
             if constexpr (decltype(rest_c)::value) {
                 next_kt();
+                if constexpr (decltype(last_c)::value) last_kt();
                 wait_next_tile(NS - 2);
             } else {
-                wait_next_tile(kfull - 2 - kt);  // tile kt+1 has landed
+                wait_next_tile(kall - 2 - kt);  // tile kt+1 has landed
             }
             lds_barrier();
             // every wavefront has read the whole of stage kt: it takes tile kt + NS
-            sub_step(work_c, next, 0, std::integral_constant<int, (C::KSUB - 1) & 1>{}, std::integral_constant<int, 0>{}, first_c, stage);
+            sub_step(work_c, std::integral_constant<int, MASK ? C::KSUB : 0>{}, next, 0, std::integral_constant<int, (C::KSUB - 1) & 1>{},
+                     std::integral_constant<int, 0>{}, first_c, stage);
             stage = next;
             kt++;
         };
+        const std::true_type yes;
+        const std::false_type no;
 #pragma unroll 1
-        while (kt < kfull - NS) k_tile(std::true_type{}, std::true_type{});
-        if (kt == kfull - NS) k_tile(std::true_type{}, std::false_type{});
+        while (kt < kall - NS - (TAIL ? 1 : 0)) k_tile(yes, yes, no, no);
+        if constexpr (TAIL) {
+            if (kt < kall - NS) k_tile(yes, yes, yes, no);
+        }
+        if (kt == kall - NS) k_tile(yes, no, no, no);
         // Past the last request nothing is fetched: a block that ends waits for no load that nobody reads.
 #pragma unroll 1
-        while (kt < kfull) k_tile(std::false_type{}, std::false_type{});
+        while (kt < kall - (TAIL ? 1 : 0)) k_tile(no, no, no, no);
+        if constexpr (TAIL) k_tile(no, no, no, yes);
         };
         bool idle = false;  // wavefront-uniform
         if constexpr (GROUPED) idle = m0 + __builtin_amdgcn_readfirstlane(wm) * C::WTM >= M || n0 + __builtin_amdgcn_readfirstlane(wn) * C::WTN >= N;
@@ -442,17 +474,15 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
         else all_tiles(std::true_type{});
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing may still be landing in LDS when it is reused or released
         lds_barrier();
-        if constexpr (!KFULL) {
+        if constexpr (!KFULL && !TAIL) {
             if (kfull < ktiles) {  // block-uniform
                 load_tile(kfull, ra[0], rb[0]);
                 store_tile(0, kfull, ra[0], rb[0]);
                 lds_barrier();
-                if (!idle) {
 #pragma unroll
-                    for (int ks = 0; ks < C::KSUB; ks++) {
-                        read_frags(0, ks, fa[0], fb[0]);
-                        mfma_step(fa[0], fb[0]);
-                    }
+                for (int ks = 0; ks < C::KSUB; ks++) {
+                    read_frags(0, ks, fa[0], fb[0]);
+                    mfma_step(fa[0], fb[0]);
                 }
                 lds_barrier();
             }
@@ -500,10 +530,21 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
 
     // Fast path (block-uniform): interior tile, fused epilogue, vector stores.  No per-element dtype
     // switches or bounds checks: ~5 VALU operations per output instead of several times that.
-    // (By experts: rows past the expert's last are computed from its last and not stored.)
-    if (!split && !acc_dump && !ep.out_scale && out_vec && (GROUPED || m0 + C::BM <= M) && n0 + C::BN <= N &&
-        (reinterpret_cast<uintptr_t>(ep.w_scale) & 15u) == 0) {
+    // By experts every tile takes it: rows past the expert's last and channels past N are computed from the last ones and not stored, and stores are as wide at any
+    // even address.
+    if (GROUPED || (!split && !acc_dump && !ep.out_scale && out_vec && m0 + C::BM <= M && n0 + C::BN <= N &&
+                    (reinterpret_cast<uintptr_t>(ep.w_scale) & 15u) == 0)) {
         auto row_in = [&](int m) __attribute__((always_inline)) { return GROUPED ? min(m, M - 1) : m; };
+        const bool scales_in_fours = !GROUPED || ((reinterpret_cast<uintptr_t>(ep.w_scale) & 15u) == 0 && n0 + C::BN <= N);  // block-uniform
+        auto scales4 = [&](int n) __attribute__((always_inline)) {
+            if (scales_in_fours) return *reinterpret_cast<const float4*>(ep.w_scale + n);
+            return make_float4(ep.w_scale[min(n, N - 1)], ep.w_scale[min(n + 1, N - 1)], ep.w_scale[min(n + 2, N - 1)], ep.w_scale[min(n + 3, N - 1)]);
+        };
+        auto bias_at = [&](int n) __attribute__((always_inline)) { return ep.beta * load_as_f32(ep.bias, ep.bias_dtype, GROUPED ? min(n, N - 1) : n); };
+        auto store_chunk = [&](uint16_t* to, int m, int n, uint4 v) __attribute__((always_inline)) {  // 8 channels
+            if constexpr (!GROUPED) store_streaming(to, v);
+            else if (m < M) store_any(to, v, N - n);
+        };
         auto fast = [&](auto out_dt_c, auto plain_c) {
             constexpr int ODT = decltype(out_dt_c)::value;
             constexpr bool PLAIN = decltype(plain_c)::value;  // no bias term and alpha = 1: the scaled accumulator is the output
@@ -523,14 +564,13 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
                     for (int g = 0; g < 4; g++) {
                         const int n = n0 + wn * C::WTN + j * 32 + 8 * g + 4 * khalf;
                         if (ep.w_scale) {
-                            const float4 v = *reinterpret_cast<const float4*>(ep.w_scale + n);
+                            const float4 v = scales4(n);
                             sw_r[j][4 * g] = v.x, sw_r[j][4 * g + 1] = v.y, sw_r[j][4 * g + 2] = v.z, sw_r[j][4 * g + 3] = v.w;
                         } else {
                             sw_r[j][4 * g] = sw_r[j][4 * g + 1] = sw_r[j][4 * g + 2] = sw_r[j][4 * g + 3] = 1.f;
                         }
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            bb_r[j][4 * g + e] = ep.bias ? ep.beta * load_as_f32(ep.bias, ep.bias_dtype, n + e) : 0.f;
+                        for (int e = 0; e < 4; e++) bb_r[j][4 * g + e] = ep.bias ? bias_at(n + e) : 0.f;
                     }
                 __syncthreads();  // every wavefront is done reading the operand stages
                 uint4* region = lds + wave * 512;
@@ -576,7 +616,7 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
                     for (int it = 0; it < 8; it++) {
                         const int q = it * kWave + lane, row = q >> 3, c = q & 7;
                         const uint4 v = region[row * 8 + (c ^ ((row >> 1) & 7))];
-                        if (!GROUPED || m0 + wm * C::WTM + p * 64 + row < M) store_streaming(obase + (int64_t)row * ldo + 8 * c, v);
+                        store_chunk(obase + (int64_t)row * ldo + 8 * c, m0 + wm * C::WTM + p * 64 + row, n0 + wn * C::WTN + jh * 64 + 8 * c, v);
                     }
                   }
                 }
@@ -596,10 +636,10 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
 #pragma unroll
                     for (int g = 0; g < 4; g++) {
                         const int n = n0 + wn * C::WTN + j * 32 + 8 * g + 4 * khalf;
-                        const float4 v = ep.w_scale ? *reinterpret_cast<const float4*>(ep.w_scale + n) : make_float4(1.f, 1.f, 1.f, 1.f);
+                        const float4 v = ep.w_scale ? scales4(n) : make_float4(1.f, 1.f, 1.f, 1.f);
                         sw_r[j][4 * g] = v.x, sw_r[j][4 * g + 1] = v.y, sw_r[j][4 * g + 2] = v.z, sw_r[j][4 * g + 3] = v.w;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) bb_r[j][4 * g + e] = ep.bias ? ep.beta * load_as_f32(ep.bias, ep.bias_dtype, n + e) : 0.f;
+                        for (int e = 0; e < 4; e++) bb_r[j][4 * g + e] = ep.bias ? bias_at(n + e) : 0.f;
                     }
                 // (the barrier behind the main loop: every wavefront is done reading the operand stages)
 #pragma unroll
@@ -636,10 +676,11 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
 #pragma unroll
                 for (int it = 0; it < C::BM * 16 / C::NT; it++) {
                     const int q = it * C::NT + tid, row = q >> 4, c = q & 15;
-                    if (!GROUPED || m0 + row < M) store_streaming(obase + (int64_t)row * ldo + 8 * c, lds[row * 16 + (c ^ (row & 15))]);
+                    store_chunk(obase + (int64_t)row * ldo + 8 * c, m0 + row, n0 + 8 * c, lds[row * 16 + (c ^ (row & 15))]);
                 }
                 return;
             }
+            static_assert(!GROUPED || LDS_EPI || BLOCK_EPI, "by experts the outputs go through LDS");
             float sa_r[C::TM];  // fetched before any store is issued (see above)
 #pragma unroll
             for (int i = 0; i < C::TM; i++) sa_r[i] = ep.a_scale ? ep.a_scale[row_in(m0 + wm * C::WTM + i * 32 + l32)] : 1.f;
@@ -685,7 +726,7 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
                             pk[2 * g][x] = sw2[0];
                             pk[2 * g + 1][x] = sw2[1];
                         }
-                        if (!GROUPED || m < M) store_streaming(orow + nb + 16 * g + 8 * khalf, make_uint4(pk[2 * g][0], pk[2 * g][1], pk[2 * g + 1][0], pk[2 * g + 1][1]));
+                        store_streaming(orow + nb + 16 * g + 8 * khalf, make_uint4(pk[2 * g][0], pk[2 * g][1], pk[2 * g + 1][0], pk[2 * g + 1][1]));
                     }
                 }
             }
@@ -699,6 +740,7 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
         }
         return;
     }
+    if constexpr (GROUPED) return;
 #pragma unroll
     for (int j = 0; j < C::TN; j++) {
         const int nb = n0 + wn * C::WTN + j * 32;  // first channel of this 32-wide MFMA tile (wave-uniform)

@@ -73,6 +73,19 @@ __device__ __forceinline__ void store_streaming(void* p, uint4 v) {
     typedef uint32_t u4v __attribute__((ext_vector_type(4)));
     __builtin_nontemporal_store(u4v{v.x, v.y, v.z, v.w}, reinterpret_cast<u4v*>(p));
 }
+// the first `left` of eight finished 16-bit outputs, to any even address
+__device__ __forceinline__ void store_any(uint16_t* to, uint4 v, int left) {
+    typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+    typedef u4v u4any __attribute__((aligned(2)));
+    if (left >= 8) {
+        __builtin_nontemporal_store(u4v{v.x, v.y, v.z, v.w}, reinterpret_cast<u4any*>(to));
+    } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 7; e++)
+            if (e < left) to[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+    }
+}
 __device__ __forceinline__ float load_as_f32(const void* p, int dtype, int64_t i) {
     if (dtype == LLMQ_F32) return ((const float*)p)[i];
     uint16_t h = ((const uint16_t*)p)[i];

@@ -90,7 +90,7 @@ def test_product_refusals(p16):
     assert grouped(p, A=p + 8) == ALIGN and grouped(p, B=p + 8) == ALIGN
     assert grouped(p, M=0) == OK and grouped(p, N=0, ldo=0) == OK and grouped(p, E=0) == OK
     L = _abi.lib()
-    assert L.llmq_gemm_w8a8_grouped_force_plan(3) == SHAPE and L.llmq_gemm_w8a8_grouped_force_plan(18) == SHAPE
+    assert L.llmq_gemm_w8a8_grouped_force_plan(3) == SHAPE and L.llmq_gemm_w8a8_grouped_force_plan(13) == SHAPE
     assert L.llmq_gemm_w8a8_grouped_force_plan(-1) == OK
 
 
