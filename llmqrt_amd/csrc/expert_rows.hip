@@ -17,22 +17,22 @@ namespace {
 
 enum { OUT_SAME = LLMQ_NORM_SAME, OUT_I8 = LLMQ_NORM_I8_TOKEN, OUT_GROUP = LLMQ_NORM_FP8_GROUP };
 constexpr int kMaxTop = 64, kMaxExperts = 4096;
-constexpr int kMaxChunks = 2048;     // of ids
 constexpr int64_t kCountAll = 2048;  // up to so many ids every token counts all of them for itself
 
 struct DispatchArgs {
     const uint16_t* x;
     const int32_t* ids;
-    const int32_t* base;  // [experts, chunks]: place of the first id of an expert in a chunk of ids; null: every token counts all ids
     void* rows;
     float* scale;
     int32_t *offsets, *places;
     int64_t ldx, K;
     int t0, ids_total;  // t0: token of block 0
-    int tokens, top, first, experts, chunks, chunk_tokens;  // tokens: of this launch
+    int tokens, top, first, experts;  // tokens: of this launch
+    int wide;           // codes are stored 16 at a time
 };
 
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_prefix(v), kWave - 1); }
+__device__ __forceinline__ uint32_t expert_of(const int32_t* ids, int i, int first) { return (uint32_t)ids[i] - (uint32_t)first; }
 
 // Exclusive prefix sums of n values in LDS, in place, by NT threads; returns the total.
 template <int NT>
@@ -56,219 +56,289 @@ __device__ __forceinline__ int scan_lds(int32_t* v, int n, int32_t* sums) {
     return total;
 }
 
-// A block per expert: how many ids go to smaller experts, and how many of its own each chunk of ids holds.
-__global__ __launch_bounds__(1024) void expert_bases_kernel(const int32_t* __restrict__ ids, int n, int first, int experts, int chunk, int chunks,
-                                                            int32_t* __restrict__ base, int32_t* __restrict__ offsets) {
-    __shared__ int32_t same[kMaxChunks], sums[1024 / kWave], s_less[1024 / kWave];
-    const int e = blockIdx.x, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    int less = 0;
-    for (int c = wave; c < chunks; c += 1024 / kWave) {
-        const int lo = c * chunk, hi = min(n - lo, chunk) + lo;
-        int mine = 0;
-#pragma unroll 4
-        for (int i = lo + lane; i < hi; i += kWave) {
-            const uint32_t v = (uint32_t)ids[i] - (uint32_t)first;
-            mine += v == (uint32_t)e, less += v < (uint32_t)e;
+// Many ids: a block per expert finds the places of its own.  Every wavefront has a run of the ids and goes over it twice: it counts those of smaller experts and
+// of this one, and hands out places from where the runs before it end.  A run of up to U * Q * 64 ids stays in registers between the two.
+// Q: ids of a lane next to each other (4: 16-byte loads).  32768 ids of 32 experts, us: 8 pieces of 64 at a time, loaded twice 11.1, so 9.6; 8000 of 60 4.4 and 5.6.
+template <int Q>
+__global__ __launch_bounds__(1024) void expert_places_kernel(const int32_t* __restrict__ ids, int n, int first, int experts, int32_t* __restrict__ places,
+                                                             int32_t* __restrict__ offsets) {
+    constexpr int NW = 1024 / kWave, U = 8, PIECE = Q * kWave;  // U pieces requested before the first is used
+    __shared__ int32_t s_same[NW], s_less[NW];
+    const int e = blockIdx.x, lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int run = ((n + NW - 1) / NW + PIECE - 1) / PIECE * PIECE, lo = (int)min((int64_t)n, (int64_t)wave * run), hi = min(n - lo, run) + lo;
+    uint32_t v[U][Q];
+    auto load = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = b + u * PIECE + lane * Q;
+            if constexpr (Q == 4) {
+                const int4 w = *reinterpret_cast<const int4*>(ids + (i < n - 3 ? i : 0));  // (n > 3; the last, partial piece below)
+                v[u][0] = (uint32_t)w.x, v[u][1] = (uint32_t)w.y, v[u][2] = (uint32_t)w.z, v[u][3] = (uint32_t)w.w;
+            } else {
+                v[u][0] = (uint32_t)ids[min(i, n - 1)];
+            }
         }
-        mine = wave_total(mine);
-        if (lane == 0) same[c] = mine;
-    }
-    less = wave_total(less);
-    if (lane == 0) s_less[wave] = less;
+        if (Q == 4 && b + U * PIECE > n - 3)  // uniform
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int i = b + u * PIECE + lane * Q;
+                if (i < n && i >= n - 3)
+#pragma unroll
+                    for (int q = 0; q < Q; q++) v[u][q] = (uint32_t)ids[min(i + q, n - 1)];
+            }
+    };
+    // the lanes whose id q of piece u is this expert's; a piece past the run has none
+    uint64_t has[U][Q];
+    int less = 0, same = 0;
+    auto look = [&](int b, bool count) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int at = b + u * PIECE;
+#pragma unroll
+            for (int q = 0; q < Q; q++) has[u][q] = 0;
+            if (at >= hi) continue;  // uniform
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+                const uint32_t id = v[u][q] - (uint32_t)first;
+                const bool in = at + PIECE <= hi || at + lane * Q + q < hi;
+                has[u][q] = __ballot(in && id == (uint32_t)e);
+                if (count) same += (int)__popcll(has[u][q]), less += (int)__popcll(__ballot(in && id < (uint32_t)e));
+            }
+        }
+    };
+    for (int b = lo; b < hi; b += U * PIECE) load(b), look(b, true);
+    if (lane == 0) s_same[wave] = same, s_less[wave] = less;
     __syncthreads();
-    const int own = scan_lds<1024>(same, chunks, sums);
-    less = 0;
-    for (int w = 0; w < 1024 / kWave; w++) less += s_less[w];
-    for (int c = threadIdx.x; c < chunks; c += 1024) base[(int64_t)e * chunks + c] = less + same[c];
+    int before = 0, all = 0, from = 0;
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        before += w < wave ? s_same[w] : 0;
+        all += s_same[w], from += s_less[w];
+    }
     if (threadIdx.x == 0) {
-        offsets[e] = less;
-        if (e == experts - 1) offsets[experts] = less + own;
+        offsets[e] = from;
+        if (e == experts - 1) offsets[experts] = from + all;
+    }
+    int at = from + before;
+    for (int b = lo; b < hi; b += U * PIECE) {
+        if (hi - lo > U * PIECE) load(b), look(b, false);  // (a short run is still there)
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = b + u * PIECE + lane * Q;
+            uint64_t any = 0;
+#pragma unroll
+            for (int q = 0; q < Q; q++) any |= has[u][q];
+            if (any) {  // uniform
+                int upto = at;  // the place of the lane's first one
+#pragma unroll
+                for (int q = 0; q < Q; q++) upto = __builtin_amdgcn_mbcnt_hi((uint32_t)(has[u][q] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has[u][q], upto));
+#pragma unroll
+                for (int q = 0; q < Q; q++) {
+                    if (has[u][q] >> lane & 1) places[i + q] = upto++;
+                    at += (int)__popcll(has[u][q]);
+                }
+            }
+            if (e == 0)
+#pragma unroll
+                for (int q = 0; q < Q; q++)
+                    if (i + q < hi && v[u][q] - (uint32_t)first >= (uint32_t)experts) places[i + q] = -1;
+        }
     }
 }
 
-// A block per token.  ALL: every token counts all ids for itself, and one more block counts them for the offsets.  NC > 0: the row stays in NC registers per thread; 0: rows of any
-// length, read again for every copy.
-template <int DT, int OUT, bool ALL, int NC, int NT>
+// A block per token; 16 neighbouring elements per thread and piece.  ALL: every token counts all ids for itself, and one more block counts them for the
+// offsets; otherwise the places are there.  NP > 0: the row stays in registers, NP pieces per thread; 0: rows of any length, read again for every copy.
+template <int DT, int OUT, bool ALL, int NP, int NT>
 __global__ __launch_bounds__(NT) void dispatch_kernel(DispatchArgs a) {
-    constexpr int NW = NT / kWave, REGS = NC > 0 ? NC : 1, JW = 4;
+    constexpr int NW = NT / kWave, REGS = NP > 0 ? NP : 1, JW = 4;
     __shared__ float smem[NW];
-    __shared__ int32_t place[kMaxTop];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    if constexpr (ALL) if (blockIdx.x == (unsigned)a.tokens) {  // block-uniform
-        __shared__ int32_t count[kMaxExperts], sums[NW];
-        for (int e = tid; e < a.experts; e += NT) count[e] = 0;
-        __syncthreads();
-        for (int i = tid; i < a.ids_total; i += NT) {
-            const uint32_t e = (uint32_t)a.ids[i] - (uint32_t)a.first;
-            if (e < (uint32_t)a.experts) atomicAdd(&count[e], 1);
+    if constexpr (ALL) {
+        if (blockIdx.x == (unsigned)a.tokens) {  // block-uniform
+            __shared__ int32_t count[kMaxExperts], sums[NW];
+            for (int e = tid; e < a.experts; e += NT) count[e] = 0;
+            __syncthreads();
+            for (int i = tid; i < a.ids_total; i += NT) {
+                const uint32_t e = expert_of(a.ids, i, a.first);
+                if (e < (uint32_t)a.experts) atomicAdd(&count[e], 1);
+            }
+            __syncthreads();
+            const int total = scan_lds<NT>(count, a.experts, sums);
+            for (int e = tid; e < a.experts; e += NT) a.offsets[e] = count[e];
+            if (tid == 0) a.offsets[a.experts] = total;
+            return;
         }
-        __syncthreads();
-        const int total = scan_lds<NT>(count, a.experts, sums);
-        for (int e = tid; e < a.experts; e += NT) a.offsets[e] = count[e];
-        if (tid == 0) a.offsets[a.experts] = total;
-        return;
     }
-    const int t = a.t0 + (int)blockIdx.x;
-    const int nchunk = (int)(a.K >> 3);
+    const int t = a.t0 + (int)blockIdx.x, mine = t * a.top;
+    const int nchunk = (int)(a.K >> 3), npiece = (nchunk + 1) / 2;
+    int goes_to = -1;  // the place of copy `lane`
+    if constexpr (!ALL) goes_to = lane < a.top ? a.places[mine + lane] : -1;
     const uint4* xr = reinterpret_cast<const uint4*>(a.x + (int64_t)t * a.ldx);
-    uint4 v[REGS];
-    if (NC > 0) {
+    auto half = [&](int c) __attribute__((always_inline)) { return c < nchunk ? xr[c] : make_uint4(0, 0, 0, 0); };
+    // the chunks of piece i: two neighbours, whose codes are 16 bytes; rows that are copied as they are: one of this half of NT chunks and one of the next
+    auto chunk = [&](int i, int h) __attribute__((always_inline)) { return OUT == OUT_SAME ? i / NT * (2 * NT) + h * NT + i % NT : 2 * i + h; };
+    uint4 v[REGS][2];
+    if (NP > 0) {
 #pragma unroll
-        for (int c = 0; c < NC; c++) v[c] = tid + c * NT < nchunk ? xr[tid + c * NT] : make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < NP; c++) {
+            const int i = tid + c * NT;
+            v[c][0] = half(chunk(i, 0)), v[c][1] = half(chunk(i, 1));
+        }
     }
 
-    // ---- places of the token's copies: JW of them per wavefront and pass over the ids
-    const int mine = t * a.top, chunk = ALL ? 0 : t / a.chunk_tokens, lo = ALL ? 0 : chunk * a.chunk_tokens * a.top;
-    for (int j0 = wave * JW; j0 < a.top; j0 += NW * JW) {
-        uint32_t e[JW];
-        int n[JW];
+    if constexpr (ALL) {  // JW copies per wavefront and pass over the ids
+        __shared__ int32_t place[kMaxTop];
+        for (int j0 = wave * JW; j0 < a.top; j0 += NW * JW) {
+            uint32_t e[JW];
+            int n[JW];
 #pragma unroll
-        for (int k = 0; k < JW; k++) {
-            e[k] = j0 + k < a.top ? (uint32_t)a.ids[mine + j0 + k] - (uint32_t)a.first : ~0u;
-            n[k] = 0;
-        }
-        if (!ALL) {
-#pragma unroll 4
-            for (int i = lo + lane; i < mine + a.top; i += kWave) {
-                const uint32_t id = (uint32_t)a.ids[i] - (uint32_t)a.first;
-#pragma unroll
-                for (int k = 0; k < JW; k++) n[k] += id == e[k] && i < mine + j0 + k;
+            for (int k = 0; k < JW; k++) {
+                e[k] = j0 + k < a.top ? expert_of(a.ids, mine + j0 + k, a.first) : ~0u;
+                n[k] = 0;
             }
-        } else {
 #pragma unroll 4
             for (int i = lane; i < a.ids_total; i += kWave) {
-                const uint32_t id = (uint32_t)a.ids[i] - (uint32_t)a.first;
+                const uint32_t id = expert_of(a.ids, i, a.first);
 #pragma unroll
                 for (int k = 0; k < JW; k++) n[k] += id < e[k] || (id == e[k] && i < mine + j0 + k);
             }
-        }
 #pragma unroll
-        for (int k = 0; k < JW; k++) {
-            if (j0 + k >= a.top) break;
-            const bool goes = e[k] < (uint32_t)a.experts;
-            int p = wave_total(n[k]);
-            if (!ALL && goes) p += a.base[(int64_t)e[k] * a.chunks + chunk];
-            if (!goes) p = -1;
-            if (lane == 0) place[j0 + k] = p, a.places[mine + j0 + k] = p;
+            for (int k = 0; k < JW; k++) {
+                if (j0 + k >= a.top) break;
+                const int p = e[k] < (uint32_t)a.experts ? wave_total(n[k]) : -1;
+                if (lane == 0) place[j0 + k] = p, a.places[mine + j0 + k] = p;
+            }
         }
+        __syncthreads();
+        goes_to = lane < a.top ? place[lane] : -1;
     }
-    __syncthreads();
+    auto each_copy = [&](auto&& f) __attribute__((always_inline)) {  // f(place)
+        for (int j = 0; j < a.top; j++) {
+            const int p = __builtin_amdgcn_readlane(goes_to, j);
+            if (p >= 0) f(p);
+        }
+    };
+    // codes of piece i to a row
+    auto store = [&](uint8_t* to, int i, uint2 q0, uint2 q1) __attribute__((always_inline)) {
+        if (a.wide) {
+            *reinterpret_cast<uint4*>(to + 16 * (int64_t)i) = make_uint4(q0.x, q0.y, q1.x, q1.y);
+        } else {
+            *reinterpret_cast<uint2*>(to + 16 * (int64_t)i) = q0;
+            if (2 * i + 1 < nchunk) *reinterpret_cast<uint2*>(to + 16 * (int64_t)i + 8) = q1;
+        }
+    };
 
     // ---- the row, in its output's form, to every place
     if (OUT == OUT_SAME) {
-        for (int j = 0; j < a.top; j++) {
-            const int p = place[j];
-            if (p < 0) continue;
+        each_copy([&](int p) __attribute__((always_inline)) {
             uint4* to = reinterpret_cast<uint4*>((uint16_t*)a.rows + (int64_t)p * a.K);
-            if (NC > 0) {
+            auto copy = [&](int i, uint4 lo, uint4 hi) __attribute__((always_inline)) {
+                if (chunk(i, 0) < nchunk) to[chunk(i, 0)] = lo;
+                if (chunk(i, 1) < nchunk) to[chunk(i, 1)] = hi;
+            };
+            if (NP > 0) {
 #pragma unroll
-                for (int c = 0; c < NC; c++)
-                    if (tid + c * NT < nchunk) to[tid + c * NT] = v[c];
+                for (int c = 0; c < NP; c++) copy(tid + c * NT, v[c][0], v[c][1]);
             } else {
-                for (int i = tid; i < nchunk; i += NT) to[i] = xr[i];
+                for (int i = tid; chunk(i, 0) < nchunk; i += NT) copy(i, half(chunk(i, 0)), half(chunk(i, 1)));
             }
-        }
+        });
         return;
     }
     if (OUT == OUT_I8) {  // the scale and the quotients are values of x's type, as in llmq_quant_i8_per_token
+        auto most = [](uint4 lo, uint4 hi) __attribute__((always_inline)) { return max_nonneg(absmax8(lo, DT == LLMQ_BF16), absmax8(hi, DT == LLMQ_BF16)); };
         float amax = 0.f;
-        if (NC > 0) {
+        if (NP > 0) {
 #pragma unroll
-            for (int c = 0; c < NC; c++) amax = max_nonneg(amax, absmax8(v[c], DT == LLMQ_BF16));
+            for (int c = 0; c < NP; c++) amax = max_nonneg(amax, most(v[c][0], v[c][1]));
         } else {
-            for (int i = tid; i < nchunk; i += NT) amax = max_nonneg(amax, absmax8(xr[i], DT == LLMQ_BF16));
+            for (int i = tid; i < npiece; i += NT) amax = max_nonneg(amax, most(half(2 * i), half(2 * i + 1)));
         }
-        amax = block_max<NW>(amax, smem);
+        amax = NW > 1 ? block_max<NW>(amax, smem) : wave_max(amax);
         const float s = scale_from_amax<DT, MODE_I8>(amax), inv_s = 1.0f / s;
         const bool fin = amax < __builtin_inff() && s > 0.f;
         auto codes = [&](uint4 r) __attribute__((always_inline)) {
             return fin ? quant8<DT, MODE_I8, Q_DT, true>(r, s, inv_s) : quant8<DT, MODE_I8, Q_DT, false>(r, s, inv_s);
         };
-        uint2 q[REGS];
-        if (NC > 0) {
+        uint2 q[REGS][2];
+        if (NP > 0) {
 #pragma unroll
-            for (int c = 0; c < NC; c++) q[c] = codes(v[c]);
+            for (int c = 0; c < NP; c++) q[c][0] = codes(v[c][0]), q[c][1] = codes(v[c][1]);
         }
-        for (int j = 0; j < a.top; j++) {
-            const int p = place[j];
-            if (p < 0) continue;
-            uint2* to = reinterpret_cast<uint2*>((uint8_t*)a.rows + (int64_t)p * a.K);
-            if (tid == 0) a.scale[p] = s;
-            if (NC > 0) {
+        if (wave == 0 && goes_to >= 0) a.scale[goes_to] = s;
+        each_copy([&](int p) __attribute__((always_inline)) {
+            uint8_t* to = (uint8_t*)a.rows + (int64_t)p * a.K;
+            if (NP > 0) {
 #pragma unroll
-                for (int c = 0; c < NC; c++)
-                    if (tid + c * NT < nchunk) to[tid + c * NT] = q[c];
+                for (int c = 0; c < NP; c++)
+                    if (tid + c * NT < npiece) store(to, tid + c * NT, q[c][0], q[c][1]);
             } else {
-                for (int i = tid; i < nchunk; i += NT) to[i] = codes(xr[i]);
+                for (int i = tid; i < npiece; i += NT) store(to, i, codes(half(2 * i)), codes(half(2 * i + 1)));
             }
-        }
+        });
         return;
     }
-    // a scale per 16 chunks, which 16 neighbouring lanes hold
-    const int groups = (nchunk + kTeam - 1) / kTeam;
-    auto group_codes = [&](uint4 r, float& s) __attribute__((always_inline)) {
-        const float amax = team_max(absmax8(r, DT == LLMQ_BF16));
-        s = scale32<MODE_F8>(amax);
-        const float inv_s = 1.0f / s;
-        float f[8];
-        widen8<DT>(r, f);
-        return __all(near_ok(amax, s)) ? codes8<MODE_F8, true>(f, s, inv_s) : codes8<MODE_F8, false>(f, s, inv_s);
+    // a scale per 8 pieces, which 8 neighbouring lanes hold
+    constexpr int TEAM = kTeam / 2;
+    const int groups = (npiece + TEAM - 1) / TEAM;
+    auto group_codes = [&](uint4 lo, uint4 hi, uint2* q) __attribute__((always_inline)) {
+        float amax = max_nonneg(absmax8(lo, DT == LLMQ_BF16), absmax8(hi, DT == LLMQ_BF16));
+        amax = max_nonneg(amax, lane_xor<1>(amax));
+        amax = max_nonneg(amax, lane_xor<2>(amax));
+        amax = max_nonneg(amax, lane_xor<4>(amax));
+        const float s = scale32<MODE_F8>(amax), inv_s = 1.0f / s;
+        float f[8], h[8];
+        widen8<DT>(lo, f), widen8<DT>(hi, h);
+        if (__all(near_ok(amax, s))) q[0] = codes8<MODE_F8, true>(f, s, inv_s), q[1] = codes8<MODE_F8, true>(h, s, inv_s);
+        else q[0] = codes8<MODE_F8, false>(f, s, inv_s), q[1] = codes8<MODE_F8, false>(h, s, inv_s);
+        return s;
     };
-    uint2 q[REGS];
+    uint2 q[REGS][2];
     float s[REGS];
-    if (NC > 0) {
+    if (NP > 0) {
 #pragma unroll
-        for (int c = 0; c < NC; c++) q[c] = group_codes(v[c], s[c]);
+        for (int c = 0; c < NP; c++) s[c] = group_codes(v[c][0], v[c][1], q[c]);
     }
-    for (int j = 0; j < a.top; j++) {
-        const int p = place[j];
-        if (p < 0) continue;  // block-uniform
-        uint2* to = reinterpret_cast<uint2*>((uint8_t*)a.rows + (int64_t)p * a.K);
+    each_copy([&](int p) __attribute__((always_inline)) {
+        uint8_t* to = (uint8_t*)a.rows + (int64_t)p * a.K;
         float* ts = a.scale + (int64_t)p * groups;
-        if (NC > 0) {
+        if (NP > 0) {
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
+            for (int c = 0; c < NP; c++) {
                 const int i = tid + c * NT;
-                if (i < nchunk) to[i] = q[c];
-                if (i < nchunk && i % kTeam == 0) ts[i / kTeam] = s[c];
+                if (i < npiece) store(to, i, q[c][0], q[c][1]);
+                if (i < npiece && i % TEAM == 0) ts[i / TEAM] = s[c];
             }
         } else {
-            for (int b = 0; b < nchunk; b += NT) {
+            for (int b = 0; b < npiece; b += NT) {
                 const int i = b + tid;
-                const uint2 c = group_codes(i < nchunk ? xr[i] : make_uint4(0, 0, 0, 0), s[0]);
-                if (i < nchunk) to[i] = c;
-                if (i < nchunk && i % kTeam == 0) ts[i / kTeam] = s[0];
+                s[0] = group_codes(half(2 * i), half(2 * i + 1), q[0]);
+                if (i < npiece) store(to, i, q[0][0], q[0][1]);
+                if (i < npiece && i % TEAM == 0) ts[i / TEAM] = s[0];
             }
         }
-    }
-}
-
-// ids per chunk, a whole number of tokens' (0: every token counts all ids)
-int64_t chunk_tokens(int64_t tokens, int64_t top) {
-    if (tokens * top <= kCountAll) return 0;
-    const int64_t least = (tokens + kMaxChunks - 1) / kMaxChunks;
-    return std::max(least, std::max<int64_t>(1, 512 / top));
+    });
 }
 
 template <int DT, int OUT, bool ALL>
 int launch_dispatch(const DispatchArgs& a, unsigned grid, hipStream_t st) {
-    const int64_t chunks = a.K >> 3;
-#define LLMQ_DISPATCH(NC, NT) hipLaunchKernelGGL((dispatch_kernel<DT, OUT, ALL, NC, NT>), dim3(grid), dim3(NT), 0, st, a)
-    if (chunks <= 128) LLMQ_DISPATCH(1, 128);
-    else if (chunks <= 256) LLMQ_DISPATCH(1, 256);
-    else if (chunks <= 512) LLMQ_DISPATCH(2, 256);
-    else if (chunks <= 1024) LLMQ_DISPATCH(4, 256);
-    else if (chunks <= 2560) LLMQ_DISPATCH(5, 512);
+    const int64_t pieces = (a.K + 15) / 16;
+#define LLMQ_DISPATCH(NP, NT) hipLaunchKernelGGL((dispatch_kernel<DT, OUT, ALL, NP, NT>), dim3(grid), dim3(NT), 0, st, a)
+    if (!ALL && pieces <= 64) LLMQ_DISPATCH(1, (ALL ? 256 : 64));
+    else if (!ALL && pieces <= 128) LLMQ_DISPATCH(1, (ALL ? 256 : 128));
+    else if (pieces <= 256) LLMQ_DISPATCH(1, 256);  // (with all ids to count, as many wavefronts as that for short rows too)
+    else if (pieces <= 512) LLMQ_DISPATCH(2, 256);
+    else if (pieces <= 1280) LLMQ_DISPATCH(5, 256);
     else LLMQ_DISPATCH(0, 512);
 #undef LLMQ_DISPATCH
     return launch_status();
 }
 template <int DT>
-int launch_dispatch_out(int out, const DispatchArgs& a, unsigned grid, hipStream_t st) {
+int launch_dispatch_out(int out, bool all, const DispatchArgs& a, unsigned grid, hipStream_t st) {
     switch (out) {
-        case OUT_SAME: return a.base ? launch_dispatch<DT, OUT_SAME, false>(a, grid, st) : launch_dispatch<DT, OUT_SAME, true>(a, grid, st);
-        case OUT_I8: return a.base ? launch_dispatch<DT, OUT_I8, false>(a, grid, st) : launch_dispatch<DT, OUT_I8, true>(a, grid, st);
-        default: return a.base ? launch_dispatch<DT, OUT_GROUP, false>(a, grid, st) : launch_dispatch<DT, OUT_GROUP, true>(a, grid, st);
+        case OUT_SAME: return all ? launch_dispatch<DT, OUT_SAME, true>(a, grid, st) : launch_dispatch<DT, OUT_SAME, false>(a, grid, st);
+        case OUT_I8: return all ? launch_dispatch<DT, OUT_I8, true>(a, grid, st) : launch_dispatch<DT, OUT_I8, false>(a, grid, st);
+        default: return all ? launch_dispatch<DT, OUT_GROUP, true>(a, grid, st) : launch_dispatch<DT, OUT_GROUP, false>(a, grid, st);
     }
 }
 
@@ -327,15 +397,9 @@ bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0
 
 using namespace llmq;
 
-extern "C" size_t llmq_dispatch_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts) {
-    if (tokens <= 0 || top_k <= 0 || top_k > kMaxTop || experts <= 0 || experts > kMaxExperts || tokens > 0x7fffff00LL / top_k) return 0;
-    const int64_t per = chunk_tokens(tokens, top_k);
-    return per ? (size_t)(experts * ((tokens + per - 1) / per) * 4) : 0;
-}
-
 extern "C" int llmq_dispatch_experts(int out, const void* x, int x_dtype, int64_t tokens, int64_t K, int64_t ldx, const int32_t* ids, int64_t top_k,
                                      int64_t first_expert, int64_t experts, void* rows, float* scale, int32_t* offsets, int32_t* places,
-                                     void* workspace, size_t workspace_bytes, llmq_stream_t stream) {
+                                     llmq_stream_t stream) {
     if ((out != OUT_SAME && out != OUT_I8 && out != OUT_GROUP) || (x_dtype != LLMQ_BF16 && x_dtype != LLMQ_F16)) return LLMQ_ERR_DTYPE;
     if (tokens < 0 || K < 0 || K > 0x7fffffffLL || ldx < K || (K & 7) || (ldx & 7) || top_k < 1 || top_k > kMaxTop || experts < 1 ||
         experts > kMaxExperts || first_expert < 0 || first_expert > 0x7fff0000LL || tokens > 0x7fffff00LL / top_k)
@@ -343,26 +407,23 @@ extern "C" int llmq_dispatch_experts(int out, const void* x, int x_dtype, int64_
     if (!offsets || (tokens > 0 && (!ids || !places || (K > 0 && (!x || !rows || (out != OUT_SAME && !scale)))))) return LLMQ_ERR_NULL;
     if (tokens > 0 && K == 0) return LLMQ_ERR_SHAPE;
     if (tokens > 0 && (!aligned16(x) || (out == OUT_SAME ? !aligned16(rows) : !aligned8(rows)))) return LLMQ_ERR_ALIGN;
-    const size_t need = llmq_dispatch_workspace_bytes(tokens, top_k, experts);
-    if (need && (!workspace || workspace_bytes < need)) return LLMQ_ERR_WORKSPACE;
-    if (need && (reinterpret_cast<uintptr_t>(workspace) & 3u)) return LLMQ_ERR_ALIGN;
     DispatchArgs a = {};
     a.x = (const uint16_t*)x, a.ids = ids, a.rows = rows, a.scale = scale, a.offsets = offsets, a.places = places;
     a.ldx = ldx, a.K = K, a.ids_total = (int)(tokens * top_k), a.top = (int)top_k, a.first = (int)first_expert, a.experts = (int)experts;
+    a.wide = K % 16 == 0 && aligned16(rows);
     const hipStream_t st = (hipStream_t)stream;
-    const int64_t per = chunk_tokens(tokens, top_k);
-    if (per) {
-        a.chunk_tokens = (int)per, a.chunks = (int)((tokens + per - 1) / per), a.base = (const int32_t*)workspace;
-        hipLaunchKernelGGL(expert_bases_kernel, dim3((unsigned)experts), dim3(1024), 0, st, ids, a.ids_total, a.first, a.experts, (int)(per * top_k), a.chunks,
-                           (int32_t*)workspace, offsets);
+    const bool all = tokens * top_k <= kCountAll;
+    if (!all) {
+        if (aligned16(ids)) hipLaunchKernelGGL((expert_places_kernel<4>), dim3((unsigned)experts), dim3(1024), 0, st, ids, a.ids_total, a.first, a.experts, places, offsets);
+        else hipLaunchKernelGGL((expert_places_kernel<1>), dim3((unsigned)experts), dim3(1024), 0, st, ids, a.ids_total, a.first, a.experts, places, offsets);
         if (launch_status() != LLMQ_OK) return LLMQ_ERR_LAUNCH;
     }
     const int64_t step = (int64_t)1 << 21;  // tokens of a grid: 2^32 threads are too many
     int rc = LLMQ_OK;
-    for (int64_t t = 0; rc == LLMQ_OK && (t < tokens || (t == 0 && !per)); t += step) {
+    for (int64_t t = 0; rc == LLMQ_OK && (t < tokens || (t == 0 && all)); t += step) {
         a.t0 = (int)t, a.tokens = (int)std::min(step, tokens - t);
-        const unsigned grid = (unsigned)a.tokens + (per ? 0 : 1);  // (every token counts all ids: one launch, with the block for the offsets)
-        rc = x_dtype == LLMQ_BF16 ? launch_dispatch_out<LLMQ_BF16>(out, a, grid, st) : launch_dispatch_out<LLMQ_F16>(out, a, grid, st);
+        const unsigned grid = (unsigned)a.tokens + (all ? 1 : 0);  // (every token counts all ids: one launch, with the block for the offsets)
+        rc = x_dtype == LLMQ_BF16 ? launch_dispatch_out<LLMQ_BF16>(out, all, a, grid, st) : launch_dispatch_out<LLMQ_F16>(out, all, a, grid, st);
     }
     return rc;
 }

@@ -676,7 +676,7 @@ std::optional<Sorted> dispatch(const Tensor& x, const Tensor& ids, int64_t exper
     if (top < 1 || top > 64) return std::nullopt;
     const at::Device dev = x.device();
     const Launch l(dev);
-    Tensor rows, scale, offsets, places, ws;
+    Tensor rows, scale, offsets, places;
     Outputs o(dev);
     const bool same = out == LLMQ_NORM_SAME;
     o.add(&rows, {n, r.K}, same ? x.scalar_type() : out == LLMQ_NORM_I8_TOKEN ? at::kChar : at::kFloat8_e4m3fn);
@@ -684,11 +684,9 @@ std::optional<Sorted> dispatch(const Tensor& x, const Tensor& ids, int64_t exper
     o.add(&offsets, {experts + 1}, at::kInt);
     o.add(&places, ids.sizes(), at::kInt);
     o.make_all();
-    const int64_t bytes = (int64_t)llmq_dispatch_workspace_bytes(r.M, top, experts);
-    if (bytes) ws = make({bytes}, at::kByte, dev);
     const int rc = llmq_dispatch_experts(out, x.data_ptr(), code(x.scalar_type()), r.M, r.K, r.K, (const int32_t*)ids.data_ptr(), top, first, experts,
                                          rows.data_ptr(), same ? nullptr : (float*)scale.data_ptr(), (int32_t*)offsets.data_ptr(),
-                                         (int32_t*)places.data_ptr(), bytes ? ws.data_ptr() : nullptr, (size_t)bytes, l.stream);
+                                         (int32_t*)places.data_ptr(), l.stream);
     if (refused(rc)) return std::nullopt;
     check(rc, "llmq_dispatch_experts");
     Sorted s;

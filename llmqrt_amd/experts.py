@@ -113,13 +113,10 @@ def _dispatch_general(x, experts, num_experts, first_expert, out):
         scale = torch.empty((n, 1 if out == _I8_TOKEN else (K + 127) // 128), dtype=torch.float32, device=dev)
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
     places = torch.empty(experts.shape, dtype=torch.int32, device=dev)
-    L = _abi.lib()
-    nws = L.llmq_dispatch_workspace_bytes(T, top, num_experts)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
     with torch.cuda.device(dev):
-        _abi.check(L.llmq_dispatch_experts(out, rows.data_ptr(), _abi.dtype_code(rows.dtype), T, K, rows.stride(0) if T > 1 else K, ids.data_ptr(), top,
-                                           first_expert, num_experts, sorted_rows.data_ptr(), _abi.ptr(scale), offsets.data_ptr(), places.data_ptr(),
-                                           _abi.ptr(ws), nws, _abi.stream_of(rows)), "llmq_dispatch_experts")
+        _abi.check(_abi.lib().llmq_dispatch_experts(
+            out, rows.data_ptr(), _abi.dtype_code(rows.dtype), T, K, rows.stride(0) if T > 1 else K, ids.data_ptr(), top, first_expert, num_experts,
+            sorted_rows.data_ptr(), _abi.ptr(scale), offsets.data_ptr(), places.data_ptr(), _abi.stream_of(rows)), "llmq_dispatch_experts")
     return (sorted_rows, offsets, places) if scale is None else (sorted_rows, scale, offsets, places)
 
 

@@ -6,7 +6,7 @@ import torch
 
 from llmqrt_amd import _abi
 
-OK, NULL, DTYPE, SHAPE, WORKSPACE, ALIGN = 0, -1, -2, -3, -4, -6
+OK, NULL, DTYPE, SHAPE, ALIGN = 0, -1, -2, -3, -6
 
 
 @pytest.fixture(scope="module")
@@ -32,9 +32,9 @@ def test_route_refusals(p16):
     assert route(p, T=0, logits=0, w=0, ids=0) == OK
 
 
-def dispatch(p, out=0, dt=0, T=4, K=64, ldx=64, k=2, first=0, E=4, x=None, ids=None, rows=None, scale=None, off=None, pl=None, ws=0, wsb=0):
+def dispatch(p, out=0, dt=0, T=4, K=64, ldx=64, k=2, first=0, E=4, x=None, ids=None, rows=None, scale=None, off=None, pl=None):
     d = lambda v: p if v is None else v  # noqa: E731
-    return _abi.lib().llmq_dispatch_experts(out, d(x), dt, T, K, ldx, d(ids), k, first, E, d(rows), d(scale), d(off), d(pl), ws, wsb, None)
+    return _abi.lib().llmq_dispatch_experts(out, d(x), dt, T, K, ldx, d(ids), k, first, E, d(rows), d(scale), d(off), d(pl), None)
 
 
 def test_dispatch_refusals(p16):
@@ -47,14 +47,6 @@ def test_dispatch_refusals(p16):
         assert dispatch(p, **{name: 0}) == NULL
     assert dispatch(p, out=1, scale=0) == NULL and dispatch(p, out=3, scale=0) == NULL and dispatch(p, T=0, off=0) == NULL
     assert dispatch(p, x=p + 8) == ALIGN and dispatch(p, rows=p + 8) == ALIGN and dispatch(p, out=1, rows=p + 4) == ALIGN
-    L = _abi.lib()
-    assert L.llmq_dispatch_workspace_bytes(16, 4, 64) == 0 and L.llmq_dispatch_workspace_bytes(0, 4, 64) == 0
-    assert L.llmq_dispatch_workspace_bytes(8192, 65, 64) == 0 and L.llmq_dispatch_workspace_bytes(8192, 4, 5000) == 0
-    need = L.llmq_dispatch_workspace_bytes(8192, 4, 64)
-    assert need > 0 and need % (4 * 64) == 0
-    assert dispatch(p, T=8192, k=4, E=64) == WORKSPACE and dispatch(p, T=8192, k=4, E=64, ws=p, wsb=need - 1) == WORKSPACE
-    assert dispatch(p, T=8192, k=4, E=64, ws=p + 2, wsb=need) == ALIGN
-    assert L.llmq_dispatch_workspace_bytes(0x7fffff00 // 8, 8, 4096) <= 4 * 4096 * 2048
 
 
 def combine(p, dt=0, R=8, N=64, ldy=64, T=4, k=2, sh=0, lds=64, y=None, pl=None, w=None, out=None):
