@@ -5,7 +5,9 @@ Layout:
   _abi.py          ctypes loader (no fallback: a missing library raises)
   quantize.py      activation quantizers (reference names), fp8 per token and 128 channels, block-scaled weights
   norm.py          RMSNorm, alone, behind the residual's addition, and with an output in 8 bits
-  sq_fp8_kernels   drop-in for runtime.sq_fp8_kernels; block-scaled fp8 products, alone and by experts
+  activation.py    silu(gate) * up, alone and with an output in 8 bits
+  experts.py       routing to experts, rows to them (with the quantizer of their product) and back
+  sq_fp8_kernels   drop-in for runtime.sq_fp8_kernels; block-scaled fp8 products, alone and by experts, W8A8 by experts
   awq_kernels      drop-in for runtime.triton_kernels.awq_kernels
   linear/          quantized Linear modules + registry
   fused_utils.py   fuse q/k/v or gate/up sibling modules into one

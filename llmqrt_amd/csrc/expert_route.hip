@@ -325,8 +325,9 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
         } else if (a.sigmoid) {
 #pragma unroll
             for (int v = 0; v < V; v++) c[v] = __builtin_amdgcn_rcpf(1.f + exp_fast(-x[v]));
-            // exp takes 2 |x| 2^-24 from its argument and 2^-23 of its own, of which s (1 - s) reaches s: less than 2^-24; the sum and the reciprocal 3 2^-24
-            off = 5 * 0x1p-24f;
+            // exp takes 2 |x| 2^-24 from its argument and 2^-23 of its own, of which s (1 - s) reaches s: less than 2^-24; the sum and the reciprocal, whose last
+            // place is worth 2^-24 at most, as much each
+            off = 3 * 0x1p-24f;
         } else {
             sum = 0.f;
 #pragma unroll
@@ -398,7 +399,6 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
             group = best;
         }
     }
-    auto apart = [&](float p, float q, float s) __attribute__((always_inline)) { return p - q > 4 * off + 0x1p-22f * s; };  // (for sums of two as well)
     if (a.groups > 1) {
         score_t left = group, least = 0;
         // the last of as many different scores as groups are asked for, or of fewer where groups are level
@@ -415,34 +415,52 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
         if constexpr (BY == BY_SCORES_32) {
             const float next = token_max<LPT>(left);
             size = token_max<LPT>(size);
-            if (least > kNone && next > kNone && !apart(least, next, 2 * size)) sure = false;
+            // (a score and its share of the sum are each rounded once, the sum once more)
+            if (least > kNone && next > kNone && !(least - next > 4 * off + 0x1p-22f * size)) sure = false;
         }
 #pragma unroll
         for (int v = 0; v < V; v++) key[v] = kept ? key[v] : kNoKey;
     }
 
     // ---- the choices; lane j keeps choice j
-    int id = -1;
+    int id = -1, last = -1;
     float before = __builtin_inff();
+    bool near_last = false;  // the last two choices were close
     for (int j = 0; j < a.top + (BY == BY_SCORES_32 ? 1 : 0); j++) {
         key_t best = key[0];
 #pragma unroll
         for (int v = 1; v < V; v++) best = larger(best, key[v]);
         best = token_max<LPT>(best);
-        if constexpr (BY == BY_SCORES_32) {
-            const float c = value32(best);
-            if (j > 0 && best != 0 && !apart(before, c, fabsf(before) + fabsf(c))) sure = false;
-            before = c;
-            if (j == a.top) break;
-        }
         int at = V;  // the lowest of the lane's experts that has it
 #pragma unroll
         for (int v = V - 1; v >= 0; v--) at = key[v] == best ? v : at;
         const uint32_t lowest = token_max<LPT>(at < V ? 0xffffu - (uint32_t)(e0 + at) : 0u);
-        const int chosen = 0xffff - (int)lowest;
+        int chosen = 0xffff - (int)lowest;
         at = chosen - e0;
 #pragma unroll
         for (int v = 0; v < V; v++) key[v] = v == at && v < count ? kNoKey : key[v];
+        if constexpr (BY == BY_SCORES_32) {
+            const float c = value32(best);
+            const bool close = j > 0 && best != 0 && !(before - c > 2 * off + 0x1p-24f * (fabsf(before) + fabsf(c)));
+            before = c;
+            if (__any(close && sure)) {
+                // Two close sigmoid scores are compared in 64 bits by themselves; three, and those of a softmax, whose sum takes part, are not.
+                if (!a.sigmoid || near_last) sure = sure && !close;
+                if (close && sure) {
+                    auto score = [&](int e) __attribute__((always_inline)) {
+                        return 1.0 / (1.0 + exp(-(double)load_as_f32(a.logits, DT, t * a.ld + e))) + (a.bias ? (double)a.bias[e] : 0.0);
+                    };
+                    const double p = score(last), q = score(chosen);
+                    if (q > p || (q == p && chosen < last)) {
+                        if (l == j - 1) id = chosen;
+                        chosen = last;
+                    }
+                }
+            }
+            near_last = close;
+            last = chosen;
+            if (j == a.top) break;
+        }
         if (l == j) id = best != kNoKey ? chosen : -1;
     }
     if (!__any(sure && wanted)) return false;

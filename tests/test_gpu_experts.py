@@ -115,6 +115,31 @@ def test_route_ties_and_zeros(cuda):
     check_route(half, 8, "sigmoid", torch.zeros(256, device=cuda), 8, 3, "top2")
 
 
+@pytest.mark.parametrize("E,groups,top_groups,score", [(48, 1, 1, "max"), (128, 1, 1, "max"), (256, 1, 1, "max"), (64, 8, 3, "top2"), (256, 8, 4, "top2"), (160, 8, 3, "max")])
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+def test_route_close_scores(cuda, E, groups, top_groups, score, scoring):
+    """Scores with the bias in pairs, threes and fours that 32 bits do not tell apart: the order is that of 64 bits.  (The biases lift neighbours, in a shuffled order, to
+    the same score up to their own rounding, 2^-25 at most; what 64 bits compute is off by 2^-52.)"""
+    g = torch.Generator().manual_seed(E + groups)
+    T = 400
+    x = torch.randn(T, E, generator=g).bfloat16().float()
+    x[1:] = x[0] + torch.randint(-1, 2, (T - 1, 1), generator=g).float() * 2.0 ** -20 * torch.randint(0, 2, (T - 1, E), generator=g)
+    s = torch.sigmoid(x[0].double()) if scoring == "sigmoid" else torch.softmax(x[0].double(), 0)
+    order = torch.randperm(E, generator=g)
+    aim = torch.empty(E, dtype=torch.float64)
+    at, value = 0, 1.5
+    while at < E:
+        n = int(torch.randint(1, 5, (1,), generator=g))
+        aim[order[at:at + n]] = value
+        at, value = at + n, value - 0.01
+    bias = (aim - s).float()
+    c = s[None] * 0 + (torch.sigmoid(x.double()) if scoring == "sigmoid" else torch.softmax(x.double(), 1)) + bias.double()
+    gaps = c.sort(1, descending=True).values.diff(dim=1).abs()
+    assert ((gaps > 0) & (gaps < 1e-7)).any(1).float().mean() > 0.9 and not ((gaps > 0) & (gaps < 1e-13)).any()
+    check_route(x.to(cuda), 8, scoring, bias.to(cuda), groups, top_groups, score)
+    check_route(x[:5].to(cuda), 8, scoring, bias.to(cuda), groups, top_groups, score)
+
+
 def test_route_masks(cuda):
     """-inf is never chosen, the type's lowest value is a value; a row without experts goes nowhere."""
     for dtype in (torch.float32, torch.bfloat16, torch.float16):
