@@ -15,11 +15,6 @@ from .quantize import _apart, _as_rows
 _SAME, _I8_TOKEN, _FP8_TOKEN, _FP8_GROUP = range(4)
 
 
-def _silu_mul(x, out):
-    y = host().silu_mul(x, out)
-    return _silu_mul_general(x, out) if y is None else y
-
-
 @torch.no_grad()
 def _silu_mul_general(x, out):
     if x.dim() < 1 or x.shape[-1] % 16:
@@ -44,19 +39,23 @@ def _silu_mul_general(x, out):
 
 def silu_mul(x: torch.Tensor) -> torch.Tensor:
     """silu(x[.., :N]) * x[.., N:], rounded once to x's type: -> [.., N]."""
-    return _silu_mul(x, _SAME)
+    y = host().silu_mul(x, _SAME)
+    return _silu_mul_general(x, _SAME) if y is None else y
 
 
 def silu_mul_quantize_activation_per_token_absmax(x: torch.Tensor):
     """silu_mul quantized to int8 per token, as it is in fp32: -> (int8 [.., N], fp32 scales [.., 1]).  scale = max(absmax, 1e-5) / 127."""
-    return _silu_mul(x, _I8_TOKEN)
+    y = host().silu_mul(x, _I8_TOKEN)
+    return _silu_mul_general(x, _I8_TOKEN) if y is None else y
 
 
 def silu_mul_per_token_quantize(x: torch.Tensor):
     """silu_mul quantized to e4m3fn per token: -> (codes [.., N], fp32 scales [.., 1]).  scale = max(absmax, 1e-12) / 448."""
-    return _silu_mul(x, _FP8_TOKEN)
+    y = host().silu_mul(x, _FP8_TOKEN)
+    return _silu_mul_general(x, _FP8_TOKEN) if y is None else y
 
 
 def silu_mul_per_group_quantize(x: torch.Tensor):
     """silu_mul quantized to e4m3fn per token and 128 channels, for a block-scaled Linear: -> (codes [.., N], fp32 scales [.., ceil(N / 128)])."""
-    return _silu_mul(x, _FP8_GROUP)
+    y = host().silu_mul(x, _FP8_GROUP)
+    return _silu_mul_general(x, _FP8_GROUP) if y is None else y

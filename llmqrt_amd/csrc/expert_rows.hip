@@ -17,7 +17,7 @@ namespace {
 
 enum { OUT_SAME = LLMQ_NORM_SAME, OUT_I8 = LLMQ_NORM_I8_TOKEN, OUT_GROUP = LLMQ_NORM_FP8_GROUP };
 constexpr int kMaxTop = 64, kMaxExperts = 4096;
-constexpr int64_t kCountAll = 2048;  // up to so many ids every token counts all of them for itself
+constexpr int kCountAll = 4096, kIndexBits = 12;  // up to so many ids every token may count all of them for itself
 
 struct DispatchArgs {
     const uint16_t* x;
@@ -186,31 +186,54 @@ __global__ __launch_bounds__(NT) void dispatch_kernel(DispatchArgs a) {
         }
     }
 
-    if constexpr (ALL) {  // JW copies per wavefront and pass over the ids
-        __shared__ int32_t place[kMaxTop];
-        for (int j0 = wave * JW; j0 < a.top; j0 += NW * JW) {
-            uint32_t e[JW];
+    if constexpr (ALL) {
+        // Expert and index in one key: a copy's place is how many keys are below its own (an id that goes nowhere is above all).  The wavefronts share JW copies
+        // each and, where there are more wavefronts than that, parts of the ids.
+        static_assert((int64_t)kMaxExperts << kIndexBits < 0xffffffffLL && kCountAll <= 1 << kIndexBits, "keys");
+        __shared__ int32_t part[NW][kMaxTop];
+        auto key = [&](int32_t id, int i) __attribute__((always_inline)) {
+            return min((uint32_t)id - (uint32_t)a.first, (uint32_t)a.experts) << kIndexBits | (uint32_t)i;
+        };
+        const bool fours = (reinterpret_cast<uintptr_t>(a.ids) & 15u) == 0 && a.ids_total % 4 == 0;  // uniform
+        const bool here = lane < a.top && key(a.ids[mine + min(lane, a.top - 1)], 0) >> kIndexBits < (uint32_t)a.experts;
+        const int share = a.top <= JW ? 0 : a.top <= 2 * JW ? 1 : 31 - __builtin_clz(NW);  // 2^share wavefronts have different copies
+        const int parts = NW >> share, mine_of = wave >> share;
+        for (int j0 = (wave & ((1 << share) - 1)) * JW; j0 < a.top; j0 += JW << share) {
+            uint32_t k0[JW];
             int n[JW];
 #pragma unroll
             for (int k = 0; k < JW; k++) {
-                e[k] = j0 + k < a.top ? expert_of(a.ids, mine + j0 + k, a.first) : ~0u;
+                k0[k] = j0 + k < a.top ? key(a.ids[mine + j0 + k], mine + j0 + k) : 0;
                 n[k] = 0;
             }
-#pragma unroll 4
-            for (int i = lane; i < a.ids_total; i += kWave) {
-                const uint32_t id = expert_of(a.ids, i, a.first);
+            auto count = [&](uint32_t id) __attribute__((always_inline)) {
 #pragma unroll
-                for (int k = 0; k < JW; k++) n[k] += id < e[k] || (id == e[k] && i < mine + j0 + k);
+                for (int k = 0; k < JW; k++) n[k] += id < k0[k];
+            };
+            if (fours) {
+#pragma unroll 4
+                for (int i = (mine_of * kWave + lane) * 4; i < a.ids_total; i += parts * kWave * 4) {
+                    const int4 v = *reinterpret_cast<const int4*>(a.ids + i);
+                    count(key(v.x, i)), count(key(v.y, i + 1)), count(key(v.z, i + 2)), count(key(v.w, i + 3));
+                }
+            } else {
+#pragma unroll 4
+                for (int i = mine_of * kWave + lane; i < a.ids_total; i += parts * kWave) count(key(a.ids[i], i));
             }
 #pragma unroll
             for (int k = 0; k < JW; k++) {
                 if (j0 + k >= a.top) break;
-                const int p = e[k] < (uint32_t)a.experts ? wave_total(n[k]) : -1;
-                if (lane == 0) place[j0 + k] = p, a.places[mine + j0 + k] = p;
+                const int total = wave_total(n[k]);
+                if (lane == 0) part[mine_of][j0 + k] = total;
             }
         }
         __syncthreads();
-        goes_to = lane < a.top ? place[lane] : -1;
+        if (here) {
+            goes_to = 0;
+#pragma unroll
+            for (int w = 0; w < NW; w++) goes_to += w < parts ? part[w][lane] : 0;
+        }
+        if (wave == 0 && lane < a.top) a.places[mine + lane] = goes_to;
     }
     auto each_copy = [&](auto&& f) __attribute__((always_inline)) {  // f(place)
         for (int j = 0; j < a.top; j++) {
@@ -412,7 +435,9 @@ extern "C" int llmq_dispatch_experts(int out, const void* x, int x_dtype, int64_
     a.ldx = ldx, a.K = K, a.ids_total = (int)(tokens * top_k), a.top = (int)top_k, a.first = (int)first_expert, a.experts = (int)experts;
     a.wide = K % 16 == 0 && aligned16(rows);
     const hipStream_t st = (hipStream_t)stream;
-    const bool all = tokens * top_k <= kCountAll;
+    // every token counts all ids, or one launch more finds the places: us, counted / found (rows of 3584 int8) 512 tokens of 4 5.6 / 8.2, 1024 of 4 7.5 / 8.8, 2000 of
+    // 4 14 / 9.6
+    const bool all = tokens * top_k <= kCountAll && tokens * tokens * top_k <= 1 << 22;
     if (!all) {
         if (aligned16(ids)) hipLaunchKernelGGL((expert_places_kernel<4>), dim3((unsigned)experts), dim3(1024), 0, st, ids, a.ids_total, a.first, a.experts, places, offsets);
         else hipLaunchKernelGGL((expert_places_kernel<1>), dim3((unsigned)experts), dim3(1024), 0, st, ids, a.ids_total, a.first, a.experts, places, offsets);

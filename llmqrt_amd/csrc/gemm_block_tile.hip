@@ -7,6 +7,7 @@
 // channels, and its factor sa sw is one register for all channel tiles of the token.
 #include <type_traits>
 
+#include "expert_tiles.h"
 #include "gemm_block.h"
 
 namespace llmq {
@@ -14,8 +15,6 @@ namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
-
-constexpr int kNumXcd = 8, kGroupM = 8;
 
 template <int B, int E, class F>
 __device__ __forceinline__ void unrolled(F&& f) {
@@ -44,34 +43,6 @@ struct TileCfg {
 
 // LDS place of 16-byte chunk c of row r: 16 rows of one chunk fall on 16 places
 __device__ __forceinline__ int chunk_at(int r, int c) { return (r * 8 + (c ^ ((r >> 1) & 7))) * 16; }
-
-// sum over lanes 0 .. lane, in registers (us, by lane shuffles through LDS / so: 256 rows of 64 experts 45.5 / 45.0, 700 of 90 8.2 / 7.5)
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int plus_lanes(int v) {  // of the rows of 16 lanes in ROWS; where there is none, plus zero
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int wave_prefix(int v) {
-    v = plus_lanes<0x111, 0xf>(v);  // the lane before, in a row of 16
-    v = plus_lanes<0x112, 0xf>(v);
-    v = plus_lanes<0x114, 0xf>(v);
-    v = plus_lanes<0x118, 0xf>(v);
-    v = plus_lanes<0x142, 0xa>(v);  // rows 1 and 3: the last lane of the row before
-    return plus_lanes<0x143, 0xc>(v);  // rows 2 and 3: lane 31
-}
-
-// flat block id -> place in the order of tiles: a contiguous range per XCD
-__device__ __forceinline__ int place_of(int bid, int nblk) {
-    const int q = nblk / kNumXcd, r = nblk % kNumXcd, xcd = bid % kNumXcd, local = bid / kNumXcd;
-    return xcd < r ? xcd * (q + 1) + local : r * (q + 1) + (xcd - r) * q + local;
-}
-// place in one matrix's order -> (tile of rows, tile of channels): groups of kGroupM tiles of rows, each of which starts its walk over the weights at
-// another place, so that the XCDs do not all wait for the same weights from HBM (us, all from the first channel / so: 8192 x 37888 x 3584 1008 / 988,
-// on 128 x 256 tiles 1175 / 1097, 8192 x 4608 x 3584 157 / 146)
-__device__ __forceinline__ void tile_of(int pid, int tiles_m, int tiles_n, int& tm, int& tn) {
-    const int width = kGroupM * tiles_n, group = pid / width, first = group * kGroupM, size = min(tiles_m - first, kGroupM);
-    tm = first + (pid % width) % size;
-    tn = (pid % width / size + group * tiles_n / ((tiles_m + kGroupM - 1) / kGroupM)) % tiles_n;
-}
 
 // TAIL: K, or a split's share of it, is not made of whole blocks for every group
 template <class C, bool GROUPED, bool SPLIT, bool TAIL>
@@ -152,7 +123,7 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     // The walk over K starts at an eighth that follows from the tile of channels and wraps around: the XCDs work on different channels, and so do not
     // all ask for the same part of the rows at once, which lie the same distance apart and fall on few memory channels (us, from 0 / so: 777 x 3584 x
     // 18944 on 128 x 256 tiles 130 / 115, in two splits 82 / 76).  A channel's sums have one order for every token of a call.
-    int ld_kb = kb0 + group + tn * kNumXcd / tiles_n * kfull / kNumXcd * KS;
+    int ld_kb = kb0 + group + tn * kExpertXcd / tiles_n * kfull / kExpertXcd * KS;
     // What the groups' whole blocks leave of this split comes last: at most a block for each group, one of them ragged.  Its missing chunks are read as
     // the block's first one (a group without a block: of any), and zeros take their place in the weights' operand; what the tokens have there belongs to the
     // same row, so where it is NaN the result is too.  A group without a block multiplies nothing: the scales that it read may be infinite.

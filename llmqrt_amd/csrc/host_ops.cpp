@@ -677,13 +677,17 @@ std::optional<Sorted> dispatch(const Tensor& x, const Tensor& ids, int64_t exper
     const at::Device dev = x.device();
     const Launch l(dev);
     Tensor rows, scale, offsets, places;
-    Outputs o(dev);
+    Outputs small(dev);
     const bool same = out == LLMQ_NORM_SAME;
-    o.add(&rows, {n, r.K}, same ? x.scalar_type() : out == LLMQ_NORM_I8_TOKEN ? at::kChar : at::kFloat8_e4m3fn);
-    if (!same) o.add(&scale, {n, out == LLMQ_NORM_FP8_GROUP ? blocks128(r.K) : 1}, at::kFloat);
-    o.add(&offsets, {experts + 1}, at::kInt);
-    o.add(&places, ids.sizes(), at::kInt);
-    o.make_all();
+    const at::ScalarType dt = same ? x.scalar_type() : out == LLMQ_NORM_I8_TOKEN ? at::kChar : at::kFloat8_e4m3fn;
+    // rows too large for one allocation with the others have one of their own, so that those still share one
+    const bool apart = n * r.K > 32 * 1024;
+    if (apart) rows = make({n, r.K}, dt, dev);
+    else small.add(&rows, {n, r.K}, dt);
+    if (!same) small.add(&scale, {n, out == LLMQ_NORM_FP8_GROUP ? blocks128(r.K) : 1}, at::kFloat);
+    small.add(&offsets, {experts + 1}, at::kInt);
+    small.add(&places, ids.sizes(), at::kInt);
+    small.make_all();
     const int rc = llmq_dispatch_experts(out, x.data_ptr(), code(x.scalar_type()), r.M, r.K, r.K, (const int32_t*)ids.data_ptr(), top, first, experts,
                                          rows.data_ptr(), same ? nullptr : (float*)scale.data_ptr(), (int32_t*)offsets.data_ptr(),
                                          (int32_t*)places.data_ptr(), l.stream);

@@ -80,11 +80,6 @@ def _route_general(logits, top_k, scoring, bias, num_groups, top_groups, group_s
 _SAME, _I8_TOKEN, _FP8_GROUP = 0, 1, 3
 
 
-def _dispatch(x, experts, num_experts, first_expert, out):
-    y = host().dispatch(x, experts, num_experts, first_expert, out)
-    return _dispatch_general(x, experts, num_experts, first_expert, out) if y is None else y
-
-
 @torch.no_grad()
 def _dispatch_general(x, experts, num_experts, first_expert, out):
     what = "dispatch to experts"
@@ -127,19 +122,22 @@ def dispatch_to_experts(x: torch.Tensor, experts: torch.Tensor, num_experts: int
     ``x`` [.., K] in bf16 or fp16; ``experts`` int32 or int64 [.., top_k], counted from ``first_expert`` (of a GPU that holds a part of the experts); ids outside
     its ``num_experts`` go nowhere.  Rows offsets[e] .. offsets[e + 1] - 1 belong to expert e; those from offsets[num_experts] on are not written.
     ``places`` says where a token's copies are (-1: nowhere), for ``combine_from_experts``."""
-    return _dispatch(x, experts, num_experts, first_expert, _SAME)
+    y = host().dispatch(x, experts, num_experts, first_expert, _SAME)
+    return _dispatch_general(x, experts, num_experts, first_expert, _SAME) if y is None else y
 
 
 def dispatch_quantize_activation_per_token_absmax(x: torch.Tensor, experts: torch.Tensor, num_experts: int, first_expert: int = 0):
     """dispatch_to_experts with rows in int8, the bits of ``quantize.quantize_activation_per_token_absmax_f32``, quantized once per token:
     -> (int8 rows, fp32 scales [rows, 1], offsets, places)."""
-    return _dispatch(x, experts, num_experts, first_expert, _I8_TOKEN)
+    y = host().dispatch(x, experts, num_experts, first_expert, _I8_TOKEN)
+    return _dispatch_general(x, experts, num_experts, first_expert, _I8_TOKEN) if y is None else y
 
 
 def dispatch_per_group_quantize(x: torch.Tensor, experts: torch.Tensor, num_experts: int, first_expert: int = 0):
     """dispatch_to_experts with rows in e4m3fn, the bits of ``quantize.per_group_quantize``, quantized once per token:
     -> (codes, fp32 scales [rows, ceil(K / 128)], offsets, places)."""
-    return _dispatch(x, experts, num_experts, first_expert, _FP8_GROUP)
+    y = host().dispatch(x, experts, num_experts, first_expert, _FP8_GROUP)
+    return _dispatch_general(x, experts, num_experts, first_expert, _FP8_GROUP) if y is None else y
 
 
 def combine_from_experts(y: torch.Tensor, places: torch.Tensor, weights: torch.Tensor, shared: torch.Tensor | None = None) -> torch.Tensor:
