@@ -8,10 +8,11 @@
 // Which experts are chosen has to follow from the scores, not from how they were rounded: without a bias the order of c is that of the logits, which are
 // compared as they are; with one, and where two scores of a group are added, scores are formed and compared in 64 bits.
 //
-// Most tokens take the short form: 16 lanes share a token, at most V neighbouring experts of one group each, in registers, with the scores in 32 bits.  A
-// choice is a maximum over a lane's experts and over the 16 lanes (row rotations, no LDS) and the lowest expert that has it.  Its order is that of the exact
-// scores wherever neighbours in it lie further apart than both scores can be off; a token with two closer ones is done over with scores in 64 bits.  Bound by
-// the vector unit: about 90 instructions for a choice of 4 tokens from 256 experts each.
+// Most tokens take the short form: 16, 32 or 64 lanes share a token, at most V neighbouring experts of one group each, in registers, with the scores in 32 bits.
+// A choice is a maximum over a lane's experts and over the lanes (row rotations and swaps, no LDS) and the lowest expert that has it.  Its order is that of the
+// exact scores wherever neighbours in it lie further apart than both scores can be off.  Two closer sigmoid scores are compared in 64 bits by themselves; a token
+// with more of them, with close groups, or with close scores of a softmax is done over with all scores in 64 bits.
+// Many tokens are bound by the vector unit (8192 of 256 experts, 8 chosen: 7 us, with a bias 12), a few by the chain of choices (16 of them: 4 and 5 us).
 // More than 256 experts, 16 groups or 16 choices, and tokens with a NaN, take the long form.
 #include <algorithm>
 #include <type_traits>
@@ -317,7 +318,10 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
                 double all = 0.0;
 #pragma unroll
                 for (int v = 0; v < V; v++) c[v] = exp((double)x[v] - (double)m), all += c[v];
-                all = token_sum<LPT>(all), sum = (float)all;
+                // (lanes add in orders of their own; equal scores need one sum)
+                static_assert(LPT == kWave, "one token");
+                all = by_halves(token_sum<LPT>(all), [](uint32_t u) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)u); });
+                sum = (float)all;
                 const double r = 1.0 / all;
 #pragma unroll
                 for (int v = 0; v < V; v++) c[v] *= r;
@@ -337,7 +341,7 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
 #pragma unroll
             for (int v = 0; v < V; v++) c[v] *= r;
             // in 2^-24 of the largest score, which is r: exp takes 2.5 d + 2 with d = m - x, of which less than 3 remain behind exp(-d); the sum's share of that
-            // is at most 2.5 ln 256 + 2 < 16, which all scores have in common but the bias does not; V + 4 additions, the reciprocal 2 and the product 1
+            // is at most 2.5 ln 256 + 2 < 16, which all scores have in common but the bias does not; V + 6 additions, the reciprocal 2 and the product 1
             off = (V + 32) * 0x1p-24f * r;
         }
         score_t best = kNone, second = kNone;
@@ -426,7 +430,8 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
     int id = -1, last = -1;
     float before = __builtin_inff();
     bool near_last = false;  // the last two choices were close
-    for (int j = 0; j < a.top + (BY == BY_SCORES_32 ? 1 : 0); j++) {
+    // (one choice more shows whether the last one is close to what is left, and if so one further whether those are two)
+    for (int j = 0, rounds = a.top + (BY == BY_SCORES_32 ? 1 : 0); j < rounds; j++) {
         key_t best = key[0];
 #pragma unroll
         for (int v = 1; v < V; v++) best = larger(best, key[v]);
@@ -444,9 +449,10 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
             const bool close = j > 0 && best != 0 && !(before - c > 2 * off + 0x1p-24f * (fabsf(before) + fabsf(c)));
             before = c;
             if (__any(close && sure)) {
+                if (j == a.top) rounds++;
                 // Two close sigmoid scores are compared in 64 bits by themselves; three, and those of a softmax, whose sum takes part, are not.
-                if (!a.sigmoid || near_last) sure = sure && !close;
-                if (close && sure) {
+                if (near_last || (!a.sigmoid && j <= a.top)) sure = sure && !close;
+                if (close && sure && j <= a.top) {
                     auto score = [&](int e) __attribute__((always_inline)) {
                         return 1.0 / (1.0 + exp(-(double)load_as_f32(a.logits, DT, t * a.ld + e))) + (a.bias ? (double)a.bias[e] : 0.0);
                     };
@@ -459,7 +465,7 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
             }
             near_last = close;
             last = chosen;
-            if (j == a.top) break;
+            if (j >= a.top) continue;
         }
         if (l == j) id = best != kNoKey ? chosen : -1;
     }

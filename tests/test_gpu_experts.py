@@ -140,6 +140,22 @@ def test_route_close_scores(cuda, E, groups, top_groups, score, scoring):
     check_route(x[:5].to(cuda), 8, scoring, bias.to(cuda), groups, top_groups, score)
 
 
+@pytest.mark.parametrize("E,groups,top_groups,score", [(4, 1, 1, "max"), (64, 1, 1, "max"), (128, 1, 1, "max"), (256, 1, 1, "max"), (64, 4, 4, "top2"), (256, 8, 8, "max")])
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("T", [5, 3500])
+def test_route_close_scores_at_the_last_choice(cuda, E, groups, top_groups, score, scoring, T):
+    """The last choice lies among two, three or four scores that 32 bits do not tell apart, some of them not chosen."""
+    g = torch.Generator().manual_seed(E + T)
+    near = 8.0 if scoring == "sigmoid" else 0.0  # sigmoids near 1, or shares of a softmax near each other
+    for top in (1, 2, 3):
+        x = torch.randn(T, E, generator=g) - 12
+        for t in range(T):
+            at = torch.randperm(E, generator=g)[:4]
+            few = 2 + t % 3 if E > 4 else 4
+            x[t, at[:few]] = near + torch.randint(-6, 7, (few,), generator=g) * 2.0 ** -20
+        check_route(x.to(cuda), min(top, E), scoring, torch.zeros(E, device=cuda), groups, top_groups, score)
+
+
 def test_route_masks(cuda):
     """-inf is never chosen, the type's lowest value is a value; a row without experts goes nowhere."""
     for dtype in (torch.float32, torch.bfloat16, torch.float16):
