@@ -44,7 +44,7 @@ int launch_grouped(const GroupedCall& g, hipStream_t st) {
     return launch_status();
 }
 
-thread_local int forced = -1;
+thread_local int forced = -1;  // llmq_gemm_w8a8_grouped_force_plan
 
 // What a launch takes, in us, as a rule of the sizes alone; the host knows the rows of all experts together, not each one's, and takes every expert that may
 // have rows to end with about half a tile:

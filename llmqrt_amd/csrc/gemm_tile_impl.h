@@ -413,60 +413,60 @@ __global__ __launch_bounds__(C::NT) void gemm_tile_kernel(
         };
         // WORK: the wavefront has rows and channels; otherwise it loads its pieces and waits with the others, and multiplies nothing
         auto all_tiles = [&](auto work_c) __attribute__((always_inline)) {
-        constexpr bool WORK = decltype(work_c)::value;
-        unrolled<0, NS - 1>([&](auto t_c) __attribute__((always_inline)) {
-            constexpr int t = decltype(t_c)::value;
-            if (t < kall) {
-                if (TAIL && t == kall - 1) last_kt();
-                unrolled<0, LPT>([&](auto d) __attribute__((always_inline)) { issue(t, d); });
-                next_kt();
-            }
-        });
-        wait_next_tile(min(kall, NS - 1) - 1);
-        lds_barrier();
-        if constexpr (WORK) read_frags(0, 0, fa[0], fb[0]);
-        // the stage NS - 1 is free from the start: the part of its tile that the loop requests behind a barrier comes first
-        if (NS - 1 < kall) {
-            if (TAIL && NS == kall) last_kt();
-            unrolled<0, (STEP < LPT ? STEP : LPT)>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
-        }
-        int stage = 0, kt = 0;
-        // rest: the part of tile kt + NS - 1 that the last iteration did not request; first: tile kt + NS exists; last: it is the last one; mask: tile kt is
-        // ragged
-        auto k_tile = [&](auto rest_c, auto first_c, auto last_c, auto mask_c) __attribute__((always_inline)) {
-            const int prev = stage == 0 ? NS - 1 : stage - 1, next = stage == NS - 1 ? 0 : stage + 1;
-            constexpr int MASK = decltype(mask_c)::value;
-            unrolled<0, C::KSUB - 1>([&](auto ks_c) __attribute__((always_inline)) {
-                constexpr int ks = decltype(ks_c)::value;
-                sub_step(work_c, std::integral_constant<int, MASK ? 1 + ks : 0>{}, stage, ks + 1, std::integral_constant<int, ks & 1>{},
-                         std::integral_constant<int, (ks + 1) * STEP>{}, rest_c, prev);
+            constexpr bool WORK = decltype(work_c)::value;
+            unrolled<0, NS - 1>([&](auto t_c) __attribute__((always_inline)) {
+                constexpr int t = decltype(t_c)::value;
+                if (t < kall) {
+                    if (TAIL && t == kall - 1) last_kt();
+                    unrolled<0, LPT>([&](auto d) __attribute__((always_inline)) { issue(t, d); });
+                    next_kt();
+                }
             });
-            if constexpr (decltype(rest_c)::value) {
-                next_kt();
-                if constexpr (decltype(last_c)::value) last_kt();
-                wait_next_tile(NS - 2);
-            } else {
-                wait_next_tile(kall - 2 - kt);  // tile kt+1 has landed
-            }
+            wait_next_tile(min(kall, NS - 1) - 1);
             lds_barrier();
-            // every wavefront has read the whole of stage kt: it takes tile kt + NS
-            sub_step(work_c, std::integral_constant<int, MASK ? C::KSUB : 0>{}, next, 0, std::integral_constant<int, (C::KSUB - 1) & 1>{},
-                     std::integral_constant<int, 0>{}, first_c, stage);
-            stage = next;
-            kt++;
-        };
-        const std::true_type yes;
-        const std::false_type no;
+            if constexpr (WORK) read_frags(0, 0, fa[0], fb[0]);
+            // the stage NS - 1 is free from the start: the part of its tile that the loop requests behind a barrier comes first
+            if (NS - 1 < kall) {
+                if (TAIL && NS == kall) last_kt();
+                unrolled<0, (STEP < LPT ? STEP : LPT)>([&](auto d) __attribute__((always_inline)) { issue(NS - 1, d); });
+            }
+            int stage = 0, kt = 0;
+            // rest: the part of tile kt + NS - 1 that the last iteration did not request; first: tile kt + NS exists; last: it is the last one; mask: tile kt is
+            // ragged
+            auto k_tile = [&](auto rest_c, auto first_c, auto last_c, auto mask_c) __attribute__((always_inline)) {
+                const int prev = stage == 0 ? NS - 1 : stage - 1, next = stage == NS - 1 ? 0 : stage + 1;
+                constexpr int MASK = decltype(mask_c)::value;
+                unrolled<0, C::KSUB - 1>([&](auto ks_c) __attribute__((always_inline)) {
+                    constexpr int ks = decltype(ks_c)::value;
+                    sub_step(work_c, std::integral_constant<int, MASK ? 1 + ks : 0>{}, stage, ks + 1, std::integral_constant<int, ks & 1>{},
+                             std::integral_constant<int, (ks + 1) * STEP>{}, rest_c, prev);
+                });
+                if constexpr (decltype(rest_c)::value) {
+                    next_kt();
+                    if constexpr (decltype(last_c)::value) last_kt();
+                    wait_next_tile(NS - 2);
+                } else {
+                    wait_next_tile(kall - 2 - kt);  // tile kt+1 has landed
+                }
+                lds_barrier();
+                // every wavefront has read the whole of stage kt: it takes tile kt + NS
+                sub_step(work_c, std::integral_constant<int, MASK ? C::KSUB : 0>{}, next, 0, std::integral_constant<int, (C::KSUB - 1) & 1>{},
+                         std::integral_constant<int, 0>{}, first_c, stage);
+                stage = next;
+                kt++;
+            };
+            const std::true_type yes;
+            const std::false_type no;
 #pragma unroll 1
-        while (kt < kall - NS - (TAIL ? 1 : 0)) k_tile(yes, yes, no, no);
-        if constexpr (TAIL) {
-            if (kt < kall - NS) k_tile(yes, yes, yes, no);
-        }
-        if (kt == kall - NS) k_tile(yes, no, no, no);
-        // Past the last request nothing is fetched: a block that ends waits for no load that nobody reads.
+            while (kt < kall - NS - (TAIL ? 1 : 0)) k_tile(yes, yes, no, no);
+            if constexpr (TAIL) {
+                if (kt < kall - NS) k_tile(yes, yes, yes, no);
+            }
+            if (kt == kall - NS) k_tile(yes, no, no, no);
+            // Past the last request nothing is fetched: a block that ends waits for no load that nobody reads.
 #pragma unroll 1
-        while (kt < kall - (TAIL ? 1 : 0)) k_tile(no, no, no, no);
-        if constexpr (TAIL) k_tile(no, no, no, yes);
+            while (kt < kall - (TAIL ? 1 : 0)) k_tile(no, no, no, no);
+            if constexpr (TAIL) k_tile(no, no, no, yes);
         };
         bool idle = false;  // wavefront-uniform
         if constexpr (GROUPED) idle = m0 + __builtin_amdgcn_readfirstlane(wm) * C::WTM >= M || n0 + __builtin_amdgcn_readfirstlane(wn) * C::WTN >= N;

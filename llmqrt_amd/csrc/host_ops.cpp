@@ -670,7 +670,7 @@ struct Sorted {
 std::optional<Sorted> dispatch(const Tensor& x, const Tensor& ids, int64_t experts, int64_t first, int out) {
     const Rows r = rows_of(x);
     if (!r.ok || !is16(x.scalar_type()) || r.K % 8 || !ids.defined() || ids.scalar_type() != at::kInt || ids.dim() != x.dim() || !plain_on(ids, x.device()) ||
-        ids.sizes().slice(0, ids.dim() - 1) != x.sizes().slice(0, x.dim() - 1) || experts < 1 || experts > 4096 || ids.numel() > 0x7fffff00LL)
+        ids.sizes().slice(0, ids.dim() - 1) != x.sizes().slice(0, x.dim() - 1) || experts < 1 || experts > 4096 || ids.numel() > 0x7fff0000LL)
         return std::nullopt;
     const int64_t top = ids.size(-1), n = r.M * top;
     if (top < 1 || top > 64) return std::nullopt;
@@ -703,7 +703,7 @@ std::optional<Tensor> combine(const Tensor& y, const Tensor& places, const Tenso
     const Rows r = rows_of(y);
     if (!r.ok || y.dim() != 2 || !is16(y.scalar_type()) || r.K % 8) return std::nullopt;
     const at::Device dev = y.device();
-    if (!places.defined() || places.scalar_type() != at::kInt || places.dim() < 1 || places.numel() == 0 || places.numel() > 0x7fffff00LL ||
+    if (!places.defined() || places.scalar_type() != at::kInt || places.dim() < 1 || places.numel() == 0 || places.numel() > 0x7fff0000LL ||
         !plain_on(places, dev) || !weights.defined() || weights.scalar_type() != at::kFloat || weights.sizes() != places.sizes() || !plain_on(weights, dev))
         return std::nullopt;
     const at::DimVector size = out_size(places, r.K);

@@ -3,7 +3,8 @@
 //   y[m, k] = g / (1 + exp(-g)) * u,   g = x[m, k], u = x[m, N + k]
 //   and y rounded once to x_dtype, or quantized:  int8 s = max(max_k |y|, 1e-5) / 127,  q = rint(y / s)
 //                                                 e4m3 s = max(max |y|, 1e-12) / 448, per token or per token and group of 128 channels
-// Everything between x and the codes is fp32.  HBM-bound: 4 bytes read and 1 or 2 written per output.
+// Everything between x and the codes is fp32.  HBM-bound: 4 bytes read and 1 or 2 written per output; a few rows are a launch and a chain of latencies (37 x 18944
+// int8 4.9 us: two loads, the formula, a maximum over 16 wavefronts, the codes).
 #include <algorithm>
 
 #include "llmq_common.h"
@@ -35,42 +36,30 @@ __device__ __forceinline__ void gated8(uint4 gv, uint4 uv, float* y) {
     for (int i = 0; i < 8; i++) y[i] = silu(g[i]) * u[i];
 }
 
-// No reduction over the whole row: 16 lanes take 128 channels of a row, U such pieces in flight per lane.
-template <int DT, bool GROUP, int U>
+// No reduction over the whole row: 16 lanes take 128 channels of a row, 8 of each half a lane.  One such piece per lane, and many blocks: with two or four
+// in flight per lane, 8192 x 18944 takes 144 and 154 us by groups where one takes 134 (5.8 TB/s), 37 x 18944 3.1 and 4.4 where 2.7.
+template <int DT, bool GROUP>
 __global__ __launch_bounds__(kSiluThreads) void silu_groups_kernel(SiluArgs a, uint32_t groups, uint32_t total) {
-    constexpr int TEAMS = kSiluThreads / kTeam;
     const int l = threadIdx.x % kTeam;
-    const uint32_t g0 = blockIdx.x * (TEAMS * U) + threadIdx.x / kTeam;
-    uint4 gv[U], uv[U];
-    int64_t to[U];  // first element of the lane's chunk in the output; < 0: none
-    uint32_t row = g0 / groups, col = g0 - row * groups;
-    const uint32_t step_rows = TEAMS / groups, step_cols = TEAMS - step_rows * groups;
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int64_t k = (int64_t)col * 128 + l * 8;
-        const bool in = g0 + u * TEAMS < total && k < a.N;
-        const uint16_t* xr = a.x + (int64_t)row * a.ldx + k;
-        to[u] = in ? (int64_t)row * a.N + k : -1;
-        gv[u] = in ? *reinterpret_cast<const uint4*>(xr) : make_uint4(0, 0, 0, 0);
-        uv[u] = in ? *reinterpret_cast<const uint4*>(xr + a.N) : make_uint4(0, 0, 0, 0);
-        row += step_rows, col += step_cols;
-        if (col >= groups) col -= groups, row++;
+    const uint32_t g = blockIdx.x * (kSiluThreads / kTeam) + threadIdx.x / kTeam, row = g / groups;
+    const int64_t k = (int64_t)(g - row * groups) * 128 + l * 8;
+    const bool in = g < total && k < a.N;
+    const uint16_t* xr = a.x + (int64_t)row * a.ldx + k;
+    const uint4 gv = in ? *reinterpret_cast<const uint4*>(xr) : make_uint4(0, 0, 0, 0);
+    const uint4 uv = in ? *reinterpret_cast<const uint4*>(xr + a.N) : make_uint4(0, 0, 0, 0);
+    const int64_t to = (int64_t)row * a.N + k;
+    float y[8];
+    gated8<DT>(gv, uv, y);
+    if (!GROUP) {
+        if (in) *reinterpret_cast<uint4*>(a.y + to) = narrow8<DT>(y);
+        return;
     }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        float y[8];
-        gated8<DT>(gv[u], uv[u], y);
-        if (!GROUP) {
-            if (to[u] >= 0) *reinterpret_cast<uint4*>(a.y + to[u]) = narrow8<DT>(y);
-            continue;
-        }
-        const float amax = team_max(absmax8f(y)), s = scale32<MODE_F8>(amax), inv_s = 1.0f / s;
-        uint2 c;
-        if (__all(near_ok(amax, s))) c = codes8<MODE_F8, true>(y, s, inv_s);
-        else c = codes8<MODE_F8, false>(y, s, inv_s);
-        if (to[u] >= 0) *reinterpret_cast<uint2*>(a.q + to[u]) = c;
-        if (l == 0 && g0 + u * TEAMS < total) a.scale[g0 + u * TEAMS] = s;
-    }
+    const float amax = team_max(absmax8f(y)), s = scale32<MODE_F8>(amax), inv_s = 1.0f / s;
+    uint2 c;
+    if (__all(near_ok(amax, s))) c = codes8<MODE_F8, true>(y, s, inv_s);
+    else c = codes8<MODE_F8, false>(y, s, inv_s);
+    if (in) *reinterpret_cast<uint2*>(a.q + to) = c;
+    if (l == 0 && g < total) a.scale[g] = s;
 }
 
 // A scale per row.  NT threads per row, RPB rows per block (more than one: a wavefront each, and no barrier).  NC > 0: a row's outputs stay in 8 NC
@@ -128,29 +117,27 @@ template <int DT, bool GROUP>
 int launch_groups(const SiluArgs& a, hipStream_t st) {
     constexpr int TEAMS = kSiluThreads / kTeam;
     const uint32_t groups = (uint32_t)((a.N + 127) / 128), total = (uint32_t)(a.M * groups);
-    if (total >= 256 * TEAMS * 8)
-        hipLaunchKernelGGL((silu_groups_kernel<DT, GROUP, 2>), dim3((total + TEAMS * 2 - 1) / (TEAMS * 2)), dim3(kSiluThreads), 0, st, a, groups, total);
-    else
-        hipLaunchKernelGGL((silu_groups_kernel<DT, GROUP, 1>), dim3((total + TEAMS - 1) / TEAMS), dim3(kSiluThreads), 0, st, a, groups, total);
+    hipLaunchKernelGGL((silu_groups_kernel<DT, GROUP>), dim3((total + TEAMS - 1) / TEAMS), dim3(kSiluThreads), 0, st, a, groups, total);
     return launch_status();
 }
 
-// Threads per row and chunks per thread as for the norm with an 8-bit output (quant_groups.hip): a few rows are a chain of latencies, many are bytes.
+// Two chunks per thread until a row takes 1024 of them: fewer threads per row mean less to wait for between the maximum and the codes, fewer chunks more wavefronts that
+// hide it.  8192 rows in int8, us, threads x chunks: 1024 channels 64 x 2 (four rows to a block) 9.2, 128 x 1 11.9, 256 x 1 14.4; 2048 128 x 2 17.0, 64 x 4 17.8, 256 x 1
+// 20.7; 3584 256 x 2 28.0, 512 x 1 34.1; 8192 512 x 2 62.9, 1024 x 1 73.7, 256 x 4 64.1; 13696 1024 x 2 96, 512 x 4 105; 18944 1024 x 3 136, 512 x 5 145; 28672 1024 x 4
+// 221, rows computed twice 294.  A few rows of 8192: 512 x 2 2.9, 1024 x 1 3.5.
 template <int DT, int MODE>
 int launch_rows(const SiluArgs& a, hipStream_t st) {
     const int64_t chunks = a.N >> 3;
 #define LLMQ_SILU(NC, NT, RPB) \
     hipLaunchKernelGGL((silu_rows_kernel<DT, MODE, NC, NT, RPB>), dim3((unsigned)((a.M + RPB - 1) / RPB)), dim3(NT * RPB), 0, st, a)
-    if (chunks <= 128 && a.M >= 256) LLMQ_SILU(2, 64, 4);
-    else if (chunks <= 256) LLMQ_SILU(1, 256, 1);
-    else if (chunks <= 512) {
-        if (a.M < 400) LLMQ_SILU(1, 512, 1);
-        else LLMQ_SILU(2, 256, 1);
-    } else if (chunks <= 1024) {
-        if (a.M < 400) LLMQ_SILU(1, 1024, 1);
-        else LLMQ_SILU(2, 512, 1);
-    } else if (chunks <= 3 * 1024) LLMQ_SILU(3, 1024, 1);
-    else LLMQ_SILU(0, 512, 1);
+    if (chunks <= 128) LLMQ_SILU(2, 64, 4);
+    else if (chunks <= 256) LLMQ_SILU(2, 128, 1);
+    else if (chunks <= 512) LLMQ_SILU(2, 256, 1);
+    else if (chunks <= 1024) LLMQ_SILU(2, 512, 1);
+    else if (chunks <= 2048) LLMQ_SILU(2, 1024, 1);
+    else if (chunks <= 3 * 1024) LLMQ_SILU(3, 1024, 1);
+    else if (chunks <= 4096) LLMQ_SILU(4, 1024, 1);
+    else LLMQ_SILU(0, 1024, 1);
 #undef LLMQ_SILU
     return launch_status();
 }

@@ -17,7 +17,7 @@ from .quantize import _apart, _as_rows
 _SCORING = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORE = {"max": 0, "top2": 1}
 MAX_ROUTED_EXPERTS, MAX_DISPATCHED_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 4096, 64, 64
-_MAX_ROWS = 0x7fffff00
+_MAX_ROWS = 0x7fff0000
 
 
 def _check(cond: bool, msg: str) -> None:
