@@ -12,7 +12,8 @@
 // A choice is a maximum over a lane's experts and over the lanes (row rotations and swaps, no LDS) and the lowest expert that has it.  Its order is that of the
 // exact scores wherever neighbours in it lie further apart than both scores can be off.  Two closer sigmoid scores are compared in 64 bits by themselves; a token
 // with more of them, with close groups, or with close scores of a softmax is done over with all scores in 64 bits.
-// Many tokens are bound by the vector unit (8192 of 256 experts, 8 chosen: 7 us, with a bias 12), a few by the chain of choices (16 of them: 4 and 5 us).
+// Many tokens are bound by the vector unit (8192 of 256 experts, 8 chosen: 6.4 us, with a bias 8.5, of 8 groups 10), a few by the chain of choices (16 of them: 4 and
+// 5 us).
 // More than 256 experts, 16 groups or 16 choices, and tokens with a NaN, take the long form.
 #include <algorithm>
 #include <type_traits>
@@ -246,8 +247,6 @@ template <int CTRL, class T>
 __device__ __forceinline__ T paired(T v) { return by_halves(v, [](uint32_t u) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)u, CTRL, 0xf, 0xf, true); }); }
 
 __device__ __forceinline__ float exp_fast(float v) { return __builtin_amdgcn_exp2f(1.44269504088896f * v); }
-__device__ __forceinline__ uint32_t key32(float c) { return (uint32_t)(key_of(c) >> 32); }
-__device__ __forceinline__ float value32(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
 
 // What choices go by: the logits; scores in 32 bits, where their neighbours lie far enough apart; scores in 64 bits
 enum { BY_LOGITS, BY_SCORES_32, BY_SCORES_64 };
@@ -259,9 +258,7 @@ struct Lay { int lanes_per_group, per_lane, vec; };
 template <int DT, int BY, int LPT, int V>
 __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t t, bool wanted) {
     using score_t = std::conditional_t<BY == BY_SCORES_64, double, float>;
-    using key_t = std::conditional_t<BY == BY_SCORES_64, double, uint32_t>;
     constexpr score_t kNone = -(score_t)__builtin_inff();
-    constexpr key_t kNoKey = BY == BY_SCORES_64 ? (key_t)kNone : (key_t)0;
     __shared__ float stage[kThreads / LPT][LPT * V];
     const int l = threadIdx.x % LPT, team = threadIdx.x / LPT, lanes_per_group = lay.lanes_per_group, per_lane = lay.per_lane;
     const uint64_t token_lanes = (LPT == 64 ? ~0ull : (1ull << (LPT & 63)) - 1) << ((threadIdx.x & (kWave - 1)) / LPT * LPT);
@@ -298,6 +295,22 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
 #pragma unroll
     for (int v = 0; v < V; v++) x[v] = v < count ? x[v] : -__builtin_inff();
 
+    float b[V];
+    if constexpr (BY != BY_LOGITS) {
+#pragma unroll
+        for (int v = 0; v < V; v++) b[v] = 0.f;
+        if (a.bias && lay.vec) {
+            const float4* p = reinterpret_cast<const float4*>(a.bias + (count ? e0 : 0));
+#pragma unroll
+            for (int v = 0; v < V / 4; v++) {
+                const float4 f = p[v];
+                b[4 * v] = f.x, b[4 * v + 1] = f.y, b[4 * v + 2] = f.z, b[4 * v + 3] = f.w;
+            }
+        } else if (a.bias) {
+#pragma unroll
+            for (int v = 0; v < V; v++) b[v] = v < count ? a.bias[e0 + v] : 0.f;
+        }
+    }
     float m = 0.f, sum = 1.f;
     if (!a.sigmoid) {
         m = x[0];
@@ -305,7 +318,7 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
         for (int v = 1; v < V; v++) m = fmaxf(m, x[v]);
         m = token_max<LPT>(m);
     }
-    key_t key[V];
+    score_t key[V];  // kNone: masked, chosen already, or no expert
     score_t group = kNone, size = 0, off = 0;  // score of the lane's group and what its rounding goes by; what a score can be off, but for its last rounding
     bool sure = true;
     if constexpr (BY != BY_LOGITS) {
@@ -344,20 +357,12 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
             // is at most 2.5 ln 256 + 2 < 16, which all scores have in common but the bias does not; V + 6 additions, the reciprocal 2 and the product 1
             off = (V + 32) * 0x1p-24f * r;
         }
-        score_t best = kNone, second = kNone;
-        bool number = true;
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            const float b = a.bias && v < count ? a.bias[e0 + v] : 0.f;
-            c[v] = x[v] == -__builtin_inff() ? kNone : c[v] + (score_t)b;
-            number &= c[v] == c[v];
-            if constexpr (BY == BY_SCORES_64) key[v] = c[v];
-            else key[v] = c[v] == kNone ? 0 : key32(c[v]);
-            second = larger(second, smaller(best, c[v]));
-            best = larger(best, c[v]);
-        }
-        sure = (__ballot(!number) & token_lanes) == 0;  // (a NaN: the long form knows its place)
+        for (int v = 0; v < V; v++) key[v] = x[v] == -__builtin_inff() ? kNone : c[v] + (score_t)b[v];
         if (a.groups > 1) {
+            score_t best = kNone, second = kNone;
+#pragma unroll
+            for (int v = 0; v < V; v++) second = larger(second, smaller(best, key[v])), best = larger(best, key[v]);
             auto merge = [&](score_t b2, score_t s2) __attribute__((always_inline)) {
                 second = larger(smaller(best, b2), larger(second, s2));
                 best = larger(best, b2);
@@ -380,11 +385,8 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
             if constexpr (BY == BY_SCORES_32) size = group == kNone ? 0.f : fabsf(best) + (two ? fabsf(second) : 0.f);
         }
     } else {
-        score_t best = kNone;
-        uint32_t top = 0;
 #pragma unroll
-        for (int v = 0; v < V; v++) key[v] = x[v] == -__builtin_inff() ? 0 : key32(x[v]), best = fmaxf(best, x[v]), top = max(top, key[v]);
-        sure = token_max<LPT>(top) != ~0u;  // a NaN's key
+        for (int v = 0; v < V; v++) key[v] = x[v];
         if (!a.sigmoid && !a.renormalize) {
             sum = 0.f;
 #pragma unroll
@@ -392,6 +394,9 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
             sum = token_sum<LPT>(sum);
         }
         if (a.groups > 1) {
+            score_t best = key[0];
+#pragma unroll
+            for (int v = 1; v < V; v++) best = fmaxf(best, key[v]);
             if (lanes_per_group > 1) best = fmaxf(best, paired<0xB1>(best));
             if (lanes_per_group > 2) best = fmaxf(best, paired<0x4E>(best));
             if (lanes_per_group > 4) best = fmaxf(best, paired<0x141>(best));
@@ -403,6 +408,10 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
             group = best;
         }
     }
+    bool number = true;
+#pragma unroll
+    for (int v = 0; v < V; v += 2) number &= !__builtin_isunordered(key[v], key[v + 1]);
+    sure = (__ballot(!number) & token_lanes) == 0;  // (a NaN: the long form knows its place)
     if (a.groups > 1) {
         score_t left = group, least = 0;
         // the last of as many different scores as groups are asked for, or of fewer where groups are level
@@ -423,16 +432,17 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
             if (least > kNone && next > kNone && !(least - next > 4 * off + 0x1p-22f * size)) sure = false;
         }
 #pragma unroll
-        for (int v = 0; v < V; v++) key[v] = kept ? key[v] : kNoKey;
+        for (int v = 0; v < V; v++) key[v] = kept ? key[v] : kNone;
     }
 
     // ---- the choices; lane j keeps choice j
-    int id = -1, last = -1;
+    int id = -1;
     float before = __builtin_inff();
     bool near_last = false;  // the last two choices were close
+    uint64_t pairs = 0;      // bit j: choices j - 1 and j are
     // (one choice more shows whether the last one is close to what is left, and if so one further whether those are two)
     for (int j = 0, rounds = a.top + (BY == BY_SCORES_32 ? 1 : 0); j < rounds; j++) {
-        key_t best = key[0];
+        score_t best = key[0];
 #pragma unroll
         for (int v = 1; v < V; v++) best = larger(best, key[v]);
         best = token_max<LPT>(best);
@@ -440,39 +450,41 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
 #pragma unroll
         for (int v = V - 1; v >= 0; v--) at = key[v] == best ? v : at;
         const uint32_t lowest = token_max<LPT>(at < V ? 0xffffu - (uint32_t)(e0 + at) : 0u);
-        int chosen = 0xffff - (int)lowest;
+        const int chosen = 0xffff - (int)lowest;
         at = chosen - e0;
 #pragma unroll
-        for (int v = 0; v < V; v++) key[v] = v == at && v < count ? kNoKey : key[v];
+        for (int v = 0; v < V; v++) key[v] = v == at ? kNone : key[v];  // (past the lane's last expert there is nothing to lose)
         if constexpr (BY == BY_SCORES_32) {
-            const float c = value32(best);
-            const bool close = j > 0 && best != 0 && !(before - c > 2 * off + 0x1p-24f * (fabsf(before) + fabsf(c)));
-            before = c;
-            if (__any(close && sure)) {
-                if (j == a.top) rounds++;
-                // Two close sigmoid scores are compared in 64 bits by themselves; three, and those of a softmax, whose sum takes part, are not.
-                if (near_last || (!a.sigmoid && j <= a.top)) sure = sure && !close;
-                if (close && sure && j <= a.top) {
-                    auto score = [&](int e) __attribute__((always_inline)) {
-                        return 1.0 / (1.0 + exp(-(double)load_as_f32(a.logits, DT, t * a.ld + e))) + (a.bias ? (double)a.bias[e] : 0.0);
-                    };
-                    const double p = score(last), q = score(chosen);
-                    if (q > p || (q == p && chosen < last)) {
-                        if (l == j - 1) id = chosen;
-                        chosen = last;
-                    }
-                }
-            }
-            near_last = close;
-            last = chosen;
-            if (j >= a.top) continue;
+            // Two close sigmoid scores are compared in 64 bits by themselves, below; three, and those of a softmax, whose sum takes part, are not.
+            const bool close = j > 0 && best != kNone && !(before - best > 2 * off + 0x1p-24f * (fabsf(before) + fabsf(best)));
+            if (close && (near_last || (j <= a.top && (!a.sigmoid || j == LPT)))) sure = false;
+            if (j == a.top && __any(close && sure)) rounds++;
+            pairs |= (uint64_t)(close && j <= a.top) << j;
+            before = best, near_last = close;
         }
-        if (l == j) id = best != kNoKey ? chosen : -1;
+        if (l == j) id = best != kNone ? chosen : -1;
     }
     if (!__any(sure && wanted)) return false;
 
+    float cx = id >= 0 ? load_as_f32(a.logits, DT, t * a.ld + id) : -__builtin_inff();
+    if constexpr (BY == BY_SCORES_32) {
+        if (__any(pairs != 0 && sure)) {
+            const double score = id >= 0 ? 1.0 / (1.0 + exp(-(double)cx)) + (a.bias ? (double)a.bias[id] : 0.0) : 0.0;
+            const bool second = pairs >> l & 1, first = pairs >> l >> 1 & 1;  // of its pair (no choice is in two)
+            const int partner = (int)(threadIdx.x & (kWave - 1)) + (second ? -1 : first ? 1 : 0);
+            auto theirs = [&](auto v) __attribute__((always_inline)) {
+                return by_halves(v, [&](uint32_t u) __attribute__((always_inline)) { return (uint32_t)__builtin_amdgcn_ds_bpermute(partner * 4, (int)u); });
+            };
+            const double other = theirs(score);
+            const int other_id = theirs(id);
+            const float other_x = theirs(cx);
+            const bool ahead = second ? score > other || (score == other && id < other_id) : other > score || (other == score && other_id < id);  // the second one is
+            if ((first || second) && ahead) id = other_id, cx = other_x;
+        }
+        if (l >= a.top) id = -1, cx = -__builtin_inff();
+    }
+
     // ---- weights, as in the long form
-    const float cx = id >= 0 ? load_as_f32(a.logits, DT, t * a.ld + id) : -__builtin_inff();
     const float top_x = token_max<LPT>(cx);
     float w = 0.f;
     if (id >= 0) {
@@ -514,7 +526,8 @@ bool lay_out(const RouteArgs& a, Lay& lay) {
     int lanes = LPT;  // of a group
     while (lanes > 1 && lanes * a.groups > LPT) lanes /= 2;
     lay.lanes_per_group = lanes, lay.per_lane = (a.group_size + lanes - 1) / lanes;
-    lay.vec = a.group_size == lanes * V && a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.logits) % (DT == LLMQ_F32 ? 16 : 8) == 0;
+    lay.vec = a.group_size == lanes * V && a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.logits) % (DT == LLMQ_F32 ? 16 : 8) == 0 &&
+              reinterpret_cast<uintptr_t>(a.bias) % 16 == 0;
     return lanes * a.groups <= LPT && lay.per_lane <= V;
 }
 template <int DT, bool EXACT, int LPT, int V>
@@ -528,15 +541,18 @@ bool try_short(const RouteArgs& a, hipStream_t st) {
 }
 
 // A few tokens are a chain of latencies, which fewer experts for a lane shorten; many are instructions, of which more experts for a lane need fewer.
-// us without / with a bias, 16, 32, 64 lanes for a token: 16 tokens of 256 experts 5.6 4.5 4.0 / 7.9 6.0 4.9, 1024 of them 5.8 4.8 4.4 / 8.2 6.4 5.3, 4096 6.2
-// 5.7 7.1, 8192 7.1 8.1 11.3; 16 of 128 4.2 3.8 4.3 / 5.8 4.8 5.0, 8192 5.5 6.6 11.6; 16 of 64 3.5 4.0 4.2 / 4.5 4.9 4.9, 8192 4.4 6.9 11.5.
+// us without / with a bias, 16, 32, 64 lanes for a token: 16 tokens of 256 experts 4.9 4.2 4.0 / 6.0 5.2 4.9, 2048 of them 5.2 4.6 5.0 / 6.4 5.7 6.0, 8192 6.4 7.7 11.3 /
+// 8.5 9.6 14.0; 16 and 32 lanes, 16 tokens of 128 4.0 3.7 / 4.8 4.5, 3000 4.2 4.5 / 5.3 5.5, 8192 4.8 6.3 / 6.0 7.9.
 template <int DT, bool EXACT>
 int launch_route(const RouteArgs& a, hipStream_t st) {
     bool done = false;
     if (a.groups <= kShortGroups && a.top <= kShortTop && a.experts <= kShortExperts) {
         done = try_short<DT, EXACT, 16, 4>(a, st);
-        if (!done && a.tokens <= 3000) done = try_short<DT, EXACT, 32, 4>(a, st) || try_short<DT, EXACT, 64, 4>(a, st);
-        if (!done) done = try_short<DT, EXACT, 16, 8>(a, st) || try_short<DT, EXACT, 16, 16>(a, st) || try_short<DT, EXACT, 64, 4>(a, st);
+        if (!done && a.tokens <= 2500) done = try_short<DT, EXACT, 32, 4>(a, st);
+        if (!done && a.tokens <= 1500) done = try_short<DT, EXACT, 64, 4>(a, st);
+        if (!done) done = try_short<DT, EXACT, 16, 8>(a, st);
+        if (!done && a.tokens <= 5000) done = try_short<DT, EXACT, 32, 8>(a, st);
+        if (!done) done = try_short<DT, EXACT, 16, 16>(a, st);
     }
     if (!done)
         hipLaunchKernelGGL((route_many_kernel<DT, EXACT>), dim3((unsigned)a.tokens), dim3(kThreads), a.groups > 1 ? (a.experts + a.groups) * 8 : 0, st, a);
