@@ -7,7 +7,7 @@
  *    nothing, never synchronises with the host and launches on the stream it is given
  *    (0 = the null stream).  Calls are asynchronous.  State kept between calls, all of
  *    it per host thread: the *_force_plan tuning hooks, the last 64 GEMM and 64 AWQ plans, and the last plan of each of the
- *    two block-scaled products (a function of sizes and format alone).  llmq_gemm_w8a8_static has a scratch array per GPU.
+ *    two block-scaled products and of the W8A8 product by experts (a function of sizes and format alone).  llmq_gemm_w8a8_static has a scratch array per GPU.
  *  - Matrices are row-major; `ld*` is the row stride in ELEMENTS.
  *  - Return value: LLMQ_OK (0) or a negative llmq_status; llmq_status_string() names it.
  *  - Paths below are relative to the reference's runtime/ directory.
