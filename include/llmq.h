@@ -449,10 +449,12 @@ int llmq_route_experts(int scoring, const void* logits, int logits_dtype, int64_
  *     LLMQ_NORM_SAME       x_dtype, 16-byte aligned
  *     LLMQ_NORM_I8_TOKEN   the codes of llmq_quant_i8_per_token, 8-byte aligned; scale: fp32 [tokens * top_k]
  *     LLMQ_NORM_FP8_GROUP  the codes of llmq_quant_fp8_per_group, 8-byte aligned; scale: fp32 [tokens * top_k, ceil(K / 128)]
- * x: [tokens, K] bf16 / f16, K % 8 == 0, ldx % 8 == 0, 16-byte aligned.  At most 4096 experts, top_k at most 64, at most 2^31 - 65536 rows. */
+ * x: [tokens, K] bf16 / f16, K % 8 == 0, ldx % 8 == 0, 16-byte aligned.  At most 4096 experts, top_k at most 64, at most 2^31 - 65536 rows.
+ * workspace: >= llmq_dispatch_experts_workspace_bytes bytes (0 up to some 20000 rows; NULL will do then), 16-byte aligned, contents irrelevant on entry. */
 int llmq_dispatch_experts(int out, const void* x, int x_dtype, int64_t tokens, int64_t K, int64_t ldx, const int32_t* ids, int64_t top_k,
                           int64_t first_expert, int64_t experts, void* rows, float* scale, int32_t* offsets, int32_t* places,
-                          llmq_stream_t stream);
+                          void* workspace, size_t workspace_bytes, llmq_stream_t stream);
+size_t llmq_dispatch_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts);
 
 /* out[t, :] = dtype( sum_j weights[t, j] y[places[t, j], :]  (+ shared[t, :]) ), fp32 sums in the order of j, the shared row last.  Places outside
  * [0, rows) add nothing, whatever their weight.  y: bf16 / f16 [rows, N], shared: [tokens, N] or null, out: [tokens, N] contiguous, all of one type; N % 8 == 0,

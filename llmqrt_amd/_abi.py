@@ -87,7 +87,8 @@ SIGNATURES = {
     "llmq_gemm_fp8_block_grouped": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _int, _vp, _int, _i64, _i64, _i64, _i64, _vp]),
     "llmq_gemm_fp8_block_force_plan": (_int, [_int, _int]),
     "llmq_route_experts": (_int, [_int, _vp, _int, _i64, _i64, _i64, _vp, _i64, _i64, _int, _i64, _int, _f32, _vp, _vp, _vp]),
-    "llmq_dispatch_experts": (_int, [_int, _vp, _int, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "llmq_dispatch_experts": (_int, [_int, _vp, _int, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "llmq_dispatch_experts_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "llmq_combine_experts": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp]),
     "llmq_gemm_w8a8_grouped": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _int, _vp, _int, _i64, _i64, _i64, _i64, _vp]),
     "llmq_gemm_w8a8_grouped_force_plan": (_int, [_int]),

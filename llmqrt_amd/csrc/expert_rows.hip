@@ -6,7 +6,7 @@
 // Ids are counted from `first`; those outside [first, first + experts) go nowhere: they have no place (-1) and are not counted.
 //
 // The order is that of a stable sort, so it is the same every time.  A token is read and quantized once and written top_k times.  HBM-bound: 8192 tokens of 3584
-// int8 to 4 of 32 experts 40 us, of which the rows take 30 (5.8 TB/s) and their places 9.5; combined again 55 us (5.3 TB/s).  A few tokens are a launch and a chain of
+// int8 to 4 of 32 experts 38 us, of which the rows take 30 (5.8 TB/s) and their places 7.7; combined again 55 us (5.3 TB/s).  A few tokens are a launch and a chain of
 // latencies: ids, places, rows (48 tokens to 4 of 64 4.0 us, combined again 2.8).
 #include <algorithm>
 
@@ -147,6 +147,126 @@ __global__ __launch_bounds__(1024) void expert_places_kernel(const int32_t* __re
         }
     }
 }
+
+// ---- very many ids: in three launches that each go over them once.  A wavefront has a run of ids; `counts` says how many of them are of each expert, then how many of
+// an expert's lie in the runs before.
+constexpr int kRunPieces = 4, kRunUnit = kRunPieces * kWave, kMaxRuns = 1024, kRunWaves = 2;
+struct Runs {
+    int n, per, runs, stride;  // ids; of a run; runs; ints of an expert in `counts`, whose last ones are the experts' totals
+    int32_t* counts;
+};
+__device__ __forceinline__ void own_lds() {  // LDS that this wavefront alone writes and reads
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+// the ids from b on that are in front of hi, as experts; the others are none
+__device__ __forceinline__ void load_run(const int32_t* ids, int64_t b, int64_t hi, int first, uint32_t* e) {
+    const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+    for (int u = 0; u < kRunPieces; u++) {
+        const int64_t i = b + u * kWave + lane;
+        e[u] = (uint32_t)ids[i < hi ? i : hi - 1] - (uint32_t)first;
+        if (i >= hi) e[u] = ~0u;
+    }
+}
+
+__global__ __launch_bounds__(kRunWaves * kWave) void run_counts_kernel(const int32_t* __restrict__ ids, Runs r, int first, int experts) {
+    extern __shared__ int32_t s_count[];  // of a wavefront: experts
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, run = blockIdx.x * kRunWaves + wave;
+    if (run >= r.runs) return;  // wavefront-uniform; no barrier follows
+    int32_t* count = s_count + wave * experts;
+    for (int e = lane; e < experts; e += kWave) count[e] = 0;
+    own_lds();
+    const int64_t lo = (int64_t)run * r.per, hi = min((int64_t)r.n, lo + r.per);
+    for (int64_t b = lo; b < hi; b += kRunUnit) {
+        uint32_t e[kRunPieces];
+        load_run(ids, b, hi, first, e);
+#pragma unroll
+        for (int u = 0; u < kRunPieces; u++)
+            if (e[u] < (uint32_t)experts) atomicAdd(&count[e[u]], 1);
+    }
+    own_lds();
+    for (int e = lane; e < experts; e += kWave) r.counts[(int64_t)e * r.stride + run] = count[e];
+}
+
+// A wavefront per expert
+__global__ __launch_bounds__(kWave) void run_sums_kernel(Runs r, int experts) {
+    const int e = blockIdx.x, lane = threadIdx.x;
+    int4* c = reinterpret_cast<int4*>(r.counts + (int64_t)e * r.stride);
+    int4 v[kMaxRuns / kRunUnit];
+#pragma unroll
+    for (int k = 0; k < kMaxRuns / kRunUnit; k++) {
+        const int i = (k * kWave + lane) * 4;
+        v[k] = i < r.stride ? c[k * kWave + lane] : make_int4(0, 0, 0, 0);
+        v[k].x = i < r.runs ? v[k].x : 0, v[k].y = i + 1 < r.runs ? v[k].y : 0, v[k].z = i + 2 < r.runs ? v[k].z : 0, v[k].w = i + 3 < r.runs ? v[k].w : 0;
+    }
+    int before = 0;
+#pragma unroll
+    for (int k = 0; k < kMaxRuns / kRunUnit; k++) {
+        const int own = v[k].x + v[k].y + v[k].z + v[k].w, upto = before + wave_prefix(own), at = upto - own;
+        if ((k * kWave + lane) * 4 < r.stride) c[k * kWave + lane] = make_int4(at, at + v[k].x, at + v[k].x + v[k].y, at + v[k].x + v[k].y + v[k].z);
+        before = __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    if (lane == 0) r.counts[(int64_t)experts * r.stride + e] = before;
+}
+
+// Every run hands out the places of its ids: among 64 at a time those of one expert find each other by the bits of its number, bits of them.
+__global__ __launch_bounds__(kRunWaves * kWave) void run_places_kernel(const int32_t* __restrict__ ids, Runs r, int first, int experts, int bits,
+                                                                       int32_t* __restrict__ places, int32_t* __restrict__ offsets) {
+    extern __shared__ int32_t s_next[];  // experts' first rows; then of a wavefront: an expert's next place
+    __shared__ int32_t sums[kRunWaves];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, run = blockIdx.x * kRunWaves + wave;
+    for (int e = threadIdx.x; e < experts; e += kRunWaves * kWave) s_next[e] = r.counts[(int64_t)experts * r.stride + e];
+    __syncthreads();
+    const int total = scan_lds<kRunWaves * kWave>(s_next, experts, sums);
+    if (blockIdx.x == 0) {
+        for (int e = threadIdx.x; e < experts; e += kRunWaves * kWave) offsets[e] = s_next[e];
+        if (threadIdx.x == 0) offsets[experts] = total;
+    }
+    if (run >= r.runs) return;  // wavefront-uniform; no barrier follows
+    int32_t* next = s_next + (wave + 1) * experts;
+    for (int e = lane; e < experts; e += kWave) next[e] = s_next[e] + r.counts[(int64_t)e * r.stride + run];
+    own_lds();
+    const int64_t lo = (int64_t)run * r.per, hi = min((int64_t)r.n, lo + r.per);
+    for (int64_t b = lo; b < hi; b += kRunUnit) {
+        uint32_t e[kRunPieces];
+        uint64_t like[kRunPieces];  // the lanes with the same expert
+        load_run(ids, b, hi, first, e);
+#pragma unroll
+        for (int u = 0; u < kRunPieces; u++) like[u] = __ballot(e[u] < (uint32_t)experts);
+        for (int k = 0; k < bits; k++) {
+#pragma unroll
+            for (int u = 0; u < kRunPieces; u++) {
+                const bool one = e[u] >> k & 1;
+                const uint64_t ones = __ballot(one);
+                like[u] &= one ? ones : ~ones;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kRunPieces; u++) {
+            const int64_t i = b + u * kWave + lane;
+            const bool in = e[u] < (uint32_t)experts;
+            int place = -1;
+            if (in) place = __builtin_amdgcn_mbcnt_hi((uint32_t)(like[u] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)like[u], next[e[u]]));
+            own_lds();
+            if (in && (like[u] >> lane >> 1) == 0) next[e[u]] = place + 1;  // the last of them
+            own_lds();
+            if (i < hi) places[i] = place;
+        }
+    }
+}
+
+// Whether there are so many ids that the three launches are faster than a block per expert over all of them, and how they share them.  us, a block per expert / in
+// runs: 16384 ids of 64 experts 6.9 / 7.9, 32768 of 32 9.2 / 7.7, of 128 9.0 / 8.4, of 256 8.6 / 9.7, 65536 of 256 19.2 / 10.2, 262144 of 64 72 / 9.3; 16000 of 512 10.2 / 12.1,
+// of 1024 17.5 / 17.6, of 4096 59 / 50.  The one grows with ids, and with experts where the chip does not hold a block of each, the other with experts.
+bool in_runs(int64_t n, int64_t experts, Runs& r) {
+    r.n = (int)n, r.per = (int)(((n + kMaxRuns - 1) / kMaxRuns + kRunUnit - 1) / kRunUnit * kRunUnit);
+    r.runs = (int)((n + r.per - 1) / r.per), r.stride = (r.runs + 3) / 4 * 4;
+    return n * std::max<int64_t>(experts, 256) > 256 * (21400 + 50 * experts);
+}
+size_t run_bytes(const Runs& r, int64_t experts) { return ((size_t)r.stride + 1) * experts * sizeof(int32_t); }
+bool count_all(int64_t tokens, int64_t top_k) { return tokens * top_k <= kCountAll && tokens * tokens * top_k <= 1 << 22; }
 
 // A block per token; 16 neighbouring elements per thread and piece.  ALL: every token counts all ids for itself, and one more block counts them for the
 // offsets; otherwise the places are there.  NP > 0: the row stays in registers, NP pieces per thread; 0: rows of any length, read again for every copy.
@@ -424,9 +544,15 @@ bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0
 
 using namespace llmq;
 
+extern "C" size_t llmq_dispatch_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts) {
+    if (tokens < 1 || top_k < 1 || top_k > kMaxTop || tokens > 0x7fff0000LL / top_k || experts < 1 || experts > kMaxExperts || count_all(tokens, top_k)) return 0;
+    Runs r;
+    return in_runs(tokens * top_k, experts, r) ? run_bytes(r, experts) : 0;
+}
+
 extern "C" int llmq_dispatch_experts(int out, const void* x, int x_dtype, int64_t tokens, int64_t K, int64_t ldx, const int32_t* ids, int64_t top_k,
                                      int64_t first_expert, int64_t experts, void* rows, float* scale, int32_t* offsets, int32_t* places,
-                                     llmq_stream_t stream) {
+                                     void* workspace, size_t workspace_bytes, llmq_stream_t stream) {
     if ((out != OUT_SAME && out != OUT_I8 && out != OUT_GROUP) || (x_dtype != LLMQ_BF16 && x_dtype != LLMQ_F16)) return LLMQ_ERR_DTYPE;
     if (tokens < 0 || K < 0 || K > 0x7fffffffLL || ldx < K || (K & 7) || (ldx & 7) || top_k < 1 || top_k > kMaxTop || experts < 1 ||
         experts > kMaxExperts || first_expert < 0 || first_expert > 0x7fff0000LL || tokens > 0x7fff0000LL / top_k)
@@ -439,10 +565,22 @@ extern "C" int llmq_dispatch_experts(int out, const void* x, int x_dtype, int64_
     a.ldx = ldx, a.K = K, a.ids_total = (int)(tokens * top_k), a.top = (int)top_k, a.first = (int)first_expert, a.experts = (int)experts;
     a.wide = K % 16 == 0 && aligned16(rows);
     const hipStream_t st = (hipStream_t)stream;
-    // every token counts all ids, or one launch more finds the places: us, counted / found (rows of 3584 int8) 512 tokens of 4 5.6 / 8.2, 1024 of 4 7.5 / 8.8, 2000 of
+    // every token counts all ids, or further launches find the places: us, counted / found (rows of 3584 int8) 512 tokens of 4 5.6 / 8.2, 1024 of 4 7.5 / 8.8, 2000 of
     // 4 14 / 9.6
-    const bool all = tokens * top_k <= kCountAll && tokens * tokens * top_k <= 1 << 22;
-    if (!all) {
+    const bool all = count_all(tokens, top_k);
+    Runs r;
+    if (!all && in_runs(a.ids_total, experts, r)) {
+        if (!workspace || workspace_bytes < run_bytes(r, experts)) return LLMQ_ERR_WORKSPACE;
+        if (!aligned16(workspace)) return LLMQ_ERR_ALIGN;
+        r.counts = (int32_t*)workspace;
+        const unsigned blocks = (unsigned)((r.runs + kRunWaves - 1) / kRunWaves), threads = kRunWaves * kWave;
+        int bits = 0;
+        while (1 << bits < experts) bits++;
+        hipLaunchKernelGGL(run_counts_kernel, dim3(blocks), dim3(threads), kRunWaves * experts * 4, st, ids, r, a.first, a.experts);
+        hipLaunchKernelGGL(run_sums_kernel, dim3((unsigned)experts), dim3(kWave), 0, st, r, a.experts);
+        hipLaunchKernelGGL(run_places_kernel, dim3(blocks), dim3(threads), (kRunWaves + 1) * experts * 4, st, ids, r, a.first, a.experts, bits, places, offsets);
+        if (launch_status() != LLMQ_OK) return LLMQ_ERR_LAUNCH;
+    } else if (!all) {
         if (aligned16(ids)) hipLaunchKernelGGL((expert_places_kernel<4>), dim3((unsigned)experts), dim3(1024), 0, st, ids, a.ids_total, a.first, a.experts, places, offsets);
         else hipLaunchKernelGGL((expert_places_kernel<1>), dim3((unsigned)experts), dim3(1024), 0, st, ids, a.ids_total, a.first, a.experts, places, offsets);
         if (launch_status() != LLMQ_OK) return LLMQ_ERR_LAUNCH;

@@ -688,9 +688,12 @@ std::optional<Sorted> dispatch(const Tensor& x, const Tensor& ids, int64_t exper
     small.add(&offsets, {experts + 1}, at::kInt);
     small.add(&places, ids.sizes(), at::kInt);
     small.make_all();
+    const size_t bytes = llmq_dispatch_experts_workspace_bytes(r.M, top, experts);
+    Tensor ws;
+    if (bytes) ws = make({(int64_t)bytes}, at::kByte, dev);
     const int rc = llmq_dispatch_experts(out, x.data_ptr(), code(x.scalar_type()), r.M, r.K, r.K, (const int32_t*)ids.data_ptr(), top, first, experts,
                                          rows.data_ptr(), same ? nullptr : (float*)scale.data_ptr(), (int32_t*)offsets.data_ptr(),
-                                         (int32_t*)places.data_ptr(), l.stream);
+                                         (int32_t*)places.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes, l.stream);
     if (refused(rc)) return std::nullopt;
     check(rc, "llmq_dispatch_experts");
     Sorted s;

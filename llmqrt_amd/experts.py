@@ -108,10 +108,12 @@ def _dispatch_general(x, experts, num_experts, first_expert, out):
         scale = torch.empty((n, 1 if out == _I8_TOKEN else (K + 127) // 128), dtype=torch.float32, device=dev)
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
     places = torch.empty(experts.shape, dtype=torch.int32, device=dev)
+    ws = torch.empty(_abi.lib().llmq_dispatch_experts_workspace_bytes(T, top, num_experts), dtype=torch.uint8, device=dev)
     with torch.cuda.device(dev):
         _abi.check(_abi.lib().llmq_dispatch_experts(
             out, rows.data_ptr(), _abi.dtype_code(rows.dtype), T, K, rows.stride(0) if T > 1 else K, ids.data_ptr(), top, first_expert, num_experts,
-            sorted_rows.data_ptr(), _abi.ptr(scale), offsets.data_ptr(), places.data_ptr(), _abi.stream_of(rows)), "llmq_dispatch_experts")
+            sorted_rows.data_ptr(), _abi.ptr(scale), offsets.data_ptr(), places.data_ptr(),
+            ws.data_ptr() or None, ws.numel(), _abi.stream_of(rows)), "llmq_dispatch_experts")
     return (sorted_rows, offsets, places) if scale is None else (sorted_rows, scale, offsets, places)
 
 

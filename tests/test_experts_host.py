@@ -6,7 +6,7 @@ import torch
 
 from llmqrt_amd import _abi
 
-OK, NULL, DTYPE, SHAPE, ALIGN = 0, -1, -2, -3, -6
+OK, NULL, DTYPE, SHAPE, WORKSPACE, ALIGN = 0, -1, -2, -3, -4, -6
 
 
 @pytest.fixture(scope="module")
@@ -32,9 +32,9 @@ def test_route_refusals(p16):
     assert route(p, T=0, logits=0, w=0, ids=0) == OK
 
 
-def dispatch(p, out=0, dt=0, T=4, K=64, ldx=64, k=2, first=0, E=4, x=None, ids=None, rows=None, scale=None, off=None, pl=None):
+def dispatch(p, out=0, dt=0, T=4, K=64, ldx=64, k=2, first=0, E=4, x=None, ids=None, rows=None, scale=None, off=None, pl=None, ws=None, wsb=0):
     d = lambda v: p if v is None else v  # noqa: E731
-    return _abi.lib().llmq_dispatch_experts(out, d(x), dt, T, K, ldx, d(ids), k, first, E, d(rows), d(scale), d(off), d(pl), None)
+    return _abi.lib().llmq_dispatch_experts(out, d(x), dt, T, K, ldx, d(ids), k, first, E, d(rows), d(scale), d(off), d(pl), ws, wsb, None)
 
 
 def test_dispatch_refusals(p16):
@@ -46,6 +46,11 @@ def test_dispatch_refusals(p16):
     for name in ("x", "ids", "rows", "off", "pl"):
         assert dispatch(p, **{name: 0}) == NULL
     assert dispatch(p, out=1, scale=0) == NULL and dispatch(p, out=3, scale=0) == NULL and dispatch(p, T=0, off=0) == NULL
+    need = _abi.lib().llmq_dispatch_experts_workspace_bytes
+    assert need(48, 4, 64) == 0 and need(4000, 4, 64) == 0 and need(0, 4, 64) == 0 and need(-1, 4, 64) == 0 and need(1 << 62, 64, 4096) == 0 and need(9, 9, 5000) == 0
+    many = need(50000, 2, 12)
+    assert many >= 12 * 4 * 2 and 0 < need((1 << 31) // 64 - 1024, 64, 4096) <= 4096 * 4 * 1025
+    assert dispatch(p, T=50000, E=12) == WORKSPACE and dispatch(p, T=50000, E=12, ws=p, wsb=many - 1) == WORKSPACE and dispatch(p, T=50000, E=12, ws=p + 4, wsb=many) == ALIGN
     assert dispatch(p, x=p + 8) == ALIGN and dispatch(p, rows=p + 8) == ALIGN and dispatch(p, out=1, rows=p + 4) == ALIGN
 
 

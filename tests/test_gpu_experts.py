@@ -272,7 +272,8 @@ def choose(T, E, top, g):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,K,E,top", [(1, 8, 1, 1), (1, 3584, 64, 8), (3, 136, 5, 2), (48, 3584, 64, 4), (17, 1000, 60, 7), (255, 896, 16, 8), (256, 896, 16, 8),
                                        (257, 896, 300, 8), (700, 264, 8, 3), (2049, 128, 128, 1), (130, 2056, 4, 40), (37, 18944, 9, 2), (33, 20488, 3, 64),
-                                       (5000, 64, 256, 8), (40, 4104, 4096, 64)])
+                                       (5000, 64, 256, 8), (40, 4104, 4096, 64), (6000, 64, 60, 8), (20001, 8, 200, 3), (41000, 16, 1, 1), (5100, 24, 257, 8), (700, 8, 4096, 5),
+                                       (150000, 8, 33, 4)])
 def test_dispatch(cuda, T, K, E, top, dtype, kind):
     g = torch.Generator().manual_seed(T + K + E)
     x = torch.randn(T, K, generator=g).to(dtype)
@@ -319,7 +320,7 @@ def test_dispatch_rows_left_alone(cuda, T):
     rows = torch.full((n + 2, K), 77, dtype=torch.int8, device=cuda)
     scale, places, offsets = torch.full((n + 2,), 7.0, device=cuda), torch.full((n + 2,), 7, dtype=torch.int32, device=cuda), torch.full((E + 3,), 7, dtype=torch.int32, device=cuda)
     _abi.check(L.llmq_dispatch_experts(1, x.data_ptr(), _abi.BF16, T, K, K, ids.data_ptr(), top, 0, E, rows[1].data_ptr(), scale[1:].data_ptr(), offsets[1:].data_ptr(),
-                                       places[1:].data_ptr(), _abi.stream_of(x)), "dispatch")
+                                       places[1:].data_ptr(), None, 0, _abi.stream_of(x)), "dispatch")
     off, pl, _ = sorted64(ids.cpu(), E, 0)
     end = int(off[-1])
     assert same(offsets[1:E + 2].cpu(), off) and same(places[1:n + 1].view(T, top).cpu(), pl) and 0 < end < n

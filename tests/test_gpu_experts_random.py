@@ -125,6 +125,26 @@ def test_many_experts(cuda, M, cfg):
             assert same(out[m:m + 8000], ((acc * alpha[m:m + 8000]) * beta[e]).to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("T,E,top", [(40, 8, 2), (3000, 16, 4), (9000, 64, 8)])
+def test_captured_dispatch(cuda, T, E, top):
+    """One launch, two and four: every replay sorts the ids that are there, beside eager calls."""
+    from llmqrt_amd.experts import dispatch_to_experts
+    g = torch.Generator().manual_seed(T)
+    x, ids = torch.randn(T, 16, generator=g).bfloat16().to(cuda), choose(T, E, top, g).to(cuda)
+    dispatch_to_experts(x, ids, E)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = dispatch_to_experts(x, ids, E)
+    for _ in range(4):
+        ids.copy_(choose(T, E, top, g))
+        want = dispatch_to_experts(x, ids, E)
+        graph.replay()
+        other = dispatch_to_experts(x, ids.flip(0), E)
+        torch.cuda.synchronize()
+        assert all(same(a, b) for a, b in zip(got, want)) and int(other[1][-1]) == T * top
+
+
 @pytest.mark.parametrize("T,top", [(5, 3), (16, 8), (3000, 4)])
 def test_dispatch_to_the_most_experts(cuda, T, top):
     g = torch.Generator().manual_seed(T)
