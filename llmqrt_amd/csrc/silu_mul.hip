@@ -62,16 +62,15 @@ __global__ __launch_bounds__(kSiluThreads) void silu_groups_kernel(SiluArgs a, u
     if (l == 0 && g < total) a.scale[g] = s;
 }
 
-// A scale per row.  NT threads per row, RPB rows per block (more than one: a wavefront each, and no barrier).  NC > 0: a row's outputs stay in 8 NC
+// A scale per row.  NT threads per row, RPB rows per block (more than one: within a wavefront each, and no barrier).  NC > 0: a row's outputs stay in 8 NC
 // registers per thread between the maximum and the codes; 0: rows of any length, computed twice.
 template <int DT, int MODE, int NC, int NT, int RPB>
 __global__ __launch_bounds__(NT * RPB) void silu_rows_kernel(SiluArgs a) {
-    static_assert(RPB == 1 || NT == kWave, "several rows per block are a wavefront each");
-    __shared__ float smem[NT / kWave];
-    const int tid = RPB > 1 ? threadIdx.x % kWave : threadIdx.x;
-    const int64_t row = RPB > 1 ? (int64_t)blockIdx.x * RPB + threadIdx.x / kWave : blockIdx.x;
-    if (RPB > 1 && row >= a.M) return;  // wavefront-uniform; no barrier follows
-    const int nchunk = (int)(a.N >> 3);
+    static_assert(RPB == 1 ? NT >= kWave : NT == 16 || NT == 32 || NT == kWave, "several rows per block are within a wavefront each");
+    __shared__ float smem[RPB > 1 ? 1 : NT / kWave];
+    const int tid = threadIdx.x % NT;
+    const int64_t own = (int64_t)blockIdx.x * RPB + threadIdx.x / NT, row = RPB > 1 ? min(own, a.M - 1) : own;
+    const int nchunk = RPB > 1 && own >= a.M ? 0 : (int)(a.N >> 3);  // (lanes without a row have no chunks)
     const uint4* gr = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
     const uint4* ur = reinterpret_cast<const uint4*>(a.x + row * a.ldx + a.N);
     uint2* qr = reinterpret_cast<uint2*>(a.q + row * a.N);
@@ -95,9 +94,14 @@ __global__ __launch_bounds__(NT * RPB) void silu_rows_kernel(SiluArgs a) {
             amax = max_nonneg(amax, absmax8f(y[0]));
         }
     }
-    amax = RPB > 1 ? wave_max(amax) : block_max<NT / kWave>(amax, smem);
+    if constexpr (RPB == 1) {
+        amax = block_max<NT / kWave>(amax, smem);
+    } else {
+        amax = NT == kWave ? wave_max(amax) : team_max(amax);
+        if constexpr (NT == 32) amax = max_nonneg(amax, lane_xor<16>(amax));
+    }
     const float s = scale32<MODE>(amax), inv_s = 1.0f / s;
-    if (tid == 0) a.scale[row] = s;
+    if (tid == 0 && (RPB == 1 || own < a.M)) a.scale[row] = s;
     const bool fast = near_ok(amax, s);  // of the row
     if (NC > 0) {
 #pragma unroll
@@ -122,7 +126,8 @@ int launch_groups(const SiluArgs& a, hipStream_t st) {
 }
 
 // Two chunks per thread until a row takes 1024 of them: fewer threads per row mean less to wait for between the maximum and the codes, fewer chunks more wavefronts that
-// hide it.  8192 rows in int8, us, threads x chunks: 1024 channels 64 x 2 (four rows to a block) 9.2, 128 x 1 11.9, 256 x 1 14.4; 2048 128 x 2 17.0, 64 x 4 17.8, 256 x 1
+// hide it.  Up to 64 threads, rows share a wavefront and a block of 256 threads.  32768 rows in int8, us, threads x chunks: 256 channels 16 x 2 8.8, 32 x 2 10.4, 64 x 1
+// 18.8; 512 32 x 2 16.7, 64 x 2 18.5; 552 64 x 2 21.8, 32 x 3 19.0, 768 23.6 and 24.3.  8192 rows: 1024 channels 64 x 2 9.2, 128 x 1 11.9, 256 x 1 14.4; 2048 128 x 2 17.0, 64 x 4 17.8, 256 x 1
 // 20.7; 3584 256 x 2 28.0, 512 x 1 34.1; 8192 512 x 2 62.9, 1024 x 1 73.7, 256 x 4 64.1; 13696 1024 x 2 96, 512 x 4 105; 18944 1024 x 3 136, 512 x 5 145; 28672 1024 x 4
 // 221, rows computed twice 294.  A few rows of 8192: 512 x 2 2.9, 1024 x 1 3.5.
 template <int DT, int MODE>
@@ -130,7 +135,9 @@ int launch_rows(const SiluArgs& a, hipStream_t st) {
     const int64_t chunks = a.N >> 3;
 #define LLMQ_SILU(NC, NT, RPB) \
     hipLaunchKernelGGL((silu_rows_kernel<DT, MODE, NC, NT, RPB>), dim3((unsigned)((a.M + RPB - 1) / RPB)), dim3(NT * RPB), 0, st, a)
-    if (chunks <= 128) LLMQ_SILU(2, 64, 4);
+    if (chunks <= 32) LLMQ_SILU(2, 16, 16);
+    else if (chunks <= 64) LLMQ_SILU(2, 32, 8);
+    else if (chunks <= 128) LLMQ_SILU(2, 64, 4);
     else if (chunks <= 256) LLMQ_SILU(2, 128, 1);
     else if (chunks <= 512) LLMQ_SILU(2, 256, 1);
     else if (chunks <= 1024) LLMQ_SILU(2, 512, 1);

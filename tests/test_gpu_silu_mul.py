@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
 KINDS = ["same", "int8", "fp8", "group"]
-SIZES = [(1, 8), (1, 3584), (3, 136), (37, 18944), (300, 896), (256, 1024), (255, 1024), (5, 2056), (399, 4096), (400, 4104), (401, 8192), (9, 24576), (7, 24584), (1030, 2432), (2100, 264), (9, 1024), (260, 1032), (2, 16384), (300, 16392), (3, 32768), (5, 32776)]
+SIZES = [(1, 8), (1, 3584), (3, 136), (37, 18944), (300, 896), (256, 1024), (255, 1024), (5, 2056), (399, 4096), (400, 4104), (401, 8192), (9, 24576), (7, 24584), (1030, 2432), (2100, 264), (9, 1024), (260, 1032), (17, 256), (300, 248), (9, 264), (31, 512), (2, 16384), (300, 16392), (3, 32768), (5, 32776)]
 
 
 def call(kind, x):
