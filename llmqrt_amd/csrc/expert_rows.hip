@@ -60,11 +60,12 @@ __device__ __forceinline__ int scan_lds(int32_t* v, int n, int32_t* sums) {
 
 // Many ids: a block per expert finds the places of its own.  Every wavefront has a run of the ids and goes over it twice: it counts those of smaller experts and
 // of this one, and hands out places from where the runs before it end.  A run of up to U * Q * 64 ids stays in registers between the two.
-// Q: ids of a lane next to each other (4: 16-byte loads).  32768 ids of 32 experts, us: 8 pieces of 64 at a time, loaded twice 11.1, so 9.6; 8000 of 60 4.4 and 5.6.
-template <int Q>
+// Q: ids of a lane next to each other (4: 16-byte loads); U: pieces of 64 Q ids that a run holds.  us, U = 2, 4, 8 with 16-byte loads, 8 with 4-byte ones: 8000 ids of 60
+// experts 3.9 4.5 5.8 4.1, 16384 of 64 6.5 5.6 6.9 7.4, 24000 of 256 8.8 9.4 7.8 9.7.
+template <int Q, int U>
 __global__ __launch_bounds__(1024) void expert_places_kernel(const int32_t* __restrict__ ids, int n, int first, int experts, int32_t* __restrict__ places,
                                                              int32_t* __restrict__ offsets) {
-    constexpr int NW = 1024 / kWave, U = 8, PIECE = Q * kWave;  // U pieces requested before the first is used
+    constexpr int NW = 1024 / kWave, PIECE = Q * kWave;  // U pieces requested before the first is used
     __shared__ int32_t s_same[NW], s_less[NW];
     const int e = blockIdx.x, lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int run = ((n + NW - 1) / NW + PIECE - 1) / PIECE * PIECE, lo = (int)min((int64_t)n, (int64_t)wave * run), hi = min(n - lo, run) + lo;
@@ -566,7 +567,7 @@ extern "C" int llmq_dispatch_experts(int out, const void* x, int x_dtype, int64_
     a.wide = K % 16 == 0 && aligned16(rows);
     const hipStream_t st = (hipStream_t)stream;
     // every token counts all ids, or further launches find the places: us, counted / found (rows of 3584 int8) 512 tokens of 4 5.6 / 8.2, 1024 of 4 7.5 / 8.8, 2000 of
-    // 4 14 / 9.6
+    // 4 14 / 8
     const bool all = count_all(tokens, top_k);
     Runs r;
     if (!all && in_runs(a.ids_total, experts, r)) {
@@ -581,8 +582,13 @@ extern "C" int llmq_dispatch_experts(int out, const void* x, int x_dtype, int64_
         hipLaunchKernelGGL(run_places_kernel, dim3(blocks), dim3(threads), (kRunWaves + 1) * experts * 4, st, ids, r, a.first, a.experts, bits, places, offsets);
         if (launch_status() != LLMQ_OK) return LLMQ_ERR_LAUNCH;
     } else if (!all) {
-        if (aligned16(ids)) hipLaunchKernelGGL((expert_places_kernel<4>), dim3((unsigned)experts), dim3(1024), 0, st, ids, a.ids_total, a.first, a.experts, places, offsets);
-        else hipLaunchKernelGGL((expert_places_kernel<1>), dim3((unsigned)experts), dim3(1024), 0, st, ids, a.ids_total, a.first, a.experts, places, offsets);
+#define LLMQ_PLACES(Q, U) \
+    hipLaunchKernelGGL((expert_places_kernel<Q, U>), dim3((unsigned)experts), dim3(1024), 0, st, ids, a.ids_total, a.first, a.experts, places, offsets)
+        if (!aligned16(ids)) LLMQ_PLACES(1, 8);
+        else if (a.ids_total <= 2 * 4 * 1024) LLMQ_PLACES(4, 2);  // (pieces of a run, ids of a lane, lanes)
+        else if (a.ids_total <= 4 * 4 * 1024) LLMQ_PLACES(4, 4);
+        else LLMQ_PLACES(4, 8);
+#undef LLMQ_PLACES
         if (launch_status() != LLMQ_OK) return LLMQ_ERR_LAUNCH;
     }
     const int64_t step = (int64_t)1 << 21;  // tokens of a grid: 2^32 threads are too many
