@@ -456,13 +456,13 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
         for (int v = 0; v < V; v++) key[v] = v == at ? kNone : key[v];  // (past the lane's last expert there is nothing to lose)
         if constexpr (BY == BY_SCORES_32) {
             // Two close sigmoid scores are compared in 64 bits by themselves, below; three, and those of a softmax, whose sum takes part, are not.
-            const bool close = j > 0 && best != kNone && !(before - best > 2 * off + 0x1p-24f * (fabsf(before) + fabsf(best)));
+            const bool close = j > 0 && best > kNone && !(before - best > 2 * off + 0x1p-24f * (fabsf(before) + fabsf(best)));
             if (close && (near_last || (j <= a.top && (!a.sigmoid || j == LPT)))) sure = false;
             if (j == a.top && __any(close && sure)) rounds++;
             pairs |= (uint64_t)(close && j <= a.top) << j;
             before = best, near_last = close;
         }
-        if (l == j) id = best != kNone ? chosen : -1;
+        if (l == j) id = best > kNone ? chosen : -1;  // (nothing left, or nothing but NaN)
     }
     if (!__any(sure && wanted)) return false;
 

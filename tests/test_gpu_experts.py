@@ -190,6 +190,27 @@ def test_route_not_finite(cuda):
         assert 7 in ids[20].tolist()
 
 
+def test_route_tokens_of_nan(cuda):
+    """A token with NaN alone, or NaN and masked experts, beside others: they get what they get without it, and it gets experts in range, none twice."""
+    from llmqrt_amd.experts import route_to_experts
+    g = torch.Generator().manual_seed(14)
+    for T, E, groups in ((40, 64, 1), (40, 256, 8), (3100, 128, 4), (4200, 256, 1), (6000, 256, 8)):
+        x = torch.randn(T, E, generator=g).to(cuda)
+        bias = (torch.randn(E, generator=g) * 0.1).to(cuda)
+        bad = x.clone()
+        bad[3] = float("nan")
+        bad[T - 1] = float("nan")
+        bad[T // 2, 1:], bad[T // 2, 0] = -INF, float("nan")
+        rest = [t for t in range(T) if t not in (3, T // 2, T - 1)]
+        for scoring, b in (("softmax", None), ("sigmoid", bias), ("softmax", bias)):
+            w, ids = route_to_experts(bad, 4, scoring, b, groups, groups, "max" if b is None else "top2")
+            w0, ids0 = route_to_experts(x, 4, scoring, b, groups, groups, "max" if b is None else "top2")
+            assert same(ids[rest], ids0[rest]) and same(w[rest], w0[rest])
+            for t in (3, T // 2, T - 1):
+                own = [i for i in ids[t].tolist() if i >= 0]
+                assert all(i < E for i in own) and len(set(own)) == len(own) and ids[t].min() >= -1
+
+
 def test_route_far_logits(cuda):
     """Renormalised weights are ratios, also of scores that underflow."""
     x = torch.full((3, 32), -200.0, device=cuda)
