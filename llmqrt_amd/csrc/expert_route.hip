@@ -449,8 +449,9 @@ __device__ __forceinline__ bool route_short(const RouteArgs& a, Lay lay, int64_t
         int at = V;  // the lowest of the lane's experts that has it
 #pragma unroll
         for (int v = V - 1; v >= 0; v--) at = key[v] == best ? v : at;
-        const uint32_t lowest = token_max<LPT>(at < V ? 0xffffu - (uint32_t)(e0 + at) : 0u);
-        const int chosen = 0xffff - (int)lowest;
+        int chosen;  // (experts lie in the order of lanes)
+        if constexpr (LPT == kWave) chosen = __builtin_amdgcn_readlane(e0 + at, (__ffsll((unsigned long long)__ballot(at < V)) - 1) & (kWave - 1));
+        else chosen = 0xffff - (int)token_max<LPT>(at < V ? 0xffffu - (uint32_t)(e0 + at) : 0u);
         at = chosen - e0;
 #pragma unroll
         for (int v = 0; v < V; v++) key[v] = v == at ? kNone : key[v];  // (past the lane's last expert there is nothing to lose)
@@ -541,15 +542,14 @@ bool try_short(const RouteArgs& a, hipStream_t st) {
 }
 
 // A few tokens are a chain of latencies, which fewer experts for a lane shorten; many are instructions, of which more experts for a lane need fewer.
-// us without / with a bias, 16, 32, 64 lanes for a token: 16 tokens of 256 experts 4.9 4.2 4.0 / 6.0 5.2 4.9, 2048 of them 5.2 4.6 5.0 / 6.4 5.7 6.0, 8192 6.4 7.7 11.3 /
-// 8.5 9.6 14.0; 16 and 32 lanes, 16 tokens of 128 4.0 3.7 / 4.8 4.5, 3000 4.2 4.5 / 5.3 5.5, 8192 4.8 6.3 / 6.0 7.9.
+// us without / with a bias, 16, 32, 64 lanes for a token: 16 tokens of 256 experts 5.0 4.2 3.7 / 6.0 5.1 4.5, 2048 of them 5.2 4.6 4.6 / 6.4 5.8 5.5, 8192 6.4 7.7 9.6 /
+// 8.5 9.6 12.2; 16 and 32 lanes, 16 tokens of 128 4.0 3.7 / 4.8 4.5, 3000 4.2 4.5 / 5.3 5.5, 8192 4.8 6.3 / 6.0 7.9.
 template <int DT, bool EXACT>
 int launch_route(const RouteArgs& a, hipStream_t st) {
     bool done = false;
     if (a.groups <= kShortGroups && a.top <= kShortTop && a.experts <= kShortExperts) {
         done = try_short<DT, EXACT, 16, 4>(a, st);
-        if (!done && a.tokens <= 2500) done = try_short<DT, EXACT, 32, 4>(a, st);
-        if (!done && a.tokens <= 1500) done = try_short<DT, EXACT, 64, 4>(a, st);
+        if (!done && a.tokens <= 2500) done = try_short<DT, EXACT, 32, 4>(a, st) || try_short<DT, EXACT, 64, 4>(a, st);
         if (!done) done = try_short<DT, EXACT, 16, 8>(a, st);
         if (!done && a.tokens <= 5000) done = try_short<DT, EXACT, 32, 8>(a, st);
         if (!done) done = try_short<DT, EXACT, 16, 16>(a, st);
