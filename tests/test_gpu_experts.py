@@ -329,7 +329,7 @@ def test_dispatch_skewed(cuda):
         check_dispatch("same", x[:50], ids[:50].to(torch.int32).to(cuda), 8)
 
 
-@pytest.mark.parametrize("T", [6, 2000])
+@pytest.mark.parametrize("T", [6, 2000, 30000])
 def test_dispatch_rows_left_alone(cuda, T):
     """The C entry writes the rows that have an expert and no other byte."""
     from llmqrt_amd import _abi
@@ -340,13 +340,16 @@ def test_dispatch_rows_left_alone(cuda, T):
     n = T * top
     rows = torch.full((n + 2, K), 77, dtype=torch.int8, device=cuda)
     scale, places, offsets = torch.full((n + 2,), 7.0, device=cuda), torch.full((n + 2,), 7, dtype=torch.int32, device=cuda), torch.full((E + 3,), 7, dtype=torch.int32, device=cuda)
+    need = L.llmq_dispatch_experts_workspace_bytes(T, top, E)
+    assert (need > 0) == (T == 30000)
+    ws = torch.full((need + 64,), 77, dtype=torch.uint8, device=cuda)
     _abi.check(L.llmq_dispatch_experts(1, x.data_ptr(), _abi.BF16, T, K, K, ids.data_ptr(), top, 0, E, rows[1].data_ptr(), scale[1:].data_ptr(), offsets[1:].data_ptr(),
-                                       places[1:].data_ptr(), None, 0, _abi.stream_of(x)), "dispatch")
+                                       places[1:].data_ptr(), ws.data_ptr(), need, _abi.stream_of(x)), "dispatch")
     off, pl, _ = sorted64(ids.cpu(), E, 0)
     end = int(off[-1])
     assert same(offsets[1:E + 2].cpu(), off) and same(places[1:n + 1].view(T, top).cpu(), pl) and 0 < end < n
     assert (rows[0] == 77).all() and (rows[end + 1:] == 77).all() and scale[0] == 7 and (scale[end + 1:] == 7).all()
-    assert offsets[0] == 7 and offsets[E + 2] == 7 and places[0] == 7 and places[n + 1] == 7
+    assert (ws[need:] == 77).all() and offsets[0] == 7 and offsets[E + 2] == 7 and places[0] == 7 and places[n + 1] == 7
 
 
 def test_dispatch_layouts(cuda):
