@@ -259,8 +259,8 @@ __global__ __launch_bounds__(kRunWaves * kWave) void run_places_kernel(const int
 }
 
 // Whether there are so many ids that the three launches are faster than a block per expert over all of them, and how they share them.  us, a block per expert / in
-// runs: 16384 ids of 64 experts 6.9 / 7.9, 32768 of 32 9.2 / 7.7, of 128 9.0 / 8.4, of 256 8.6 / 9.7, 65536 of 256 19.2 / 10.2, 262144 of 64 72 / 9.3; 16000 of 512 10.2 / 12.1,
-// of 1024 17.5 / 17.6, of 4096 59 / 50.  The one grows with ids, and with experts where the chip does not hold a block of each, the other with experts.
+// runs: 16384 ids of 64 experts 6.9 / 7.9, 32768 of 32 9.2 / 7.7, of 128 9.0 / 8.4, of 256 8.6 / 9.7, 65536 of 256 19.2 / 10.2, 262144 of 64 72 / 9.3; 16000 of 512
+// 10.2 / 12.1, of 1024 17.5 / 17.6, of 4096 59 / 50.  The one grows with ids, and with experts where the chip does not hold a block of each, the other with experts.
 bool in_runs(int64_t n, int64_t experts, Runs& r) {
     r.n = (int)n, r.per = (int)(((n + kMaxRuns - 1) / kMaxRuns + kRunUnit - 1) / kRunUnit * kRunUnit);
     r.runs = (int)((n + r.per - 1) / r.per), r.stride = (r.runs + 3) / 4 * 4;

@@ -125,11 +125,11 @@ int launch_groups(const SiluArgs& a, hipStream_t st) {
     return launch_status();
 }
 
-// Two chunks per thread until a row takes 1024 of them: fewer threads per row mean less to wait for between the maximum and the codes, fewer chunks more wavefronts that
-// hide it.  Up to 64 threads, rows share a wavefront and a block of 256 threads.  32768 rows in int8, us, threads x chunks: 256 channels 16 x 2 8.8, 32 x 2 10.4, 64 x 1
-// 18.8; 512 32 x 2 16.7, 64 x 2 18.5; 552 64 x 2 21.8, 32 x 3 19.0, 768 23.6 and 24.3.  8192 rows: 1024 channels 64 x 2 9.2, 128 x 1 11.9, 256 x 1 14.4; 2048 128 x 2 17.0, 64 x 4 17.8, 256 x 1
-// 20.7; 3584 256 x 2 28.0, 512 x 1 34.1; 8192 512 x 2 62.9, 1024 x 1 73.7, 256 x 4 64.1; 13696 1024 x 2 96, 512 x 4 105; 18944 1024 x 3 136, 512 x 5 145; 28672 1024 x 4
-// 221, rows computed twice 294.  A few rows of 8192: 512 x 2 2.9, 1024 x 1 3.5.
+// Two chunks per thread until a row takes 1024 of them: fewer threads per row mean less to wait for between the maximum and the codes, fewer chunks more
+// wavefronts that hide it.  Up to 64 threads, rows share a wavefront and a block of 256 threads.  32768 rows in int8, us, threads x chunks: 256 channels 16 x 2
+// 8.8, 32 x 2 10.4, 64 x 1 18.8; 512 32 x 2 16.7, 64 x 2 18.5; 552 64 x 2 21.8, 32 x 3 19.0, 768 23.6 and 24.3.  8192 rows: 1024 channels 64 x 2 9.2, 128 x 1
+// 11.9, 256 x 1 14.4; 2048 128 x 2 17.0, 64 x 4 17.8, 256 x 1 20.7; 3584 256 x 2 28.0, 512 x 1 34.1; 8192 512 x 2 62.9, 1024 x 1 73.7, 256 x 4 64.1; 13696 1024
+// x 2 96, 512 x 4 105; 18944 1024 x 3 136, 512 x 5 145; 28672 1024 x 4 221, rows computed twice 294.  A few rows of 8192: 512 x 2 2.9, 1024 x 1 3.5.
 template <int DT, int MODE>
 int launch_rows(const SiluArgs& a, hipStream_t st) {
     const int64_t chunks = a.N >> 3;
