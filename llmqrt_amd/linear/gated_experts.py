@@ -39,12 +39,12 @@ class GatedExperts(torch.nn.Module):
         self.register_buffer("score_bias", score_bias)
 
     def _apply(self, fn, *args, **kwargs):
-        bias = self._buffers.pop("score_bias")  # .half() and .bfloat16() are for the activations: scores stay fp32
-        try:
-            out = super()._apply(fn, *args, **kwargs)
-        finally:
-            self._buffers["score_bias"] = None if bias is None else bias.to(fn(bias).device)
-        return out
+        kept = self.score_bias
+
+        def moved(t):  # .half() and .bfloat16() are for the activations: scores stay fp32
+            u = fn(t)
+            return t.to(u.device) if t is kept and u.dtype != t.dtype else u
+        return super()._apply(moved, *args, **kwargs)
 
     def forward(self, x, logits, shared=None):
         """``x`` [.., K] in the modules' dtype, ``logits`` [.., experts of the router]; ``shared`` [.., K'] is added to the result (an expert that all tokens

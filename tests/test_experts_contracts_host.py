@@ -1,0 +1,37 @@
+"""CPU-only checks of what the modules and entries by experts promise beyond their results: conversions, constructor refusals, size queries."""
+import pytest
+import torch
+
+
+def layer(dev="cpu", bias=True):
+    from llmqrt_amd.linear import GatedExperts, SqW8A8GroupedLinear
+    up, down = SqW8A8GroupedLinear(4, 64, 96, dev=dev), SqW8A8GroupedLinear(4, 48, 64, dev=dev)
+    return GatedExperts(up, down, 2, torch.arange(4.0, device=dev) if bias else None)
+
+
+@pytest.mark.parametrize("bias", [True, False])
+def test_layer_from_the_meta_device(bias):
+    """A layer that was built without memory takes memory and then its values, the scores' bias among them."""
+    m = layer("meta", bias).to_empty(device="cpu")
+    assert m.gate_up.qweight.device.type == "cpu" and (m.score_bias is None) == (not bias)
+    m.load_state_dict(layer("cpu", bias).state_dict())
+    if bias:
+        assert m.score_bias.dtype == torch.float32 and torch.equal(m.score_bias, torch.arange(4.0))
+
+
+def test_conversions_keep_the_scores_bias():
+    for f in (lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.to(torch.float16), lambda m: m.to("cpu", torch.bfloat16), lambda m: m.to("meta").half()):
+        m = f(layer())
+        assert m.score_bias.dtype == torch.float32 and "score_bias" in m.state_dict() and m.gate_up.dtype in (torch.float16, torch.bfloat16)
+
+
+def test_a_failed_conversion_leaves_the_layer_whole():
+    m = layer()
+
+    def fails(t):
+        if t is m.score_bias:
+            raise NotImplementedError("no")
+        return t
+    with pytest.raises(NotImplementedError):
+        m._apply(fails)
+    assert torch.equal(m.score_bias, torch.arange(4.0)) and "score_bias" in m.state_dict()
