@@ -18,10 +18,10 @@ _KINDS = {SqW8A8GroupedLinear: (dispatch_quantize_activation_per_token_absmax, s
 
 
 class GatedExperts(torch.nn.Module):
-    """``gate_up``: the experts' gate and up projections joined, [2 I, K] each, ``down``: their down projections [K', I]; both SqW8A8GroupedLinear or both
-    FP8BlockGroupedLinear.  ``score_bias``: fp32 [experts of the router] or None; ``routing``: the other arguments of route_to_experts (scoring, num_groups,
-    top_groups, group_score, renormalize, scale).  ``first_expert``: the router's number of the first expert here, where a GPU holds a part of them; its output is
-    then its part of the sum."""
+    """``gate_up``: the experts' gate and up projections joined, [2 I, K] each, ``down``: their down projections [K', I], K' a multiple of 8; both
+    SqW8A8GroupedLinear or both FP8BlockGroupedLinear.  ``score_bias``: fp32 [experts of the router] or None; ``routing``: the other arguments of route_to_experts
+    (scoring, num_groups, top_groups, group_score, renormalize, scale).  ``first_expert``: the router's number of the first expert here, where a GPU holds a part
+    of them; its output is then its part of the sum."""
 
     def __init__(self, gate_up, down, top_k, score_bias=None, first_expert=0, **routing):
         super().__init__()
@@ -29,6 +29,8 @@ class GatedExperts(torch.nn.Module):
             raise RuntimeError("gate_up and down must both be SqW8A8GroupedLinear or both FP8BlockGroupedLinear")
         if gate_up.num_experts != down.num_experts or gate_up.out_features != 2 * down.in_features or gate_up.out_features % 16:
             raise RuntimeError("gate_up and down must have as many experts, and gate_up twice the channels that down takes, a multiple of 8")
+        if down.out_features % 8:
+            raise RuntimeError(f"down must have a multiple of 8 output channels, got {down.out_features}")
         if gate_up.dtype != down.dtype:
             raise RuntimeError("gate_up and down must have one dtype")
         unknown = set(routing) - {"scoring", "num_groups", "top_groups", "group_score", "renormalize", "scale"}

@@ -35,3 +35,14 @@ def test_a_failed_conversion_leaves_the_layer_whole():
     with pytest.raises(NotImplementedError):
         m._apply(fails)
     assert torch.equal(m.score_bias, torch.arange(4.0)) and "score_bias" in m.state_dict()
+
+
+def test_a_layer_whose_sum_cannot_be_formed_is_refused():
+    """combine_from_experts takes multiples of 8 channels: said when the layer is built, not behind four of its steps."""
+    from llmqrt_amd.linear import FP8BlockGroupedLinear, GatedExperts, SqW8A8GroupedLinear
+    for kind in (SqW8A8GroupedLinear, FP8BlockGroupedLinear):
+        up = kind(4, 64, 96, dev="cpu")
+        for n in (100, 4, 65):
+            with pytest.raises(RuntimeError, match="multiple of 8"):
+                GatedExperts(up, kind(4, 48, n, dev="cpu"), 2)
+        GatedExperts(up, kind(4, 48, 104, dev="cpu"), 2)
