@@ -24,7 +24,7 @@ from typing import Iterable
 import torch
 from torch import nn
 
-from .linear import FP8BlockGroupedLinear, FP8BlockLinear, SqW8A8BBF16OBF16PerChannel, method_to_linear
+from .linear import FP8BlockGroupedLinear, FP8BlockLinear, SqW8A8BBF16OBF16PerChannel, SqW8A8GroupedLinear, method_to_linear
 
 
 @dataclass
@@ -95,7 +95,7 @@ def replace_linears(model: nn.Module, cfg: QuantConfig, dtype=torch.bfloat16) ->
     which the reference declares but does not implement; ``quant_method == "fp8_dynamic_quant"`` with ``q_group_size == 128`` the block-scaled FP8
     module, whose weight is stored in e4m3fn with a scale per 128 x 128 block (the reference's FP8 modules refuse any group size but 0).  With
     ``skip_whole_names`` a name is skipped only where whole parts of it are listed ("mlp.gate" is no part of "mlp.gate_proj").  The modules of a list of experts are replaced one by
-    one; FP8BlockGroupedLinear.from_linears joins them once they are filled."""
+    one; the from_linears of FP8BlockGroupedLinear and SqW8A8GroupedLinear joins them once they are filled."""
     if cfg.quant_method not in method_to_linear:
         raise RuntimeError(f"quant_method {cfg.quant_method!r} is not supported: {sorted(method_to_linear)}, or \"fp8\" with a weight_block_size of 128 x 128 "
                            "and dynamic activation scales")
@@ -184,5 +184,5 @@ def load_quantized_weights(model: nn.Module, path: str, device=None) -> tuple[li
 
 
 def named_quantized_linears(model: nn.Module) -> Iterable[tuple[str, nn.Module]]:
-    kinds = tuple(set(method_to_linear.values()) | {SqW8A8BBF16OBF16PerChannel, FP8BlockLinear, FP8BlockGroupedLinear})
+    kinds = tuple(set(method_to_linear.values()) | {SqW8A8BBF16OBF16PerChannel, SqW8A8GroupedLinear, FP8BlockLinear, FP8BlockGroupedLinear})
     return ((n, m) for n, m in model.named_modules() if isinstance(m, kinds))

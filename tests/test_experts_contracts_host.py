@@ -46,3 +46,11 @@ def test_a_layer_whose_sum_cannot_be_formed_is_refused():
             with pytest.raises(RuntimeError, match="multiple of 8"):
                 GatedExperts(up, kind(4, 48, n, dev="cpu"), 2)
         GatedExperts(up, kind(4, 48, 104, dev="cpu"), 2)
+
+
+def test_named_quantized_linears_names_the_modules_by_experts():
+    from llmqrt_amd.checkpoint import named_quantized_linears
+    from llmqrt_amd.linear import FP8BlockGroupedLinear, GatedExperts
+    model = torch.nn.ModuleDict({"a": layer(), "b": GatedExperts(FP8BlockGroupedLinear(2, 64, 96, dev="cpu"), FP8BlockGroupedLinear(2, 48, 64, dev="cpu"), 1),
+                                 "router": torch.nn.Linear(64, 4)})
+    assert [n for n, _ in named_quantized_linears(model)] == ["a.gate_up", "a.down", "b.gate_up", "b.down"]
