@@ -450,7 +450,8 @@ int llmq_route_experts(int scoring, const void* logits, int logits_dtype, int64_
  *     LLMQ_NORM_I8_TOKEN   the codes of llmq_quant_i8_per_token, 8-byte aligned; scale: fp32 [tokens * top_k]
  *     LLMQ_NORM_FP8_GROUP  the codes of llmq_quant_fp8_per_group, 8-byte aligned; scale: fp32 [tokens * top_k, ceil(K / 128)]
  * x: [tokens, K] bf16 / f16, K % 8 == 0, ldx % 8 == 0, 16-byte aligned.  At most 4096 experts, top_k at most 64, at most 2^31 - 65536 rows.
- * workspace: >= llmq_dispatch_experts_workspace_bytes bytes (0 up to some 20000 rows; NULL will do then), 16-byte aligned, contents irrelevant on entry. */
+ * workspace: >= llmq_dispatch_experts_workspace_bytes(tokens, top_k, experts) bytes, 16-byte aligned, contents irrelevant on entry; NULL will do where that is 0
+ * (it depends on the experts too: none is needed for up to 14000 rows, whatever the experts). */
 int llmq_dispatch_experts(int out, const void* x, int x_dtype, int64_t tokens, int64_t K, int64_t ldx, const int32_t* ids, int64_t top_k,
                           int64_t first_expert, int64_t experts, void* rows, float* scale, int32_t* offsets, int32_t* places,
                           void* workspace, size_t workspace_bytes, llmq_stream_t stream);

@@ -54,3 +54,18 @@ def test_named_quantized_linears_names_the_modules_by_experts():
     model = torch.nn.ModuleDict({"a": layer(), "b": GatedExperts(FP8BlockGroupedLinear(2, 64, 96, dev="cpu"), FP8BlockGroupedLinear(2, 48, 64, dev="cpu"), 1),
                                  "router": torch.nn.Linear(64, 4)})
     assert [n for n, _ in named_quantized_linears(model)] == ["a.gate_up", "a.down", "b.gate_up", "b.down"]
+
+
+def test_dispatch_workspace_bound_of_the_header():
+    """The header names a number of rows up to which no workspace is needed, whatever the experts; it says nothing that the size query does not."""
+    import pathlib
+    import re
+    from llmqrt_amd import _abi
+    need = _abi.lib().llmq_dispatch_experts_workspace_bytes
+    text = (pathlib.Path(__file__).resolve().parent.parent / "include" / "llmq.h").read_text()
+    rows = int(re.search(r"none is needed for up to (\d+) rows, whatever the experts", text)[1])
+    for experts in (1, 60, 255, 256, 257, 512, 1000, 1024, 2048, 4095, 4096):
+        for top in (1, 2, 7, 8, 64):
+            for n in range(max(1, rows // top - 300), rows // top + 1):
+                assert need(n, top, experts) == 0
+    assert need(14200, 1, 4096) > 0 and need(18200, 1, 1024) > 0  # near the bound: another figure would not do
