@@ -413,8 +413,8 @@ size_t llmq_gemm_fp8_block_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 /* The same product by experts: rows offsets[e] .. offsets[e + 1] - 1 of A with the weights of expert e.  B: [experts, N, K], w_scale:
  * [experts, ceil(N / 128), ceil(K / 128)], bias: [experts, N] or null, all contiguous; offsets: int32 [experts + 1] on the device, ascending;
- * values outside [0, M] are taken as the nearest inside.  Rows that belong to no expert are not written.  At most 65536 experts.  No workspace;
- * nothing is read back by the host, so a captured call follows the offsets of its replay. */
+ * values outside [0, M] are taken as the nearest inside, and one below an earlier one as that, so that no row has two experts.  Rows that belong to no expert
+ * are not written.  At most 65536 experts.  No workspace; nothing is read back by the host, so a captured call follows the offsets of its replay. */
 int llmq_gemm_fp8_block_grouped(const uint8_t* A, int64_t lda, const float* a_scale, const uint8_t* B, const float* w_scale,
                                 const int32_t* offsets, int64_t experts, const void* bias, int bias_dtype, void* out, int out_dtype,
                                 int64_t ldo, int64_t M, int64_t N, int64_t K, llmq_stream_t stream);

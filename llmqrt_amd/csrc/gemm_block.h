@@ -25,12 +25,6 @@ struct BlockArgs {
     int bias_dtype, out_dtype;
 };
 
-// Rows [first, last) of expert e, whatever the offsets hold: never outside [0, M].
-__device__ __forceinline__ void expert_rows(const BlockArgs& g, int e, int& first, int& last) {
-    first = min(max(g.offsets[e], 0), g.M);
-    last = min(max(g.offsets[e + 1], first), g.M);
-}
-
 struct BlockTile { int bm, bn, ks; };  // tokens, channels, groups of wavefronts of a block
 constexpr BlockTile kBlockTiles[] = {
     {256, 256, 1},  // 0: 8 wavefronts of 128 x 64

@@ -55,44 +55,14 @@ __global__ __launch_bounds__(C::NT) void block_tile_kernel(BlockArgs g) {
     const int tiles_n = (g.N + C::BN - 1) / C::BN;
 
     // ---- the block's rows [row0, row_end) and channels from n0
-    int tm, tn, row0, row_end, expert = 0;
-    if (!GROUPED) {
+    int tn, row0, row_end, expert = 0;
+    if constexpr (GROUPED) {
+        if (!expert_tile<C::BM>(g.offsets, g.experts, g.M, tiles_n, expert, row0, row_end, tn)) return;  // block-uniform
+    } else {
         const int tiles_m = (g.M + C::BM - 1) / C::BM;
+        int tm;
         tile_of(place_of(blockIdx.x, gridDim.x), tiles_m, tiles_n, tm, tn);
         row0 = tm * C::BM, row_end = g.M;
-    } else {
-        // the experts' tiles of rows, counted by every wavefront for itself: 64 experts at a time
-        int total = 0, first, last, mine, upto;
-        auto count = [&](int e0, int before) __attribute__((always_inline)) {
-            first = last = 0;
-            if (e0 + lane < g.experts) expert_rows(g, e0 + lane, first, last);
-            mine = (last - first + C::BM - 1) / C::BM, upto = before + wave_prefix(mine);
-        };
-        for (int e0 = 0; e0 < g.experts; e0 += kWave) count(e0, total), total = __builtin_amdgcn_readlane(upto, kWave - 1);
-        const int64_t nblk = min((int64_t)gridDim.x, (int64_t)total * tiles_n);
-        if (blockIdx.x >= nblk) return;  // block-uniform
-        // one expert's tiles after the other's, so that neighbours share its weights
-        const int pid = place_of(blockIdx.x, (int)nblk), flat = pid / tiles_n;
-        int before = 0, tiles = 1;
-        row0 = row_end = 0;
-        for (int e0 = 0; e0 < g.experts; e0 += kWave) {
-            if (g.experts > kWave) count(e0, before);  // (not again what is still there)
-            const uint64_t has = __ballot(flat >= upto - mine && flat < upto);
-            if (has) {
-                const int at = __ffsll((unsigned long long)has) - 1;
-                expert = e0 + at;
-                row0 = __builtin_amdgcn_readlane(first, at), row_end = __builtin_amdgcn_readlane(last, at);
-                tiles = __builtin_amdgcn_readlane(mine, at), before = __builtin_amdgcn_readlane(upto, at) - tiles;
-                break;
-            }
-            before = __builtin_amdgcn_readlane(upto, kWave - 1);
-        }
-        tile_of(pid - before * tiles_n, tiles, tiles_n, tm, tn);
-        row0 += tm * C::BM;
-        expert = __builtin_amdgcn_readfirstlane(expert);
-        row0 = __builtin_amdgcn_readfirstlane(row0);
-        row_end = __builtin_amdgcn_readfirstlane(row_end);
-        if (row0 >= row_end) return;  // block-uniform
     }
     const int n0 = tn * C::BN;
     const int kb0 = SPLIT ? blockIdx.y * g.blocks_per_split : 0, kb1 = SPLIT ? min(g.KB, kb0 + g.blocks_per_split) : g.KB;
