@@ -476,7 +476,8 @@ int llmq_gemm_w8a8_grouped(const int8_t* A, int64_t lda, const float* a_scale, c
  * experts, -1: the built-in choice.  Per host thread. */
 int llmq_gemm_w8a8_grouped_force_plan(int cfg);
 
-/* y[m, n] = g / (1 + exp(-g)) * u with g = x[m, n], u = x[m, N + n], in fp32; out as llmq_add_rmsnorm's:
+/* y[m, n] = g / (1 + exp(-g)) * u with g = x[m, n], u = x[m, N + n], in fp32, also where exp(-g) is no fp32 number (from g = -174 down, where y is less than
+ * 3e-74 |u|, it may be 0); out as llmq_add_rmsnorm's:
  *   LLMQ_NORM_SAME y = x_dtype(y) (16-byte aligned); otherwise codes of the fp32 y (8-byte aligned) and scale: fp32 [M] or [M, ceil(N / 128)]
  * x: [M, 2 N] bf16 / f16, N % 8 == 0, ldx % 8 == 0, 16-byte aligned; y: [M, N] contiguous, must not overlap x. */
 int llmq_silu_mul(int out, const void* x, int x_dtype, int64_t M, int64_t N, int64_t ldx, void* y, float* scale, llmq_stream_t stream);

@@ -24,16 +24,26 @@ struct SiluArgs {
     int64_t ldx, M, N;
 };
 
-// exp by the base-2 instruction: |g| 2^-24 off relative to itself, far below what 16 or 8 bits keep.  g of -inf gives -inf * 0 = NaN, as the formula does.
+// exp by the base-2 instruction: y is off by (2 |g| + 8) 2^-24 of itself.  g of -inf gives -inf * 0 = NaN, as the formula does.
 __device__ __forceinline__ float silu(float g) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896f * g));
+}
+// Below -87 the reciprocal, below -88 exp(-g) itself leaves the range of fp32, while y still has bits where u is large.  From kFarGate on 1 is nothing beside exp(-g),
+// which is taken 2^-126 of, and u as well: y is then 0 only where it is less than 3e-74 |u| (g below -174).
+constexpr float kFarGate = -80.0f;
+__device__ __forceinline__ float far_silu_mul(float g, float u) {
+    return g * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(-1.44269504088896f * g - 126.0f)) * (u * 0x1p-126f);
 }
 template <int DT>
 __device__ __forceinline__ void gated8(uint4 gv, uint4 uv, float* y) {
     float g[8], u[8];
     widen8<DT>(gv, g), widen8<DT>(uv, u);
+    uint32_t most = 0;  // of negative numbers, the bits of the lowest
 #pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = silu(g[i]) * u[i];
+    for (int i = 0; i < 8; i++) y[i] = silu(g[i]) * u[i], most = max(most, __float_as_uint(g[i]));
+    if (__any(most > __float_as_uint(kFarGate)))  // uniform, and rare
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = g[i] < kFarGate ? far_silu_mul(g[i], u[i]) : y[i];
 }
 
 // No reduction over the whole row: 16 lanes take 128 channels of a row, 8 of each half a lane.  One such piece per lane, and many blocks: with two or four

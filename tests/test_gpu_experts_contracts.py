@@ -29,3 +29,30 @@ def test_block_scaled_offsets_that_descend(cuda, E, M):
             finally:
                 _abi.lib().llmq_gemm_fp8_block_force_plan(-1, 0)
             assert torch.equal(room[1:-1], want) and (room[0] == 7).all() and (room[-1] == 7).all(), (at[:6], cfg)
+
+
+@pytest.mark.parametrize("kind", ["same", "int8", "fp8", "group"])
+@pytest.mark.parametrize("N", [256, 18944, 33000])
+def test_gates_whose_exponential_leaves_fp32(cuda, kind, N, monkeypatch):
+    """exp(-g) is no fp32 number below -88, g sigmoid(g) u still one where u is large: the bound of ordinary gates, u_32 (2 |g| + 8) |y|, holds for far ones too,
+    without a term in u of more than 3e-74 (exp(-174), behind which y is 0) and fp32's smallest normal number."""
+    import test_gpu_silu_mul as ordinary
+
+    def exact(x):
+        g, u = x.double().chunk(2, dim=-1)
+        y = g * torch.sigmoid(g) * u
+        return y, ordinary.U * (2 * g.abs() + 8) * y.abs() + 3e-74 * u.abs() + 2.0 ** -126
+    monkeypatch.setattr(ordinary, "exact", exact)
+    x = torch.ones(9, 2 * N, dtype=torch.float64)
+    x[:, :N] = torch.linspace(-200, -60, N, dtype=torch.float64)
+    x[1, N:], x[2, N:], x[3, N:], x[4, N:] = 3e38, -1e30, 1e-30, 6e4
+    x[5, :N], x[5, N:] = -89.0, 3e38
+    x[6, : N - 1] = 2.0  # one far gate in a row of others
+    x[7, :N], x[7, N:] = torch.linspace(-81, -79, N, dtype=torch.float64), 2e35
+    x[8, :N], x[8, N:] = torch.linspace(-178, -170, N, dtype=torch.float64), 3e38
+    x = x.to(torch.bfloat16)
+    ordinary.check(kind, x.to(cuda))
+    if kind == "same":
+        y = ordinary.call(kind, x.to(cuda))
+        assert ((y[5].double().cpu() / (x[5, :N].double() * torch.sigmoid(x[5, :N].double()) * x[5, N:].double()) - 1).abs() < 0.0041).all()
+    ordinary.check(kind, x[[0, 4]].half().to(cuda))
