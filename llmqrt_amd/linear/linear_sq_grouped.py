@@ -71,9 +71,10 @@ class SqW8A8GroupedLinear(LinearBase):
     def forward(self, x, offsets, out=None):
         """``x`` [M, K] in bf16 or fp16, sorted by expert; ``offsets``: int32 [num_experts + 1] on the GPU, the experts' first rows and the end of the last.
         Rows of no expert are not written (sq_fp8_kernels.w8a8_int8_linear_per_channel_grouped).  -> [M, N] in x's type."""
-        if x.dim() != 2 or x.shape[1] != self.in_features or x.dtype not in _NAMES:
-            raise RuntimeError(f"the input must be [rows, {self.in_features}] in bf16 or fp16")
-        q, s = quantize_activation_per_token_absmax_f32(x)
+        if x.dim() != 2 or x.shape[1] != self.in_features or x.dtype not in _NAMES or not x.is_cuda:
+            raise RuntimeError(f"the input must be [rows, {self.in_features}] in bf16 or fp16 on a GPU")
+        with torch.cuda.device(x.device):  # (the quantizer launches on the current one)
+            q, s = quantize_activation_per_token_absmax_f32(x)
         return w8a8_int8_linear_per_channel_grouped(q, self.qweight, self.bias, s, self.weight_scale, offsets, _NAMES[x.dtype], out)
 
     def forward_quantized(self, qinput, x_scale, offsets, out=None):

@@ -69,3 +69,32 @@ def test_dispatch_workspace_bound_of_the_header():
             for n in range(max(1, rows // top - 300), rows // top + 1):
                 assert need(n, top, experts) == 0
     assert need(14200, 1, 4096) > 0 and need(18200, 1, 1024) > 0  # near the bound: another figure would not do
+
+
+def test_rows_are_quantized_on_their_own_device(monkeypatch):
+    """The current device may be another than the activations': the quantizer in front of the product launches with theirs as the current one."""
+    import contextlib
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from llmqrt_amd.linear import SqW8A8GroupedLinear
+    from llmqrt_amd.linear import linear_sq_grouped as mod
+    current, seen = [torch.device("cuda:0")], []
+
+    @contextlib.contextmanager
+    def device(d):
+        current.append(torch.device(d))
+        yield
+        current.pop()
+
+    def quantizer(x):
+        seen.append((x.device, current[-1]))
+        return x, x
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(mod, "quantize_activation_per_token_absmax_f32", quantizer)
+    monkeypatch.setattr(mod, "w8a8_int8_linear_per_channel_grouped", lambda *a: a[0])
+    m = SqW8A8GroupedLinear(2, 64, 40, dev="cpu")
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        x = torch.empty(3, 64, dtype=torch.bfloat16, device="cuda:1")
+        m(x, None)
+    assert seen == [(torch.device("cuda:1"), torch.device("cuda:1"))] and current == [torch.device("cuda:0")]
+    with pytest.raises(RuntimeError):
+        m(torch.zeros(3, 64, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32))
