@@ -190,7 +190,7 @@ __device__ __forceinline__ void route_long(const RouteArgs& a, int64_t t) {
         return expf(v - top_x) / (1.f + expf(v));
     };
     if (a.renormalize) {
-        sum = 0.f;
+        sum = sum == sum ? 0.f : sum;  // (a softmax that has no value gives none to weights, also where the logit that took it away is not chosen)
         for (int j = 0; j < a.top; j++)
             if (s_id[j] >= 0) sum += part(s_x[j]);
     } else if (a.sigmoid) {

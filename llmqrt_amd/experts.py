@@ -34,8 +34,8 @@ def route_to_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax",
     ``scale``.  With ``num_groups`` > 1 only the experts of the ``top_groups`` groups of neighbours with the largest score take part: the largest c of the group
     (``group_score`` "max") or the sum of its two largest ("top2").
     An expert whose logit or bias is -inf is never chosen; a place that is left over has expert -1 and weight 0, and goes nowhere in the functions below.
-    The order is that of the exact scores: without a bias the logits' own, otherwise that of scores in 64 bits.  A token with a NaN among its logits gets
-    experts in range, none twice; its softmax weights are NaN."""
+    The order is that of the exact scores: without a bias the logits' own, otherwise that of scores in 64 bits.  A token with a NaN (or, for
+    softmax, +inf) among its logits gets experts in range, none twice; its softmax weights are NaN."""
     if scoring in _SCORING and group_score in _GROUP_SCORE:
         y = host().route(logits, bias, top_k, _SCORING[scoring], num_groups, top_groups, _GROUP_SCORE[group_score], bool(renormalize), scale)
         if y is not None:

@@ -56,3 +56,23 @@ def test_gates_whose_exponential_leaves_fp32(cuda, kind, N, monkeypatch):
         y = ordinary.call(kind, x.to(cuda))
         assert ((y[5].double().cpu() / (x[5, :N].double() * torch.sigmoid(x[5, :N].double()) * x[5, N:].double()) - 1).abs() < 0.0041).all()
     ordinary.check(kind, x[[0, 4]].half().to(cuda))
+
+
+@pytest.mark.parametrize("T,E,groups", [(3, 40, 1), (9, 64, 4), (70, 256, 8), (3000, 128, 1), (5, 300, 5), (4, 1024, 1)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_weights_of_a_softmax_without_value_are_nan(cuda, T, E, groups, bad):
+    """A NaN or an infinity among the logits leaves the softmax of a token no value: its weights are NaN, with a bias and without, divided by their sum or not; its
+    experts are in range and none twice, and other tokens do not notice."""
+    from llmqrt_amd.experts import route_to_experts
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, E, generator=g).to(cuda)
+    wrong = x.clone()
+    wrong[1, E - 3] = bad  # (not among the lowest experts, which are chosen where all scores are NaN)
+    rest = [t for t in range(T) if t != 1]
+    for bias in (None, (torch.randn(E, generator=g) * 0.1).to(cuda)):
+        for score in ("max", "top2"):
+            for renormalize in (True, False):
+                args = (4, "softmax", bias, groups, max(1, groups // 2), score, renormalize, 2.0)
+                (w, ids), (w0, ids0) = route_to_experts(wrong, *args), route_to_experts(x, *args)
+                assert w[1].isnan().all() and len(set(ids[1].tolist())) == 4 and ((ids[1] >= 0) & (ids[1] < E)).all()
+                assert torch.equal(w[rest], w0[rest]) and torch.equal(ids[rest], ids0[rest])
