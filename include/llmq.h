@@ -430,10 +430,10 @@ int llmq_gemm_fp8_block_force_plan(int cfg, int splits);
 /* experts[t, :] = the top_k experts with the largest c = s + bias, largest first, ties to the lowest expert; weights[t, :] = their s, divided by
  * their sum where renormalize != 0, times scale;  s = softmax(logits[t, :]) or 1 / (1 + exp(-logits)).  bias: fp32 [experts] or null; it takes part in the choice
  * alone.  With groups > 1 (it divides experts; at most 64) only the experts of the top_groups groups of neighbours with the largest score are
- * chosen from: the largest c of the group, or the sum of its two largest.
- * An expert whose logit or bias is -inf is never chosen; a place that is left over has expert -1 and weight 0.  The order is that of the exact scores: without a
- * bias the logits' own, otherwise that of scores in 64 bits.  A token with a NaN or, for softmax, +inf among its logits gets experts of that range, none twice, and for
- * softmax weights that are NaN.
+ * chosen from: the largest c of the group, or the sum of its two largest (where masks leave one expert of a group, that one's c alone).
+ * An expert whose logit or bias is -inf is never chosen; a place that is left over has expert -1 and weight 0.  The order is that of the exact scores: the
+ * logits' own, or with a bias or where two scores of a group are added that of scores in 64 bits, where those closer than 64 bits tell apart are ties.  A token
+ * with a NaN or, for softmax, +inf among its logits gets experts of that range, none twice, and for softmax weights that are NaN.
  * logits: bf16 / f16 / f32 [tokens, experts], row stride ld, at any address of its type; at most 1024 experts, top_k at most 64 and at most experts /
  * groups * top_groups.  weights: fp32 [tokens, top_k]; experts: int32 [tokens, top_k]. */
 enum { LLMQ_ROUTE_SOFTMAX = 0, LLMQ_ROUTE_SIGMOID = 1 };

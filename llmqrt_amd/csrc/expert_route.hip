@@ -2,7 +2,7 @@
 //
 //   s = softmax(l) or 1 / (1 + exp(-l));  c = s + bias;  experts = the top_k largest c, ties to the lowest expert;  weights = s of those, divided by their
 //   sum if asked for, times a factor
-// Groups: of neighbouring experts; only the top_groups groups with the largest score (max c, or the sum of the two largest c) take part.
+// Groups: of neighbouring experts; only the top_groups groups with the largest score (max c, or the sum of the two largest c, of one that is left alone) take part.
 // l or bias of -inf: the expert is masked, never chosen.  A place that is left over has expert -1 and weight 0.
 //
 // Which experts are chosen has to follow from the scores, not from how they were rounded: without a bias the order of c is that of the logits, which are
@@ -12,9 +12,14 @@
 // A choice is a maximum over a lane's experts and over the lanes (row rotations and swaps, no LDS) and the lowest expert that has it.  Its order is that of the
 // exact scores wherever neighbours in it lie further apart than both scores can be off.  Two closer sigmoid scores are compared in 64 bits by themselves; a token
 // with more of them, with close groups, or with close scores of a softmax is done over with all scores in 64 bits.
-// Many tokens are bound by the vector unit (8192 of 256 experts, 8 chosen: 6.4 us, with a bias 8.5, of 8 groups 10), a few by the chain of choices (16 of them: 4 and
-// 5 us).
-// More than 256 experts, 16 groups or 16 choices, and tokens with a NaN, take the long form.
+// Many tokens are bound by the vector unit (8192 of 256 experts, 8 chosen: 6.5 us, with a bias 8.4, of 8 groups 9.5 to 11 by inputs), a few by the chain of choices
+// (16 of them: 4 and 4.4 us).
+// The long form takes tokens with a NaN, more than 256 experts, 16 groups or 16 choices, and groups too large for their lanes: with 64 lanes shared among the
+// groups, as many for each as the largest power of two that they have room for, four experts a lane (240 experts in 3, 5 or 6 groups do not fit, 256 in 8 do).  A
+// wavefront takes a token there, 16 experts a lane, all scores with a bias or of added pairs in 64 bits.  us, 8 chosen: 8192 tokens of 384 with a bias 47, of 1024
+// 31 and with a bias 52, of 240 in 6 groups 49 and 68; 16 tokens of 384 with a bias 15, of 240 in 6 groups 25.
+// The sum under the weights is of fp32 terms in the order of the lanes, of scores in 64 bits where those were formed: weights that are not divided by their own sum
+// may differ in their last places with the number of tokens, and with whether theirs was done over.
 #include <algorithm>
 #include <type_traits>
 

@@ -32,10 +32,10 @@ def route_to_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax",
     ``logits`` [.., experts] in bf16, fp16 or fp32; s = softmax(logits) or sigmoid(logits) in fp32.  Chosen are the largest c = s + ``bias`` (fp32 [experts], for
     balance; it takes part in the choice alone), ties going to the lowest expert; the weights are their s, divided by their sum if ``renormalize``, times
     ``scale``.  With ``num_groups`` > 1 only the experts of the ``top_groups`` groups of neighbours with the largest score take part: the largest c of the group
-    (``group_score`` "max") or the sum of its two largest ("top2").
+    (``group_score`` "max") or the sum of its two largest ("top2"; where masks leave one expert of a group, that one's c alone).
     An expert whose logit or bias is -inf is never chosen; a place that is left over has expert -1 and weight 0, and goes nowhere in the functions below.
-    The order is that of the exact scores: without a bias the logits' own, otherwise that of scores in 64 bits.  A token with a NaN (or, for
-    softmax, +inf) among its logits gets experts in range, none twice; its softmax weights are NaN."""
+    The order is that of the exact scores: the logits' own, or with a bias or "top2" groups that of scores in 64 bits, where those closer than 64 bits tell apart
+    are ties.  A token with a NaN (or, for softmax, +inf) among its logits gets experts in range, none twice; its softmax weights are NaN."""
     if scoring in _SCORING and group_score in _GROUP_SCORE:
         y = host().route(logits, bias, top_k, _SCORING[scoring], num_groups, top_groups, _GROUP_SCORE[group_score], bool(renormalize), scale)
         if y is not None:

@@ -76,3 +76,29 @@ def test_weights_of_a_softmax_without_value_are_nan(cuda, T, E, groups, bad):
                 (w, ids), (w0, ids0) = route_to_experts(wrong, *args), route_to_experts(x, *args)
                 assert w[1].isnan().all() and len(set(ids[1].tolist())) == 4 and ((ids[1] >= 0) & (ids[1] < E)).all()
                 assert torch.equal(w[rest], w0[rest]) and torch.equal(ids[rest], ids0[rest])
+
+
+def test_a_group_with_one_expert_left(cuda):
+    """Where masks leave one expert of a group, the sum of its two largest scores is that one's alone, in the short form and in the long one."""
+    from llmqrt_amd.experts import route_to_experts
+    for T, E, groups in ((3, 16, 4), (40, 256, 8), (3000, 64, 2), (4, 600, 4)):
+        n = E // groups
+        x = torch.full((T, E), -8.0, device=cuda)
+        x[:, :n] = -float("inf")
+        x[:, 1] = 3.0  # sigmoid 0.953, alone
+        x[:, n:n + 2] = torch.tensor([-0.4, -0.5], device=cuda)  # 0.401 + 0.378
+        w, ids = route_to_experts(x, 1, "sigmoid", None, groups, 1, "top2")
+        assert (ids == 1).all() and (w == 1).all()
+        x[:, 2] = -3.0  # and 0.047: 1.0
+        x[:, n:n + 2] = 0.05  # 0.5125 twice
+        assert (route_to_experts(x, 1, "sigmoid", None, groups, 1, "top2")[1] == n).all()
+
+
+def test_order_of_saturated_scores(cuda):
+    """Logits decide without a bias; where scores are formed, in 64 bits, those that are level there are ties."""
+    from llmqrt_amd.experts import route_to_experts
+    x = torch.tensor([[40.0, 41.0, 42.0, 39.0]], device=cuda)
+    assert route_to_experts(x, 4, "sigmoid")[1].tolist() == [[2, 1, 0, 3]]
+    assert route_to_experts(x, 2, "sigmoid", None, 2, 2, "max")[1].tolist() == [[2, 1]]
+    assert route_to_experts(x, 4, "sigmoid", None, 2, 2, "top2")[1].tolist() == [[0, 1, 2, 3]]
+    assert route_to_experts(x, 4, "sigmoid", torch.zeros(4, device=cuda))[1].tolist() == [[0, 1, 2, 3]]
