@@ -1,7 +1,8 @@
 """The gated activation between two Linear modules, silu(gate) * up, alone or with the quantizer of the second one in the same pass.
 
 No counterpart in the reference, whose modules call torch's.  ``x`` [.., 2 N] holds the gates in its first N channels and what they scale in the others, as the
-output of gate and up projections joined by ``fused_utils.fuse_linears`` does.  Arithmetic is fp32 from x to the output's one rounding or its codes.
+output of gate and up projections joined by ``fused_utils.fuse_linears`` does.  Arithmetic is fp32 from x to the output's one rounding or its codes.  None of
+these calls has a backward pass.
 """
 from __future__ import annotations
 
